@@ -86,6 +86,98 @@ class OptimizerConfig(ctypes.Structure):
     ]
 
 
+# geo_b200_type_t, geo_b200_position_type_t and the rotary enums (geo/geo_b200.h)
+F64, F32, BF16, F16 = 1, 2, 3, 4
+I32, I64 = 1, 2
+ROTARY_INTERLEAVED, ROTARY_HALF = 0, 1
+ROTARY_SCALING_NONE, ROTARY_SCALING_LINEAR, ROTARY_SCALING_BASE, ROTARY_SCALING_BANDED = 0, 1, 2, 3
+ROTARY_MAX_DIM = 256
+
+
+class LayerNormConfig(ctypes.Structure):
+    """geo_b200_layer_norm_config_t: strides in values, 0 for packed rows."""
+
+    _fields_ = [
+        ("type", ctypes.c_uint32),
+        ("parameter_type", ctypes.c_uint32),
+        ("rows", ctypes.c_size_t),
+        ("cols", ctypes.c_size_t),
+        ("x_stride", ctypes.c_size_t),
+        ("y_stride", ctypes.c_size_t),
+        ("y_cotangent_stride", ctypes.c_size_t),
+        ("x_cotangent_stride", ctypes.c_size_t),
+        ("epsilon", ctypes.c_double),
+    ]
+
+
+class DropoutConfig(ctypes.Structure):
+    """geo_b200_dropout_config_t: units of 2^dimension values are kept or dropped as one."""
+
+    _fields_ = [
+        ("type", ctypes.c_uint32),
+        ("dimension", ctypes.c_uint32),
+        ("rows", ctypes.c_size_t),
+        ("cols", ctypes.c_size_t),
+        ("x_stride", ctypes.c_size_t),
+        ("residual_stride", ctypes.c_size_t),
+        ("y_stride", ctypes.c_size_t),
+        ("y_cotangent_stride", ctypes.c_size_t),
+        ("x_cotangent_stride", ctypes.c_size_t),
+        ("rate", ctypes.c_double),
+        ("seed", ctypes.c_uint64),
+        ("offset", ctypes.c_uint64),
+    ]
+
+
+class RotaryConfig(ctypes.Structure):
+    _fields_ = [
+        ("layout", ctypes.c_uint32),
+        ("rotary_dim", ctypes.c_uint32),
+        ("base", ctypes.c_double),
+        ("scaling", ctypes.c_uint32),
+        ("factor", ctypes.c_double),
+        ("original_length", ctypes.c_double),
+        ("low_rotations", ctypes.c_double),
+        ("high_rotations", ctypes.c_double),
+        ("amplitude", ctypes.c_double),
+    ]
+
+
+class RotaryPlan(ctypes.Structure):
+    """geo_b200_rotary_plan_t: turns per position of each pair, as the sum of two float64."""
+
+    _fields_ = [
+        ("abi_version", ctypes.c_uint32),
+        ("layout", ctypes.c_uint32),
+        ("rotary_dim", ctypes.c_uint32),
+        ("reserved", ctypes.c_uint32),
+        ("amplitude", ctypes.c_double),
+        ("turns", ctypes.c_double * (ROTARY_MAX_DIM // 2)),
+        ("turns_low", ctypes.c_double * (ROTARY_MAX_DIM // 2)),
+    ]
+
+
+class RotaryShape(ctypes.Structure):
+    """geo_b200_rotary_shape_t: [batch][tokens][heads][head_dim], strides in values (0: packed)."""
+
+    _fields_ = [
+        ("type", ctypes.c_uint32),
+        ("position_type", ctypes.c_uint32),
+        ("batch", ctypes.c_size_t),
+        ("tokens", ctypes.c_size_t),
+        ("heads", ctypes.c_size_t),
+        ("head_dim", ctypes.c_size_t),
+        ("x_batch_stride", ctypes.c_size_t),
+        ("x_token_stride", ctypes.c_size_t),
+        ("x_head_stride", ctypes.c_size_t),
+        ("y_batch_stride", ctypes.c_size_t),
+        ("y_token_stride", ctypes.c_size_t),
+        ("y_head_stride", ctypes.c_size_t),
+        ("position_batch_stride", ctypes.c_size_t),
+        ("first_position", ctypes.c_int64),
+    ]
+
+
 _P = ctypes.c_void_p
 _D = ctypes.c_double
 _SZ = ctypes.c_size_t
@@ -177,6 +269,20 @@ SIGNATURES: dict[str, tuple] = {
     "geo_b200_sparse_apply_vjp_f64": (_I, [ctypes.POINTER(OperatorPlanI32), _P, _P, _SZ, _P]),
     "geo_b200_sparse_apply_parametric_vjp_f64": (
         _I, [ctypes.POINTER(OperatorPlanI32), _P, _P, _P, _P, _P, _SZ, _P]),
+    "geo_b200_layer_norm": (_I, [ctypes.POINTER(LayerNormConfig), _P, _P, _P, _P, _P, _P, _P]),
+    "geo_b200_layer_norm_vjp_workspace": (_SZ, [ctypes.POINTER(LayerNormConfig)]),
+    "geo_b200_layer_norm_vjp": (
+        _I, [ctypes.POINTER(LayerNormConfig), _P, _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P]),
+    "geo_b200_dropout": (_I, [ctypes.POINTER(DropoutConfig), _P, _P, _P, _P, _P]),
+    "geo_b200_dropout_vjp": (_I, [ctypes.POINTER(DropoutConfig), _P, _P, _P, _P]),
+    "geo_b200_residual_dropout_layer_norm": (
+        _I, [ctypes.POINTER(LayerNormConfig), ctypes.POINTER(DropoutConfig), _P, _P, _P, _P, _P, _P, _P, _P, _P, _P]),
+    "geo_b200_residual_dropout_layer_norm_vjp": (
+        _I, [ctypes.POINTER(LayerNormConfig), ctypes.POINTER(DropoutConfig), _P, _P, _P, _P, _P, _P, _P, _P, _P, _P,
+             _P, _P, _SZ, _P]),
+    "geo_b200_rotary_plan_init": (_I, [ctypes.POINTER(RotaryPlan), ctypes.POINTER(RotaryConfig)]),
+    "geo_b200_rotary": (_I, [ctypes.POINTER(RotaryPlan), ctypes.POINTER(RotaryShape), _P, _P, _P, _P]),
+    "geo_b200_rotary_vjp": (_I, [ctypes.POINTER(RotaryPlan), ctypes.POINTER(RotaryShape), _P, _P, _P, _P]),
 }
 
 

@@ -21,6 +21,9 @@
  *     float64, plus a float32 build of the forward.
  *  4. Sparse fixed-multivector operators over a batch (reference
  *     src/operator_kernel.c:191-334, geo_operator_apply_*_f64 and VJPs).
+ *  5. Layer operators over rows of coefficients (no counterpart in the
+ *     reference): layer norm, dropout, the two fused with a residual, and
+ *     rotary positions, each with its VJP; float64, float32, bfloat16, float16.
  *
  * All device-pointer calls are asynchronous on the given stream; host-pointer
  * calls are synchronous. Arrays are sample-major [batch][2^n].
@@ -338,6 +341,209 @@ geo_b200_status_t geo_b200_sparse_apply_parametric_vjp_f64(const geo_operator_pl
                                                            double *device_in_cotangent,
                                                            double *device_parameter_cotangent, size_t batch,
                                                            cudaStream_t stream);
+
+/* ---- 5. layer operators over rows of coefficients ---------------------- */
+
+/* What a model of several layers does between its products, on arrays of
+ * `rows` rows of `cols` values in device memory (a row: the coefficients of
+ * one or several multivectors, or of any other layer). None of these has a
+ * counterpart in the reference. Common to all of section 5:
+ *   - asynchronous on `stream`, which belongs to the current device, as does
+ *     every array (device memory, managed memory, or pinned host memory);
+ *     other pointers are refused with GEO_B200_INVALID_ARGUMENT, as is an array
+ *     that is not aligned to its value type, before anything is launched. Only
+ *     argument and launch errors are reported. Nothing is allocated and nothing
+ *     is kept between calls; calls may be captured into a CUDA graph.
+ *   - strides are in values; 0 means packed rows, otherwise stride >= cols.
+ *     Values between the rows are neither read nor written.
+ *   - an output may be the same array (pointer and stride) as an input of the
+ *     call that it overwrites; arrays must not overlap otherwise.
+ *   - arithmetic and sums are float64 for GEO_B200_F64 and float32 otherwise,
+ *     rounded once (to nearest, ties to even) to the array's type. Sums are
+ *     taken in a fixed order: the same call gives the same bits.
+ *   - infinities and NaN reach every output that depends on them. */
+typedef enum {
+    GEO_B200_F64 = 1,
+    GEO_B200_F32 = 2,
+    GEO_B200_BF16 = 3,
+    GEO_B200_F16 = 4
+} geo_b200_type_t;
+
+#define GEO_B200_LAYER_MAX_COLS 16777216u  /* 2^24 values a row */
+#define GEO_B200_LAYER_MAX_ROWS 4294967296ull
+
+/* Layer norm over each row: with mean m and variance v (divided by cols),
+ *   rstd = 1 / sqrt(v + epsilon),  y = (x - m) rstd weight + bias. */
+typedef struct {
+    uint32_t type;              /* geo_b200_type_t of x, y and their cotangents */
+    uint32_t parameter_type;    /* of weight, bias and their cotangents: `type`, or F32 for the 16-bit types */
+    size_t rows, cols;          /* 1 .. GEO_B200_LAYER_MAX_ROWS, 1 .. GEO_B200_LAYER_MAX_COLS */
+    size_t x_stride, y_stride, y_cotangent_stride, x_cotangent_stride;
+    double epsilon;             /* finite, >= 0 */
+} geo_b200_layer_norm_config_t;
+
+/* weight, bias (cols values each) may be NULL: 1 and 0. mean and rstd (rows
+ * values each, float64 for GEO_B200_F64, else float32; what the VJP needs) may
+ * be NULL. The statistics of a row are taken about its own mean (no difference
+ * of large squares). */
+geo_b200_status_t geo_b200_layer_norm(const geo_b200_layer_norm_config_t *config, const void *device_x,
+                                      const void *device_weight, const void *device_bias, void *device_y,
+                                      void *device_mean, void *device_rstd, cudaStream_t stream);
+
+/* Bytes of device workspace of the VJP of `config` on the current device (the
+ * partial sums of the weight's and the bias's cotangent); 0 for a config that
+ * the VJP would refuse. */
+size_t geo_b200_layer_norm_vjp_workspace(const geo_b200_layer_norm_config_t *config);
+
+/* VJP: with xh = (x - mean) rstd, g = y_bar weight (means over the row),
+ *   x_bar = rstd (g - mean(g) - xh mean(g xh)),
+ *   weight_bar = sum over the rows of y_bar xh, bias_bar = sum of y_bar.
+ * Any of the three outputs may be NULL, not all; outputs are overwritten.
+ * workspace: geo_b200_layer_norm_vjp_workspace bytes, 16-byte aligned, not
+ * needed (may be NULL) when weight_bar and bias_bar are both NULL. Calls that
+ * may overlap on the GPU, captured graphs among them, need a workspace each. */
+geo_b200_status_t geo_b200_layer_norm_vjp(const geo_b200_layer_norm_config_t *config, const void *device_x,
+                                          const void *device_weight, const void *device_mean,
+                                          const void *device_rstd, const void *device_y_cotangent,
+                                          void *device_x_cotangent, void *device_weight_cotangent,
+                                          void *device_bias_cotangent, void *device_workspace,
+                                          size_t workspace_bytes, cudaStream_t stream);
+
+/* Dropout, y = [residual +] keep x / (1 - rate), whose mask is computed from a
+ * counter and never stored. What is kept or dropped as one is a unit of
+ * 2^dimension consecutive values of a row: a single value (dimension 0), or a
+ * whole multivector, which keeps a layer of multivectors equivariant (dropping
+ * coefficients one by one does not commute with a rotor).
+ * Unit u = (row cols + col) >> dimension (strides do not enter) draws 16 bits:
+ * half u & 1 (0: the low one) of word (u & 7) / 2 of the block
+ *   Philox4x32-10(counter = {lo, hi of u >> 3, lo, hi of the offset}, key = {lo, hi of the seed})
+ * (Salmon, Moraes, Dror, Shaw: Parallel random numbers: as easy as 1, 2, 3; SC
+ * 2011), and is kept when they are >= T = rate in steps of 2^-16, rounded to
+ * the nearest (ties to even); x is scaled by 65536 / (65536 - T), so the mean
+ * over masks is x at the rounded rate, and T = 65536 drops everything.
+ * A dropped unit gives 0 (or the residual) whatever its x holds, NaN included. */
+typedef struct {
+    uint32_t type;              /* geo_b200_type_t of all arrays */
+    uint32_t dimension;         /* 0 .. 6; cols is a multiple of 2^dimension */
+    size_t rows, cols;
+    size_t x_stride, residual_stride, y_stride, y_cotangent_stride, x_cotangent_stride;
+    double rate;                /* 0 .. 1 */
+    uint64_t seed;
+    uint64_t offset;            /* another mask for each call of a training run */
+} geo_b200_dropout_config_t;
+
+/* residual may be NULL. device_offset may be NULL; else the value it points to
+ * when the kernel runs is added to config->offset (modulo 2^64), so that a
+ * captured graph draws another mask at each replay. */
+geo_b200_status_t geo_b200_dropout(const geo_b200_dropout_config_t *config, const void *device_x,
+                                   const void *device_residual, const uint64_t *device_offset, void *device_y,
+                                   cudaStream_t stream);
+/* x_bar = keep y_bar / (1 - rate), of the forward's seed and offset (the
+ * residual's cotangent is y_bar itself). */
+geo_b200_status_t geo_b200_dropout_vjp(const geo_b200_dropout_config_t *config, const uint64_t *device_offset,
+                                       const void *device_y_cotangent, void *device_x_cotangent,
+                                       cudaStream_t stream);
+
+/* Both in one pass over a residual stream: z = residual + dropout(x) and
+ * y = layer_norm(z). z is dropout's y (dropout->y_stride) and layer norm's x
+ * (norm->x_stride, the same value); type, rows and cols agree. The statistics
+ * and y are taken from z before it is rounded to its type. */
+geo_b200_status_t geo_b200_residual_dropout_layer_norm(
+    const geo_b200_layer_norm_config_t *norm, const geo_b200_dropout_config_t *dropout, const void *device_x,
+    const void *device_residual, const uint64_t *device_offset, const void *device_weight, const void *device_bias,
+    void *device_z, void *device_y, void *device_mean, void *device_rstd, cudaStream_t stream);
+/* VJP from y_bar (norm->y_cotangent_stride) and, where z is used further on,
+ * its own cotangent z_bar (dropout->y_cotangent_stride; may be NULL):
+ *   residual_bar = layer_norm_vjp(y_bar) + z_bar  (norm->x_cotangent_stride),
+ *   x_bar = keep residual_bar / (1 - rate)        (dropout->x_cotangent_stride).
+ * Any output may be NULL, not all. Workspace as geo_b200_layer_norm_vjp, from
+ * geo_b200_layer_norm_vjp_workspace(norm). */
+geo_b200_status_t geo_b200_residual_dropout_layer_norm_vjp(
+    const geo_b200_layer_norm_config_t *norm, const geo_b200_dropout_config_t *dropout,
+    const uint64_t *device_offset, const void *device_z, const void *device_weight, const void *device_mean,
+    const void *device_rstd, const void *device_y_cotangent, const void *device_z_cotangent,
+    void *device_residual_cotangent, void *device_x_cotangent, void *device_weight_cotangent,
+    void *device_bias_cotangent, void *device_workspace, size_t workspace_bytes, cudaStream_t stream);
+
+/* Rotary positions: the vector of a token's head is turned, pair of
+ * coordinates by pair, by the rotor of its position,
+ *   (a, b) -> amplitude (a cos t - b sin t, a sin t + b cos t), t = position f_i,
+ * which makes the product of two turned vectors a function of the difference
+ * of their positions. Pairs i < rotary_dim / 2 are coordinates (2i, 2i + 1)
+ * (INTERLEAVED) or (i, i + rotary_dim / 2) (HALF); coordinates from rotary_dim
+ * on are copied. f_i = base^(-2i / rotary_dim) radians per position, and for
+ * contexts longer than a model was trained on:
+ *   LINEAR: f_i / factor;
+ *   BASE:   base replaced by base factor^(d / (d - 2)), d = rotary_dim > 2
+ *           (d = 2 has the single frequency 1 and is left alone);
+ *   BANDED: f_i k_i + f_i / factor (1 - k_i), k_i = (r_i - low) / (high - low)
+ *           clamped to [0, 1], r_i = original_length f_i / (2 pi) the turns
+ *           that pair i makes over the original context. */
+typedef enum { GEO_B200_ROTARY_INTERLEAVED = 0, GEO_B200_ROTARY_HALF = 1 } geo_b200_rotary_layout_t;
+typedef enum {
+    GEO_B200_ROTARY_SCALING_NONE = 0,
+    GEO_B200_ROTARY_SCALING_LINEAR = 1,
+    GEO_B200_ROTARY_SCALING_BASE = 2,
+    GEO_B200_ROTARY_SCALING_BANDED = 3
+} geo_b200_rotary_scaling_t;
+typedef enum { GEO_B200_I32 = 1, GEO_B200_I64 = 2 } geo_b200_position_type_t;
+
+#define GEO_B200_ROTARY_MAX_DIM 256u
+
+typedef struct {
+    uint32_t layout;            /* geo_b200_rotary_layout_t */
+    uint32_t rotary_dim;        /* even, 2 .. GEO_B200_ROTARY_MAX_DIM */
+    double base;                /* finite, > 0 */
+    uint32_t scaling;           /* geo_b200_rotary_scaling_t */
+    double factor;              /* finite, > 0; unless NONE */
+    double original_length;     /* BANDED: finite, > 0 */
+    double low_rotations;       /* BANDED: finite, < high_rotations */
+    double high_rotations;
+    double amplitude;           /* finite */
+} geo_b200_rotary_config_t;
+
+/* Filled by geo_b200_rotary_plan_init (host code, no GPU), owned by the caller:
+ * turns per position of each pair, as the sum of two float64, so that the
+ * angle of a far position keeps its accuracy (an error of at most
+ * 2^-63 |position| turns times the pair's own turns per position, next to
+ * float64 rounding). */
+typedef struct {
+    uint32_t abi_version;       /* GEO_B200_ABI_VERSION */
+    uint32_t layout;
+    uint32_t rotary_dim;
+    uint32_t reserved;
+    double amplitude;
+    double turns[GEO_B200_ROTARY_MAX_DIM / 2];
+    double turns_low[GEO_B200_ROTARY_MAX_DIM / 2];
+} geo_b200_rotary_plan_t;
+
+geo_b200_status_t geo_b200_rotary_plan_init(geo_b200_rotary_plan_t *plan, const geo_b200_rotary_config_t *config);
+
+/* Arrays [batch][tokens][heads][head_dim] with any strides between batches,
+ * tokens and heads (0: packed, in that order); the head_dim values of a head
+ * are adjacent, and heads must not overlap. Queries and keys that lie side by
+ * side in one projection are one call. */
+typedef struct {
+    uint32_t type;              /* geo_b200_type_t of x and y */
+    uint32_t position_type;     /* geo_b200_position_type_t */
+    size_t batch, tokens, heads, head_dim;  /* >= 1; rotary_dim <= head_dim <= 65536 */
+    size_t x_batch_stride, x_token_stride, x_head_stride;
+    size_t y_batch_stride, y_token_stride, y_head_stride;
+    size_t position_batch_stride;  /* 0: every sequence has the same positions */
+    int64_t first_position;     /* position of token t is first_position + t when no positions are given */
+} geo_b200_rotary_shape_t;
+
+/* device_positions (may be NULL) holds the position of token t of sequence b
+ * at [b position_batch_stride + t]; positions may be negative, in any order and
+ * repeated, |position| <= 2^31. */
+geo_b200_status_t geo_b200_rotary(const geo_b200_rotary_plan_t *plan, const geo_b200_rotary_shape_t *shape,
+                                  const void *device_x, const void *device_positions, void *device_y,
+                                  cudaStream_t stream);
+/* x_bar from y_bar: the reversed rotor. The shape's x strides describe
+ * device_y_cotangent, its y strides device_x_cotangent. */
+geo_b200_status_t geo_b200_rotary_vjp(const geo_b200_rotary_plan_t *plan, const geo_b200_rotary_shape_t *shape,
+                                      const void *device_y_cotangent, const void *device_positions,
+                                      void *device_x_cotangent, cudaStream_t stream);
 
 #ifdef __cplusplus
 }
