@@ -9,32 +9,160 @@ using namespace geo::layers;
 
 constexpr int kThreads = 256;
 
-// One value per thread.
+struct Rows {
+    const void *x, *residual;
+    void *y;
+    size_t x_stride, residual_stride, y_stride;
+    size_t rows, cols;  // packed arrays: one row of all values
+};
+
 template <typename T>
-__global__ void __launch_bounds__(kThreads)
-    drop_kernel(const T *x, size_t x_stride, const T *residual, size_t residual_stride, T *y, size_t y_stride,
-                size_t rows, uint32_t cols, const Drop drop) {
+__device__ __forceinline__ Wide<T> drop_value(bool kept, T x, Wide<T> scale, Wide<T> residual) {
+    using W = Wide<T>;
+    const W v = kept ? (W)widen(x) : W(0);  // selected, not multiplied: a dropped NaN is gone
+    if constexpr (std::is_same_v<W, double>)
+        return ::fma(v, scale, residual);
+    else
+        return fmaf(v, scale, residual);
+}
+
+// Vectors of 16 bytes. A warp takes 256 values at a time, kChunks times: lane l
+// works out the block of values 8 l .. 8 l + 7, once for every eight values at
+// every type, and the eight decisions go to the lanes that hold the values.
+constexpr int kChunks = 4;
+template <typename T, bool PACKED, bool RESIDUAL>
+__global__ void __launch_bounds__(kThreads) drop_vectors_kernel(const Rows a, const Drop drop) {
+    using W = Wide<T>;
+    constexpr int V = 16 / sizeof(T), R = 8 / V;
+    const uint64_t offset = drop_offset(drop);
+    const W scale = (W)drop.scale;
+    const uint32_t lane = threadIdx.x & 31;
+    const size_t count = a.rows * a.cols;
+    const size_t warp = (blockIdx.x * (size_t)kThreads + threadIdx.x) / 32;
+    Vec<T, V> x[kChunks][R], res[RESIDUAL ? kChunks : 1][R];
+    size_t y_at[PACKED ? 1 : kChunks][R];
+    auto value = [&](int m, int i) { return (warp * kChunks + m) * 256 + (i * 32 + lane) * V; };
+#pragma unroll
+    for (int m = 0; m < kChunks; ++m)
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const size_t e = value(m, i);
+            x[m][i] = Vec<T, V>{};
+            if constexpr (RESIDUAL) res[m][i] = Vec<T, V>{};
+            if (e >= count) continue;
+            if constexpr (PACKED) {
+                if (e + V <= count) {
+                    x[m][i] = load<T, V>((const T *)a.x + e);
+                    if constexpr (RESIDUAL) res[m][i] = load<T, V>((const T *)a.residual + e);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < V; ++j)
+                        if (e + j < count) {
+                            x[m][i].v[j] = ((const T *)a.x)[e + j];
+                            if constexpr (RESIDUAL) res[m][i].v[j] = ((const T *)a.residual)[e + j];
+                        }
+                }
+            } else {
+                const size_t row = count <= 0xFFFFFFFFu ? (uint32_t)e / (uint32_t)a.cols : e / a.cols;
+                const size_t c = e - row * a.cols;
+                y_at[m][i] = row * a.y_stride + c;
+                x[m][i] = load<T, V>((const T *)a.x + row * a.x_stride + c);
+                if constexpr (RESIDUAL) res[m][i] = load<T, V>((const T *)a.residual + row * a.residual_stride + c);
+            }
+        }
+#pragma unroll
+    for (int m = 0; m < kChunks; ++m) {
+        const uint32_t mine = kept_of_eight(drop, offset, (warp * kChunks + m) * 256 + lane * 8);
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const size_t e = value(m, i);
+            uint32_t kept = mine;
+            if constexpr (R > 1) kept = __shfl_sync(0xffffffffu, mine, (i * 32 + lane) / R) >> (lane % R * V);
+            Vec<T, V> out;
+#pragma unroll
+            for (int j = 0; j < V; j += 2) {
+                Pair<W> v = widen_pair(x[m][i].v[j], x[m][i].v[j + 1]);
+                v.x = (kept >> j) & 1 ? v.x : W(0);  // selected, not multiplied: a dropped NaN is gone
+                v.y = (kept >> (j + 1)) & 1 ? v.y : W(0);
+                if constexpr (RESIDUAL)
+                    v = fma(v, both(scale), widen_pair(res[m][i].v[j], res[m][i].v[j + 1]));
+                else
+                    v = v * both(scale);
+                narrow_pair<T>(v, out.v[j], out.v[j + 1]);
+            }
+            if (e >= count) continue;
+            if constexpr (PACKED) {
+                if (e + V <= count) {
+                    store<T, V>((T *)a.y + e, out);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < V; ++j)
+                        if (e + j < count) ((T *)a.y)[e + j] = out.v[j];
+                }
+            } else {
+                store<T, V>((T *)a.y + y_at[m][i], out);
+            }
+        }
+    }
+}
+
+// Rows that do not start on 16 bytes, or are not made of whole eights: a warp
+// takes 256 values of one row, lane by lane.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) drop_values_kernel(const Rows a, const Drop drop) {
     using W = Wide<T>;
     const uint64_t offset = drop_offset(drop);
     const W scale = (W)drop.scale;
-    const size_t count = rows * cols;
-    for (size_t i = blockIdx.x * (size_t)kThreads + threadIdx.x; i < count; i += (size_t)gridDim.x * kThreads) {
-        const size_t row = i / cols, c = i - row * cols;
-        W v = drop.threshold == 0 || unit_kept(drop, offset, i >> drop.shift) ? widen(x[row * x_stride + c]) * scale
-                                                                              : W(0);
-        if (residual != nullptr) v += widen(residual[row * residual_stride + c]);
-        y[row * y_stride + c] = narrow<T>(v);
+    const uint32_t lane = threadIdx.x & 31;
+    const size_t pieces = (a.cols + 255) / 256, count = a.rows * pieces;
+    const size_t step = (size_t)gridDim.x * (kThreads / 32);
+    for (size_t piece = (blockIdx.x * (size_t)kThreads + threadIdx.x) / 32; piece < count; piece += step) {
+        const size_t row = piece / pieces, first = (piece - row * pieces) * 256;
+        const T *x = (const T *)a.x + row * a.x_stride;
+        const T *residual = a.residual != nullptr ? (const T *)a.residual + row * a.residual_stride : nullptr;
+        T v[8], r[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const size_t c = first + i * 32 + lane;
+            v[i] = c < a.cols ? x[c] : T{};
+            r[i] = residual != nullptr && c < a.cols ? residual[c] : T{};
+        }
+        const uint32_t kept = kept_by_warp<8>(drop, offset, row * a.cols + first, 32);
+        T *y = (T *)a.y + row * a.y_stride;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const size_t c = first + i * 32 + lane;
+            if (c < a.cols) y[c] = narrow<T>(drop_value<T>((kept >> i) & 1, v[i], scale, widen(r[i])));
+        }
     }
 }
 
 cudaError_t launch(uint32_t type, const void *x, size_t x_stride, const void *residual, size_t residual_stride,
                    void *y, size_t y_stride, size_t rows, size_t cols, const Drop &drop, cudaStream_t stream) {
+    Rows a = {x, residual, y, x_stride, residual_stride, y_stride, rows, cols};
+    const bool packed = x_stride == cols && y_stride == cols && (residual == nullptr || residual_stride == cols);
+    if (packed) a.cols = rows * cols, a.rows = 1;
+    const size_t b = type_bytes(type), low = (uintptr_t)x | (uintptr_t)y | (uintptr_t)residual;
+    const size_t strides = x_stride | y_stride | (residual != nullptr ? residual_stride : 0);
+    const bool vectors = low % 16 == 0 && (packed || (cols % 8 == 0 && strides * b % 16 == 0));
     return by_type(type, [&](auto t) {
         using T = decltype(t);
-        const size_t blocks = (rows * cols + kThreads - 1) / kThreads, most = (size_t)geo::device_sm_count() * 32;
-        drop_kernel<T><<<(unsigned)(blocks < most ? blocks : most), kThreads, 0, stream>>>(
-            (const T *)x, x_stride, (const T *)residual, residual_stride, (T *)y, y_stride, rows, (uint32_t)cols,
-            drop);
+        if (vectors) {
+            const size_t each = (size_t)kThreads * 8 * kChunks;
+            const size_t grid = (rows * cols + each - 1) / each;
+            if (grid > 0x7fffffff) return cudaErrorInvalidValue;
+            if (packed && residual != nullptr)
+                drop_vectors_kernel<T, true, true><<<(unsigned)grid, kThreads, 0, stream>>>(a, drop);
+            else if (packed)
+                drop_vectors_kernel<T, true, false><<<(unsigned)grid, kThreads, 0, stream>>>(a, drop);
+            else if (residual != nullptr)
+                drop_vectors_kernel<T, false, true><<<(unsigned)grid, kThreads, 0, stream>>>(a, drop);
+            else
+                drop_vectors_kernel<T, false, false><<<(unsigned)grid, kThreads, 0, stream>>>(a, drop);
+        } else {
+            const size_t pieces = a.rows * ((a.cols + 255) / 256), blocks = (pieces + kThreads / 32 - 1) / (kThreads / 32);
+            drop_values_kernel<T><<<(unsigned)(blocks < 0x7fffffff ? blocks : 0x7fffffff), kThreads, 0, stream>>>(a, drop);
+        }
         return cudaGetLastError();
     });
 }

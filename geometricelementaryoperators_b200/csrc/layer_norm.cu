@@ -6,6 +6,8 @@
 //   x_bar = rstd (g - mean(g) - xh mean(g xh)),
 //   w_bar = sum_rows y_bar xh, b_bar = sum_rows y_bar.
 // Every variant does a few multiply-adds per value, so HBM bounds it.
+#include <cooperative_groups.h>
+
 #include <cmath>
 
 #include "geo_runtime.h"
@@ -46,6 +48,477 @@ struct BackwardArgs {
     int cols;
     Drop drop;
 };
+
+// ---- rows held on chip ---------------------------------------------------------
+
+// A team of lanes holds one row, thread `lane` the vectors lane, lane + lanes, ...
+// (K of them, V values each; pair q of the thread's values is 2q, 2q + 1 in that
+// order): part of a warp (lanes a power of two up to 32, several rows a warp), a
+// whole block, or (backward) the blocks of a cluster.
+
+template <typename W>
+__device__ __forceinline__ W team_sum(W v, int lanes) {
+    for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+// Weight or bias at V columns, of the value type or (16-bit values only) float32.
+template <typename T, int V>
+__device__ __forceinline__ void load_parameter(const void *p, bool is_float, int c, Wide<T> *out) {
+    if constexpr (sizeof(T) == 2) {
+        if (is_float) {
+            constexpr int U = V < 4 ? V : 4;
+#pragma unroll
+            for (int j = 0; j < V; j += U) {
+                const Vec<float, U> w = load<float, U>((const float *)p + c + j);
+#pragma unroll
+                for (int i = 0; i < U; ++i) out[j + i] = w.v[i];
+            }
+            return;
+        }
+    }
+    const Vec<T, V> w = load<T, V>((const T *)p + c);
+#pragma unroll
+    for (int j = 0; j < V; ++j) out[j] = widen(w.v[j]);
+}
+
+// The thread's parameters as pairs in the order of its values; `absent` past the row.
+template <typename T, int V, int K>
+__device__ __forceinline__ void load_parameters(const void *p, bool is_float, int lane, int threads, int cols,
+                                                Wide<T> absent, Pair<Wide<T>> (&out)[K * V / 2]) {
+    Wide<T> flat[K * V];
+#pragma unroll
+    for (int i = 0; i < K; ++i) {
+        const int c = (lane + i * threads) * V;
+#pragma unroll
+        for (int j = 0; j < V; ++j) flat[i * V + j] = absent;
+        if (p != nullptr && c < cols) load_parameter<T, V>(p, is_float, c, flat + i * V);
+    }
+#pragma unroll
+    for (int q = 0; q < K * V / 2; ++q) out[q] = {flat[2 * q], flat[2 * q + 1]};
+}
+
+template <typename T, int V, int K>
+__device__ __forceinline__ Pair<Wide<T>> pair_at(const Vec<T, V> (&raw)[K], int q) {
+    return widen_pair(raw[2 * q / V].v[2 * q % V], raw[(2 * q + 1) / V].v[(2 * q + 1) % V]);
+}
+
+template <typename T, int V, int K>
+__device__ __forceinline__ void set_pair(Vec<T, V> (&raw)[K], int q, Pair<Wide<T>> v) {
+    narrow_pair<T>(v, raw[2 * q / V].v[2 * q % V], raw[(2 * q + 1) / V].v[(2 * q + 1) % V]);
+}
+
+// Which of the thread's values dropout keeps, bit i V + j.
+template <int V, int K>
+__device__ __forceinline__ uint32_t kept_of_row(const Drop &drop, uint64_t offset, uint64_t row_start, int lane,
+                                                int threads, int cols) {
+    if constexpr (V == 1) {
+        return kept_by_warp<K>(drop, offset, row_start + (lane & ~31), threads);
+    } else {
+        uint32_t bits = 0;
+#pragma unroll
+        for (int i = 0; i < K; ++i) {
+            const int c = (lane + i * threads) * V;
+            if (c >= cols) continue;
+            bits |= (kept_values<V>(drop, offset, row_start + c) & ((1u << V) - 1u)) << (i * V);
+        }
+        return bits;
+    }
+}
+
+template <typename T, int V, int K, bool DROP, bool BLOCK, int THREADS>
+__global__ void __launch_bounds__(THREADS, THREADS == 1024 ? 1 : 768 / THREADS) norm_kernel(const ForwardArgs a, int lanes, bool float_parameters) {
+    using W = Wide<T>;
+    constexpr int Q = K * V / 2;
+    __shared__ W sums[2][BLOCK ? 32 : 1][2];
+    const int threads = BLOCK ? (int)blockDim.x : lanes;
+    const int lane = BLOCK ? (int)threadIdx.x : (int)threadIdx.x & (lanes - 1);
+    const int warp = (int)threadIdx.x >> 5, wlane = (int)threadIdx.x & 31;
+    const int teams = BLOCK ? 1 : 128 / lanes;
+    const size_t step = (size_t)gridDim.x * teams;
+    const uint64_t offset = DROP ? drop_offset(a.drop) : 0;
+    const W scale = (W)a.drop.scale, over = W(1) / (W)a.cols;
+    // BLOCK: how many values of the row warp w holds.
+    auto held_by = [&](int w) {
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < K; ++i) {
+            const int left = a.cols / V - (w * 32 + i * threads);
+            n += left < 0 ? 0 : (left < 32 ? left : 32);
+        }
+        return (W)(n * V);
+    };
+    const W held = BLOCK ? held_by(warp) : (W)a.cols;
+    const W over_held = held > W(0) ? W(1) / held : W(0);
+    // BLOCK: thread `wlane` of every warp joins what warp `wlane` held.
+    const W joined = BLOCK && wlane < threads / 32 ? held_by(wlane) : W(0);
+    const W over_joined = joined > W(0) ? W(1) / joined : W(0);
+    int flip = 0;
+    // The bound is the warp's first row, so that all its lanes stay for the shuffles.
+    for (size_t first = (size_t)blockIdx.x * teams + (BLOCK ? 0 : warp * (32 / lanes)); first < a.rows;
+         first += step, flip ^= 1) {
+        const size_t row = BLOCK ? first : first + wlane / lanes;
+        const bool live = BLOCK || row < a.rows;
+        Pair<W> v[Q];
+        {
+            Vec<T, V> raw[K], res[DROP ? K : 1];
+            const T *x = (const T *)a.x + row * a.x_stride;
+            const T *r = DROP ? (const T *)a.residual + row * a.residual_stride : nullptr;
+#pragma unroll
+            for (int i = 0; i < K; ++i) {
+                const int c = (lane + i * threads) * V;
+                raw[i] = Vec<T, V>{};
+                if constexpr (DROP) res[i] = Vec<T, V>{};
+                if (live && c < a.cols) {
+                    raw[i] = load<T, V>(x + c);
+                    if constexpr (DROP) res[i] = load<T, V>(r + c);
+                }
+            }
+            if constexpr (DROP) {
+                const uint32_t kept = kept_of_row<V, K>(a.drop, offset, row * (size_t)a.cols, lane, threads, a.cols);
+#pragma unroll
+                for (int q = 0; q < Q; ++q) {
+                    Pair<W> p = pair_at(raw, q);
+                    p.x = (kept >> (2 * q)) & 1 ? p.x : W(0);
+                    p.y = (kept >> (2 * q + 1)) & 1 ? p.y : W(0);
+                    v[q] = fma(p, both(scale), pair_at(res, q));
+                }
+            } else {
+#pragma unroll
+                for (int q = 0; q < Q; ++q) v[q] = pair_at(raw, q);
+            }
+        }
+        // Two sweeps over registers: the mean of what the warp (or its team)
+        // holds, then the squares about it. Values past the row are 0 in the
+        // first, the mean itself in the second.
+        Pair<W> two = both(W(0));
+#pragma unroll
+        for (int q = 0; q < Q; ++q) two = two + v[q];
+        W sum = team_sum(two.x + two.y, BLOCK ? 32 : lanes);
+        W mean = BLOCK ? sum * over_held : sum / held;
+#pragma unroll
+        for (int i = 0; i < K; ++i)
+            if ((lane + i * threads) * V >= a.cols) {
+                if constexpr (V == 1) {
+                    (i & 1 ? v[i / 2].y : v[i / 2].x) = mean;
+                } else {
+#pragma unroll
+                    for (int q = i * V / 2; q < (i + 1) * V / 2; ++q) v[q] = both(mean);
+                }
+            }
+        two = both(W(0));
+#pragma unroll
+        for (int q = 0; q < Q; ++q) {
+            const Pair<W> d = v[q] + both(-mean);
+            two = fma(d, d, two);
+        }
+        W squares = team_sum(two.x + two.y, BLOCK ? 32 : lanes);
+        if constexpr (BLOCK) {
+            // Warps joined about the row's mean: squares + held (warp's mean - mean)^2. Two buffers, one barrier a row.
+            if (wlane == 0) {
+                sums[flip][warp][0] = sum;
+                sums[flip][warp][1] = squares;
+            }
+            __syncthreads();
+            const W other = wlane < threads / 32 ? sums[flip][wlane][0] : W(0);
+            mean = team_sum(other, 32) / (W)a.cols;  // divided, so that a row of one value has no spread
+            const W d = other * over_joined - mean;
+            squares = team_sum(wlane < threads / 32 ? sums[flip][wlane][1] + joined * d * d : W(0), 32);
+        }
+        const W rstd = rsqrt(squares * over + (W)a.epsilon);
+        if (live && lane == 0) {
+            if (a.mean != nullptr) ((W *)a.mean)[row] = mean;
+            if (a.rstd != nullptr) ((W *)a.rstd)[row] = rstd;
+        }
+        // A vector (or two single values) at a time, so that few parameters are held.
+        constexpr int G = V > 1 ? V : 2;
+#pragma unroll
+        for (int m = 0; m < K * V / G; ++m) {
+            Vec<T, V> z[G / V], y[G / V];
+            W w[G], b[G];
+#pragma unroll
+            for (int i = 0; i < G / V; ++i) {
+                const int c = (lane + (m * G / V + i) * threads) * V;
+#pragma unroll
+                for (int j = 0; j < V; ++j) w[i * V + j] = W(1), b[i * V + j] = W(0);
+                if (c < a.cols) {
+                    if (a.weight != nullptr) load_parameter<T, V>(a.weight, float_parameters, c, w + i * V);
+                    if (a.bias != nullptr) load_parameter<T, V>(a.bias, float_parameters, c, b + i * V);
+                }
+            }
+#pragma unroll
+            for (int q = 0; q < G / 2; ++q) {
+                const Pair<W> p = v[m * G / 2 + q];
+                if constexpr (DROP) set_pair(z, q, p);
+                const Pair<W> hat = (p + both(-mean)) * both(rstd);
+                set_pair(y, q, fma(hat, Pair<W>{w[2 * q], w[2 * q + 1]}, Pair<W>{b[2 * q], b[2 * q + 1]}));
+            }
+#pragma unroll
+            for (int i = 0; i < G / V; ++i) {
+                const int c = (lane + (m * G / V + i) * threads) * V;
+                if (!live || c >= a.cols) continue;
+                if constexpr (DROP) store<T, V>((T *)a.z + row * a.z_stride + c, z[i]);
+                store<T, V>((T *)a.y + row * a.y_stride + c, y[i]);
+            }
+        }
+    }
+}
+
+// ---- backward ------------------------------------------------------------------
+
+__device__ __forceinline__ uint32_t shared_address(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+template <int BYTES>
+__device__ __forceinline__ void copy_async(uint32_t to, const void *from, bool live) {
+    if constexpr (BYTES == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(live ? 16 : 0) : "memory");
+    else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(to), "l"(from), "n"(BYTES),
+                     "r"(live ? BYTES : 0)
+                     : "memory");
+}
+__device__ __forceinline__ void commit_async() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT>
+__device__ __forceinline__ void wait_async() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
+}
+
+// Bytes of shared memory behind one vector of one thread: 16, or a whole copy
+// of 4 or 8 bytes for single values.
+template <typename T, int V>
+constexpr int kSlot = V > 1 ? 16 : (sizeof(T) == 8 ? 8 : 4);
+
+// Copies a vector into its slot (zeros when not `live`). A single 16-bit value
+// travels as the aligned 4-byte word around it, whose other half is not used;
+// where that word would reach over an end of the array (`edge`: the array's
+// first or last value), the value alone is loaded and stored.
+template <typename T, int V>
+__device__ __forceinline__ void fetch(uint32_t slot, const T *from, bool live, bool edge) {
+    if constexpr (kSlot<T, V> > sizeof(T) * V) {
+        if (edge) {
+            const uint16_t v = *reinterpret_cast<const uint16_t *>(from);
+            asm volatile("st.shared.u16 [%0], %1;" ::"r"(slot + (uint32_t)((uintptr_t)from & 2)), "h"(v) : "memory");
+        } else {
+            copy_async<4>(slot, (const void *)((uintptr_t)from & ~(uintptr_t)3), live);
+        }
+    } else {
+        copy_async<kSlot<T, V>>(slot, from, live);
+    }
+}
+
+// One pass over x and y_bar (and z_bar): x_bar row by row, and the column sums
+// of y_bar xh and y_bar in the registers of the thread that owns the column; at
+// the end partial[cluster][0: weight, 1: bias][col]. Rows come through a ring of
+// `stages` in shared memory, each thread copying and waiting for its own vectors
+// only, stages - 1 rows ahead. CLUSTER: the row is cut into the cluster's blocks,
+// which hand each other their warps' sums through distributed shared memory.
+template <typename T, int V, int K, bool DROP, bool BLOCK, bool CLUSTER, int STAGES>
+__global__ void __launch_bounds__(BLOCK ? 256 : 128, BLOCK ? 2 : 4)
+    vjp_kernel(const BackwardArgs a, int lanes, bool float_parameters, Wide<T> *partial) {
+    using W = Wide<T>;
+    constexpr int Q = K * V / 2;
+    constexpr int kColumns = BLOCK ? 1 : (V == 1 ? 32 * K : 32 * K * V);
+    constexpr int S = kSlot<T, V>;
+    extern __shared__ __align__(16) unsigned char ring[];
+    __shared__ W sums[2][CLUSTER ? 64 : 8][2];
+    __shared__ W columns[2][kColumns];
+    namespace cg = cooperative_groups;
+    const int rank = CLUSTER ? (int)cg::this_cluster().block_rank() : 0;
+    const int ranks = CLUSTER ? (int)cg::this_cluster().num_blocks() : 1;
+    const int threads = BLOCK ? (int)blockDim.x * ranks : lanes;
+    const int lane = BLOCK ? (int)threadIdx.x + rank * (int)blockDim.x : (int)threadIdx.x & (lanes - 1);
+    const int warp = (int)threadIdx.x >> 5, wlane = (int)threadIdx.x & 31;
+    const int teams = BLOCK ? 1 : 128 / lanes;
+    const int warps = BLOCK ? (int)blockDim.x / 32 : 1;
+    const size_t cluster = blockIdx.x / ranks;
+    const size_t step = (size_t)(gridDim.x / ranks) * teams;
+    const uint64_t offset = DROP ? drop_offset(a.drop) : 0;
+    const W scale = (W)a.drop.scale, over = W(1) / (W)a.cols;
+    const bool has_dz = DROP && a.dz != nullptr;
+    const int arrays = has_dz ? 3 : 2;
+
+    Pair<W> weight[Q], dw[Q], db[Q];
+    load_parameters<T, V, K>(a.weight, float_parameters, lane, threads, a.cols, W(1), weight);
+#pragma unroll
+    for (int q = 0; q < Q; ++q) dw[q] = db[q] = both(W(0));
+
+    const uint32_t slots = shared_address(ring) + threadIdx.x * S;
+    const uint32_t next_vector = blockDim.x * S, next_array = K * next_vector, next_stage = arrays * next_array;
+    auto enqueue = [&](size_t row, uint32_t stage) {
+        const bool live = row < a.rows;
+#pragma unroll
+        for (int i = 0; i < K; ++i) {
+            const int c = (lane + i * threads) * V;
+            const bool inside = live && c < a.cols;
+            const bool edge = inside && ((row == 0 && c == 0) || (row == a.rows - 1 && c == a.cols - 1));
+            const size_t r = inside ? row : 0, at = inside ? c : 0;
+            const uint32_t slot = slots + stage * next_stage + i * next_vector;
+            fetch<T, V>(slot, (const T *)a.x + r * a.x_stride + at, inside, edge);
+            fetch<T, V>(slot + next_array, (const T *)a.dy + r * a.dy_stride + at, inside, edge);
+            if constexpr (DROP)
+                if (has_dz) fetch<T, V>(slot + 2 * next_array, (const T *)a.dz + r * a.dz_stride + at, inside, edge);
+        }
+        commit_async();
+    };
+    auto vectors = [&](Vec<T, V> (&out)[K], uint32_t stage, int array, const T *row_start) {
+        const unsigned char *from = ring + threadIdx.x * S + stage * next_stage + array * next_array;
+        // Where in its word a single 16-bit value is: the same for all of a thread's, which are 32 n apart.
+        if constexpr (S > sizeof(T) * V) from += (uintptr_t)(row_start + lane) & 2;
+#pragma unroll
+        for (int i = 0; i < K; ++i) out[i] = *reinterpret_cast<const Vec<T, V> *>(from + i * next_vector);
+    };
+
+    const size_t begin = cluster * teams + (BLOCK ? 0 : warp * (32 / lanes));
+    const size_t within = BLOCK ? 0 : wlane / lanes;
+#pragma unroll
+    for (int s = 0; s < STAGES - 1; ++s) enqueue(begin + within + s * step, s);
+    W next_mean = 0, next_rstd = 0;
+    if (begin + within < a.rows) {
+        next_mean = ((const W *)a.mean)[begin + within];
+        next_rstd = ((const W *)a.rstd)[begin + within];
+    }
+    if constexpr (CLUSTER) cg::this_cluster().sync();  // every block runs before its memory is written
+    int flip = 0;
+    uint32_t stage = 0;
+    for (size_t first = begin; first < a.rows; first += step, flip ^= 1) {
+        const size_t row = first + within;
+        const bool live = row < a.rows;
+        const W mean = next_mean, rstd = next_rstd;
+        next_mean = next_rstd = 0;
+        if (row + step < a.rows) {
+            next_mean = ((const W *)a.mean)[row + step];
+            next_rstd = ((const W *)a.rstd)[row + step];
+        }
+        // Into the slot that this thread read in the last round.
+        enqueue(row + (STAGES - 1) * step, stage == 0 ? STAGES - 1 : stage - 1);
+        wait_async<STAGES - 1>();
+        const T *x_row = (const T *)a.x + (live ? row : 0) * a.x_stride;
+        const T *dy_row = (const T *)a.dy + (live ? row : 0) * a.dy_stride;
+        const T *dz_row = has_dz ? (const T *)a.dz + (live ? row : 0) * a.dz_stride : nullptr;
+        Vec<T, V> x[K], dy[K];
+        vectors(x, stage, 0, x_row);
+        vectors(dy, stage, 1, dy_row);
+        Pair<W> sum2 = both(W(0)), along2 = both(W(0));
+#pragma unroll
+        for (int q = 0; q < Q; ++q) {
+            const Pair<W> d = pair_at(dy, q), xh = (pair_at(x, q) + both(-mean)) * both(rstd), g = d * weight[q];
+            sum2 = sum2 + g;
+            along2 = fma(g, xh, along2);
+            dw[q] = fma(d, xh, dw[q]);
+            db[q] = db[q] + d;
+        }
+        W sum = team_sum(sum2.x + sum2.y, BLOCK ? 32 : lanes);
+        W along = team_sum(along2.x + along2.y, BLOCK ? 32 : lanes);
+        if constexpr (BLOCK) {
+            if constexpr (CLUSTER) {
+                if (wlane < ranks) {
+                    W *there = cg::this_cluster().map_shared_rank(&sums[flip][rank * warps + warp][0], wlane);
+                    there[0] = sum;
+                    there[1] = along;
+                }
+                cg::this_cluster().sync();
+            } else {
+                if (wlane == 0) {
+                    sums[flip][warp][0] = sum;
+                    sums[flip][warp][1] = along;
+                }
+                __syncthreads();
+            }
+            const int n = ranks * warps;
+            sum = wlane < n ? sums[flip][wlane][0] : W(0);
+            along = wlane < n ? sums[flip][wlane][1] : W(0);
+            if (CLUSTER && wlane + 32 < n) {
+                sum += sums[flip][wlane + 32][0];
+                along += sums[flip][wlane + 32][1];
+            }
+            sum = team_sum(sum, 32);
+            along = team_sum(along, 32);
+        }
+        sum *= over;
+        along *= over;
+        if (BLOCK) {
+            vectors(x, stage, 0, x_row);
+            vectors(dy, stage, 1, dy_row);
+        }
+        Pair<W> v[Q];
+#pragma unroll
+        for (int q = 0; q < Q; ++q) {
+            const Pair<W> xh = (pair_at(x, q) + both(-mean)) * both(rstd);
+            v[q] = (fma(xh, both(-along), pair_at(dy, q) * weight[q]) + both(-sum)) * both(rstd);
+        }
+        if constexpr (DROP)
+            if (has_dz) {
+                vectors(x, stage, 2, dz_row);
+#pragma unroll
+                for (int q = 0; q < Q; ++q) v[q] = v[q] + pair_at(x, q);
+            }
+        if (a.dsum != nullptr) {
+#pragma unroll
+            for (int q = 0; q < Q; ++q) set_pair(x, q, v[q]);
+#pragma unroll
+            for (int i = 0; i < K; ++i) {
+                const int c = (lane + i * threads) * V;
+                if (live && c < a.cols) store<T, V>((T *)a.dsum + row * a.dsum_stride + c, x[i]);
+            }
+        }
+        if constexpr (DROP) {
+            if (a.dx != nullptr) {
+                const uint32_t kept = kept_of_row<V, K>(a.drop, offset, row * (size_t)a.cols, lane, threads, a.cols);
+#pragma unroll
+                for (int q = 0; q < Q; ++q) {
+                    v[q] = v[q] * both(scale);
+                    v[q].x = (kept >> (2 * q)) & 1 ? v[q].x : W(0);
+                    v[q].y = (kept >> (2 * q + 1)) & 1 ? v[q].y : W(0);
+                    set_pair(x, q, v[q]);
+                }
+#pragma unroll
+                for (int i = 0; i < K; ++i) {
+                    const int c = (lane + i * threads) * V;
+                    if (live && c < a.cols) store<T, V>((T *)a.dx + row * a.dx_stride + c, x[i]);
+                }
+            }
+        }
+        stage = stage == STAGES - 1 ? 0 : stage + 1;
+    }
+    if (partial == nullptr) return;
+    W *mine = partial + cluster * 2 * a.cols;
+    W flat[2][K * V];
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+        flat[0][2 * q] = dw[q].x, flat[0][2 * q + 1] = dw[q].y;
+        flat[1][2 * q] = db[q].x, flat[1][2 * q + 1] = db[q].y;
+    }
+    if constexpr (BLOCK) {
+#pragma unroll
+        for (int i = 0; i < K; ++i) {
+            const int c = (lane + i * threads) * V;
+            if (c < a.cols)
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    mine[c + j] = flat[0][i * V + j];
+                    mine[a.cols + c + j] = flat[1][i * V + j];
+                }
+        }
+    } else {
+        // The block's teams in order.
+        for (int team = 0; team < teams; ++team) {
+            if ((int)threadIdx.x / lanes == team)
+#pragma unroll
+                for (int i = 0; i < K; ++i)
+#pragma unroll
+                    for (int j = 0; j < V; ++j) {
+                        const int c = (lane + i * threads) * V + j;
+                        columns[0][c] = flat[0][i * V + j] + (team > 0 ? columns[0][c] : W(0));
+                        columns[1][c] = flat[1][i * V + j] + (team > 0 ? columns[1][c] : W(0));
+                    }
+            __syncthreads();
+        }
+        for (int c = threadIdx.x; c < a.cols; c += 128) {
+            mine[c] = columns[0][c];
+            mine[a.cols + c] = columns[1][c];
+        }
+    }
+}
 
 // ---- any row length ----------------------------------------------------------
 
@@ -163,20 +636,92 @@ __global__ void __launch_bounds__(kThreads) vjp_columns_any_kernel(const Backwar
     }
 }
 
-// out[c] = sum over the blocks of partial[block][which][c], in block order.
+// out[c] = sum over the blocks of partial[block][which][c]. `wide` columns a
+// block of threads, 1024 / wide threads a column, each over every so many
+// blocks in order, then those in order.
 template <typename W, typename P>
-__global__ void __launch_bounds__(kThreads) join_columns_kernel(const W *partial, int blocks, int cols, void *dweight,
-                                                                void *dbias) {
-    const int c = (int)blockIdx.x * kThreads + threadIdx.x;
-    if (c >= cols) return;
+__global__ void __launch_bounds__(1024) join_columns_kernel(const W *partial, int blocks, int cols, int wide,
+                                                            void *dweight, void *dbias) {
+    __shared__ W sums[1024];
     P *out = (P *)(blockIdx.y == 0 ? dweight : dbias);
     if (out == nullptr) return;
+    const int column = threadIdx.x & (wide - 1), part = threadIdx.x / wide, parts = 1024 / wide;
+    const int c = (int)blockIdx.x * wide + column;
     W sum = 0;
-    for (int i = 0; i < blocks; ++i) sum += partial[((size_t)i * 2 + blockIdx.y) * cols + c];
-    out[c] = narrow<P>((Wide<P>)sum);
+    if (c < cols) {
+#pragma unroll 8
+        for (int i = part; i < blocks; i += parts) sum += partial[((size_t)i * 2 + blockIdx.y) * cols + c];
+    }
+    sums[threadIdx.x] = sum;
+    for (int n = parts / 2; n > 0; n /= 2) {
+        __syncthreads();
+        if (part < n) sums[threadIdx.x] += sums[threadIdx.x + n * wide];
+    }
+    if (part == 0 && c < cols) out[c] = narrow<P>((Wide<P>)sums[threadIdx.x]);
 }
 
 // ---- launches ----------------------------------------------------------------
+
+// How a row is held: values a thread loads at once, vectors a thread, threads.
+struct Shape {
+    int vector;   // 16 bytes of values, or one value
+    int vectors;  // K; 0: rows too long, the kernels for any row length
+    int lanes;    // threads of a row in a block: a power of two up to 32, or a whole block
+    int blocks;   // blocks of a row (backward)
+    int grid;     // backward: clusters of `blocks`, each with a partial sum of the columns
+};
+
+// Single values are spread over whole warps, which work their draws out together.
+int threads_for(size_t vectors, int k, bool aligned) {
+    const size_t lanes = (vectors + k - 1) / k;
+    if (lanes > 32 || !aligned) return (int)((lanes + 31) / 32 * 32);
+    int n = 1;
+    while (n < (int)lanes) n *= 2;
+    return n;
+}
+
+// Forward: the fewest threads a row that still fill the device, because sums
+// across threads cost a fixed number of instructions a thread; with few rows as
+// many threads as vectors, because then the chain of one row is the time.
+Shape forward_shape(size_t rows, size_t cols, uint32_t type, bool aligned) {
+    const int b = (int)type_bytes(type);
+    Shape s = {aligned ? 16 / b : 1, 0, 0, 1, 0};
+    const size_t vectors = cols / s.vector;
+    const int most = !aligned ? 16 : (type == GEO_B200_F64 ? 8 : 4);
+    for (int k = aligned ? 1 : 4; k <= most; k *= aligned ? 2 : 4) {
+        const int lanes = threads_for(vectors, k, aligned);
+        if (lanes > 1024) continue;
+        if (k == 8 && s.vectors != 0) break;  // 8: only where 4 cannot hold the row
+        s.vectors = k;
+        s.lanes = lanes;
+        if (rows * lanes <= (size_t)geo::device_sm_count() * 2048) break;
+    }
+    return s;
+}
+
+constexpr int kBackwardThreads = 256;
+
+// Backward: 16 values a thread (8 in float64), whose two column sums and weight
+// fit 128 registers beside the arithmetic; 512 threads a multiprocessor.
+Shape backward_shape(size_t rows, size_t cols, uint32_t type, bool aligned) {
+    const int b = (int)type_bytes(type);
+    const int each = type == GEO_B200_F64 ? 8 : 16;
+    Shape s = {aligned ? 16 / b : 1, 0, 0, 1, 0};
+    const int k = each / s.vector;
+    int lanes = threads_for(cols / s.vector, k, aligned);
+    while (lanes > kBackwardThreads * s.blocks) s.blocks *= 2;
+    if (s.blocks > 8) return s;
+    if (s.blocks > 1) lanes = (lanes / s.blocks + 31) / 32 * 32;
+    if (s.blocks * lanes * (size_t)k < cols / s.vector) lanes += 32;
+    s.vectors = k;
+    s.lanes = lanes;
+    const size_t teams = lanes <= 32 ? 128 / lanes : 1;
+    const size_t wanted = (rows + teams - 1) / teams;
+    const size_t resident = lanes <= 128 ? 4 : 2;  // blocks a multiprocessor
+    const size_t most = geo::device_sm_count() * resident / s.blocks;
+    s.grid = (int)(wanted < most ? wanted : most);
+    return s;
+}
 
 // Row blocks of the column sums: enough for four CTAs per SM, at least 64 rows each.
 size_t column_blocks(size_t rows, size_t cols) {
@@ -198,33 +743,153 @@ cudaError_t by_types(uint32_t type, uint32_t parameter_type, F &&f) {
     });
 }
 
+// f(V, K) as compile-time constants.
+template <typename T, typename F>
+void by_shape(const Shape &s, F &&f) {
+    constexpr int V = 16 / (int)sizeof(T);
+    using std::integral_constant;
+    if (s.vector == 1) {
+        if (s.vectors == 4) f(integral_constant<int, 1>{}, integral_constant<int, 4>{});
+        if (s.vectors == 8) f(integral_constant<int, 1>{}, integral_constant<int, 8>{});
+        if (s.vectors == 16) f(integral_constant<int, 1>{}, integral_constant<int, 16>{});
+    } else {
+        if (s.vectors == 1) f(integral_constant<int, V>{}, integral_constant<int, 1>{});
+        if (s.vectors == 2) f(integral_constant<int, V>{}, integral_constant<int, 2>{});
+        if (s.vectors == 4) f(integral_constant<int, V>{}, integral_constant<int, 4>{});
+        if constexpr (V == 2)
+            if (s.vectors == 8) f(integral_constant<int, V>{}, integral_constant<int, 8>{});
+    }
+}
+
+// Whether every array starts on, and every row is a multiple of, 16 bytes.
+struct Rows {
+    const void *pointer;
+    size_t stride;
+};
+bool aligned16(size_t cols, size_t bytes, size_t parameter_bytes, std::initializer_list<Rows> arrays,
+               std::initializer_list<const void *> parameters) {
+    if (cols * bytes % 16 != 0) return false;
+    for (const Rows &r : arrays)
+        if (r.pointer != nullptr && ((uintptr_t)r.pointer % 16 != 0 || r.stride * bytes % 16 != 0)) return false;
+    // A thread's parameters are loaded by up to 16 bytes at multiples of the same.
+    const size_t need = 16 / bytes * parameter_bytes < 16 ? 16 / bytes * parameter_bytes : 16;
+    for (const void *p : parameters)
+        if ((uintptr_t)p % need != 0) return false;
+    return true;
+}
+
 template <bool DROP>
 cudaError_t launch_forward(const geo_b200_layer_norm_config_t &c, const ForwardArgs &a, cudaStream_t stream) {
-    return by_types(c.type, c.parameter_type, [&](auto t, auto p) {
-        norm_any_kernel<decltype(t), decltype(p), DROP><<<row_grid(a.rows), kThreads, 0, stream>>>(a);
+    const bool aligned = aligned16(a.cols, type_bytes(c.type), type_bytes(c.parameter_type),
+                                   {{a.x, a.x_stride}, {a.residual, a.residual_stride}, {a.z, a.z_stride}, {a.y, a.y_stride}},
+                                   {a.weight, a.bias});
+    const Shape s = forward_shape(a.rows, a.cols, c.type, aligned);
+    if (s.vectors == 0)
+        return by_types(c.type, c.parameter_type, [&](auto t, auto p) {
+            norm_any_kernel<decltype(t), decltype(p), DROP><<<row_grid(a.rows), kThreads, 0, stream>>>(a);
+            return cudaGetLastError();
+        });
+    const bool float_parameters = c.parameter_type == GEO_B200_F32;
+    return by_type(c.type, [&](auto t) {
+        using T = decltype(t);
+        by_shape<T>(s, [&](auto v, auto k) {
+            constexpr int V = decltype(v)::value, K = decltype(k)::value;
+            if constexpr (V > 1 || K != 8) {  // 8 single values a thread: the backward pass only
+                // As many blocks as are resident, each over several rows.
+                const size_t teams = s.lanes <= 32 ? 128 / s.lanes : 1, threads = s.lanes <= 32 ? 128 : s.lanes;
+                const size_t wanted = (a.rows + teams - 1) / teams;
+                const size_t most = (size_t)geo::device_sm_count() * (threads > 256 ? 1024 / threads : 768 / threads);
+                const unsigned grid = (unsigned)(wanted < most ? wanted : most);
+                if (s.lanes <= 32)
+                    norm_kernel<T, V, K, DROP, false, 128><<<grid, 128, 0, stream>>>(a, s.lanes, float_parameters);
+                else if (s.lanes <= 256)
+                    norm_kernel<T, V, K, DROP, true, 256><<<grid, s.lanes, 0, stream>>>(a, s.lanes, float_parameters);
+                else
+                    norm_kernel<T, V, K, DROP, true, 1024><<<grid, s.lanes, 0, stream>>>(a, s.lanes, float_parameters);
+            }
+        });
         return cudaGetLastError();
     });
+}
+
+template <typename T, int V, int K, bool DROP, bool BLOCK, bool CLUSTER, int STAGES>
+cudaError_t launch_vjp(const Shape &s, const BackwardArgs &a, bool float_parameters, size_t ring, Wide<T> *partial,
+                       cudaStream_t stream) {
+    auto kernel = vjp_kernel<T, V, K, DROP, BLOCK, CLUSTER, STAGES>;
+    if (ring > 40 * 1024) {
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)ring);
+        if (e != cudaSuccess) return e;
+    }
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3((unsigned)(s.grid * s.blocks));
+    config.blockDim = dim3((unsigned)(BLOCK ? s.lanes : 128));
+    config.dynamicSmemBytes = ring;
+    config.stream = stream;
+    cudaLaunchAttribute attribute = {};
+    attribute.id = cudaLaunchAttributeClusterDimension;
+    attribute.val.clusterDim = {(unsigned)s.blocks, 1, 1};
+    config.attrs = &attribute;
+    config.numAttrs = CLUSTER ? 1 : 0;
+    return cudaLaunchKernelEx(&config, kernel, a, s.lanes, float_parameters, partial);
 }
 
 template <bool DROP>
 cudaError_t launch_backward(const geo_b200_layer_norm_config_t &c, const BackwardArgs &a, void *workspace,
                             cudaStream_t stream) {
+    const bool sums = a.dweight != nullptr || a.dbias != nullptr;
+    const bool aligned =
+        aligned16(a.cols, type_bytes(c.type), type_bytes(c.parameter_type),
+                  {{a.x, a.x_stride}, {a.dy, a.dy_stride}, {a.dz, a.dz_stride}, {a.dsum, a.dsum_stride}, {a.dx, a.dx_stride}},
+                  {a.weight});
+    const Shape s = backward_shape(a.rows, a.cols, c.type, aligned);
+    const bool float_parameters = c.parameter_type == GEO_B200_F32;
     return by_types(c.type, c.parameter_type, [&](auto t, auto p) {
         using T = decltype(t);
         using P = decltype(p);
         using W = Wide<T>;
-        // Columns first: the row kernel may overwrite x or y_bar.
-        if (a.dweight != nullptr || a.dbias != nullptr) {
-            const size_t blocks = column_blocks(a.rows, a.cols);
-            const dim3 grid((unsigned)((a.cols + 31) / 32), (unsigned)blocks);
-            vjp_columns_any_kernel<T>
-                <<<grid, kThreads, 0, stream>>>(a, (W *)workspace, (a.rows + blocks - 1) / blocks);
-            const dim3 join((unsigned)((a.cols + kThreads - 1) / kThreads), 2);
-            join_columns_kernel<W, P><<<join, kThreads, 0, stream>>>((const W *)workspace, (int)blocks, a.cols,
-                                                                     a.dweight, a.dbias);
+        int blocks = s.grid;
+        cudaError_t e = cudaSuccess;
+        if (s.vectors != 0) {
+            W *partial = sums ? (W *)workspace : nullptr;
+            by_shape<T>(s, [&](auto v, auto k) {
+                constexpr int V = decltype(v)::value, K = decltype(k)::value;
+                if constexpr (V * K == (sizeof(T) == 8 ? 8 : 16)) {
+                    // Four rows in flight where shared memory holds them at 512 threads a multiprocessor, else two.
+                    const int threads = s.lanes <= 32 ? 128 : s.lanes;
+                    const size_t stage = (size_t)(a.dz != nullptr ? 3 : 2) * K * threads * kSlot<T, V>;
+                    const size_t room = (size_t)208 * 1024 * (threads <= 128 ? 128 : 256) / 512;
+                    const bool deep = 4 * stage <= room;
+                    const size_t ring = (deep ? 4 : 2) * stage;
+                    auto go = [&](auto block, auto cluster) {
+                        constexpr bool B = decltype(block)::value, C = decltype(cluster)::value;
+                        e = deep ? launch_vjp<T, V, K, DROP, B, C, 4>(s, a, float_parameters, ring, partial, stream)
+                                 : launch_vjp<T, V, K, DROP, B, C, 2>(s, a, float_parameters, ring, partial, stream);
+                    };
+                    if (s.lanes <= 32 && s.blocks == 1)
+                        go(std::false_type{}, std::false_type{});
+                    else if (s.blocks == 1)
+                        go(std::true_type{}, std::false_type{});
+                    else
+                        go(std::true_type{}, std::true_type{});
+                }
+            });
+        } else {
+            // Columns first: the row kernel may overwrite x or y_bar.
+            if (sums) {
+                blocks = (int)column_blocks(a.rows, a.cols);
+                const dim3 grid((unsigned)((a.cols + 31) / 32), (unsigned)blocks);
+                vjp_columns_any_kernel<T>
+                    <<<grid, kThreads, 0, stream>>>(a, (W *)workspace, (a.rows + blocks - 1) / blocks);
+            }
+            if (a.dsum != nullptr || a.dx != nullptr)
+                vjp_rows_any_kernel<T, P, DROP><<<row_grid(a.rows), kThreads, 0, stream>>>(a);
+            e = cudaGetLastError();
         }
-        if (a.dsum != nullptr || a.dx != nullptr)
-            vjp_rows_any_kernel<T, P, DROP><<<row_grid(a.rows), kThreads, 0, stream>>>(a);
+        if (e != cudaSuccess || !sums) return e;
+        const int wide = a.cols >= 2048 ? 32 : 8;
+        const dim3 join((unsigned)((a.cols + wide - 1) / wide), 2);
+        join_columns_kernel<W, P><<<join, 1024, 0, stream>>>((const W *)workspace, blocks, a.cols, wide, a.dweight,
+                                                             a.dbias);
         return cudaGetLastError();
     });
 }
@@ -236,8 +901,16 @@ bool config_valid(const geo_b200_layer_norm_config_t *c) {
            std::isfinite(c->epsilon) && c->epsilon >= 0.0;
 }
 
+// Enough for whatever alignment the arrays turn out to have.
 size_t workspace_bytes_of(const geo_b200_layer_norm_config_t &c) {
-    return column_blocks(c.rows, c.cols) * 2 * c.cols * wide_bytes(c.type);
+    size_t blocks = 0;
+    for (const bool aligned : {false, true}) {
+        if (aligned && c.cols * type_bytes(c.type) % 16 != 0) continue;
+        const Shape s = backward_shape(c.rows, c.cols, c.type, aligned);
+        const size_t n = s.vectors != 0 ? (size_t)s.grid : column_blocks(c.rows, c.cols);
+        if (n > blocks) blocks = n;
+    }
+    return blocks * 2 * c.cols * wide_bytes(c.type);
 }
 
 bool workspace_usable(const geo_b200_layer_norm_config_t &c, const void *workspace, size_t bytes) {

@@ -47,6 +47,7 @@ bool make_drop(const geo_b200_dropout_config_t &config, const uint64_t *device_o
     out->offset = config.offset;
     out->device_offset = device_offset;
     out->threshold = (uint32_t)threshold;
+    out->bound = (uint32_t)((uint64_t)out->threshold * 65536u - 1u);  // 2^32 - 1 when everything is dropped
     out->scale = threshold < 65536.0 ? 65536.0 / (65536.0 - threshold) : 0.0;
     out->shift = config.dimension;
     return true;

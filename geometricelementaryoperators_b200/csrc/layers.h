@@ -40,6 +40,75 @@ __device__ __forceinline__ T narrow(Wide<T> v) {
         return v;
 }
 
+// Two values of the arithmetic type. float32 pairs go through the packed
+// two-wide add, multiply and multiply-add of sm_100a: half the instructions of
+// kernels that would otherwise issue more than HBM lets them.
+template <typename W>
+struct alignas(2 * sizeof(W)) Pair {
+    W x, y;
+};
+
+__device__ __forceinline__ uint64_t bits_of(Pair<float> a) {
+    return (uint64_t)__float_as_uint(a.x) | (uint64_t)__float_as_uint(a.y) << 32;
+}
+__device__ __forceinline__ Pair<float> pair_of(uint64_t b) {
+    return {__uint_as_float((uint32_t)b), __uint_as_float((uint32_t)(b >> 32))};
+}
+__device__ __forceinline__ Pair<float> operator+(Pair<float> a, Pair<float> b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits_of(a)), "l"(bits_of(b)));
+    return pair_of(r);
+}
+__device__ __forceinline__ Pair<float> operator*(Pair<float> a, Pair<float> b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits_of(a)), "l"(bits_of(b)));
+    return pair_of(r);
+}
+__device__ __forceinline__ Pair<float> fma(Pair<float> a, Pair<float> b, Pair<float> c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(bits_of(a)), "l"(bits_of(b)), "l"(bits_of(c)));
+    return pair_of(r);
+}
+__device__ __forceinline__ Pair<double> operator+(Pair<double> a, Pair<double> b) { return {a.x + b.x, a.y + b.y}; }
+__device__ __forceinline__ Pair<double> operator*(Pair<double> a, Pair<double> b) { return {a.x * b.x, a.y * b.y}; }
+__device__ __forceinline__ Pair<double> fma(Pair<double> a, Pair<double> b, Pair<double> c) {
+    return {::fma(a.x, b.x, c.x), ::fma(a.y, b.y, c.y)};
+}
+template <typename W>
+__device__ __forceinline__ Pair<W> both(W v) {
+    return {v, v};
+}
+
+// V adjacent values, moved as one access.
+template <typename T, int V>
+struct alignas(sizeof(T) * V) Vec {
+    T v[V];
+};
+template <typename T, int V>
+__device__ __forceinline__ Vec<T, V> load(const T *p) {
+    return *reinterpret_cast<const Vec<T, V> *>(p);
+}
+template <typename T, int V>
+__device__ __forceinline__ void store(T *p, const Vec<T, V> &v) {
+    *reinterpret_cast<Vec<T, V> *>(p) = v;
+}
+
+template <typename T>
+__device__ __forceinline__ Pair<Wide<T>> widen_pair(T a, T b) {
+    return {widen(a), widen(b)};
+}
+template <typename T>
+__device__ __forceinline__ void narrow_pair(Pair<Wide<T>> v, T &a, T &b) {
+    if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+        const __nv_bfloat162 r = __floats2bfloat162_rn(v.x, v.y);
+        a = r.x, b = r.y;
+    } else if constexpr (std::is_same_v<T, __half>) {
+        const __half2 r = __floats2half2_rn(v.x, v.y);
+        a = r.x, b = r.y;
+    } else {
+        a = v.x, b = v.y;
+    }
+}
 #endif
 
 inline size_t type_bytes(uint32_t type) {
@@ -102,6 +171,7 @@ struct Drop {
     const uint64_t *device_offset;
     double scale;        // 65536 / (65536 - threshold); 0 when everything is dropped
     uint32_t threshold;  // drop when draw < threshold, 0 .. 65536
+    uint32_t bound;      // (threshold << 16) - 1: keep when draw << 16 is above it (threshold > 0)
     uint32_t shift;      // a unit is 2^shift values
 };
 // Checks everything but strides and arrays; false when a field is out of range.
@@ -135,11 +205,69 @@ __device__ __forceinline__ uint64_t drop_offset(const Drop &drop) {
     return drop.offset + (drop.device_offset != nullptr ? *drop.device_offset : 0);
 }
 
+// Bit i: whether draw i of the block is kept.
+__device__ __forceinline__ uint32_t kept_of_block(const Drop &drop, uint64_t offset, uint64_t index) {
+    const Block b = philox(index, offset, drop.seed);
+    uint32_t bits = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        bits |= (uint32_t)((b.word[i] << 16) > drop.bound) << (2 * i);
+        bits |= (uint32_t)(b.word[i] > drop.bound) << (2 * i + 1);
+    }
+    return bits;
+}
+
+// Bit j: whether value e + j is kept, j < 8, e a multiple of 8: their units are
+// draws of one block.
+__device__ __forceinline__ uint32_t kept_of_eight(const Drop &drop, uint64_t offset, uint64_t e) {
+    if (drop.threshold == 0) return 0xFFu;
+    const uint64_t unit = e >> drop.shift;
+    const uint32_t bits = kept_of_block(drop, offset, unit >> 3);
+    if (drop.shift == 0) return bits;
+    uint32_t out = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) out |= ((bits >> (((uint32_t)unit + ((uint32_t)j >> drop.shift)) & 7u)) & 1u) << j;
+    return out;
+}
+
+// The same of V values, V = 2, 4 or 8 dividing e.
+template <int V>
+__device__ __forceinline__ uint32_t kept_values(const Drop &drop, uint64_t offset, uint64_t e) {
+    return kept_of_eight(drop, offset, e & ~(uint64_t)7) >> ((uint32_t)e & 7u);
+}
+
+// Rows that are not made of whole vectors: bit i of the result is whether value
+// base + i step + lane is kept (i < K), lane = thread of the warp, the same base
+// and step on every lane, all lanes taking part. The 32 values of one i lie in at
+// most five blocks, so each lane works one block out for six i at a time and
+// hands its eight decisions round: a sixth of a block a value instead of one.
+template <int K>
+__device__ __forceinline__ uint32_t kept_by_warp(const Drop &drop, uint64_t offset, uint64_t base, uint32_t step) {
+    if (drop.threshold == 0) return 0xFFFFFFFFu;
+    // Places relative to the start of the first value's block, in 32 bits.
+    const uint32_t lane = threadIdx.x & 31, whole = drop.shift + 3;
+    const uint64_t block = base >> whole;
+    const uint32_t in_block = (uint32_t)base & ((8u << drop.shift) - 1u);
+    uint32_t kept = 0;
+#pragma unroll
+    for (int i0 = 0; i0 < K; i0 += 6) {
+        const uint32_t from = (in_block + (i0 + lane / 5) * step) >> whole;
+        const uint32_t mine = kept_of_block(drop, offset, block + from + lane % 5);
+#pragma unroll
+        for (int m = 0; m < 6 && i0 + m < K; ++m) {
+            const uint32_t first = in_block + (i0 + m) * step, place = first + lane;
+            const uint32_t bits = __shfl_sync(0xffffffffu, mine, m * 5 + (place >> whole) - (first >> whole));
+            kept |= ((bits >> ((place >> drop.shift) & 7u)) & 1u) << (i0 + m);
+        }
+    }
+    return kept;
+}
+
 // Whether the unit is kept; for callers that look at one unit at a time.
 __device__ __forceinline__ bool unit_kept(const Drop &drop, uint64_t offset, uint64_t unit) {
     const Block b = philox(unit >> 3, offset, drop.seed);
     const uint32_t word = (unit & 4) ? ((unit & 2) ? b.word[3] : b.word[2]) : ((unit & 2) ? b.word[1] : b.word[0]);
-    return ((unit & 1) ? word >> 16 : word & 0xFFFFu) >= drop.threshold;
+    return ((unit & 1) ? word : word << 16) > drop.bound;
 }
 #endif
 

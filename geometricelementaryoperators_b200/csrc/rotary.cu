@@ -23,6 +23,8 @@ struct RotaryArgs {
     size_t batch, tokens, heads, head_dim;
     size_t xb, xt, xh, yb, yt, yh, pb;
     int64_t first_position;
+    size_t groups, share;  // heads are split into `groups` of `share`
+    int narrow_positions;
 };
 
 template <typename W>
@@ -42,37 +44,87 @@ __device__ __forceinline__ void rotor(int64_t position, double hi, double lo, W 
     s = amplitude * ((q & 1) ? (q == 1 ? cosine : -cosine) : (q == 0 ? sine : -sine));
 }
 
-// One pair (or one copied coordinate past rotary_dim) of one token per thread,
-// all heads.
-template <typename T, typename I>
+// A thread takes the pairs that one vector (INTERLEAVED: V / 2 pairs) or two
+// vectors half a head apart (HALF: V pairs) hold of one token, works their rotors
+// out once, and turns them in `share` heads, kHeads loads ahead; the coordinates
+// past rotary_dim go the same way as vectors that are only copied. Where nothing
+// wider than a value is aligned, a pair is two values.
+constexpr int kHeads = 4;
+template <typename T, int V, bool HALF>
 __global__ void __launch_bounds__(kThreads)
     rotary_kernel(const RotaryArgs a, const __grid_constant__ geo_b200_rotary_plan_t plan, int backward) {
     using W = Wide<T>;
-    const size_t pairs = plan.rotary_dim / 2, columns = a.head_dim - pairs;
-    const size_t count = a.batch * a.tokens * columns;
-    for (size_t i = blockIdx.x * (size_t)kThreads + threadIdx.x; i < count; i += (size_t)gridDim.x * kThreads) {
-        const size_t bt = i / columns, column = i - bt * columns;
+    constexpr bool SPLIT = HALF || V == 1;     // a pair's coordinates are in two vectors
+    constexpr int N = SPLIT ? 2 : 1;           // vectors a head
+    constexpr int PAIRS = SPLIT ? V : V / 2;   // pairs a thread
+    const uint32_t half = plan.rotary_dim / 2, second = HALF ? half : 1;
+    const uint32_t turned = plan.rotary_dim / (N * V);
+    const uint32_t units = turned + ((uint32_t)a.head_dim - plan.rotary_dim) / V;
+    const size_t count = a.batch * a.tokens * a.groups * units;
+    for (size_t id = blockIdx.x * (size_t)kThreads + threadIdx.x; id < count; id += (size_t)gridDim.x * kThreads) {
+        size_t rest = id / units;
+        const uint32_t unit = (uint32_t)(id - rest * units);
+        const size_t bt = rest / a.groups, group = rest - bt * a.groups;
         const size_t b = bt / a.tokens, t = bt - b * a.tokens;
-        const T *x = (const T *)a.x + b * a.xb + t * a.xt;
-        T *y = (T *)a.y + b * a.yb + t * a.yt;
-        if (column >= pairs) {
-            const size_t at = column + pairs;
-            for (size_t h = 0; h < a.heads; ++h) y[h * a.yh + at] = x[h * a.xh + at];
-            continue;
+        const size_t from = group * a.share, left = a.heads - from;
+        const size_t heads = left < a.share ? left : a.share;
+        const bool copied = unit >= turned;
+        if (copied && a.x == a.y) continue;
+        const size_t at = copied ? plan.rotary_dim + (size_t)(unit - turned) * V : (size_t)unit * (HALF ? V : N * V);
+        const T *x = (const T *)a.x + b * a.xb + t * a.xt + from * a.xh + at;
+        T *y = (T *)a.y + b * a.yb + t * a.yt + from * a.yh + at;
+        W c[PAIRS], s[PAIRS];
+        if (!copied) {
+            const size_t where = b * a.pb + t;
+            const int64_t position = a.positions == nullptr ? a.first_position + (int64_t)t
+                                     : a.narrow_positions   ? (int64_t)((const int32_t *)a.positions)[where]
+                                                            : ((const int64_t *)a.positions)[where];
+#pragma unroll
+            for (int j = 0; j < PAIRS; ++j) {
+                const uint32_t pair = unit * PAIRS + j;
+                rotor<W>(position, plan.turns[pair], plan.turns_low[pair], (W)plan.amplitude, c[j], s[j]);
+                if (backward) s[j] = -s[j];
+            }
         }
-        const int64_t position = a.positions != nullptr ? (int64_t)((const I *)a.positions)[b * a.pb + t]
-                                                        : a.first_position + (int64_t)t;
-        W c, s;
-        rotor<W>(position, plan.turns[column], plan.turns_low[column], (W)plan.amplitude, c, s);
-        if (backward) s = -s;
-        const bool half = plan.layout == GEO_B200_ROTARY_HALF;
-        const size_t ia = half ? column : 2 * column, ib = half ? column + pairs : 2 * column + 1;
-        for (size_t h = 0; h < a.heads; ++h) {
-            const W u = widen(x[h * a.xh + ia]), v = widen(x[h * a.xh + ib]);
-            y[h * a.yh + ia] = narrow<T>(u * c - v * s);
-            y[h * a.yh + ib] = narrow<T>(u * s + v * c);
+        for (size_t h = 0; h < heads; h += kHeads) {
+            Vec<T, V> v[kHeads][N];
+#pragma unroll
+            for (int k = 0; k < kHeads; ++k)
+                if (h + k < heads) {
+                    v[k][0] = load<T, V>(x + (h + k) * a.xh);
+                    if (SPLIT && !copied) v[k][N - 1] = load<T, V>(x + (h + k) * a.xh + second);
+                }
+#pragma unroll
+            for (int k = 0; k < kHeads; ++k)
+                if (h + k < heads) {
+                    if (!copied) {
+#pragma unroll
+                        for (int j = 0; j < PAIRS; ++j) {
+                            T &p = v[k][0].v[SPLIT ? j : 2 * j];
+                            T &q = v[k][N - 1].v[SPLIT ? j : 2 * j + 1];
+                            const W u = widen(p), w = widen(q);
+                            narrow_pair<T>({u * c[j] - w * s[j], u * s[j] + w * c[j]}, p, q);
+                        }
+                    }
+                    store<T, V>(y + (h + k) * a.yh, v[k][0]);
+                    if (SPLIT && !copied) store<T, V>(y + (h + k) * a.yh + second, v[k][N - 1]);
+                }
         }
     }
+}
+
+// The widest vector, up to 16 bytes, that every head, half and row starts on.
+int vector_width(const RotaryArgs &a, const geo_b200_rotary_plan_t &plan, size_t bytes) {
+    const bool half = plan.layout == GEO_B200_ROTARY_HALF;
+    size_t strides = a.head_dim | plan.rotary_dim;
+    if (a.heads > 1) strides |= a.xh | a.yh;
+    if (a.tokens > 1) strides |= a.xt | a.yt;
+    if (a.batch > 1) strides |= a.xb | a.yb;
+    if (half) strides |= plan.rotary_dim / 2;
+    const uintptr_t low = (uintptr_t)a.x | (uintptr_t)a.y;
+    int v = 16 / (int)bytes;
+    while (v > 1 && (strides % v != 0 || low % (v * bytes) != 0)) v /= 2;
+    return v;
 }
 
 // Strides (0 = packed) of one array; false when an offset would not fit.
@@ -153,15 +205,34 @@ geo_b200_status_t rotary(const geo_b200_rotary_plan_t *plan, const geo_b200_rota
     a.yh = s.y_head_stride;
     a.pb = s.position_batch_stride;
     a.first_position = s.first_position;
+    a.narrow_positions = s.position_type == GEO_B200_I32;
+    // A rotor costs about as much as turning four heads: heads are shared out
+    // only as far as it takes to give every multiprocessor 1024 threads.
+    const int v = vector_width(a, *plan, b);
+    const bool half = plan->layout == GEO_B200_ROTARY_HALF;
+    const size_t units = plan->rotary_dim / (half || v == 1 ? 2 * v : v) + (s.head_dim - plan->rotary_dim) / v;
+    const size_t wanted = (size_t)geo::device_sm_count() * 1024, threads = tokens * units;
+    size_t groups = threads < wanted ? (wanted + threads - 1) / threads : 1;
+    if (groups > s.heads) groups = s.heads;
+    a.share = (s.heads + groups - 1) / groups;
+    a.groups = (s.heads + a.share - 1) / a.share;
+    const size_t blocks = (threads * a.groups + kThreads - 1) / kThreads;
+    const unsigned grid = (unsigned)(blocks < 0x7fffffff ? blocks : 0x7fffffff);
     return status_of(by_type(s.type, [&](auto t) {
         using T = decltype(t);
-        const size_t count = tokens * (s.head_dim - plan->rotary_dim / 2);
-        const size_t blocks = (count + kThreads - 1) / kThreads, most = (size_t)geo::device_sm_count() * 32;
-        const unsigned grid = (unsigned)(blocks < most ? blocks : most);
-        if (s.position_type == GEO_B200_I32)
-            rotary_kernel<T, int32_t><<<grid, kThreads, 0, stream>>>(a, *plan, backward);
-        else
-            rotary_kernel<T, int64_t><<<grid, kThreads, 0, stream>>>(a, *plan, backward);
+        auto go = [&](auto width) {
+            constexpr int V = decltype(width)::value;
+            if (half)
+                rotary_kernel<T, V, true><<<grid, kThreads, 0, stream>>>(a, *plan, backward);
+            else
+                rotary_kernel<T, V, false><<<grid, kThreads, 0, stream>>>(a, *plan, backward);
+        };
+        if (v == 1) go(std::integral_constant<int, 1>{});
+        if (v == 2) go(std::integral_constant<int, 2>{});
+        if constexpr (sizeof(T) <= 4)
+            if (v == 4) go(std::integral_constant<int, 4>{});
+        if constexpr (sizeof(T) == 2)
+            if (v == 8) go(std::integral_constant<int, 8>{});
         return cudaGetLastError();
     }));
 }
