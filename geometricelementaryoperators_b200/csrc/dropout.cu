@@ -47,20 +47,13 @@ __global__ void __launch_bounds__(kThreads) drop_vectors_kernel(const Rows a, co
 #pragma unroll
         for (int i = 0; i < R; ++i) {
             const size_t e = value(m, i);
-            x[m][i] = Vec<T, V>{};
-            if constexpr (RESIDUAL) res[m][i] = Vec<T, V>{};
+            x[m][i] = Vec<T, V>::zero();
+            if constexpr (RESIDUAL) res[m][i] = Vec<T, V>::zero();
             if (e >= count) continue;
             if constexpr (PACKED) {
                 if (e + V <= count) {
                     x[m][i] = load<T, V>((const T *)a.x + e);
                     if constexpr (RESIDUAL) res[m][i] = load<T, V>((const T *)a.residual + e);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < V; ++j)
-                        if (e + j < count) {
-                            x[m][i].v[j] = ((const T *)a.x)[e + j];
-                            if constexpr (RESIDUAL) res[m][i].v[j] = ((const T *)a.residual)[e + j];
-                        }
                 }
             } else {
                 const size_t row = count <= 0xFFFFFFFFu ? (uint32_t)e / (uint32_t)a.cols : e / a.cols;
@@ -80,24 +73,26 @@ __global__ void __launch_bounds__(kThreads) drop_vectors_kernel(const Rows a, co
             if constexpr (R > 1) kept = __shfl_sync(0xffffffffu, mine, (i * 32 + lane) / R) >> (lane % R * V);
             Vec<T, V> out;
 #pragma unroll
-            for (int j = 0; j < V; j += 2) {
-                Pair<W> v = widen_pair(x[m][i].v[j], x[m][i].v[j + 1]);
-                v.x = (kept >> j) & 1 ? v.x : W(0);  // selected, not multiplied: a dropped NaN is gone
-                v.y = (kept >> (j + 1)) & 1 ? v.y : W(0);
+            for (int q = 0; q < V / 2; ++q) {
+                Pair<W> v = x[m][i].pair(q);
+                v.x = (kept >> (2 * q)) & 1 ? v.x : W(0);  // selected, not multiplied: a dropped NaN is gone
+                v.y = (kept >> (2 * q + 1)) & 1 ? v.y : W(0);
                 if constexpr (RESIDUAL)
-                    v = fma(v, both(scale), widen_pair(res[m][i].v[j], res[m][i].v[j + 1]));
+                    v = fma(v, both(scale), res[m][i].pair(q));
                 else
                     v = v * both(scale);
-                narrow_pair<T>(v, out.v[j], out.v[j + 1]);
+                out.set(q, v);
             }
             if (e >= count) continue;
             if constexpr (PACKED) {
                 if (e + V <= count) {
                     store<T, V>((T *)a.y + e, out);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < V; ++j)
-                        if (e + j < count) ((T *)a.y)[e + j] = out.v[j];
+                } else {  // the last values of all, one by one
+                    for (int j = 0; e + j < count; ++j) {
+                        const W residual = RESIDUAL ? (W)widen(((const T *)a.residual)[e + j]) : W(0);
+                        ((T *)a.y)[e + j] =
+                            narrow<T>(drop_value<T>((kept >> j) & 1, ((const T *)a.x)[e + j], scale, residual));
+                    }
                 }
             } else {
                 store<T, V>((T *)a.y + y_at[m][i], out);

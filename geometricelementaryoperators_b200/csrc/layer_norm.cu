@@ -62,50 +62,64 @@ __device__ __forceinline__ W team_sum(W v, int lanes) {
     return v;
 }
 
-// Weight or bias at V columns, of the value type or (16-bit values only) float32.
-template <typename T, int V>
-__device__ __forceinline__ void load_parameter(const void *p, bool is_float, int c, Wide<T> *out) {
-    if constexpr (sizeof(T) == 2) {
-        if (is_float) {
-            constexpr int U = V < 4 ? V : 4;
+// Pairs of weight or bias for values [first, first + G) of the thread, of the
+// value type or (16-bit values only) float32; `absent` past the row or without
+// the array. G: whole vectors, at least two values.
+template <typename T, int V, int G>
+__device__ __forceinline__ void load_parameters(const void *p, bool is_float, int first_vector, int lane, int threads,
+                                                int cols, Wide<T> absent, Pair<Wide<T>> (&out)[G / 2]) {
+    using W = Wide<T>;
 #pragma unroll
-            for (int j = 0; j < V; j += U) {
-                const Vec<float, U> w = load<float, U>((const float *)p + c + j);
-#pragma unroll
-                for (int i = 0; i < U; ++i) out[j + i] = w.v[i];
+    for (int i = 0; i < G / V; ++i) {
+        const int c = (lane + (first_vector + i) * threads) * V;
+        const bool there = p != nullptr && c < cols;
+        if constexpr (V == 1) {
+            W v = absent;
+            if (there) {
+                if (sizeof(T) == 2 && is_float)
+                    v = (W)((const float *)p)[c];
+                else
+                    v = load<T, 1>((const T *)p + c).one();
             }
-            return;
+            (i & 1 ? out[i / 2].y : out[i / 2].x) = v;
+        } else {
+#pragma unroll
+            for (int q = 0; q < V / 2; ++q) out[i * V / 2 + q] = both(absent);
+            if (!there) continue;
+            if (sizeof(T) == 2 && is_float) {
+                if constexpr (sizeof(T) == 2) {
+#pragma unroll
+                    for (int j = 0; j < V; j += 4) {
+                        const Vec<float, 4> w = load<float, 4>((const float *)p + c + j);
+                        out[i * V / 2 + j / 2] = w.pair(0);
+                        out[i * V / 2 + j / 2 + 1] = w.pair(1);
+                    }
+                }
+            } else {
+                const Vec<T, V> w = load<T, V>((const T *)p + c);
+#pragma unroll
+                for (int q = 0; q < V / 2; ++q) out[i * V / 2 + q] = w.pair(q);
+            }
         }
     }
-    const Vec<T, V> w = load<T, V>((const T *)p + c);
-#pragma unroll
-    for (int j = 0; j < V; ++j) out[j] = widen(w.v[j]);
-}
-
-// The thread's parameters as pairs in the order of its values; `absent` past the row.
-template <typename T, int V, int K>
-__device__ __forceinline__ void load_parameters(const void *p, bool is_float, int lane, int threads, int cols,
-                                                Wide<T> absent, Pair<Wide<T>> (&out)[K * V / 2]) {
-    Wide<T> flat[K * V];
-#pragma unroll
-    for (int i = 0; i < K; ++i) {
-        const int c = (lane + i * threads) * V;
-#pragma unroll
-        for (int j = 0; j < V; ++j) flat[i * V + j] = absent;
-        if (p != nullptr && c < cols) load_parameter<T, V>(p, is_float, c, flat + i * V);
-    }
-#pragma unroll
-    for (int q = 0; q < K * V / 2; ++q) out[q] = {flat[2 * q], flat[2 * q + 1]};
 }
 
 template <typename T, int V, int K>
 __device__ __forceinline__ Pair<Wide<T>> pair_at(const Vec<T, V> (&raw)[K], int q) {
-    return widen_pair(raw[2 * q / V].v[2 * q % V], raw[(2 * q + 1) / V].v[(2 * q + 1) % V]);
+    if constexpr (V == 1)
+        return {raw[2 * q].one(), raw[2 * q + 1].one()};
+    else
+        return raw[2 * q / V].pair(q % (V / 2));
 }
 
 template <typename T, int V, int K>
 __device__ __forceinline__ void set_pair(Vec<T, V> (&raw)[K], int q, Pair<Wide<T>> v) {
-    narrow_pair<T>(v, raw[2 * q / V].v[2 * q % V], raw[(2 * q + 1) / V].v[(2 * q + 1) % V]);
+    if constexpr (V == 1) {
+        raw[2 * q].set_one(v.x);
+        raw[2 * q + 1].set_one(v.y);
+    } else {
+        raw[2 * q / V].set(q % (V / 2), v);
+    }
 }
 
 // Which of the thread's values dropout keeps, bit i V + j.
@@ -153,6 +167,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 1024 ? 1 : 768 / THREADS) 
     // BLOCK: thread `wlane` of every warp joins what warp `wlane` held.
     const W joined = BLOCK && wlane < threads / 32 ? held_by(wlane) : W(0);
     const W over_joined = joined > W(0) ? W(1) / joined : W(0);
+    const bool ragged = threads * K * V != a.cols;
     int flip = 0;
     // The bound is the warp's first row, so that all its lanes stay for the shuffles.
     for (size_t first = (size_t)blockIdx.x * teams + (BLOCK ? 0 : warp * (32 / lanes)); first < a.rows;
@@ -167,8 +182,8 @@ __global__ void __launch_bounds__(THREADS, THREADS == 1024 ? 1 : 768 / THREADS) 
 #pragma unroll
             for (int i = 0; i < K; ++i) {
                 const int c = (lane + i * threads) * V;
-                raw[i] = Vec<T, V>{};
-                if constexpr (DROP) res[i] = Vec<T, V>{};
+                raw[i] = Vec<T, V>::zero();
+                if constexpr (DROP) res[i] = Vec<T, V>::zero();
                 if (live && c < a.cols) {
                     raw[i] = load<T, V>(x + c);
                     if constexpr (DROP) res[i] = load<T, V>(r + c);
@@ -196,9 +211,10 @@ __global__ void __launch_bounds__(THREADS, THREADS == 1024 ? 1 : 768 / THREADS) 
         for (int q = 0; q < Q; ++q) two = two + v[q];
         W sum = team_sum(two.x + two.y, BLOCK ? 32 : lanes);
         W mean = BLOCK ? sum * over_held : sum / held;
+        if (ragged)
 #pragma unroll
-        for (int i = 0; i < K; ++i)
-            if ((lane + i * threads) * V >= a.cols) {
+            for (int i = 0; i < K; ++i) {
+                if ((lane + i * threads) * V < a.cols) continue;
                 if constexpr (V == 1) {
                     (i & 1 ? v[i / 2].y : v[i / 2].x) = mean;
                 } else {
@@ -235,23 +251,15 @@ __global__ void __launch_bounds__(THREADS, THREADS == 1024 ? 1 : 768 / THREADS) 
 #pragma unroll
         for (int m = 0; m < K * V / G; ++m) {
             Vec<T, V> z[G / V], y[G / V];
-            W w[G], b[G];
-#pragma unroll
-            for (int i = 0; i < G / V; ++i) {
-                const int c = (lane + (m * G / V + i) * threads) * V;
-#pragma unroll
-                for (int j = 0; j < V; ++j) w[i * V + j] = W(1), b[i * V + j] = W(0);
-                if (c < a.cols) {
-                    if (a.weight != nullptr) load_parameter<T, V>(a.weight, float_parameters, c, w + i * V);
-                    if (a.bias != nullptr) load_parameter<T, V>(a.bias, float_parameters, c, b + i * V);
-                }
-            }
+            Pair<W> w[G / 2], b[G / 2];
+            load_parameters<T, V, G>(a.weight, float_parameters, m * G / V, lane, threads, a.cols, W(1), w);
+            load_parameters<T, V, G>(a.bias, float_parameters, m * G / V, lane, threads, a.cols, W(0), b);
 #pragma unroll
             for (int q = 0; q < G / 2; ++q) {
                 const Pair<W> p = v[m * G / 2 + q];
                 if constexpr (DROP) set_pair(z, q, p);
                 const Pair<W> hat = (p + both(-mean)) * both(rstd);
-                set_pair(y, q, fma(hat, Pair<W>{w[2 * q], w[2 * q + 1]}, Pair<W>{b[2 * q], b[2 * q + 1]}));
+                set_pair(y, q, fma(hat, w[q], b[q]));
             }
 #pragma unroll
             for (int i = 0; i < G / V; ++i) {
@@ -338,7 +346,7 @@ __global__ void __launch_bounds__(BLOCK ? 256 : 128, BLOCK ? 2 : 4)
     const int arrays = has_dz ? 3 : 2;
 
     Pair<W> weight[Q], dw[Q], db[Q];
-    load_parameters<T, V, K>(a.weight, float_parameters, lane, threads, a.cols, W(1), weight);
+    load_parameters<T, V, K * V>(a.weight, float_parameters, 0, lane, threads, a.cols, W(1), weight);
 #pragma unroll
     for (int q = 0; q < Q; ++q) dw[q] = db[q] = both(W(0));
 
@@ -365,7 +373,7 @@ __global__ void __launch_bounds__(BLOCK ? 256 : 128, BLOCK ? 2 : 4)
         // Where in its word a single 16-bit value is: the same for all of a thread's, which are 32 n apart.
         if constexpr (S > sizeof(T) * V) from += (uintptr_t)(row_start + lane) & 2;
 #pragma unroll
-        for (int i = 0; i < K; ++i) out[i] = *reinterpret_cast<const Vec<T, V> *>(from + i * next_vector);
+        for (int i = 0; i < K; ++i) out[i] = load<T, V>((const T *)(from + i * next_vector));
     };
 
     const size_t begin = cluster * teams + (BLOCK ? 0 : warp * (32 / lanes));

@@ -79,35 +79,104 @@ __device__ __forceinline__ Pair<W> both(W v) {
     return {v, v};
 }
 
-// V adjacent values, moved as one access.
+// One value from, and to, its bits in the low half of a word.
+template <typename T>
+__device__ __forceinline__ float half_of_word(uint32_t w) {
+    if constexpr (std::is_same_v<T, __nv_bfloat16>)
+        return __uint_as_float(w << 16);
+    else
+        return __half2float(__ushort_as_half((unsigned short)w));
+}
+
+// V adjacent values, moved as one access and held as 32-bit words: 16-bit values
+// are taken from and put into a word two at a time (a bfloat16's float32 is its
+// own bits: one instruction a value).
 template <typename T, int V>
-struct alignas(sizeof(T) * V) Vec {
-    T v[V];
+struct Vec {
+    static constexpr int kBytes = (int)sizeof(T) * V;
+    uint32_t w[kBytes < 4 ? 1 : kBytes / 4];
+
+    __device__ __forceinline__ static Vec zero() {
+        Vec r;
+#pragma unroll
+        for (uint32_t &x : r.w) x = 0;
+        return r;
+    }
+    // Values 2q and 2q + 1.
+    __device__ __forceinline__ Pair<Wide<T>> pair(int q) const {
+        if constexpr (sizeof(T) == 8) {
+            return {__hiloint2double((int)w[4 * q + 1], (int)w[4 * q]),
+                    __hiloint2double((int)w[4 * q + 3], (int)w[4 * q + 2])};
+        } else if constexpr (sizeof(T) == 4) {
+            return {__uint_as_float(w[2 * q]), __uint_as_float(w[2 * q + 1])};
+        } else if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+            return {__uint_as_float(w[q] << 16), __uint_as_float(w[q] & 0xFFFF0000u)};
+        } else {
+            return {half_of_word<T>(w[q]), half_of_word<T>(w[q] >> 16)};
+        }
+    }
+    __device__ __forceinline__ void set(int q, Pair<Wide<T>> v) {
+        if constexpr (sizeof(T) == 8) {
+            w[4 * q] = (uint32_t)__double2loint(v.x), w[4 * q + 1] = (uint32_t)__double2hiint(v.x);
+            w[4 * q + 2] = (uint32_t)__double2loint(v.y), w[4 * q + 3] = (uint32_t)__double2hiint(v.y);
+        } else if constexpr (sizeof(T) == 4) {
+            w[2 * q] = __float_as_uint(v.x), w[2 * q + 1] = __float_as_uint(v.y);
+        } else if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+            const __nv_bfloat162 r = __floats2bfloat162_rn(v.x, v.y);
+            w[q] = *reinterpret_cast<const uint32_t *>(&r);
+        } else {
+            const __half2 r = __floats2half2_rn(v.x, v.y);
+            w[q] = *reinterpret_cast<const uint32_t *>(&r);
+        }
+    }
+    // The value of a Vec of one.
+    __device__ __forceinline__ Wide<T> one() const {
+        static_assert(V == 1, "one value");
+        if constexpr (sizeof(T) == 8)
+            return __hiloint2double((int)w[1], (int)w[0]);
+        else if constexpr (sizeof(T) == 4)
+            return __uint_as_float(w[0]);
+        else
+            return half_of_word<T>(w[0]);
+    }
+    __device__ __forceinline__ void set_one(Wide<T> v) {
+        static_assert(V == 1, "one value");
+        if constexpr (sizeof(T) == 8)
+            w[0] = (uint32_t)__double2loint(v), w[1] = (uint32_t)__double2hiint(v);
+        else if constexpr (sizeof(T) == 4)
+            w[0] = __float_as_uint(v);
+        else if constexpr (std::is_same_v<T, __nv_bfloat16>)
+            w[0] = __bfloat16_as_ushort(__float2bfloat16_rn(v));
+        else
+            w[0] = __half_as_ushort(__float2half_rn(v));
+    }
 };
 template <typename T, int V>
 __device__ __forceinline__ Vec<T, V> load(const T *p) {
-    return *reinterpret_cast<const Vec<T, V> *>(p);
+    Vec<T, V> r;
+    if constexpr (Vec<T, V>::kBytes == 16) {
+        const uint4 v = *reinterpret_cast<const uint4 *>(p);
+        r.w[0] = v.x, r.w[1] = v.y, r.w[2] = v.z, r.w[3] = v.w;
+    } else if constexpr (Vec<T, V>::kBytes == 8) {
+        const uint2 v = *reinterpret_cast<const uint2 *>(p);
+        r.w[0] = v.x, r.w[1] = v.y;
+    } else if constexpr (Vec<T, V>::kBytes == 4) {
+        r.w[0] = *reinterpret_cast<const uint32_t *>(p);
+    } else {
+        r.w[0] = *reinterpret_cast<const unsigned short *>(p);
+    }
+    return r;
 }
 template <typename T, int V>
 __device__ __forceinline__ void store(T *p, const Vec<T, V> &v) {
-    *reinterpret_cast<Vec<T, V> *>(p) = v;
-}
-
-template <typename T>
-__device__ __forceinline__ Pair<Wide<T>> widen_pair(T a, T b) {
-    return {widen(a), widen(b)};
-}
-template <typename T>
-__device__ __forceinline__ void narrow_pair(Pair<Wide<T>> v, T &a, T &b) {
-    if constexpr (std::is_same_v<T, __nv_bfloat16>) {
-        const __nv_bfloat162 r = __floats2bfloat162_rn(v.x, v.y);
-        a = r.x, b = r.y;
-    } else if constexpr (std::is_same_v<T, __half>) {
-        const __half2 r = __floats2half2_rn(v.x, v.y);
-        a = r.x, b = r.y;
-    } else {
-        a = v.x, b = v.y;
-    }
+    if constexpr (Vec<T, V>::kBytes == 16)
+        *reinterpret_cast<uint4 *>(p) = make_uint4(v.w[0], v.w[1], v.w[2], v.w[3]);
+    else if constexpr (Vec<T, V>::kBytes == 8)
+        *reinterpret_cast<uint2 *>(p) = make_uint2(v.w[0], v.w[1]);
+    else if constexpr (Vec<T, V>::kBytes == 4)
+        *reinterpret_cast<uint32_t *>(p) = v.w[0];
+    else
+        *reinterpret_cast<unsigned short *>(p) = (unsigned short)v.w[0];
 }
 #endif
 

@@ -44,6 +44,32 @@ __device__ __forceinline__ void rotor(int64_t position, double hi, double lo, W 
     s = amplitude * ((q & 1) ? (q == 1 ? cosine : -cosine) : (q == 0 ? sine : -sine));
 }
 
+// SPLIT: pair j is value j of p and of q; else pair j is values 2j, 2j + 1 of p.
+template <typename T, int V, bool SPLIT, int C>
+__device__ __forceinline__ void turn(Vec<T, V> &p, Vec<T, V> &q, const Pair<Wide<T>> (&c)[C],
+                                     const Pair<Wide<T>> (&s)[C]) {
+    using W = Wide<T>;
+    if constexpr (V == 1) {
+        const W a = p.one(), b = q.one();
+        p.set_one(a * c[0].x - b * s[0].x);
+        q.set_one(a * s[0].x + b * c[0].x);
+    } else if constexpr (SPLIT) {
+#pragma unroll
+        for (int j = 0; j < V / 2; ++j) {
+            const Pair<W> a = p.pair(j), b = q.pair(j);
+            p.set(j, fma(a, c[j], b * Pair<W>{-s[j].x, -s[j].y}));
+            q.set(j, fma(a, s[j], b * c[j]));
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < V / 2; ++j) {
+            const Pair<W> a = p.pair(j);
+            const W cosine = j & 1 ? c[j / 2].y : c[j / 2].x, sine = j & 1 ? s[j / 2].y : s[j / 2].x;
+            p.set(j, {a.x * cosine - a.y * sine, a.x * sine + a.y * cosine});
+        }
+    }
+}
+
 // A thread takes the pairs that one vector (INTERLEAVED: V / 2 pairs) or two
 // vectors half a head apart (HALF: V pairs) hold of one token, works their rotors
 // out once, and turns them in `share` heads, kHeads loads ahead; the coordinates
@@ -73,7 +99,7 @@ __global__ void __launch_bounds__(kThreads)
         const size_t at = copied ? plan.rotary_dim + (size_t)(unit - turned) * V : (size_t)unit * (HALF ? V : N * V);
         const T *x = (const T *)a.x + b * a.xb + t * a.xt + from * a.xh + at;
         T *y = (T *)a.y + b * a.yb + t * a.yt + from * a.yh + at;
-        W c[PAIRS], s[PAIRS];
+        Pair<W> c[(PAIRS + 1) / 2], s[(PAIRS + 1) / 2];
         if (!copied) {
             const size_t where = b * a.pb + t;
             const int64_t position = a.positions == nullptr ? a.first_position + (int64_t)t
@@ -82,8 +108,11 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
             for (int j = 0; j < PAIRS; ++j) {
                 const uint32_t pair = unit * PAIRS + j;
-                rotor<W>(position, plan.turns[pair], plan.turns_low[pair], (W)plan.amplitude, c[j], s[j]);
-                if (backward) s[j] = -s[j];
+                W cosine, sine;
+                rotor<W>(position, plan.turns[pair], plan.turns_low[pair], (W)plan.amplitude, cosine, sine);
+                if (backward) sine = -sine;
+                (j & 1 ? c[j / 2].y : c[j / 2].x) = cosine;
+                (j & 1 ? s[j / 2].y : s[j / 2].x) = sine;
             }
         }
         for (size_t h = 0; h < heads; h += kHeads) {
@@ -97,15 +126,7 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
             for (int k = 0; k < kHeads; ++k)
                 if (h + k < heads) {
-                    if (!copied) {
-#pragma unroll
-                        for (int j = 0; j < PAIRS; ++j) {
-                            T &p = v[k][0].v[SPLIT ? j : 2 * j];
-                            T &q = v[k][N - 1].v[SPLIT ? j : 2 * j + 1];
-                            const W u = widen(p), w = widen(q);
-                            narrow_pair<T>({u * c[j] - w * s[j], u * s[j] + w * c[j]}, p, q);
-                        }
-                    }
+                    if (!copied) turn<T, V, SPLIT>(v[k][0], v[k][N - 1], c, s);
                     store<T, V>(y + (h + k) * a.yh, v[k][0]);
                     if (SPLIT && !copied) store<T, V>(y + (h + k) * a.yh + second, v[k][N - 1]);
                 }
