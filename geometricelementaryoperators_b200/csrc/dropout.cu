@@ -65,7 +65,15 @@ __global__ void __launch_bounds__(kThreads) drop_vectors_kernel(const Rows a, co
         }
 #pragma unroll
     for (int m = 0; m < kChunks; ++m) {
-        const uint32_t mine = kept_of_eight(drop, offset, (warp * kChunks + m) * 256 + lane * 8);
+        // 16-bit values: the eight of the vector. Wider ones: a block's decisions, handed round.
+        uint32_t draws[4] = {}, mine = 0xFFu;
+        if (drop.threshold != 0) {
+            const size_t eight = (warp * kChunks + m) * 256 + lane * 8;
+            if constexpr (R == 1)
+                draws_of_pairs<8>(drop, offset, eight, draws);
+            else
+                mine = kept_of_eight(drop, offset, eight);
+        }
 #pragma unroll
         for (int i = 0; i < R; ++i) {
             const size_t e = value(m, i);
@@ -75,8 +83,12 @@ __global__ void __launch_bounds__(kThreads) drop_vectors_kernel(const Rows a, co
 #pragma unroll
             for (int q = 0; q < V / 2; ++q) {
                 Pair<W> v = x[m][i].pair(q);
-                v.x = (kept >> (2 * q)) & 1 ? v.x : W(0);  // selected, not multiplied: a dropped NaN is gone
-                v.y = (kept >> (2 * q + 1)) & 1 ? v.y : W(0);
+                if constexpr (R == 1) {
+                    if (drop.threshold != 0) v = drop_pair(v, draws[q], drop.bound);
+                } else {
+                    v.x = (kept >> (2 * q)) & 1 ? v.x : W(0);
+                    v.y = (kept >> (2 * q + 1)) & 1 ? v.y : W(0);
+                }
                 if constexpr (RESIDUAL)
                     v = fma(v, both(scale), res[m][i].pair(q));
                 else
@@ -90,8 +102,8 @@ __global__ void __launch_bounds__(kThreads) drop_vectors_kernel(const Rows a, co
                 } else {  // the last values of all, one by one
                     for (int j = 0; e + j < count; ++j) {
                         const W residual = RESIDUAL ? (W)widen(((const T *)a.residual)[e + j]) : W(0);
-                        ((T *)a.y)[e + j] =
-                            narrow<T>(drop_value<T>((kept >> j) & 1, ((const T *)a.x)[e + j], scale, residual));
+                        const bool live = drop.threshold == 0 || unit_kept(drop, offset, (e + j) >> drop.shift);
+                        ((T *)a.y)[e + j] = narrow<T>(drop_value<T>(live, ((const T *)a.x)[e + j], scale, residual));
                     }
                 }
             } else {

@@ -1,0 +1,346 @@
+// layer_norm_vjp.cu -- VJPs of layer norm, alone and behind residual + dropout
+// (geo/geo_b200.h section 5); entry points in layer_norm.cu.
+//
+// With xh = (x - m) rstd and g = y_bar w (means over the row):
+//   x_bar = rstd (g - mean(g) - xh mean(g xh)),
+//   w_bar = sum_rows y_bar xh, b_bar = sum_rows y_bar.
+#include "layer_norm.h"
+
+#include "geo_runtime.h"
+
+namespace geo {
+namespace layers {
+
+namespace {
+
+// One pass over x and y_bar (and z_bar): x_bar row by row, and the column sums
+// of y_bar xh and y_bar in the registers of the thread that owns the column; at
+// the end partial[team][0: weight, 1: bias][col] (teams that are parts of a warp:
+// one partial for their block).
+template <typename T, int V, int K, bool DROP, int TEAM, bool FULL>
+__global__ void __launch_bounds__(TEAM == kWarp ? kWarpBlock : kTeamThreads, TEAM == kWarp ? 4 : 2)
+    vjp_kernel(const BackwardArgs a, int lanes, bool float_parameters, int stages, Wide<T> *partial) {
+    using W = Wide<T>;
+    constexpr int Q = K * V / 2;
+    constexpr int kColumns = TEAM == kWarp ? 32 * K * V : 1;
+    extern __shared__ __align__(16) unsigned char memory[];
+    __shared__ W sums[2][kSums<TEAM>][2];
+    __shared__ W columns[2][kColumns];
+    const Place<TEAM> at(lanes);
+    const bool has_dz = DROP && a.dz != nullptr;
+    Ring<T, V, K, TEAM, FULL> ring(memory, stages, has_dz ? 3 : 2, at, a.rows, a.cols);
+    auto next = [&] {
+        ring.copy(0, a.x, a.x_stride);
+        ring.copy(1, a.dy, a.dy_stride);
+        if constexpr (DROP)
+            if (has_dz) ring.copy(2, a.dz, a.dz_stride);
+        ring.fetched();
+    };
+    for (int s = 0; s < stages - 1; ++s) next();
+
+    const uint64_t offset = DROP ? drop_offset(a.drop) : 0;
+    const W scale = (W)a.drop.scale, over = W(1) / (W)a.cols;
+    Pair<W> w[Q], dw[Q], db[Q];
+    load_parameters<T, V, K * V>(a.weight, float_parameters, 0, at.lane, at.threads, a.cols, W(1), w);
+#pragma unroll
+    for (int q = 0; q < Q; ++q) dw[q] = db[q] = both(W(0));
+    const int joiner = at.wlane & (kJoiners<TEAM> - 1), entries = at.ranks * at.warps;
+
+    W next_mean = 0, next_rstd = 0;
+    if (at.begin + at.within < a.rows) {
+        next_mean = ((const W *)a.mean)[at.begin + at.within];
+        next_rstd = ((const W *)a.rstd)[at.begin + at.within];
+    }
+    if constexpr (TEAM == kCluster) cooperative_groups::this_cluster().sync();  // every block runs before it is written to
+    int flip = 0;
+    for (size_t first = at.begin; first < a.rows; first += at.step, flip ^= 1) {
+        const size_t row = first + at.within;
+        const bool live = TEAM != kWarp || row < a.rows;
+        // A row past the last one (kWarp) is zeros with mean and rstd zero: it adds nothing.
+        const W mean = next_mean, rstd = next_rstd;
+        next_mean = next_rstd = 0;
+        if (row + at.step < a.rows) {
+            next_mean = ((const W *)a.mean)[row + at.step];
+            next_rstd = ((const W *)a.rstd)[row + at.step];
+        }
+        next();
+        ring.wait();
+        const size_t r = live ? row : 0;
+        Vec<T, V> x[K], dy[K];
+        ring.get(x, 0, (const T *)a.x + r * a.x_stride);
+        ring.get(dy, 1, (const T *)a.dy + r * a.dy_stride);
+        Pair<W> sum2 = both(W(0)), along2 = both(W(0));
+#pragma unroll
+        for (int q = 0; q < Q; ++q) {
+            const Pair<W> d = pair_at(dy, q), xh = (pair_at(x, q) + both(-mean)) * both(rstd), g = d * w[q];
+            sum2 = sum2 + g;
+            along2 = fma(g, xh, along2);
+            dw[q] = fma(d, xh, dw[q]);
+            db[q] = db[q] + d;
+        }
+        W sum = team_sum(sum2.x + sum2.y, TEAM == kWarp ? at.threads : 32);
+        W along = team_sum(along2.x + along2.y, TEAM == kWarp ? at.threads : 32);
+        if constexpr (TEAM != kWarp) {
+            publish<W, TEAM>(sums[flip], at, sum, along);
+            sum = joiner < entries ? sums[flip][joiner][0] : W(0);
+            along = joiner < entries ? sums[flip][joiner][1] : W(0);
+            if (TEAM == kCluster && joiner + 32 < entries) {
+                sum += sums[flip][joiner + 32][0];
+                along += sums[flip][joiner + 32][1];
+            }
+            sum = team_sum(sum, kJoiners<TEAM>);
+            along = team_sum(along, kJoiners<TEAM>);
+            // Read again rather than held over the barrier: registers.
+            ring.get(x, 0, (const T *)a.x + r * a.x_stride);
+            ring.get(dy, 1, (const T *)a.dy + r * a.dy_stride);
+        }
+        sum *= over;
+        along *= over;
+        Pair<W> v[Q];
+#pragma unroll
+        for (int q = 0; q < Q; ++q) {
+            const Pair<W> xh = (pair_at(x, q) + both(-mean)) * both(rstd);
+            v[q] = (fma(xh, both(-along), pair_at(dy, q) * w[q]) + both(-sum)) * both(rstd);
+        }
+        if constexpr (DROP)
+            if (has_dz) {
+                ring.get(x, 2, (const T *)a.dz + r * a.dz_stride);
+#pragma unroll
+                for (int q = 0; q < Q; ++q) v[q] = v[q] + pair_at(x, q);
+            }
+        ring.done();
+        if (a.dsum != nullptr) {
+#pragma unroll
+            for (int q = 0; q < Q; ++q) set_pair(x, q, v[q]);
+            T *to = (T *)a.dsum + row * a.dsum_stride;
+#pragma unroll
+            for (int i = 0; i < K; ++i) {
+                const int c = (at.lane + i * at.threads) * V;
+                if (live && (FULL || c < a.cols)) store<T, V>(to + c, x[i]);
+            }
+        }
+        if constexpr (DROP) {
+            if (a.dx != nullptr) {
+                drop_row<T, V, K, FULL>(a.drop, offset, row * (size_t)a.cols, at.lane, at.threads, a.cols, v);
+#pragma unroll
+                for (int q = 0; q < Q; ++q) set_pair(x, q, v[q] * both(scale));
+                T *to = (T *)a.dx + row * a.dx_stride;
+#pragma unroll
+                for (int i = 0; i < K; ++i) {
+                    const int c = (at.lane + i * at.threads) * V;
+                    if (live && (FULL || c < a.cols)) store<T, V>(to + c, x[i]);
+                }
+            }
+        }
+    }
+    if (partial == nullptr) return;
+    W *mine = partial + at.team * 2 * a.cols;
+    auto value = [&](const Pair<W> (&p)[Q], int e) { return e & 1 ? p[e / 2].y : p[e / 2].x; };
+    if constexpr (TEAM != kWarp) {
+#pragma unroll
+        for (int e = 0; e < K * V; ++e) {
+            const int c = (at.lane + e / V * at.threads) * V + e % V;
+            if (c < a.cols) {
+                mine[c] = value(dw, e);
+                mine[a.cols + c] = value(db, e);
+            }
+        }
+    } else {
+        // The block's teams in order.
+        for (int team = 0; team < (int)at.teams; ++team) {
+            if ((int)threadIdx.x / lanes == team)
+#pragma unroll
+                for (int e = 0; e < K * V; ++e) {
+                    const int c = (at.lane + e / V * at.threads) * V + e % V;
+                    columns[0][c] = value(dw, e) + (team > 0 ? columns[0][c] : W(0));
+                    columns[1][c] = value(db, e) + (team > 0 ? columns[1][c] : W(0));
+                }
+            __syncthreads();
+        }
+        for (int c = threadIdx.x; c < a.cols; c += kWarpBlock) {
+            mine[c] = columns[0][c];
+            mine[a.cols + c] = columns[1][c];
+        }
+    }
+}
+
+// out[c] = sum over the blocks of partial[block][which][c]. `wide` columns a
+// block of threads, 1024 / wide threads a column, each over every so many
+// blocks in order, then those in order.
+template <typename W, typename P>
+__global__ void __launch_bounds__(1024) join_columns_kernel(const W *partial, int blocks, int cols, int wide,
+                                                            void *dweight, void *dbias) {
+    __shared__ W sums[1024];
+    P *out = (P *)(blockIdx.y == 0 ? dweight : dbias);
+    if (out == nullptr) return;
+    const int column = threadIdx.x & (wide - 1), part = threadIdx.x / wide, parts = 1024 / wide;
+    const int c = (int)blockIdx.x * wide + column;
+    W sum = 0;
+    if (c < cols) {
+#pragma unroll 8
+        for (int i = part; i < blocks; i += parts) sum += partial[((size_t)i * 2 + blockIdx.y) * cols + c];
+    }
+    sums[threadIdx.x] = sum;
+    for (int n = parts / 2; n > 0; n /= 2) {
+        __syncthreads();
+        if (part < n) sums[threadIdx.x] += sums[threadIdx.x + n * wide];
+    }
+    if (part == 0 && c < cols) out[c] = narrow<P>((Wide<P>)sums[threadIdx.x]);
+}
+
+
+// ---- rows of any length --------------------------------------------------------
+
+// x_bar of one row per CTA, two sweeps.
+template <typename T, typename P, bool DROP>
+__global__ void __launch_bounds__(kThreads) vjp_rows_any_kernel(const BackwardArgs a) {
+    using W = Wide<T>;
+    __shared__ W scratch[kThreads / 32];
+    const uint64_t offset = DROP ? drop_offset(a.drop) : 0;
+    const W scale = (W)a.drop.scale;
+    for (size_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const T *x = (const T *)a.x + row * a.x_stride;
+        const T *dy = (const T *)a.dy + row * a.dy_stride;
+        const T *dz = DROP && a.dz != nullptr ? (const T *)a.dz + row * a.dz_stride : nullptr;
+        T *dsum = a.dsum != nullptr ? (T *)a.dsum + row * a.dsum_stride : nullptr;
+        T *dx = DROP && a.dx != nullptr ? (T *)a.dx + row * a.dx_stride : nullptr;
+        const W mean = ((const W *)a.mean)[row], rstd = ((const W *)a.rstd)[row];
+        auto scaled = [&](int c) -> W {
+            const W v = widen(dy[c]);
+            return a.weight != nullptr ? v * (W)widen(((const P *)a.weight)[c]) : v;
+        };
+        W sum = 0, along = 0;
+        for (int c = threadIdx.x; c < a.cols; c += kThreads) {
+            const W g = scaled(c);
+            sum += g;
+            along += g * ((widen(x[c]) - mean) * rstd);
+        }
+        sum = block_sum(sum, scratch) / (W)a.cols;
+        along = block_sum(along, scratch) / (W)a.cols;
+        for (int c = threadIdx.x; c < a.cols; c += kThreads) {
+            W v = rstd * (scaled(c) - sum - (widen(x[c]) - mean) * rstd * along);
+            if (dz != nullptr) v += widen(dz[c]);
+            if (dx != nullptr) {
+                const bool kept =
+                    a.drop.threshold == 0 || unit_kept(a.drop, offset, (row * (size_t)a.cols + c) >> a.drop.shift);
+                dx[c] = narrow<T>(kept ? v * scale : W(0));
+            }
+            if (dsum != nullptr) dsum[c] = narrow<T>(v);
+        }
+    }
+}
+
+// Partial sums over rows [first, last) of block column range blockIdx.x:
+// partial[blockIdx.y][0: weight, 1: bias][col].
+template <typename T>
+__global__ void __launch_bounds__(kThreads) vjp_columns_any_kernel(const BackwardArgs a, Wide<T> *partial,
+                                                                   size_t rows_per_block) {
+    using W = Wide<T>;
+    __shared__ W sums[2][8][33];
+    const int lane = threadIdx.x & 31, group = threadIdx.x >> 5;
+    const int c = (int)blockIdx.x * 32 + lane;
+    const size_t first = blockIdx.y * rows_per_block;
+    const size_t last = first + rows_per_block < a.rows ? first + rows_per_block : a.rows;
+    W dw = 0, db = 0;
+    if (c < a.cols)
+        for (size_t row = first + group; row < last; row += 8) {
+            const W v = widen(((const T *)a.dy)[row * a.dy_stride + c]);
+            const W xh = (widen(((const T *)a.x)[row * a.x_stride + c]) - ((const W *)a.mean)[row]) *
+                         ((const W *)a.rstd)[row];
+            dw += v * xh;
+            db += v;
+        }
+    sums[0][group][lane] = dw;
+    sums[1][group][lane] = db;
+    __syncthreads();
+    if (group < 2 && c < a.cols) {
+        W total = 0;
+        for (int i = 0; i < 8; ++i) total += sums[group][i][lane];
+        partial[((size_t)blockIdx.y * 2 + group) * a.cols + c] = total;
+    }
+}
+
+// Row blocks of the column sums: enough for four CTAs per SM, at least 64 rows each.
+size_t column_blocks(size_t rows, size_t cols) {
+    const size_t wide = (cols + 31) / 32, want = ((size_t)geo::device_sm_count() * 4 + wide - 1) / wide;
+    const size_t most = (rows + 63) / 64;
+    return want < most ? want : most;
+}
+
+// Teams (blocks of teams, kWarp) of the pass: as many as 512 threads a
+// multiprocessor make, each with a partial sum of the columns.
+size_t team_grid(const Shape &s, size_t rows) {
+    const size_t wanted = (rows + s.teams() - 1) / s.teams();
+    const size_t most = (size_t)geo::device_sm_count() * (512 / s.threads()) / s.blocks;
+    return wanted < most ? wanted : most;
+}
+
+template <bool DROP>
+cudaError_t launch(NormTypes n, const BackwardArgs &a, void *workspace, cudaStream_t stream) {
+    const bool sums = a.dweight != nullptr || a.dbias != nullptr;
+    const size_t bytes = type_bytes(n.type);
+    const bool aligned = aligned16(a.cols, bytes, type_bytes(n.parameter_type),
+                                   {{a.x, a.x_stride}, {a.dy, a.dy_stride}, {a.dz, a.dz_stride},
+                                    {a.dsum, a.dsum_stride}, {a.dx, a.dx_stride}},
+                                   {a.weight});
+    const Shape s = shape_of(a.cols, bytes, aligned);
+    const bool float_parameters = n.parameter_type == GEO_B200_F32;
+    return by_types(n, [&](auto t, auto p) {
+        using T = decltype(t);
+        using P = decltype(p);
+        using W = Wide<T>;
+        size_t blocks = 0;
+        cudaError_t e = cudaSuccess;
+        if (s.lanes != 0) {
+            blocks = team_grid(s, a.rows);
+            W *partial = sums ? (W *)workspace : nullptr;
+            e = by_shape<T>(s, [&](auto v, auto k, auto team, auto full) {
+                constexpr int V = decltype(v)::value, K = decltype(k)::value;
+                const size_t stage = (size_t)(a.dz != nullptr ? 3 : 2) * K * s.threads() * kSlot<T, V>;
+                const int stages = ring_stages(stage, s.threads(), 512);
+                return launch_team(vjp_kernel<T, V, K, DROP, decltype(team)::value, decltype(full)::value>, s, blocks,
+                                   stages * stage, stream, a, s.lanes, float_parameters, stages, partial);
+            });
+        } else {
+            // Columns first: the row kernel may overwrite x or y_bar.
+            if (sums) {
+                blocks = column_blocks(a.rows, a.cols);
+                const dim3 grid((unsigned)((a.cols + 31) / 32), (unsigned)blocks);
+                vjp_columns_any_kernel<T>
+                    <<<grid, kThreads, 0, stream>>>(a, (W *)workspace, (a.rows + blocks - 1) / blocks);
+            }
+            const unsigned grid = (unsigned)(a.rows < (1u << 20) ? a.rows : (1u << 20));
+            if (a.dsum != nullptr || a.dx != nullptr)
+                vjp_rows_any_kernel<T, P, DROP><<<grid, kThreads, 0, stream>>>(a);
+            e = cudaGetLastError();
+        }
+        if (e != cudaSuccess || !sums) return e;
+        const int wide = a.cols >= 2048 ? 32 : 8;
+        const dim3 join((unsigned)((a.cols + wide - 1) / wide), 2);
+        join_columns_kernel<W, P><<<join, 1024, 0, stream>>>((const W *)workspace, (int)blocks, a.cols, wide,
+                                                             a.dweight, a.dbias);
+        return cudaGetLastError();
+    });
+}
+
+}  // namespace
+
+// Enough for whatever alignment the arrays turn out to have.
+size_t vjp_workspace(NormTypes t, size_t rows, size_t cols) {
+    const size_t bytes = type_bytes(t.type);
+    size_t blocks = 0;
+    for (const bool aligned : {false, true}) {
+        if (aligned && cols * bytes % 16 != 0) continue;
+        const Shape s = shape_of(cols, bytes, aligned);
+        const size_t n = s.lanes != 0 ? team_grid(s, rows) : column_blocks(rows, cols);
+        if (n > blocks) blocks = n;
+    }
+    return blocks * 2 * cols * wide_bytes(t.type);
+}
+
+cudaError_t launch_norm_vjp(NormTypes t, const BackwardArgs &a, bool drop, void *partial, cudaStream_t stream) {
+    return drop ? launch<true>(t, a, partial, stream) : launch<false>(t, a, partial, stream);
+}
+
+}  // namespace layers
+}  // namespace geo

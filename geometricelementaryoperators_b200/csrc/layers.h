@@ -299,10 +299,34 @@ __device__ __forceinline__ uint32_t kept_of_eight(const Drop &drop, uint64_t off
     return out;
 }
 
-// The same of V values, V = 2, 4 or 8 dividing e.
+// Words whose low and high halves are the draws of values e + 2q and e + 2q + 1,
+// V = 2, 4 or 8 values, V dividing e.
 template <int V>
-__device__ __forceinline__ uint32_t kept_values(const Drop &drop, uint64_t offset, uint64_t e) {
-    return kept_of_eight(drop, offset, e & ~(uint64_t)7) >> ((uint32_t)e & 7u);
+__device__ __forceinline__ void draws_of_pairs(const Drop &drop, uint64_t offset, uint64_t e, uint32_t (&out)[V / 2]) {
+    const uint64_t unit = e >> drop.shift;
+    const Block b = philox(unit >> 3, offset, drop.seed);
+    if (drop.shift == 0) {
+#pragma unroll
+        for (int q = 0; q < V / 2; ++q) {
+            out[q] = b.word[q];
+            if (V == 4) out[q] = (e & 4) ? b.word[q + 2] : out[q];
+            if (V == 2) out[q] = (e & 4) ? ((e & 2) ? b.word[3] : b.word[2]) : ((e & 2) ? b.word[1] : b.word[0]);
+        }
+    } else {  // both values of a pair are of one unit
+#pragma unroll
+        for (int q = 0; q < V / 2; ++q) {
+            const uint32_t i = (uint32_t)unit + (2u * q >> drop.shift);
+            const uint32_t w = (i & 4) ? ((i & 2) ? b.word[3] : b.word[2]) : ((i & 2) ? b.word[1] : b.word[0]);
+            out[q] = __byte_perm(w, 0, (i & 1) ? 0x3232 : 0x1010);
+        }
+    }
+}
+
+// Zero where the draw is below the threshold (threshold > 0): selected, not
+// multiplied, so that a dropped NaN is gone.
+template <typename W>
+__device__ __forceinline__ Pair<W> drop_pair(Pair<W> v, uint32_t draws, uint32_t bound) {
+    return {(draws << 16) > bound ? v.x : W(0), draws > bound ? v.y : W(0)};
 }
 
 // Rows that are not made of whole vectors: bit i of the result is whether value
