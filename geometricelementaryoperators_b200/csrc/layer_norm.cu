@@ -43,140 +43,159 @@ bool aligned16(size_t cols, size_t bytes, size_t parameter_bytes, std::initializ
 
 namespace {
 
+// Threads that a multiprocessor holds: 80 registers a thread, 128 where two
+// rows, or single values, are held at a time.
+constexpr int resident_threads(size_t bytes, int vector, int team) {
+    return vector == 1 || rows_at_once(bytes, vector, team) == 2 ? 512 : 768;
+}
+
 template <typename T, int V, int K, bool DROP, int TEAM, bool FULL>
 __global__ void __launch_bounds__(TEAM == kWarp ? kWarpBlock : kTeamThreads,
-                                  (V == 1 ? 512 : 768) / (TEAM == kWarp ? kWarpBlock : kTeamThreads))
+                                  resident_threads(sizeof(T), V, TEAM) / (TEAM == kWarp ? kWarpBlock : kTeamThreads))
     norm_kernel(const ForwardArgs a, int lanes, bool float_parameters, int stages) {
     using W = Wide<T>;
-    constexpr int Q = K * V / 2;
+    constexpr int Q = K * V / 2, R = rows_at_once(sizeof(T), V, TEAM);
     extern __shared__ __align__(16) unsigned char memory[];
-    __shared__ W sums[2][kSums<TEAM>][2];
-    const Place<TEAM> at(lanes);
-    Ring<T, V, K, TEAM, FULL> ring(memory, stages, DROP ? 2 : 1, at, a.rows, a.cols);
+    __shared__ W sums[2][2 * R][kSums<TEAM>];
+    const Place<TEAM, V, K> at(lanes);
+    Ring<T, V, K, TEAM, FULL, R> ring(memory, stages, DROP ? 2 : 1, at, a.rows, a.cols);
     auto next = [&] {
         ring.copy(0, a.x, a.x_stride);
         if constexpr (DROP) ring.copy(1, a.residual, a.residual_stride);
         ring.fetched();
     };
-    for (int s = 0; s < stages - 1; ++s) next();
+    for (int s = 0; s < stages - R; ++s) next();
 
     const uint64_t offset = DROP ? drop_offset(a.drop) : 0;
     const W scale = (W)a.drop.scale, over = W(1) / (W)a.cols;
     Pair<W> w[Q], b[Q];
-    load_parameters<T, V, K * V>(a.weight, float_parameters, 0, at.lane, at.threads, a.cols, W(1), w);
-    load_parameters<T, V, K * V>(a.bias, float_parameters, 0, at.lane, at.threads, a.cols, W(0), b);
+    load_parameters<T, V, K>(a.weight, float_parameters, at.first, at.gap, a.cols, W(1), w);
+    load_parameters<T, V, K>(a.bias, float_parameters, at.first, at.gap, a.cols, W(0), b);
 
     // How many values of the row warp `n` of the team holds.
     auto held_by = [&](int n) {
-        if (n >= at.ranks * at.warps) return W(0);
-        int held = 0;
-#pragma unroll
-        for (int i = 0; i < K; ++i) {
-            const int left = a.cols / V - (n * 32 + i * at.threads);
-            held += left < 0 ? 0 : (left < 32 ? left : 32);
-        }
-        return (W)(held * V);
+        if (FULL) return (W)(32 * K * V);
+        const int left = a.cols - n * (32 * K * V);
+        return (W)(left < 0 ? 0 : (left < 32 * K * V ? left : 32 * K * V));
     };
-    const int joiner = at.wlane & (kJoiners<TEAM> - 1);
-    W held = (W)a.cols, joined[2] = {}, over_held = 0, over_joined[2] = {};
-    if constexpr (TEAM != kWarp) {
-        held = held_by(at.rank * at.warps + at.warp);
-        over_held = held > W(0) ? W(1) / held : W(0);
+    // The team's warps are joined by 8 lanes a row in a block, 32 / R in a cluster, each over every so many warps.
+    constexpr int kJoin = TEAM == kCluster ? 32 / R : 8, kEach = TEAM == kCluster ? 64 / kJoin : 1;
+    const int joiner = at.wlane % kJoin, joined_row = at.wlane / kJoin % R;
+    const W held = TEAM == kWarp ? (W)a.cols : held_by(at.warp);
+    const W over_held = held > W(0) ? W(1) / held : W(0);
+    W joined[kEach], over_joined[kEach];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            joined[j] = TEAM == kCluster || j == 0 ? held_by(joiner + 32 * j) : W(0);
-            over_joined[j] = joined[j] > W(0) ? W(1) / joined[j] : W(0);
-        }
+    for (int j = 0; j < kEach; ++j) {
+        joined[j] = joiner + j * kJoin < at.entries ? held_by(joiner + j * kJoin) : W(0);
+        over_joined[j] = joined[j] > W(0) ? W(1) / joined[j] : W(0);
     }
     if constexpr (TEAM == kCluster) cooperative_groups::this_cluster().sync();  // every block runs before it is written to
 
     int flip = 0;
-    for (size_t first = at.begin; first < a.rows; first += at.step, flip ^= 1) {
-        const size_t row = first + at.within;
-        const bool live = TEAM != kWarp || row < a.rows;
-        next();
+    for (size_t first = at.begin; first < a.rows; first += R * at.step, flip ^= 1) {
+        for (int u = 0; u < R; ++u) next();
         ring.wait();
-        Pair<W> v[Q];
-        {
+        Pair<W> v[R][Q];
+        W sum[R], mean[R], squares[R];
+#pragma unroll
+        for (int u = 0; u < R; ++u) {
+            const size_t row = first + at.within + u * at.step, r = row < a.rows ? row : 0;
             Vec<T, V> raw[K];
-            const size_t r = live ? row : 0;
-            ring.get(raw, 0, (const T *)a.x + r * a.x_stride);
+            ring.get(raw, u, 0, (const T *)a.x + r * a.x_stride);
 #pragma unroll
-            for (int q = 0; q < Q; ++q) v[q] = pair_at(raw, q);
+            for (int q = 0; q < Q; ++q) v[u][q] = pair_at(raw, q);
             if constexpr (DROP) {
-                drop_row<T, V, K, FULL>(a.drop, offset, row * (size_t)a.cols, at.lane, at.threads, a.cols, v);
-                ring.get(raw, 1, (const T *)a.residual + r * a.residual_stride);
+                drop_row<T, V, K, FULL>(a.drop, offset, row * (size_t)a.cols, at, a.cols, v[u]);
+                ring.get(raw, u, 1, (const T *)a.residual + r * a.residual_stride);
 #pragma unroll
-                for (int q = 0; q < Q; ++q) v[q] = fma(v[q], both(scale), pair_at(raw, q));
+                for (int q = 0; q < Q; ++q) v[u][q] = fma(v[u][q], both(scale), pair_at(raw, q));
             }
-            ring.done();
+            Pair<W> two = both(W(0));
+#pragma unroll
+            for (int q = 0; q < Q; ++q) two = two + v[u][q];
+            sum[u] = two.x + two.y;
         }
+        ring.done();
         // Two sweeps over registers: the mean of what the warp (or its team)
         // holds, then the squares about it. Values past the row are 0 in the
         // first, the mean itself in the second.
-        Pair<W> two = both(W(0));
+        if constexpr (R == 2) {
+            sum[0] = folded_sums(sum);  // rows in halves of the warp
+            mean[0] = __shfl_sync(0xffffffffu, sum[0], 0) * over_held;
+            mean[1] = __shfl_sync(0xffffffffu, sum[0], 16) * over_held;
+        } else {
+            sum[0] = team_sum(sum[0], TEAM == kWarp ? at.threads : 32);
+            mean[0] = TEAM == kWarp ? sum[0] / held : sum[0] * over_held;
+        }
 #pragma unroll
-        for (int q = 0; q < Q; ++q) two = two + v[q];
-        const W sum = team_sum(two.x + two.y, TEAM == kWarp ? at.threads : 32);
-        W mean = TEAM == kWarp ? sum / held : sum * over_held;
-        if constexpr (!FULL) {
+        for (int u = 0; u < R; ++u) {
+            if constexpr (!FULL) {
 #pragma unroll
-            for (int i = 0; i < K; ++i) {
-                if ((at.lane + i * at.threads) * V < a.cols) continue;
-                if constexpr (V == 1) {
-                    (i & 1 ? v[i / 2].y : v[i / 2].x) = mean;
-                } else {
+                for (int i = 0; i < K; ++i) {
+                    if (at.column(i) < a.cols) continue;
+                    if constexpr (V == 1) {
+                        (i & 1 ? v[u][i / 2].y : v[u][i / 2].x) = mean[u];
+                    } else {
 #pragma unroll
-                    for (int q = i * V / 2; q < (i + 1) * V / 2; ++q) v[q] = both(mean);
+                        for (int q = i * V / 2; q < (i + 1) * V / 2; ++q) v[u][q] = both(mean[u]);
+                    }
                 }
             }
-        }
-        two = both(W(0));
+            Pair<W> two = both(W(0));
 #pragma unroll
-        for (int q = 0; q < Q; ++q) {
-            const Pair<W> d = v[q] + both(-mean);
-            two = fma(d, d, two);
+            for (int q = 0; q < Q; ++q) {
+                const Pair<W> d = v[u][q] + both(-mean[u]);
+                two = fma(d, d, two);
+            }
+            squares[u] = two.x + two.y;
         }
-        W squares = team_sum(two.x + two.y, TEAM == kWarp ? at.threads : 32);
-        if constexpr (TEAM != kWarp) {
+        W rstd[R];
+        if constexpr (TEAM == kWarp) {
+            rstd[0] = rsqrt(team_sum(squares[0], at.threads) * over + (W)a.epsilon);
+        } else {
+            squares[0] = R == 2 ? folded_sums(squares) : team_sum(squares[0], 32);
+            // sums[2 u]: sum of row u, sums[2 u + 1]: its squares.
+            publish<2 * R>(sums[flip], at, at.wlane / (16 / R) % 2 ? squares[0] : sum[0]);
             // Warps joined about the row's mean: squares + held (warp's mean - mean)^2.
-            publish<W, TEAM>(sums[flip], at, sum, squares);
-            W other[2] = {};
-            other[0] = joined[0] > W(0) ? sums[flip][joiner][0] : W(0);
-            if (TEAM == kCluster) other[1] = joined[1] > W(0) ? sums[flip][joiner + 32][0] : W(0);
+            W total = 0, other[kEach];
+#pragma unroll
+            for (int j = 0; j < kEach; ++j) {
+                other[j] = joined[j] > W(0) ? sums[flip][2 * joined_row][joiner + j * kJoin] : W(0);
+                total += other[j];
+            }
             // Divided, so that a row of one value has no spread.
-            mean = team_sum(other[0] + other[1], kJoiners<TEAM>) / (W)a.cols;
-            squares = 0;
+            const W middle = team_sum(total, kJoin) / (W)a.cols;
+            W spread = 0;
 #pragma unroll
-            for (int j = 0; j < (TEAM == kCluster ? 2 : 1); ++j) {
-                const W d = other[j] * over_joined[j] - mean;
-                if (joined[j] > W(0)) squares += sums[flip][joiner + 32 * j][1] + joined[j] * d * d;
+            for (int j = 0; j < kEach; ++j) {
+                const W d = other[j] * over_joined[j] - middle;
+                if (joined[j] > W(0)) spread += sums[flip][2 * joined_row + 1][joiner + j * kJoin] + joined[j] * d * d;
             }
-            squares = team_sum(squares, kJoiners<TEAM>);
-        }
-        const W rstd = rsqrt(squares * over + (W)a.epsilon);
-        if (live && at.lane == 0) {
-            if (a.mean != nullptr) ((W *)a.mean)[row] = mean;
-            if (a.rstd != nullptr) ((W *)a.rstd)[row] = rstd;
-        }
-        Vec<T, V> out[K];
-        if constexpr (DROP) {
+            const W inverse = rsqrt(team_sum(spread, kJoin) * over + (W)a.epsilon);
 #pragma unroll
-            for (int q = 0; q < Q; ++q) set_pair(out, q, v[q]);
-            T *z = (T *)a.z + row * a.z_stride;
-#pragma unroll
-            for (int i = 0; i < K; ++i) {
-                const int c = (at.lane + i * at.threads) * V;
-                if (live && (FULL || c < a.cols)) store<T, V>(z + c, out[i]);
+            for (int u = 0; u < R; ++u) {
+                mean[u] = R == 1 ? middle : __shfl_sync(0xffffffffu, middle, u * kJoin);
+                rstd[u] = R == 1 ? inverse : __shfl_sync(0xffffffffu, inverse, u * kJoin);
             }
         }
 #pragma unroll
-        for (int q = 0; q < Q; ++q) set_pair(out, q, fma((v[q] + both(-mean)) * both(rstd), w[q], b[q]));
-        T *y = (T *)a.y + row * a.y_stride;
+        for (int u = 0; u < R; ++u) {
+            const size_t row = first + at.within + u * at.step;
+            const bool live = (TEAM != kWarp && u == 0) || row < a.rows;
+            if (live && at.lane == 0) {
+                if (a.mean != nullptr) ((W *)a.mean)[row] = mean[u];
+                if (a.rstd != nullptr) ((W *)a.rstd)[row] = rstd[u];
+            }
+            Vec<T, V> out[K];
+            if constexpr (DROP) {
 #pragma unroll
-        for (int i = 0; i < K; ++i) {
-            const int c = (at.lane + i * at.threads) * V;
-            if (live && (FULL || c < a.cols)) store<T, V>(y + c, out[i]);
+                for (int q = 0; q < Q; ++q) set_pair(out, q, v[u][q]);
+                store_row<T, V, K, FULL>((T *)a.z + row * a.z_stride, at, live, a.cols, out);
+            }
+#pragma unroll
+            for (int q = 0; q < Q; ++q)
+                set_pair(out, q, fma((v[u][q] + both(-mean[u])) * both(rstd[u]), w[q], b[q]));
+            store_row<T, V, K, FULL>((T *)a.y + row * a.y_stride, at, live, a.cols, out);
         }
     }
 }
@@ -247,9 +266,10 @@ cudaError_t launch(NormTypes n, const ForwardArgs &a, cudaStream_t stream) {
         using T = decltype(t);
         return by_shape<T>(s, [&](auto v, auto k, auto team, auto full) {
             constexpr int V = decltype(v)::value, K = decltype(k)::value;
-            constexpr int resident = V == 1 ? 512 : 768;  // threads a multiprocessor holds (registers)
+            constexpr int resident = resident_threads(sizeof(T), V, decltype(team)::value);
+            constexpr int at_once = rows_at_once(sizeof(T), V, decltype(team)::value);
             const size_t stage = (size_t)(DROP ? 2 : 1) * K * s.threads() * kSlot<T, V>;
-            const int stages = ring_stages(stage, s.threads(), resident);
+            const int stages = ring_stages(stage, at_once, s.threads(), resident);
             const size_t wanted = (a.rows + s.teams() - 1) / s.teams();
             const size_t most = (size_t)geo::device_sm_count() * (resident / s.threads()) / s.blocks;
             return launch_team(norm_kernel<T, V, K, DROP, decltype(team)::value, decltype(full)::value>, s,

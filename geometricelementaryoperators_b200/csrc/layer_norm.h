@@ -5,13 +5,17 @@
 // threads holds it: part of a warp (a power of two up to 32 lanes, several rows a
 // warp), a block of up to 256 threads, or a cluster of up to eight such blocks
 // that exchange their warps' sums through distributed shared memory. Thread
-// `lane` of the team holds the K vectors lane, lane + threads, ... of V values
-// (16 bytes, or single values where rows are not aligned), 16 values in all (8 in
+// `lane` of the team holds K vectors of V values
+// (16 bytes, or single values where rows are not aligned; a warp's vectors are
+// adjacent: lane, lane + 32, ... of its part), 16 values in all (8 in
 // float64), so that a column belongs to one thread: weight, bias and the column
 // sums of the backward pass stay in its registers over all its rows. Rows come
 // through a ring in shared memory filled by asynchronous copies, each thread
-// copying and waiting for its own vectors only (no barrier), one to three rows
-// ahead: with few warps (registers) that keeps enough bytes in flight.
+// copying and waiting for its own vectors only (no barrier), one to four rows
+// ahead: with few warps (registers) that keeps enough bytes in flight. What is
+// left to wait for is the sums' way across the team, so teams of several warps
+// take two rows of 16-bit values at a time: one barrier for both, two chains of
+// additions side by side.
 #pragma once
 
 #include <cooperative_groups.h>
@@ -72,12 +76,16 @@ struct RowArray {
 bool aligned16(size_t cols, size_t bytes, size_t parameter_bytes, std::initializer_list<RowArray> arrays,
                std::initializer_list<const void *> parameters);
 
-// Rows in the ring: four where the multiprocessor's shared memory holds them for
-// `resident` threads, at least two.
-inline int ring_stages(size_t stage_bytes, int threads, int resident) {
-    const size_t room = (size_t)220 * 1024 * threads / resident;
-    const size_t n = room / stage_bytes;
-    return n >= 4 ? 4 : (n >= 3 ? 3 : 2);
+// Rows that a team takes at a time.
+constexpr int rows_at_once(size_t bytes, int vector, int team) { return bytes == 2 && vector > 1 && team != kWarp ? 2 : 1; }
+
+// Rows in the ring: up to four beyond those being read, where the
+// multiprocessor's shared memory holds them for `resident` threads, at least as
+// many as are read at once.
+inline int ring_stages(size_t row_bytes, int at_once, int threads, int resident) {
+    const int most = at_once == 2 ? 6 : 4;
+    const int n = (int)((size_t)220 * 1024 * threads / resident / row_bytes) / at_once * at_once;
+    return n >= most ? most : (n > 2 * at_once ? n : 2 * at_once);
 }
 
 #ifdef __CUDACC__
@@ -107,16 +115,16 @@ __device__ __forceinline__ W team_sum(W v, int lanes) {
     return v;
 }
 
-// Pairs of weight or bias for values [first, first + G) of the thread, of the
-// value type or (16-bit values only) float32; `absent` past the row or without
-// the array. G: whole vectors, at least two values.
-template <typename T, int V, int G>
-__device__ __forceinline__ void load_parameters(const void *p, bool is_float, int first_vector, int lane, int threads,
-                                                int cols, Wide<T> absent, Pair<Wide<T>> (&out)[G / 2]) {
+// Pairs of weight or bias for the thread's values, which start at column `first`
+// and go on every `gap` columns, of the value type or (16-bit values only)
+// float32; `absent` past the row or without the array.
+template <typename T, int V, int K>
+__device__ __forceinline__ void load_parameters(const void *p, bool is_float, int first, int gap, int cols,
+                                                Wide<T> absent, Pair<Wide<T>> (&out)[K * V / 2]) {
     using W = Wide<T>;
 #pragma unroll
-    for (int i = 0; i < G / V; ++i) {
-        const int c = (lane + (first_vector + i) * threads) * V;
+    for (int i = 0; i < K; ++i) {
+        const int c = first + i * gap;
         const bool there = p != nullptr && c < cols;
         if constexpr (V == 1) {
             W v = absent;
@@ -213,121 +221,131 @@ __device__ __forceinline__ void fetch(uint32_t slot, const T *from, bool live, b
 }
 
 // Where this thread stands.
-template <int TEAM>
+template <int TEAM, int V, int K>
 struct Place {
-    int threads, lane, warp, wlane, rank, ranks, warps;
-    size_t teams, team, step, begin, within;  // rows begin + within, + step, ...: `begin` is the warp's
+    int threads, lane, warp, wlane, rank, ranks, entries;  // entries: warps of the team
+    int first, gap;                                        // its vectors' columns: first, first + gap, ...
+    size_t team, step, begin, within;  // rows begin + within, + step, ...: `begin` is the warp's
     __device__ __forceinline__ explicit Place(int lanes) {
         namespace cg = cooperative_groups;
         rank = TEAM == kCluster ? (int)cg::this_cluster().block_rank() : 0;
         ranks = TEAM == kCluster ? (int)cg::this_cluster().num_blocks() : 1;
         threads = TEAM == kWarp ? lanes : (int)blockDim.x * ranks;
         lane = TEAM == kWarp ? (int)threadIdx.x & (lanes - 1) : (int)threadIdx.x + rank * (int)blockDim.x;
-        warp = (int)threadIdx.x >> 5;
         wlane = (int)threadIdx.x & 31;
-        warps = (int)blockDim.x / 32;
-        teams = TEAM == kWarp ? kWarpBlock / lanes : 1;
+        warp = TEAM == kWarp ? (int)threadIdx.x >> 5 : lane >> 5;
+        entries = threads / 32;
+        first = (TEAM == kWarp ? lane : warp * 32 * K + wlane) * V;
+        gap = (TEAM == kWarp ? lanes : 32) * V;
+        const size_t teams = TEAM == kWarp ? kWarpBlock / lanes : 1;
         team = blockIdx.x / ranks;
         step = gridDim.x / ranks * teams;
         begin = team * teams + (TEAM == kWarp ? warp * (32 / lanes) : 0);
         within = TEAM == kWarp ? wlane / lanes : 0;
     }
+    __device__ __forceinline__ int column(int i) const { return first + i * (TEAM == kWarp ? gap : 32 * V); }
 };
 
 // The slots of one thread, for `arrays` arrays of rows.
-template <typename T, int V, int K, int TEAM, bool FULL>
+template <typename T, int V, int K, int TEAM, bool FULL, int R>
 struct Ring {
+    static constexpr uint32_t kVector = 32 * kSlot<T, V>;  // bytes between a thread's vectors: its warp's lie together
+    const Place<TEAM, V, K> &at;
     const unsigned char *slots;
-    uint32_t address, next_vector, next_array, next_stage;
-    int stages, read, write;
-    size_t row, step, rows;  // of the next row to fetch
-    int cols, lane, threads;
+    uint32_t next_array, next_stage;
+    int stages, read, write, cols;
+    size_t row, rows;  // row: the next to fetch
 
-    __device__ __forceinline__ Ring(unsigned char *memory, int stages, int arrays, const Place<TEAM> &at, size_t rows,
-                                    int cols)
-        : slots(memory + threadIdx.x * kSlot<T, V>), stages(stages), read(0), write(0), row(at.begin + at.within),
-          step(at.step), rows(rows), cols(cols), lane(at.lane), threads(at.threads) {
-        address = shared_address(slots);
-        next_vector = blockDim.x * kSlot<T, V>;
-        next_array = K * next_vector;
+    __device__ __forceinline__ Ring(unsigned char *memory, int stages, int arrays, const Place<TEAM, V, K> &at,
+                                    size_t rows, int cols)
+        : at(at), slots(memory + ((threadIdx.x >> 5) * (32 * K) + (threadIdx.x & 31)) * kSlot<T, V>), stages(stages),
+          read(0), write(0), cols(cols), row(at.begin + at.within), rows(rows) {
+        next_array = K * blockDim.x * kSlot<T, V>;
         next_stage = arrays * next_array;
     }
-    // Starts the copies of array `array` of the row to fetch, which begins at `start`.
+    // Starts the copies of array `array` of the row to fetch; zeros past the last row.
     __device__ __forceinline__ void copy(int array, const void *base, size_t stride) {
-        if (TEAM != kWarp && row >= rows) return;
-        const bool live = TEAM != kWarp || row < rows;
-        const T *start = (const T *)base + (live ? row : 0) * stride;
-        const uint32_t slot = address + write * next_stage + array * next_array;
+        const bool live = row < rows;
+        const T *start = (const T *)base + (live ? row : 0) * stride + at.first;
+        const uint32_t slot = shared_address(slots) + write * next_stage + array * next_array;
 #pragma unroll
         for (int i = 0; i < K; ++i) {
-            const int c = (lane + i * threads) * V;
+            const int c = at.column(i);
             const bool inside = live && (FULL || c < cols);
             const bool edge = kSlot<T, V> > (int)sizeof(T) * V && inside &&
                               ((row == 0 && c == 0) || (row == rows - 1 && c == cols - 1));
-            fetch<T, V>(slot + i * next_vector, FULL || inside ? start + c : (const T *)base, inside, edge);
+            fetch<T, V>(slot + i * kVector, FULL || inside ? start + (c - at.first) : (const T *)base, inside, edge);
         }
     }
     __device__ __forceinline__ void fetched() {
         commit_async();
-        row += step;
+        row += at.step;
         write = write == stages - 1 ? 0 : write + 1;
     }
-    // All but the newest stages - 1 rows have arrived.
+    // All but the newest stages - R rows have arrived.
     __device__ __forceinline__ void wait() const {
-        if (stages == 4)
-            wait_async<3>();
-        else if (stages == 3)
-            wait_async<2>();
-        else
-            wait_async<1>();
+        switch (stages - R) {
+            case 1: wait_async<1>(); break;
+            case 2: wait_async<2>(); break;
+            case 3: wait_async<3>(); break;
+            default: wait_async<4>(); break;
+        }
     }
-    // This thread's part of the row being read; row_start: where it lies in global memory.
-    __device__ __forceinline__ void get(Vec<T, V> (&out)[K], int array, const T *row_start) const {
-        const unsigned char *from = slots + read * next_stage + array * next_array;
-        // A thread's single 16-bit values are 32 n apart: all in the same half of their words.
-        from += word_offset<T, V>(row_start + lane);
+    // This thread's part of row u of those being read; row_start: where it lies in global memory.
+    __device__ __forceinline__ void get(Vec<T, V> (&out)[K], int u, int array, const T *row_start) const {
+        const unsigned char *from = slots + (read + u) * next_stage + array * next_array;
+        // A thread's single 16-bit values are 32 apart: all in the same half of their words.
+        from += word_offset<T, V>(row_start + at.first);
 #pragma unroll
-        for (int i = 0; i < K; ++i) out[i] = load<T, V>((const T *)(from + i * next_vector));
+        for (int i = 0; i < K; ++i) out[i] = load<T, V>((const T *)(from + i * kVector));
     }
-    __device__ __forceinline__ void done() { read = read == stages - 1 ? 0 : read + 1; }
+    __device__ __forceinline__ void done() { read = read == stages - R ? 0 : read + R; }
 };
 
-// Two sums of every warp of the team, where all its threads find them after the
-// barrier (of the block or the cluster) in here. Two buffers in turn, so that one
-// barrier a row is enough.
-template <typename W, int TEAM>
-__device__ __forceinline__ void publish(W (*sums)[2], const Place<TEAM> &at, W a, W b) {
+// One step of a sum that leaves two values in the two halves of 2 o lanes.
+template <typename W>
+__device__ __forceinline__ W fold(W low, W high, int o) {
+    const bool upper = threadIdx.x & o;
+    return (upper ? high : low) + __shfl_xor_sync(0xffffffffu, upper ? low : high, o);
+}
+
+// Warp sums of N = 2 or 4 values: lanes 32 / N n and on hold value n.
+template <typename W, int N>
+__device__ __forceinline__ W folded_sums(const W (&v)[N]) {
+    W s;
+    if constexpr (N == 4)
+        s = fold(fold(v[0], v[2], 16), fold(v[1], v[3], 16), 8);
+    else
+        s = fold(v[0], v[1], 16);
+    return team_sum(s, 32 / N);
+}
+
+// Every warp's N values, value n in lanes 32 / N n and on, to where all the
+// team's threads find them after the barrier (of the block or the cluster) in
+// here, sums[n][warp]. Two buffers in turn, so that one barrier is enough.
+template <int TEAM>
+constexpr int kSums = TEAM == kCluster ? 64 : (TEAM == kBlock ? 8 : 1);
+template <int N, typename W, int TEAM, int V, int K>
+__device__ __forceinline__ void publish(W (*sums)[kSums<TEAM>], const Place<TEAM, V, K> &at, W value) {
     namespace cg = cooperative_groups;
-    const int mine = at.rank * at.warps + at.warp;
+    const int n = at.wlane / (32 / N), sub = at.wlane % (32 / N);
     if constexpr (TEAM == kCluster) {
-        if (at.wlane < at.ranks) {
-            W *there = cg::this_cluster().map_shared_rank(&sums[mine][0], at.wlane);
-            there[0] = a;
-            there[1] = b;
-        }
+        if (sub < at.ranks) *cg::this_cluster().map_shared_rank(&sums[n][at.warp], sub) = value;
         cg::this_cluster().sync();
     } else {
-        if (at.wlane == 0) {
-            sums[mine][0] = a;
-            sums[mine][1] = b;
-        }
+        if (sub == 0) sums[n][at.warp] = value;
         __syncthreads();
     }
 }
-template <int TEAM>
-constexpr int kSums = TEAM == kCluster ? 64 : (TEAM == kBlock ? 8 : 1);
-// Lanes that add the published sums up: a block has at most eight, a cluster 64, two a lane.
-template <int TEAM>
-constexpr int kJoiners = TEAM == kCluster ? 32 : 8;
 
 // Zeroes the values that dropout drops.
-template <typename T, int V, int K, bool FULL>
-__device__ __forceinline__ void drop_row(const Drop &drop, uint64_t offset, uint64_t row_start, int lane, int threads,
-                                         int cols, Pair<Wide<T>> (&v)[K * V / 2]) {
+template <typename T, int V, int K, bool FULL, int TEAM>
+__device__ __forceinline__ void drop_row(const Drop &drop, uint64_t offset, uint64_t row_start,
+                                         const Place<TEAM, V, K> &at, int cols, Pair<Wide<T>> (&v)[K * V / 2]) {
     using W = Wide<T>;
     if (drop.threshold == 0) return;
     if constexpr (V == 1) {
-        const uint32_t kept = kept_by_warp<K>(drop, offset, row_start + (lane & ~31), (uint32_t)threads);
+        const uint32_t kept = kept_by_warp<K>(drop, offset, row_start + at.first - at.wlane, 32);
 #pragma unroll
         for (int q = 0; q < K / 2; ++q) {
             v[q].x = (kept >> (2 * q)) & 1 ? v[q].x : W(0);
@@ -336,14 +354,23 @@ __device__ __forceinline__ void drop_row(const Drop &drop, uint64_t offset, uint
     } else {
 #pragma unroll
         for (int i = 0; i < K; ++i) {
-            const int c = (lane + i * threads) * V;
-            if (!FULL && c >= cols) continue;
+            if (!FULL && at.column(i) >= cols) continue;
             uint32_t draws[V / 2];
-            draws_of_pairs<V>(drop, offset, row_start + c, draws);
+            draws_of_pairs<V>(drop, offset, row_start + at.column(i), draws);
 #pragma unroll
             for (int q = 0; q < V / 2; ++q) v[i * V / 2 + q] = drop_pair(v[i * V / 2 + q], draws[q], drop.bound);
         }
     }
+}
+
+// The thread's part of a row to global memory.
+template <typename T, int V, int K, bool FULL, int TEAM>
+__device__ __forceinline__ void store_row(T *row_start, const Place<TEAM, V, K> &at, bool live, int cols,
+                                          const Vec<T, V> (&v)[K]) {
+    T *to = row_start + at.first;
+#pragma unroll
+    for (int i = 0; i < K; ++i)
+        if (live && (FULL || at.column(i) < cols)) store<T, V>(to + (at.column(i) - at.first), v[i]);
 }
 
 // f(V, K, TEAM, FULL) of a shape as compile-time constants, as far as they occur.

@@ -21,14 +21,14 @@ template <typename T, int V, int K, bool DROP, int TEAM, bool FULL>
 __global__ void __launch_bounds__(TEAM == kWarp ? kWarpBlock : kTeamThreads, TEAM == kWarp ? 4 : 2)
     vjp_kernel(const BackwardArgs a, int lanes, bool float_parameters, int stages, Wide<T> *partial) {
     using W = Wide<T>;
-    constexpr int Q = K * V / 2;
+    constexpr int Q = K * V / 2, R = rows_at_once(sizeof(T), V, TEAM);
     constexpr int kColumns = TEAM == kWarp ? 32 * K * V : 1;
     extern __shared__ __align__(16) unsigned char memory[];
-    __shared__ W sums[2][kSums<TEAM>][2];
+    __shared__ W sums[2][2 * R][kSums<TEAM>];
     __shared__ W columns[2][kColumns];
-    const Place<TEAM> at(lanes);
+    const Place<TEAM, V, K> at(lanes);
     const bool has_dz = DROP && a.dz != nullptr;
-    Ring<T, V, K, TEAM, FULL> ring(memory, stages, has_dz ? 3 : 2, at, a.rows, a.cols);
+    Ring<T, V, K, TEAM, FULL, R> ring(memory, stages, has_dz ? 3 : 2, at, a.rows, a.cols);
     auto next = [&] {
         ring.copy(0, a.x, a.x_stride);
         ring.copy(1, a.dy, a.dy_stride);
@@ -36,102 +36,104 @@ __global__ void __launch_bounds__(TEAM == kWarp ? kWarpBlock : kTeamThreads, TEA
             if (has_dz) ring.copy(2, a.dz, a.dz_stride);
         ring.fetched();
     };
-    for (int s = 0; s < stages - 1; ++s) next();
+    for (int s = 0; s < stages - R; ++s) next();
 
     const uint64_t offset = DROP ? drop_offset(a.drop) : 0;
     const W scale = (W)a.drop.scale, over = W(1) / (W)a.cols;
     Pair<W> w[Q], dw[Q], db[Q];
-    load_parameters<T, V, K * V>(a.weight, float_parameters, 0, at.lane, at.threads, a.cols, W(1), w);
+    load_parameters<T, V, K>(a.weight, float_parameters, at.first, at.gap, a.cols, W(1), w);
 #pragma unroll
     for (int q = 0; q < Q; ++q) dw[q] = db[q] = both(W(0));
-    const int joiner = at.wlane & (kJoiners<TEAM> - 1), entries = at.ranks * at.warps;
 
-    W next_mean = 0, next_rstd = 0;
-    if (at.begin + at.within < a.rows) {
-        next_mean = ((const W *)a.mean)[at.begin + at.within];
-        next_rstd = ((const W *)a.rstd)[at.begin + at.within];
-    }
+    // A row past the last one is zeros with mean and rstd zero: it adds nothing.
+    W next_mean[R], next_rstd[R];
+    auto statistics = [&](size_t first) {
+#pragma unroll
+        for (int u = 0; u < R; ++u) {
+            const size_t row = first + at.within + u * at.step;
+            next_mean[u] = row < a.rows ? ((const W *)a.mean)[row] : W(0);
+            next_rstd[u] = row < a.rows ? ((const W *)a.rstd)[row] : W(0);
+        }
+    };
+    statistics(at.begin);
     if constexpr (TEAM == kCluster) cooperative_groups::this_cluster().sync();  // every block runs before it is written to
     int flip = 0;
-    for (size_t first = at.begin; first < a.rows; first += at.step, flip ^= 1) {
-        const size_t row = first + at.within;
-        const bool live = TEAM != kWarp || row < a.rows;
-        // A row past the last one (kWarp) is zeros with mean and rstd zero: it adds nothing.
-        const W mean = next_mean, rstd = next_rstd;
-        next_mean = next_rstd = 0;
-        if (row + at.step < a.rows) {
-            next_mean = ((const W *)a.mean)[row + at.step];
-            next_rstd = ((const W *)a.rstd)[row + at.step];
-        }
-        next();
+    for (size_t first = at.begin; first < a.rows; first += R * at.step, flip ^= 1) {
+        W mean[R], rstd[R], part[2 * R];
+#pragma unroll
+        for (int u = 0; u < R; ++u) mean[u] = next_mean[u], rstd[u] = next_rstd[u];
+        statistics(first + R * at.step);
+        for (int u = 0; u < R; ++u) next();
         ring.wait();
-        const size_t r = live ? row : 0;
         Vec<T, V> x[K], dy[K];
-        ring.get(x, 0, (const T *)a.x + r * a.x_stride);
-        ring.get(dy, 1, (const T *)a.dy + r * a.dy_stride);
-        Pair<W> sum2 = both(W(0)), along2 = both(W(0));
 #pragma unroll
-        for (int q = 0; q < Q; ++q) {
-            const Pair<W> d = pair_at(dy, q), xh = (pair_at(x, q) + both(-mean)) * both(rstd), g = d * w[q];
-            sum2 = sum2 + g;
-            along2 = fma(g, xh, along2);
-            dw[q] = fma(d, xh, dw[q]);
-            db[q] = db[q] + d;
-        }
-        W sum = team_sum(sum2.x + sum2.y, TEAM == kWarp ? at.threads : 32);
-        W along = team_sum(along2.x + along2.y, TEAM == kWarp ? at.threads : 32);
-        if constexpr (TEAM != kWarp) {
-            publish<W, TEAM>(sums[flip], at, sum, along);
-            sum = joiner < entries ? sums[flip][joiner][0] : W(0);
-            along = joiner < entries ? sums[flip][joiner][1] : W(0);
-            if (TEAM == kCluster && joiner + 32 < entries) {
-                sum += sums[flip][joiner + 32][0];
-                along += sums[flip][joiner + 32][1];
+        for (int u = 0; u < R; ++u) {
+            const size_t row = first + at.within + u * at.step, r = row < a.rows ? row : 0;
+            ring.get(x, u, 0, (const T *)a.x + r * a.x_stride);
+            ring.get(dy, u, 1, (const T *)a.dy + r * a.dy_stride);
+            Pair<W> sum = both(W(0)), along = both(W(0));
+#pragma unroll
+            for (int q = 0; q < Q; ++q) {
+                const Pair<W> d = pair_at(dy, q), xh = (pair_at(x, q) + both(-mean[u])) * both(rstd[u]), g = d * w[q];
+                sum = sum + g;
+                along = fma(g, xh, along);
+                dw[q] = fma(d, xh, dw[q]);
+                db[q] = db[q] + d;
             }
-            sum = team_sum(sum, kJoiners<TEAM>);
-            along = team_sum(along, kJoiners<TEAM>);
-            // Read again rather than held over the barrier: registers.
-            ring.get(x, 0, (const T *)a.x + r * a.x_stride);
-            ring.get(dy, 1, (const T *)a.dy + r * a.dy_stride);
+            part[2 * u] = sum.x + sum.y;
+            part[2 * u + 1] = along.x + along.y;
         }
-        sum *= over;
-        along *= over;
-        Pair<W> v[Q];
+        if constexpr (TEAM == kWarp) {
+            part[0] = team_sum(part[0], at.threads) * over;
+            part[1] = team_sum(part[1], at.threads) * over;
+        } else {
+            publish<2 * R>(sums[flip], at, folded_sums(part));
+            constexpr int kJoin = 32 / (2 * R);  // lanes that add one value up
+            W total = 0;
 #pragma unroll
-        for (int q = 0; q < Q; ++q) {
-            const Pair<W> xh = (pair_at(x, q) + both(-mean)) * both(rstd);
-            v[q] = (fma(xh, both(-along), pair_at(dy, q) * w[q]) + both(-sum)) * both(rstd);
-        }
-        if constexpr (DROP)
-            if (has_dz) {
-                ring.get(x, 2, (const T *)a.dz + r * a.dz_stride);
-#pragma unroll
-                for (int q = 0; q < Q; ++q) v[q] = v[q] + pair_at(x, q);
+            for (int j = 0; j < (TEAM == kCluster ? 64 / kJoin : 1); ++j) {
+                const int e = at.wlane % kJoin + j * kJoin;
+                if (e < at.entries) total += sums[flip][at.wlane / kJoin][e];
             }
-        ring.done();
-        if (a.dsum != nullptr) {
+            total = team_sum(total, kJoin) * over;
 #pragma unroll
-            for (int q = 0; q < Q; ++q) set_pair(x, q, v[q]);
-            T *to = (T *)a.dsum + row * a.dsum_stride;
-#pragma unroll
-            for (int i = 0; i < K; ++i) {
-                const int c = (at.lane + i * at.threads) * V;
-                if (live && (FULL || c < a.cols)) store<T, V>(to + c, x[i]);
-            }
+            for (int n = 0; n < 2 * R; ++n) part[n] = __shfl_sync(0xffffffffu, total, n * kJoin);
         }
-        if constexpr (DROP) {
-            if (a.dx != nullptr) {
-                drop_row<T, V, K, FULL>(a.drop, offset, row * (size_t)a.cols, at.lane, at.threads, a.cols, v);
 #pragma unroll
-                for (int q = 0; q < Q; ++q) set_pair(x, q, v[q] * both(scale));
-                T *to = (T *)a.dx + row * a.dx_stride;
+        for (int u = 0; u < R; ++u) {
+            const size_t row = first + at.within + u * at.step, r = row < a.rows ? row : 0;
+            const bool live = (TEAM != kWarp && u == 0) || row < a.rows;
+            if constexpr (TEAM != kWarp) {  // read again rather than held over the barrier: registers
+                ring.get(x, u, 0, (const T *)a.x + r * a.x_stride);
+                ring.get(dy, u, 1, (const T *)a.dy + r * a.dy_stride);
+            }
+            Pair<W> v[Q];
 #pragma unroll
-                for (int i = 0; i < K; ++i) {
-                    const int c = (at.lane + i * at.threads) * V;
-                    if (live && (FULL || c < a.cols)) store<T, V>(to + c, x[i]);
+            for (int q = 0; q < Q; ++q) {
+                const Pair<W> xh = (pair_at(x, q) + both(-mean[u])) * both(rstd[u]);
+                v[q] = (fma(xh, both(-part[2 * u + 1]), pair_at(dy, q) * w[q]) + both(-part[2 * u])) * both(rstd[u]);
+            }
+            if constexpr (DROP)
+                if (has_dz) {
+                    ring.get(x, u, 2, (const T *)a.dz + r * a.dz_stride);
+#pragma unroll
+                    for (int q = 0; q < Q; ++q) v[q] = v[q] + pair_at(x, q);
+                }
+            if (a.dsum != nullptr) {
+#pragma unroll
+                for (int q = 0; q < Q; ++q) set_pair(x, q, v[q]);
+                store_row<T, V, K, FULL>((T *)a.dsum + row * a.dsum_stride, at, live, a.cols, x);
+            }
+            if constexpr (DROP) {
+                if (a.dx != nullptr) {
+                    drop_row<T, V, K, FULL>(a.drop, offset, row * (size_t)a.cols, at, a.cols, v);
+#pragma unroll
+                    for (int q = 0; q < Q; ++q) set_pair(x, q, v[q] * both(scale));
+                    store_row<T, V, K, FULL>((T *)a.dx + row * a.dx_stride, at, live, a.cols, x);
                 }
             }
         }
+        ring.done();
     }
     if (partial == nullptr) return;
     W *mine = partial + at.team * 2 * a.cols;
@@ -139,7 +141,7 @@ __global__ void __launch_bounds__(TEAM == kWarp ? kWarpBlock : kTeamThreads, TEA
     if constexpr (TEAM != kWarp) {
 #pragma unroll
         for (int e = 0; e < K * V; ++e) {
-            const int c = (at.lane + e / V * at.threads) * V + e % V;
+            const int c = at.column(e / V) + e % V;
             if (c < a.cols) {
                 mine[c] = value(dw, e);
                 mine[a.cols + c] = value(db, e);
@@ -147,11 +149,11 @@ __global__ void __launch_bounds__(TEAM == kWarp ? kWarpBlock : kTeamThreads, TEA
         }
     } else {
         // The block's teams in order.
-        for (int team = 0; team < (int)at.teams; ++team) {
+        for (int team = 0; team < kWarpBlock / lanes; ++team) {
             if ((int)threadIdx.x / lanes == team)
 #pragma unroll
                 for (int e = 0; e < K * V; ++e) {
-                    const int c = (at.lane + e / V * at.threads) * V + e % V;
+                    const int c = at.column(e / V) + e % V;
                     columns[0][c] = value(dw, e) + (team > 0 ? columns[0][c] : W(0));
                     columns[1][c] = value(db, e) + (team > 0 ? columns[1][c] : W(0));
                 }
@@ -297,7 +299,8 @@ cudaError_t launch(NormTypes n, const BackwardArgs &a, void *workspace, cudaStre
             e = by_shape<T>(s, [&](auto v, auto k, auto team, auto full) {
                 constexpr int V = decltype(v)::value, K = decltype(k)::value;
                 const size_t stage = (size_t)(a.dz != nullptr ? 3 : 2) * K * s.threads() * kSlot<T, V>;
-                const int stages = ring_stages(stage, s.threads(), 512);
+                const int stages =
+                    ring_stages(stage, rows_at_once(sizeof(T), V, decltype(team)::value), s.threads(), 512);
                 return launch_team(vjp_kernel<T, V, K, DROP, decltype(team)::value, decltype(full)::value>, s, blocks,
                                    stages * stage, stream, a, s.lanes, float_parameters, stages, partial);
             });
