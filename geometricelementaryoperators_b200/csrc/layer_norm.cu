@@ -14,11 +14,10 @@ namespace geo {
 namespace layers {
 
 Shape shape_of(size_t cols, size_t bytes, bool aligned) {
-    Shape s = {aligned ? 16 / (int)bytes : 1, 0, 1, false};
+    Shape s = {!aligned, 0, 1, false};
     const size_t held = values_per_thread(bytes), threads = (cols + held - 1) / held;
     if (threads <= 32) {
-        // Single values are spread over whole warps, which work their draws out together.
-        s.lanes = aligned ? 1 : 32;
+        s.lanes = 1;
         while (s.lanes < (int)threads) s.lanes *= 2;
     } else {
         while (threads > (size_t)kTeamThreads * s.blocks) s.blocks *= 2;
@@ -44,24 +43,26 @@ bool aligned16(size_t cols, size_t bytes, size_t parameter_bytes, std::initializ
 namespace {
 
 // Threads that a multiprocessor holds: 80 registers a thread, 128 where two
-// rows, or single values, are held at a time.
-constexpr int resident_threads(size_t bytes, int vector, int team) {
-    return vector == 1 || rows_at_once(bytes, vector, team) == 2 ? 512 : 768;
+// rows are held at a time or vectors are put together from two.
+constexpr int resident_threads(size_t bytes, bool shift, int team) {
+    return shift || rows_at_once(bytes, shift, team) == 2 ? 512 : 768;
 }
 
-template <typename T, int V, int K, bool DROP, int TEAM, bool FULL>
+template <typename T, bool DROP, int TEAM, bool SHIFT, bool FULL>
 __global__ void __launch_bounds__(TEAM == kWarp ? kWarpBlock : kTeamThreads,
-                                  resident_threads(sizeof(T), V, TEAM) / (TEAM == kWarp ? kWarpBlock : kTeamThreads))
+                                  resident_threads(sizeof(T), SHIFT, TEAM) / (TEAM == kWarp ? kWarpBlock : kTeamThreads))
     norm_kernel(const ForwardArgs a, int lanes, bool float_parameters, int stages) {
     using W = Wide<T>;
-    constexpr int Q = K * V / 2, R = rows_at_once(sizeof(T), V, TEAM);
+    constexpr int V = 16 / (int)sizeof(T), K = values_per_thread(sizeof(T)) / V, Q = K * V / 2;
+    constexpr int R = rows_at_once(sizeof(T), SHIFT, TEAM);
     extern __shared__ __align__(16) unsigned char memory[];
     __shared__ W sums[2][2 * R][kSums<TEAM>];
+    __shared__ unsigned char drop_bytes[SHIFT && DROP ? kDropBytes : 1];
     const Place<TEAM, V, K> at(lanes);
-    Ring<T, V, K, TEAM, FULL, R> ring(memory, stages, DROP ? 2 : 1, at, a.rows, a.cols);
+    Ring<T, V, K, TEAM, SHIFT, FULL, R> ring(memory, stages, DROP ? 2 : 1, at, a.rows, a.cols);
     auto next = [&] {
-        ring.copy(0, a.x, a.x_stride);
-        if constexpr (DROP) ring.copy(1, a.residual, a.residual_stride);
+        ring.copy(0, (const T *)a.x, a.x_stride);
+        if constexpr (DROP) ring.copy(1, (const T *)a.residual, a.residual_stride);
         ring.fetched();
     };
     for (int s = 0; s < stages - R; ++s) next();
@@ -69,8 +70,8 @@ __global__ void __launch_bounds__(TEAM == kWarp ? kWarpBlock : kTeamThreads,
     const uint64_t offset = DROP ? drop_offset(a.drop) : 0;
     const W scale = (W)a.drop.scale, over = W(1) / (W)a.cols;
     Pair<W> w[Q], b[Q];
-    load_parameters<T, V, K>(a.weight, float_parameters, at.first, at.gap, a.cols, W(1), w);
-    load_parameters<T, V, K>(a.bias, float_parameters, at.first, at.gap, a.cols, W(0), b);
+    load_parameters<T, V, K, SHIFT>(a.weight, float_parameters, at, a.cols, W(1), w);
+    load_parameters<T, V, K, SHIFT>(a.bias, float_parameters, at, a.cols, W(0), b);
 
     // How many values of the row warp `n` of the team holds.
     auto held_by = [&](int n) {
@@ -105,11 +106,12 @@ __global__ void __launch_bounds__(TEAM == kWarp ? kWarpBlock : kTeamThreads,
 #pragma unroll
             for (int q = 0; q < Q; ++q) v[u][q] = pair_at(raw, q);
             if constexpr (DROP) {
-                drop_row<T, V, K, FULL>(a.drop, offset, row * (size_t)a.cols, at, a.cols, v[u]);
+                drop_row<T, V, K, SHIFT, FULL>(a.drop, offset, row * (size_t)a.cols, at, a.cols, drop_bytes, v[u]);
                 ring.get(raw, u, 1, (const T *)a.residual + r * a.residual_stride);
 #pragma unroll
                 for (int q = 0; q < Q; ++q) v[u][q] = fma(v[u][q], both(scale), pair_at(raw, q));
             }
+            if constexpr (SHIFT) set_past(v[u], at, row < a.rows, a.cols, W(0));
             Pair<W> two = both(W(0));
 #pragma unroll
             for (int q = 0; q < Q; ++q) two = two + v[u][q];
@@ -129,18 +131,7 @@ __global__ void __launch_bounds__(TEAM == kWarp ? kWarpBlock : kTeamThreads,
         }
 #pragma unroll
         for (int u = 0; u < R; ++u) {
-            if constexpr (!FULL) {
-#pragma unroll
-                for (int i = 0; i < K; ++i) {
-                    if (at.column(i) < a.cols) continue;
-                    if constexpr (V == 1) {
-                        (i & 1 ? v[u][i / 2].y : v[u][i / 2].x) = mean[u];
-                    } else {
-#pragma unroll
-                        for (int q = i * V / 2; q < (i + 1) * V / 2; ++q) v[u][q] = both(mean[u]);
-                    }
-                }
-            }
+            if constexpr (!FULL) set_past(v[u], at, true, a.cols, mean[u]);
             Pair<W> two = both(W(0));
 #pragma unroll
             for (int q = 0; q < Q; ++q) {
@@ -190,12 +181,12 @@ __global__ void __launch_bounds__(TEAM == kWarp ? kWarpBlock : kTeamThreads,
             if constexpr (DROP) {
 #pragma unroll
                 for (int q = 0; q < Q; ++q) set_pair(out, q, v[u][q]);
-                store_row<T, V, K, FULL>((T *)a.z + row * a.z_stride, at, live, a.cols, out);
+                store_row<T, V, K, SHIFT, FULL>((T *)a.z + row * a.z_stride, at, live, a.cols, out);
             }
 #pragma unroll
             for (int q = 0; q < Q; ++q)
                 set_pair(out, q, fma((v[u][q] + both(-mean[u])) * both(rstd[u]), w[q], b[q]));
-            store_row<T, V, K, FULL>((T *)a.y + row * a.y_stride, at, live, a.cols, out);
+            store_row<T, V, K, SHIFT, FULL>((T *)a.y + row * a.y_stride, at, live, a.cols, out);
         }
     }
 }
@@ -264,17 +255,16 @@ cudaError_t launch(NormTypes n, const ForwardArgs &a, cudaStream_t stream) {
     const bool float_parameters = n.parameter_type == GEO_B200_F32;
     return by_type(n.type, [&](auto t) {
         using T = decltype(t);
-        return by_shape<T>(s, [&](auto v, auto k, auto team, auto full) {
-            constexpr int V = decltype(v)::value, K = decltype(k)::value;
-            constexpr int resident = resident_threads(sizeof(T), V, decltype(team)::value);
-            constexpr int at_once = rows_at_once(sizeof(T), V, decltype(team)::value);
-            const size_t stage = (size_t)(DROP ? 2 : 1) * K * s.threads() * kSlot<T, V>;
+        return by_shape(s, [&](auto team, auto shift, auto full) {
+            constexpr int G = decltype(team)::value;
+            constexpr bool S = decltype(shift)::value, F = decltype(full)::value;
+            constexpr int resident = resident_threads(sizeof(T), S, G), at_once = rows_at_once(sizeof(T), S, G);
+            const size_t stage = (DROP ? 2 : 1) * s.part(sizeof(T));
             const int stages = ring_stages(stage, at_once, s.threads(), resident);
             const size_t wanted = (a.rows + s.teams() - 1) / s.teams();
             const size_t most = (size_t)geo::device_sm_count() * (resident / s.threads()) / s.blocks;
-            return launch_team(norm_kernel<T, V, K, DROP, decltype(team)::value, decltype(full)::value>, s,
-                               wanted < most ? wanted : most, stages * stage, stream, a, s.lanes, float_parameters,
-                               stages);
+            return launch_team(norm_kernel<T, DROP, G, S, F>, s, wanted < most ? wanted : most, stages * stage, stream,
+                               a, s.lanes, float_parameters, stages);
         });
     });
 }

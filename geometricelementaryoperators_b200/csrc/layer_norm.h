@@ -6,9 +6,8 @@
 // warp), a block of up to 256 threads, or a cluster of up to eight such blocks
 // that exchange their warps' sums through distributed shared memory. Thread
 // `lane` of the team holds K vectors of V values
-// (16 bytes, or single values where rows are not aligned; a warp's vectors are
-// adjacent: lane, lane + 32, ... of its part), 16 values in all (8 in
-// float64), so that a column belongs to one thread: weight, bias and the column
+// (16 bytes; a warp's vectors are adjacent: lane, lane + 32, ... of its part), 16
+// values in all (8 in float64), so that a column belongs to one thread: weight, bias and the column
 // sums of the backward pass stay in its registers over all its rows. Rows come
 // through a ring in shared memory filled by asynchronous copies, each thread
 // copying and waiting for its own vectors only (no barrier), one to four rows
@@ -16,6 +15,14 @@
 // left to wait for is the sums' way across the team, so teams of several warps
 // take two rows of 16-bit values at a time: one barrier for both, two chains of
 // additions side by side.
+//
+// Rows that do not start on 16 bytes (SHIFT) are moved in the aligned 16-byte
+// chunks that they lie in, by the warp whose part they hold, one more than the
+// part has vectors; a thread takes its vector out of two neighbouring chunks by
+// shifting, and puts one together for storing from its own and its neighbour's
+// vector. A chunk that is shared with another warp's part or another row is
+// written value by value. The first and last chunk of an array, which may reach
+// over its ends, are read value by value.
 #pragma once
 
 #include <cooperative_groups.h>
@@ -57,12 +64,17 @@ enum Team : int { kWarp = 0, kBlock = 1, kCluster = 2 };
 constexpr int kTeamThreads = 256;  // of a block, at most
 constexpr int kWarpBlock = 128;    // threads of a block of kWarp teams
 struct Shape {
-    int vector;  // values a thread moves at once: 16 bytes, or one value
+    bool shift;  // rows are not whole aligned vectors
     int lanes;   // threads of the team in a block; 0: rows too long for a team
     int blocks;  // blocks of the team
     bool full;   // the team's threads hold the row exactly
     Team team() const { return lanes > 32 || blocks > 1 ? (blocks > 1 ? kCluster : kBlock) : kWarp; }
     int threads() const { return team() == kWarp ? kWarpBlock : lanes; }
+    // Bytes of one array's part of a row in a block's ring.
+    size_t part(size_t bytes) const {
+        const size_t units = (size_t)threads() / (team() == kWarp ? lanes : 32);
+        return (size_t)threads() * (bytes == 8 ? 8 : 16) * bytes + (shift ? units * 16 : 0);
+    }
     size_t teams() const { return team() == kWarp ? kWarpBlock / lanes : 1; }  // of a block
 };
 constexpr int values_per_thread(size_t bytes) { return bytes == 8 ? 8 : 16; }
@@ -77,7 +89,7 @@ bool aligned16(size_t cols, size_t bytes, size_t parameter_bytes, std::initializ
                std::initializer_list<const void *> parameters);
 
 // Rows that a team takes at a time.
-constexpr int rows_at_once(size_t bytes, int vector, int team) { return bytes == 2 && vector > 1 && team != kWarp ? 2 : 1; }
+constexpr int rows_at_once(size_t bytes, bool shift, int team) { return bytes == 2 && !shift && team != kWarp ? 2 : 1; }
 
 // Rows in the ring: up to four beyond those being read, where the
 // multiprocessor's shared memory holds them for `resident` threads, at least as
@@ -115,116 +127,12 @@ __device__ __forceinline__ W team_sum(W v, int lanes) {
     return v;
 }
 
-// Pairs of weight or bias for the thread's values, which start at column `first`
-// and go on every `gap` columns, of the value type or (16-bit values only)
-// float32; `absent` past the row or without the array.
-template <typename T, int V, int K>
-__device__ __forceinline__ void load_parameters(const void *p, bool is_float, int first, int gap, int cols,
-                                                Wide<T> absent, Pair<Wide<T>> (&out)[K * V / 2]) {
-    using W = Wide<T>;
-#pragma unroll
-    for (int i = 0; i < K; ++i) {
-        const int c = first + i * gap;
-        const bool there = p != nullptr && c < cols;
-        if constexpr (V == 1) {
-            W v = absent;
-            if (there) {
-                if (sizeof(T) == 2 && is_float)
-                    v = (W)((const float *)p)[c];
-                else
-                    v = load<T, 1>((const T *)p + c).one();
-            }
-            (i & 1 ? out[i / 2].y : out[i / 2].x) = v;
-        } else {
-#pragma unroll
-            for (int q = 0; q < V / 2; ++q) out[i * V / 2 + q] = both(absent);
-            if (!there) continue;
-            if (sizeof(T) == 2 && is_float) {
-                if constexpr (sizeof(T) == 2) {
-#pragma unroll
-                    for (int j = 0; j < V; j += 4) {
-                        const Vec<float, 4> w = load<float, 4>((const float *)p + c + j);
-                        out[i * V / 2 + j / 2] = w.pair(0);
-                        out[i * V / 2 + j / 2 + 1] = w.pair(1);
-                    }
-                }
-            } else {
-                const Vec<T, V> w = load<T, V>((const T *)p + c);
-#pragma unroll
-                for (int q = 0; q < V / 2; ++q) out[i * V / 2 + q] = w.pair(q);
-            }
-        }
-    }
-}
-
-template <typename T, int V, int K>
-__device__ __forceinline__ Pair<Wide<T>> pair_at(const Vec<T, V> (&raw)[K], int q) {
-    if constexpr (V == 1)
-        return {raw[2 * q].one(), raw[2 * q + 1].one()};
-    else
-        return raw[2 * q / V].pair(q % (V / 2));
-}
-
-template <typename T, int V, int K>
-__device__ __forceinline__ void set_pair(Vec<T, V> (&raw)[K], int q, Pair<Wide<T>> v) {
-    if constexpr (V == 1) {
-        raw[2 * q].set_one(v.x);
-        raw[2 * q + 1].set_one(v.y);
-    } else {
-        raw[2 * q / V].set(q % (V / 2), v);
-    }
-}
-
-__device__ __forceinline__ uint32_t shared_address(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
-
-template <int BYTES>
-__device__ __forceinline__ void copy_async(uint32_t to, const void *from, bool live) {
-    if constexpr (BYTES == 16)
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(live ? 16 : 0) : "memory");
-    else
-        asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(to), "l"(from), "n"(BYTES),
-                     "r"(live ? BYTES : 0)
-                     : "memory");
-}
-__device__ __forceinline__ void commit_async() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int LEFT>
-__device__ __forceinline__ void wait_async() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
-}
-
-// Bytes of shared memory behind one vector of one thread: 16, or a whole copy
-// of 4 or 8 bytes for single values.
-template <typename T, int V>
-constexpr int kSlot = V > 1 ? 16 : (sizeof(T) == 8 ? 8 : 4);
-
-template <typename T, int V>
-__device__ __forceinline__ uint32_t word_offset(const T *p) {
-    return kSlot<T, V> > (int)sizeof(T) * V ? (uint32_t)((uintptr_t)p & 2) : 0u;
-}
-
-// Copies a vector into its slot (zeros when not `live`). A single 16-bit value
-// travels as the aligned 4-byte word around it, whose other half is not used;
-// where that word would reach over an end of the array (`edge`: the array's
-// first or last value), the value alone is loaded and stored.
-template <typename T, int V>
-__device__ __forceinline__ void fetch(uint32_t slot, const T *from, bool live, bool edge) {
-    if constexpr (kSlot<T, V> > (int)sizeof(T) * V) {
-        if (edge) {
-            const uint16_t v = *reinterpret_cast<const uint16_t *>(from);
-            asm volatile("st.shared.u16 [%0], %1;" ::"r"(slot + word_offset<T, V>(from)), "h"(v) : "memory");
-        } else {
-            copy_async<4>(slot, (const void *)((uintptr_t)from & ~(uintptr_t)3), live);
-        }
-    } else {
-        copy_async<kSlot<T, V>>(slot, from, live);
-    }
-}
-
-// Where this thread stands.
+// Where this thread stands. A unit is what lies side by side in a ring: a team
+// within a warp, or a warp's part of the row.
 template <int TEAM, int V, int K>
 struct Place {
     int threads, lane, warp, wlane, rank, ranks, entries;  // entries: warps of the team
-    int first, gap;                                        // its vectors' columns: first, first + gap, ...
+    int unit, unit_lanes, unit_lane, unit_first;           // of the block; the unit's first column
     size_t team, step, begin, within;  // rows begin + within, + step, ...: `begin` is the warp's
     __device__ __forceinline__ explicit Place(int lanes) {
         namespace cg = cooperative_groups;
@@ -235,46 +143,179 @@ struct Place {
         wlane = (int)threadIdx.x & 31;
         warp = TEAM == kWarp ? (int)threadIdx.x >> 5 : lane >> 5;
         entries = threads / 32;
-        first = (TEAM == kWarp ? lane : warp * 32 * K + wlane) * V;
-        gap = (TEAM == kWarp ? lanes : 32) * V;
+        unit = TEAM == kWarp ? (int)threadIdx.x / lanes : (int)threadIdx.x >> 5;
+        unit_lanes = TEAM == kWarp ? lanes : 32;
+        unit_lane = TEAM == kWarp ? lane : wlane;
+        unit_first = TEAM == kWarp ? 0 : warp * 32 * K * V;
         const size_t teams = TEAM == kWarp ? kWarpBlock / lanes : 1;
         team = blockIdx.x / ranks;
         step = gridDim.x / ranks * teams;
         begin = team * teams + (TEAM == kWarp ? warp * (32 / lanes) : 0);
         within = TEAM == kWarp ? wlane / lanes : 0;
     }
-    __device__ __forceinline__ int column(int i) const { return first + i * (TEAM == kWarp ? gap : 32 * V); }
+    // First column of the thread's vector i.
+    __device__ __forceinline__ int column(int i) const {
+        return unit_first + (i * (TEAM == kWarp ? unit_lanes : 32) + unit_lane) * V;
+    }
 };
 
+// Weight or bias of the thread's values as pairs, of the value type or (16-bit
+// values only) float32; `absent` past the row or without the array.
+template <typename T, int V, int K, bool SHIFT, int TEAM>
+__device__ __forceinline__ void load_parameters(const void *p, bool is_float, const Place<TEAM, V, K> &at, int cols,
+                                                Wide<T> absent, Pair<Wide<T>> (&out)[K * V / 2]) {
+    using W = Wide<T>;
+#pragma unroll
+    for (int i = 0; i < K; ++i) {
+        const int c = at.column(i);
+#pragma unroll
+        for (int q = 0; q < V / 2; ++q) out[i * V / 2 + q] = both(absent);
+        if (p == nullptr || c >= cols) continue;
+        if constexpr (SHIFT) {
+#pragma unroll
+            for (int j = 0; j < V; ++j)
+                if (c + j < cols) {
+                    const W v = sizeof(T) == 2 && is_float ? (W)((const float *)p)[c + j] : (W)widen(((const T *)p)[c + j]);
+                    (j & 1 ? out[i * V / 2 + j / 2].y : out[i * V / 2 + j / 2].x) = v;
+                }
+        } else if (sizeof(T) == 2 && is_float) {
+            if constexpr (sizeof(T) == 2) {
+#pragma unroll
+                for (int j = 0; j < V; j += 4) {
+                    const Vec<float, 4> w = load<float, 4>((const float *)p + c + j);
+                    out[i * V / 2 + j / 2] = w.pair(0);
+                    out[i * V / 2 + j / 2 + 1] = w.pair(1);
+                }
+            }
+        } else {
+            const Vec<T, V> w = load<T, V>((const T *)p + c);
+#pragma unroll
+            for (int q = 0; q < V / 2; ++q) out[i * V / 2 + q] = w.pair(q);
+        }
+    }
+}
+
+template <typename T, int V, int K>
+__device__ __forceinline__ Pair<Wide<T>> pair_at(const Vec<T, V> (&raw)[K], int q) {
+    return raw[2 * q / V].pair(q % (V / 2));
+}
+
+template <typename T, int V, int K>
+__device__ __forceinline__ void set_pair(Vec<T, V> (&raw)[K], int q, Pair<Wide<T>> v) {
+    raw[2 * q / V].set(q % (V / 2), v);
+}
+
+// Sets the thread's values past the row's end (all of them when not `live`) to `value`.
+template <int V, int K, int TEAM, typename W>
+__device__ __forceinline__ void set_past(Pair<W> (&v)[K * V / 2], const Place<TEAM, V, K> &at, bool live, int cols,
+                                         W value) {
+#pragma unroll
+    for (int i = 0; i < K; ++i) {
+        const int left = live ? cols - at.column(i) : 0;
+        if (left >= V) continue;
+#pragma unroll
+        for (int q = 0; q < V / 2; ++q) {
+            Pair<W> &p = v[i * V / 2 + q];
+            p.x = 2 * q < left ? p.x : value;
+            p.y = 2 * q + 1 < left ? p.y : value;
+        }
+    }
+}
+
+__device__ __forceinline__ uint32_t shared_address(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+__device__ __forceinline__ void copy_async(uint32_t to, const void *from, bool live) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(live ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void commit_async() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT>
+__device__ __forceinline__ void wait_async() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
+}
+
+// Bytes [shift, shift + 16) of 32, shift a multiple of the value size below 16.
+template <typename T, int V>
+__device__ __forceinline__ Vec<T, V> shifted(const Vec<T, V> &low, const Vec<T, V> &high, uint32_t shift) {
+    uint32_t w[8] = {low.w[0], low.w[1], low.w[2], low.w[3], high.w[0], high.w[1], high.w[2], high.w[3]};
+#pragma unroll
+    for (int k = 0; k < 6; ++k) w[k] = (shift & 8) ? w[k + 2] : w[k];
+    if constexpr (sizeof(T) <= 4) {
+#pragma unroll
+        for (int k = 0; k < 5; ++k) w[k] = (shift & 4) ? w[k + 1] : w[k];
+    }
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) w[k] = __funnelshift_r(w[k], w[k + 1], (shift & 2) * 8);
+    }
+    Vec<T, V> r;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) r.w[k] = w[k];
+    return r;
+}
+
+// Value j of a vector, as it is stored.
+template <typename T, int V>
+__device__ __forceinline__ void store_value(T *p, const Vec<T, V> &v, int j) {
+    if constexpr (sizeof(T) == 8)
+        *reinterpret_cast<uint2 *>(p) = make_uint2(v.w[2 * j], v.w[2 * j + 1]);
+    else if constexpr (sizeof(T) == 4)
+        *reinterpret_cast<uint32_t *>(p) = v.w[j];
+    else
+        *reinterpret_cast<unsigned short *>(p) = (unsigned short)(v.w[j / 2] >> (j % 2 * 16));
+}
+
 // The slots of one thread, for `arrays` arrays of rows.
-template <typename T, int V, int K, int TEAM, bool FULL, int R>
+template <typename T, int V, int K, int TEAM, bool SHIFT, bool FULL, int R>
 struct Ring {
-    static constexpr uint32_t kVector = 32 * kSlot<T, V>;  // bytes between a thread's vectors: its warp's lie together
     const Place<TEAM, V, K> &at;
-    const unsigned char *slots;
+    const unsigned char *slots;  // 16 bytes each; the unit's lie together
     uint32_t next_array, next_stage;
     int stages, read, write, cols;
     size_t row, rows;  // row: the next to fetch
 
+    // Bytes of one array's part of a row, in a block of so many units of so many lanes.
+    __host__ __device__ static constexpr uint32_t part(int units, int lanes) {
+        return (uint32_t)units * (lanes * K + (SHIFT ? 1 : 0)) * 16;
+    }
     __device__ __forceinline__ Ring(unsigned char *memory, int stages, int arrays, const Place<TEAM, V, K> &at,
                                     size_t rows, int cols)
-        : at(at), slots(memory + ((threadIdx.x >> 5) * (32 * K) + (threadIdx.x & 31)) * kSlot<T, V>), stages(stages),
-          read(0), write(0), cols(cols), row(at.begin + at.within), rows(rows) {
-        next_array = K * blockDim.x * kSlot<T, V>;
+        : at(at), slots(memory + part(at.unit, at.unit_lanes) + at.unit_lane * 16), stages(stages), read(0), write(0),
+          cols(cols), row(at.begin + at.within), rows(rows) {
+        next_array = part((int)blockDim.x / at.unit_lanes, at.unit_lanes);
         next_stage = arrays * next_array;
     }
-    // Starts the copies of array `array` of the row to fetch; zeros past the last row.
-    __device__ __forceinline__ void copy(int array, const void *base, size_t stride) {
+    __device__ __forceinline__ uint32_t vector_gap() const { return TEAM == kWarp ? at.unit_lanes * 16 : 512; }
+
+    // Starts the copies of array `array` of the row to fetch (not SHIFT: zeros past the last row).
+    __device__ __forceinline__ void copy(int array, const T *base, size_t stride) {
         const bool live = row < rows;
-        const T *start = (const T *)base + (live ? row : 0) * stride + at.first;
         const uint32_t slot = shared_address(slots) + write * next_stage + array * next_array;
+        if constexpr (SHIFT) {
+            if (!live) return;
+            const T *start = base + row * stride, *first = start + at.unit_first, *end = start + cols;
+            const T *chunk = (const T *)((uintptr_t)first & ~(uintptr_t)15) + at.unit_lane * V;
+            const T *whole_end = base + (rows - 1) * stride + cols;
 #pragma unroll
-        for (int i = 0; i < K; ++i) {
-            const int c = at.column(i);
-            const bool inside = live && (FULL || c < cols);
-            const bool edge = kSlot<T, V> > (int)sizeof(T) * V && inside &&
-                              ((row == 0 && c == 0) || (row == rows - 1 && c == cols - 1));
-            fetch<T, V>(slot + i * kVector, FULL || inside ? start + (c - at.first) : (const T *)base, inside, edge);
+            for (int i = 0; i <= K; ++i) {
+                const T *from = chunk + i * (int)(vector_gap() / sizeof(T));
+                if ((i == K && at.unit_lane != 0) || from >= end) continue;
+                if (from < base || from + V > whole_end) {
+                    unsigned char *to = const_cast<unsigned char *>(slots) + write * next_stage + array * next_array +
+                                        i * vector_gap();
+                    for (int j = 0; j < V; ++j)
+                        if (from + j >= start && from + j < end) ((T *)to)[j] = from[j];
+                } else {
+                    copy_async(slot + i * vector_gap(), from, true);
+                }
+            }
+        } else {
+            const T *start = base + (live ? row : 0) * stride + at.column(0);
+#pragma unroll
+            for (int i = 0; i < K; ++i) {
+                const int c = at.column(i);
+                const bool inside = live && (FULL || c < cols);
+                copy_async(slot + i * vector_gap(), FULL || inside ? start + (c - at.column(0)) : base, inside);
+            }
         }
     }
     __device__ __forceinline__ void fetched() {
@@ -290,16 +331,23 @@ struct Ring {
             case 3: wait_async<3>(); break;
             default: wait_async<4>(); break;
         }
+        if constexpr (SHIFT) __syncwarp();  // chunks of the neighbours
     }
-    // This thread's part of row u of those being read; row_start: where it lies in global memory.
+    // This thread's part of row u of those being read; row_start: where it lies in
+    // global memory. SHIFT: what is past the row's end is anything.
     __device__ __forceinline__ void get(Vec<T, V> (&out)[K], int u, int array, const T *row_start) const {
         const unsigned char *from = slots + (read + u) * next_stage + array * next_array;
-        // A thread's single 16-bit values are 32 apart: all in the same half of their words.
-        from += word_offset<T, V>(row_start + at.first);
+        const uint32_t shift = SHIFT ? (uint32_t)(uintptr_t)(row_start + at.unit_first) & 15 : 0;
 #pragma unroll
-        for (int i = 0; i < K; ++i) out[i] = load<T, V>((const T *)(from + i * kVector));
+        for (int i = 0; i < K; ++i) {
+            out[i] = load<T, V>((const T *)(from + i * vector_gap()));
+            if constexpr (SHIFT) out[i] = shifted(out[i], load<T, V>((const T *)(from + i * vector_gap() + 16)), shift);
+        }
     }
-    __device__ __forceinline__ void done() { read = read == stages - R ? 0 : read + R; }
+    __device__ __forceinline__ void done() {
+        if constexpr (SHIFT) __syncwarp();  // the neighbours have read this thread's chunks
+        read = read == stages - R ? 0 : read + R;
+    }
 };
 
 // One step of a sum that leaves two values in the two halves of 2 o lanes.
@@ -338,18 +386,36 @@ __device__ __forceinline__ void publish(W (*sums)[kSums<TEAM>], const Place<TEAM
     }
 }
 
-// Zeroes the values that dropout drops.
-template <typename T, int V, int K, bool FULL, int TEAM>
+// Zeroes the values that dropout drops. SHIFT: a vector's values are of two
+// blocks; the unit's blocks are worked out once, their decisions (a byte each) in
+// `bytes` of shared memory.
+constexpr int kDropBytes = 576;  // eight warps' 65, or 128 threads' 3 and fewer
+template <typename T, int V, int K, bool SHIFT, bool FULL, int TEAM>
 __device__ __forceinline__ void drop_row(const Drop &drop, uint64_t offset, uint64_t row_start,
-                                         const Place<TEAM, V, K> &at, int cols, Pair<Wide<T>> (&v)[K * V / 2]) {
-    using W = Wide<T>;
+                                         const Place<TEAM, V, K> &at, int cols, unsigned char *bytes,
+                                         Pair<Wide<T>> (&v)[K * V / 2]) {
     if (drop.threshold == 0) return;
-    if constexpr (V == 1) {
-        const uint32_t kept = kept_by_warp<K>(drop, offset, row_start + at.first - at.wlane, 32);
+    if constexpr (SHIFT) {
+        const uint64_t first = row_start + at.unit_first;
+        const uint32_t in_block = (uint32_t)first & 7u;
+        const int blocks = at.unit_lanes * K * V / 8 + 1;
+        unsigned char *mine = bytes + at.unit * blocks;
+        __syncwarp();
+        for (int n = at.unit_lane; n < blocks; n += at.unit_lanes)
+            mine[n] = (unsigned char)kept_of_eight(drop, offset, (first & ~(uint64_t)7) + 8 * n);
+        __syncwarp();
 #pragma unroll
-        for (int q = 0; q < K / 2; ++q) {
-            v[q].x = (kept >> (2 * q)) & 1 ? v[q].x : W(0);
-            v[q].y = (kept >> (2 * q + 1)) & 1 ? v[q].y : W(0);
+        for (int i = 0; i < K; ++i) {
+            const uint32_t place = in_block + (uint32_t)(at.column(i) - at.unit_first);
+            // The vector's last value is in the next block only if the first is not the block's first.
+            const uint32_t low = mine[place >> 3], high = mine[(place + V - 1) >> 3];
+            const uint32_t kept = (low | high << 8) >> (place & 7u);
+#pragma unroll
+            for (int q = 0; q < V / 2; ++q) {
+                Pair<Wide<T>> &p = v[i * V / 2 + q];
+                p.x = (kept >> (2 * q)) & 1 ? p.x : Wide<T>(0);
+                p.y = (kept >> (2 * q + 1)) & 1 ? p.y : Wide<T>(0);
+            }
         }
     } else {
 #pragma unroll
@@ -363,29 +429,60 @@ __device__ __forceinline__ void drop_row(const Drop &drop, uint64_t offset, uint
     }
 }
 
-// The thread's part of a row to global memory.
-template <typename T, int V, int K, bool FULL, int TEAM>
+// The thread's part of a row to global memory (every lane of the warp takes part).
+template <typename T, int V, int K, bool SHIFT, bool FULL, int TEAM>
 __device__ __forceinline__ void store_row(T *row_start, const Place<TEAM, V, K> &at, bool live, int cols,
                                           const Vec<T, V> (&v)[K]) {
-    T *to = row_start + at.first;
+    if constexpr (SHIFT) {
+        // Chunk (i, lane) begins `back` values before the thread's vector i: the
+        // end of the vector before it, then its own beginning.
+        const uint32_t shift = (uint32_t)(uintptr_t)(row_start + at.unit_first) & 15;
+        const int back = (int)(shift / sizeof(T));
+        const int from = at.unit_first, last = at.unit_first + at.unit_lanes * K * V;
+        const int to = last < cols ? last : cols;  // the unit's columns are [from, to)
+        const int before = ((int)threadIdx.x & 31 & ~(at.unit_lanes - 1)) + ((at.unit_lane - 1) & (at.unit_lanes - 1));
 #pragma unroll
-    for (int i = 0; i < K; ++i)
-        if (live && (FULL || at.column(i) < cols)) store<T, V>(to + (at.column(i) - at.first), v[i]);
+        for (int i = 0; i <= K; ++i) {
+            Vec<T, V> previous, out;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                // Lane 0's previous vector is the last lane's of the round before.
+                const uint32_t other = i > 0 ? v[i > 0 ? i - 1 : 0].w[k] : 0u, own = i < K ? v[i < K ? i : 0].w[k] : 0u;
+                previous.w[k] =
+                    __shfl_sync(0xffffffffu, at.unit_lane == at.unit_lanes - 1 ? other : own, before);
+                out.w[k] = own;
+            }
+            if (shift != 0) out = shifted(previous, out, 16 - shift);
+            const int start = from + (i * at.unit_lanes + at.unit_lane) * V - back;
+            if (!live || (i == K && at.unit_lane != 0) || start >= to) continue;
+            if (start >= from && start + V <= to) {
+                store<T, V>(row_start + start, out);
+            } else {
+#pragma unroll
+                for (int j = 0; j < V; ++j)
+                    if (start + j >= from && start + j < to) store_value<T, V>(row_start + start + j, out, j);
+            }
+        }
+    } else {
+        T *to = row_start + at.column(0);
+#pragma unroll
+        for (int i = 0; i < K; ++i)
+            if (live && (FULL || at.column(i) < cols)) store<T, V>(to + (at.column(i) - at.column(0)), v[i]);
+    }
 }
 
-// f(V, K, TEAM, FULL) of a shape as compile-time constants, as far as they occur.
-template <typename T, typename F>
+// f(TEAM, SHIFT, FULL) of a shape as compile-time constants, as far as they occur.
+template <typename F>
 cudaError_t by_shape(const Shape &s, F &&f) {
     using std::integral_constant;
-    constexpr int E = values_per_thread(sizeof(T)), V = 16 / (int)sizeof(T);
-    auto team = [&](auto v, auto k, auto full) {
-        if (s.team() == kWarp) return f(v, k, integral_constant<int, kWarp>{}, full);
-        if (s.team() == kBlock) return f(v, k, integral_constant<int, kBlock>{}, full);
-        return f(v, k, integral_constant<int, kCluster>{}, full);
+    auto team = [&](auto shift, auto full) {
+        if (s.team() == kWarp) return f(integral_constant<int, kWarp>{}, shift, full);
+        if (s.team() == kBlock) return f(integral_constant<int, kBlock>{}, shift, full);
+        return f(integral_constant<int, kCluster>{}, shift, full);
     };
-    if (s.vector == 1) return team(integral_constant<int, 1>{}, integral_constant<int, E>{}, std::false_type{});
-    if (s.full) return team(integral_constant<int, V>{}, integral_constant<int, E / V>{}, std::true_type{});
-    return team(integral_constant<int, V>{}, integral_constant<int, E / V>{}, std::false_type{});
+    if (s.shift) return team(std::true_type{}, std::false_type{});
+    if (s.full) return team(std::false_type{}, std::true_type{});
+    return team(std::false_type{}, std::false_type{});
 }
 
 template <typename F>

@@ -17,23 +17,25 @@ namespace {
 // of y_bar xh and y_bar in the registers of the thread that owns the column; at
 // the end partial[team][0: weight, 1: bias][col] (teams that are parts of a warp:
 // one partial for their block).
-template <typename T, int V, int K, bool DROP, int TEAM, bool FULL>
+template <typename T, bool DROP, int TEAM, bool SHIFT, bool FULL>
 __global__ void __launch_bounds__(TEAM == kWarp ? kWarpBlock : kTeamThreads, TEAM == kWarp ? 4 : 2)
     vjp_kernel(const BackwardArgs a, int lanes, bool float_parameters, int stages, Wide<T> *partial) {
     using W = Wide<T>;
-    constexpr int Q = K * V / 2, R = rows_at_once(sizeof(T), V, TEAM);
+    constexpr int V = 16 / (int)sizeof(T), K = values_per_thread(sizeof(T)) / V, Q = K * V / 2;
+    constexpr int R = rows_at_once(sizeof(T), SHIFT, TEAM);
     constexpr int kColumns = TEAM == kWarp ? 32 * K * V : 1;
     extern __shared__ __align__(16) unsigned char memory[];
     __shared__ W sums[2][2 * R][kSums<TEAM>];
     __shared__ W columns[2][kColumns];
+    __shared__ unsigned char drop_bytes[SHIFT && DROP ? kDropBytes : 1];
     const Place<TEAM, V, K> at(lanes);
     const bool has_dz = DROP && a.dz != nullptr;
-    Ring<T, V, K, TEAM, FULL, R> ring(memory, stages, has_dz ? 3 : 2, at, a.rows, a.cols);
+    Ring<T, V, K, TEAM, SHIFT, FULL, R> ring(memory, stages, has_dz ? 3 : 2, at, a.rows, a.cols);
     auto next = [&] {
-        ring.copy(0, a.x, a.x_stride);
-        ring.copy(1, a.dy, a.dy_stride);
+        ring.copy(0, (const T *)a.x, a.x_stride);
+        ring.copy(1, (const T *)a.dy, a.dy_stride);
         if constexpr (DROP)
-            if (has_dz) ring.copy(2, a.dz, a.dz_stride);
+            if (has_dz) ring.copy(2, (const T *)a.dz, a.dz_stride);
         ring.fetched();
     };
     for (int s = 0; s < stages - R; ++s) next();
@@ -41,7 +43,7 @@ __global__ void __launch_bounds__(TEAM == kWarp ? kWarpBlock : kTeamThreads, TEA
     const uint64_t offset = DROP ? drop_offset(a.drop) : 0;
     const W scale = (W)a.drop.scale, over = W(1) / (W)a.cols;
     Pair<W> w[Q], dw[Q], db[Q];
-    load_parameters<T, V, K>(a.weight, float_parameters, at.first, at.gap, a.cols, W(1), w);
+    load_parameters<T, V, K, SHIFT>(a.weight, float_parameters, at, a.cols, W(1), w);
 #pragma unroll
     for (int q = 0; q < Q; ++q) dw[q] = db[q] = both(W(0));
 
@@ -72,13 +74,27 @@ __global__ void __launch_bounds__(TEAM == kWarp ? kWarpBlock : kTeamThreads, TEA
             ring.get(x, u, 0, (const T *)a.x + r * a.x_stride);
             ring.get(dy, u, 1, (const T *)a.dy + r * a.dy_stride);
             Pair<W> sum = both(W(0)), along = both(W(0));
-#pragma unroll
-            for (int q = 0; q < Q; ++q) {
-                const Pair<W> d = pair_at(dy, q), xh = (pair_at(x, q) + both(-mean[u])) * both(rstd[u]), g = d * w[q];
+            auto add = [&](int q, Pair<W> d, Pair<W> xh) {
+                const Pair<W> g = d * w[q];
                 sum = sum + g;
                 along = fma(g, xh, along);
                 dw[q] = fma(d, xh, dw[q]);
                 db[q] = db[q] + d;
+            };
+            if constexpr (SHIFT) {
+                Pair<W> d[Q], xh[Q];
+#pragma unroll
+                for (int q = 0; q < Q; ++q) {
+                    d[q] = pair_at(dy, q);
+                    xh[q] = (pair_at(x, q) + both(-mean[u])) * both(rstd[u]);
+                }
+                set_past(d, at, row < a.rows, a.cols, W(0));
+                set_past(xh, at, row < a.rows, a.cols, W(0));
+#pragma unroll
+                for (int q = 0; q < Q; ++q) add(q, d[q], xh[q]);
+            } else {
+#pragma unroll
+                for (int q = 0; q < Q; ++q) add(q, pair_at(dy, q), (pair_at(x, q) + both(-mean[u])) * both(rstd[u]));
             }
             part[2 * u] = sum.x + sum.y;
             part[2 * u + 1] = along.x + along.y;
@@ -122,14 +138,14 @@ __global__ void __launch_bounds__(TEAM == kWarp ? kWarpBlock : kTeamThreads, TEA
             if (a.dsum != nullptr) {
 #pragma unroll
                 for (int q = 0; q < Q; ++q) set_pair(x, q, v[q]);
-                store_row<T, V, K, FULL>((T *)a.dsum + row * a.dsum_stride, at, live, a.cols, x);
+                store_row<T, V, K, SHIFT, FULL>((T *)a.dsum + row * a.dsum_stride, at, live, a.cols, x);
             }
             if constexpr (DROP) {
                 if (a.dx != nullptr) {
-                    drop_row<T, V, K, FULL>(a.drop, offset, row * (size_t)a.cols, at, a.cols, v);
+                    drop_row<T, V, K, SHIFT, FULL>(a.drop, offset, row * (size_t)a.cols, at, a.cols, drop_bytes, v);
 #pragma unroll
                     for (int q = 0; q < Q; ++q) set_pair(x, q, v[q] * both(scale));
-                    store_row<T, V, K, FULL>((T *)a.dx + row * a.dx_stride, at, live, a.cols, x);
+                    store_row<T, V, K, SHIFT, FULL>((T *)a.dx + row * a.dx_stride, at, live, a.cols, x);
                 }
             }
         }
@@ -296,13 +312,13 @@ cudaError_t launch(NormTypes n, const BackwardArgs &a, void *workspace, cudaStre
         if (s.lanes != 0) {
             blocks = team_grid(s, a.rows);
             W *partial = sums ? (W *)workspace : nullptr;
-            e = by_shape<T>(s, [&](auto v, auto k, auto team, auto full) {
-                constexpr int V = decltype(v)::value, K = decltype(k)::value;
-                const size_t stage = (size_t)(a.dz != nullptr ? 3 : 2) * K * s.threads() * kSlot<T, V>;
-                const int stages =
-                    ring_stages(stage, rows_at_once(sizeof(T), V, decltype(team)::value), s.threads(), 512);
-                return launch_team(vjp_kernel<T, V, K, DROP, decltype(team)::value, decltype(full)::value>, s, blocks,
-                                   stages * stage, stream, a, s.lanes, float_parameters, stages, partial);
+            e = by_shape(s, [&](auto team, auto shift, auto full) {
+                constexpr int G = decltype(team)::value;
+                constexpr bool S = decltype(shift)::value, F = decltype(full)::value;
+                const size_t stage = (a.dz != nullptr ? 3 : 2) * s.part(sizeof(T));
+                const int stages = ring_stages(stage, rows_at_once(sizeof(T), S, G), s.threads(), 512);
+                return launch_team(vjp_kernel<T, DROP, G, S, F>, s, blocks, stages * stage, stream, a, s.lanes,
+                                   float_parameters, stages, partial);
             });
         } else {
             // Columns first: the row kernel may overwrite x or y_bar.

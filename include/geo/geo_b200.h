@@ -355,7 +355,8 @@ geo_b200_status_t geo_b200_sparse_apply_parametric_vjp_f64(const geo_operator_pl
  *     argument and launch errors are reported. Nothing is allocated and nothing
  *     is kept between calls; calls may be captured into a CUDA graph.
  *   - strides are in values; 0 means packed rows, otherwise stride >= cols.
- *     Values between the rows are neither read nor written.
+ *     Nothing is written between the rows; what lies there may be read along
+ *     with its neighbours and has no effect.
  *   - an output may be the same array (pointer and stride) as an input of the
  *     call that it overwrites; arrays must not overlap otherwise.
  *   - arithmetic and sums are float64 for GEO_B200_F64 and float32 otherwise,
