@@ -55,8 +55,8 @@ __global__ void __launch_bounds__(TEAM == kWarp ? kWarpBlock : kTeamThreads,
     using W = Wide<T>;
     constexpr int V = 16 / (int)sizeof(T), K = values_per_thread(sizeof(T)) / V, Q = K * V / 2;
     constexpr int R = rows_at_once(sizeof(T), SHIFT, TEAM);
-    extern __shared__ __align__(16) unsigned char memory[];
-    __shared__ W sums[2][2 * R][kSums<TEAM>];
+    extern __shared__ __align__(128) unsigned char memory[];  // a row of copies or reads is whole 128-byte lines
+    __shared__ Exchange<W, 2 * R, TEAM> sums;
     __shared__ unsigned char drop_bytes[SHIFT && DROP ? kDropBytes : 1];
     const Place<TEAM, V, K> at(lanes);
     Ring<T, V, K, TEAM, SHIFT, FULL, R> ring(memory, stages, DROP ? 2 : 1, at, a.rows, a.cols);
@@ -90,10 +90,10 @@ __global__ void __launch_bounds__(TEAM == kWarp ? kWarpBlock : kTeamThreads,
         joined[j] = joiner + j * kJoin < at.entries ? held_by(joiner + j * kJoin) : W(0);
         over_joined[j] = joined[j] > W(0) ? W(1) / joined[j] : W(0);
     }
-    if constexpr (TEAM == kCluster) cooperative_groups::this_cluster().sync();  // every block runs before it is written to
+    open_exchange(sums);
 
-    int flip = 0;
-    for (size_t first = at.begin; first < a.rows; first += R * at.step, flip ^= 1) {
+    uint32_t round = 0;
+    for (size_t first = at.begin; first < a.rows; first += R * at.step, ++round) {
         for (int u = 0; u < R; ++u) next();
         ring.wait();
         Pair<W> v[R][Q];
@@ -145,22 +145,24 @@ __global__ void __launch_bounds__(TEAM == kWarp ? kWarpBlock : kTeamThreads,
             rstd[0] = rsqrt(team_sum(squares[0], at.threads) * over + (W)a.epsilon);
         } else {
             squares[0] = R == 2 ? folded_sums(squares) : team_sum(squares[0], 32);
-            // sums[2 u]: sum of row u, sums[2 u + 1]: its squares.
-            publish<2 * R>(sums[flip], at, at.wlane / (16 / R) % 2 ? squares[0] : sum[0]);
+            // Values 2 u: sum of row u, 2 u + 1: its squares.
+            const bool complete = exchange(sums, round, at, at.wlane / (16 / R) % 2 ? squares[0] : sum[0]);
+            auto found = [&](int n, int j) { return sums.values[round & 1][n][at.first_entry + joiner + j * kJoin]; };
             // Warps joined about the row's mean: squares + held (warp's mean - mean)^2.
             W total = 0, other[kEach];
 #pragma unroll
             for (int j = 0; j < kEach; ++j) {
-                other[j] = joined[j] > W(0) ? sums[flip][2 * joined_row][joiner + j * kJoin] : W(0);
+                other[j] = joined[j] > W(0) ? found(2 * joined_row, j) : W(0);
                 total += other[j];
             }
             // Divided, so that a row of one value has no spread.
-            const W middle = team_sum(total, kJoin) / (W)a.cols;
+            W middle = team_sum(total, kJoin) / (W)a.cols;
+            if (!complete) middle = (W)NAN;
             W spread = 0;
 #pragma unroll
             for (int j = 0; j < kEach; ++j) {
                 const W d = other[j] * over_joined[j] - middle;
-                if (joined[j] > W(0)) spread += sums[flip][2 * joined_row + 1][joiner + j * kJoin] + joined[j] * d * d;
+                if (joined[j] > W(0)) spread += found(2 * joined_row + 1, j) + joined[j] * d * d;
             }
             const W inverse = rsqrt(team_sum(spread, kJoin) * over + (W)a.epsilon);
 #pragma unroll
@@ -189,6 +191,7 @@ __global__ void __launch_bounds__(TEAM == kWarp ? kWarpBlock : kTeamThreads,
             store_row<T, V, K, SHIFT, FULL>((T *)a.y + row * a.y_stride, at, live, a.cols, out);
         }
     }
+    close_exchange<TEAM>();
 }
 
 // ---- rows of any length --------------------------------------------------------

@@ -3,8 +3,9 @@
 //
 // A row lives on chip between the two sweeps that its sums need. A team of
 // threads holds it: part of a warp (a power of two up to 32 lanes, several rows a
-// warp), a block of up to 256 threads, or a cluster of up to eight such blocks
-// that exchange their warps' sums through distributed shared memory. Thread
+// warp), several warps of a block (up to 256 threads; smaller teams share a
+// block, each with a barrier of its own), or a cluster of up to eight blocks that
+// exchange their warps' sums through distributed shared memory. Thread
 // `lane` of the team holds K vectors of V values
 // (16 bytes; a warp's vectors are adjacent: lane, lane + 32, ... of its part), 16
 // values in all (8 in float64), so that a column belongs to one thread: weight, bias and the column
@@ -60,7 +61,7 @@ cudaError_t launch_norm_vjp(NormTypes t, const BackwardArgs &a, bool drop, void 
 size_t vjp_workspace(NormTypes t, size_t rows, size_t cols);
 
 // How a row is held.
-enum Team : int { kWarp = 0, kBlock = 1, kCluster = 2 };
+enum Team : int { kWarp = 0, kPart = 1, kBlock = 2, kCluster = 3 };  // part of a warp, of a block; a block; several
 constexpr int kTeamThreads = 256;  // of a block, at most
 constexpr int kWarpBlock = 128;    // threads of a block of kWarp teams
 struct Shape {
@@ -68,14 +69,18 @@ struct Shape {
     int lanes;   // threads of the team in a block; 0: rows too long for a team
     int blocks;  // blocks of the team
     bool full;   // the team's threads hold the row exactly
-    Team team() const { return lanes > 32 || blocks > 1 ? (blocks > 1 ? kCluster : kBlock) : kWarp; }
-    int threads() const { return team() == kWarp ? kWarpBlock : lanes; }
+    Team team() const {
+        return blocks > 1 ? kCluster : (lanes <= 32 ? kWarp : (lanes <= kTeamThreads / 2 ? kPart : kBlock));
+    }
+    int threads() const { return (int)teams() * lanes; }  // of a block
     // Bytes of one array's part of a row in a block's ring.
     size_t part(size_t bytes) const {
-        const size_t units = (size_t)threads() / (team() == kWarp ? lanes : 32);
+        const size_t units = team() == kWarp ? teams() : threads() / 32;
         return (size_t)threads() * (bytes == 8 ? 8 : 16) * bytes + (shift ? units * 16 : 0);
     }
-    size_t teams() const { return team() == kWarp ? kWarpBlock / lanes : 1; }  // of a block
+    size_t teams() const {  // of a block
+        return team() == kWarp ? kWarpBlock / lanes : (team() == kPart ? kTeamThreads / lanes : 1);
+    }
 };
 constexpr int values_per_thread(size_t bytes) { return bytes == 8 ? 8 : 16; }
 Shape shape_of(size_t cols, size_t bytes, bool aligned);
@@ -131,26 +136,29 @@ __device__ __forceinline__ W team_sum(W v, int lanes) {
 // within a warp, or a warp's part of the row.
 template <int TEAM, int V, int K>
 struct Place {
-    int threads, lane, warp, wlane, rank, ranks, entries;  // entries: warps of the team
-    int unit, unit_lanes, unit_lane, unit_first;           // of the block; the unit's first column
-    size_t team, step, begin, within;  // rows begin + within, + step, ...: `begin` is the warp's
+    int threads, lane, warp, wlane, rank, ranks;  // threads: of the team
+    int teams, team, entries, first_entry;        // in the block; entries: warps of the team, in order from first_entry
+    int unit, unit_lanes, unit_lane, unit_first;  // of the block; the unit's first column
+    size_t slice, step, begin, within;  // rows begin + within, + step, ...: `begin` is the warp's; slice: block or cluster
     __device__ __forceinline__ explicit Place(int lanes) {
         namespace cg = cooperative_groups;
         rank = TEAM == kCluster ? (int)cg::this_cluster().block_rank() : 0;
         ranks = TEAM == kCluster ? (int)cg::this_cluster().num_blocks() : 1;
-        threads = TEAM == kWarp ? lanes : (int)blockDim.x * ranks;
-        lane = TEAM == kWarp ? (int)threadIdx.x & (lanes - 1) : (int)threadIdx.x + rank * (int)blockDim.x;
+        threads = lanes * ranks;
+        teams = TEAM == kWarp ? kWarpBlock / lanes : (TEAM == kPart ? kTeamThreads / lanes : 1);
+        team = TEAM <= kPart ? (int)threadIdx.x / lanes : 0;
+        lane = (int)threadIdx.x + (TEAM == kCluster ? rank * lanes : -team * lanes);
         wlane = (int)threadIdx.x & 31;
-        warp = TEAM == kWarp ? (int)threadIdx.x >> 5 : lane >> 5;
+        warp = lane >> 5;
         entries = threads / 32;
-        unit = TEAM == kWarp ? (int)threadIdx.x / lanes : (int)threadIdx.x >> 5;
+        first_entry = TEAM == kPart ? team * entries : 0;
+        unit = TEAM == kWarp ? team : (int)threadIdx.x >> 5;
         unit_lanes = TEAM == kWarp ? lanes : 32;
         unit_lane = TEAM == kWarp ? lane : wlane;
         unit_first = TEAM == kWarp ? 0 : warp * 32 * K * V;
-        const size_t teams = TEAM == kWarp ? kWarpBlock / lanes : 1;
-        team = blockIdx.x / ranks;
-        step = gridDim.x / ranks * teams;
-        begin = team * teams + (TEAM == kWarp ? warp * (32 / lanes) : 0);
+        slice = blockIdx.x / ranks;
+        step = gridDim.x / ranks * (size_t)teams;
+        begin = slice * teams + (TEAM == kWarp ? (threadIdx.x >> 5) * (32 / lanes) : team);
         within = TEAM == kWarp ? wlane / lanes : 0;
     }
     // First column of the thread's vector i.
@@ -281,7 +289,7 @@ struct Ring {
                                     size_t rows, int cols)
         : at(at), slots(memory + part(at.unit, at.unit_lanes) + at.unit_lane * 16), stages(stages), read(0), write(0),
           cols(cols), row(at.begin + at.within), rows(rows) {
-        next_array = part((int)blockDim.x / at.unit_lanes, at.unit_lanes);
+        next_array = part(TEAM == kWarp ? at.teams : (int)blockDim.x / 32, at.unit_lanes);
         next_stage = arrays * next_array;
     }
     __device__ __forceinline__ uint32_t vector_gap() const { return TEAM == kWarp ? at.unit_lanes * 16 : 512; }
@@ -368,21 +376,81 @@ __device__ __forceinline__ W folded_sums(const W (&v)[N]) {
     return team_sum(s, 32 / N);
 }
 
-// Every warp's N values, value n in lanes 32 / N n and on, to where all the
-// team's threads find them after the barrier (of the block or the cluster) in
-// here, sums[n][warp]. Two buffers in turn, so that one barrier is enough.
+// Where the warps of a team leave N values for one another: values[n][entry]
+// of the block's (or cluster's) warps. Two of them in turn, so that one wait a
+// round is enough: a warp writes round t + 2 only after every warp has sent its
+// values of round t + 1, for which it has read those of round t.
 template <int TEAM>
-constexpr int kSums = TEAM == kCluster ? 64 : (TEAM == kBlock ? 8 : 1);
-template <int N, typename W, int TEAM, int V, int K>
-__device__ __forceinline__ void publish(W (*sums)[kSums<TEAM>], const Place<TEAM, V, K> &at, W value) {
-    namespace cg = cooperative_groups;
-    const int n = at.wlane / (32 / N), sub = at.wlane % (32 / N);
+constexpr int kEntries = TEAM == kCluster ? 64 : (TEAM == kWarp ? 1 : 8);
+template <typename W, int N, int TEAM>
+struct Exchange {
+    W values[2][N][kEntries<TEAM>];
+    uint64_t arrived[2];  // kCluster: mbarriers that count the bytes which other blocks send
+};
+constexpr uint32_t kWaitPolls = 1u << 22;  // seconds; a round takes microseconds
+
+template <typename W, int N, int TEAM>
+__device__ __forceinline__ void open_exchange(Exchange<W, N, TEAM> &x) {
     if constexpr (TEAM == kCluster) {
-        if (sub < at.ranks) *cg::this_cluster().map_shared_rank(&sums[n][at.warp], sub) = value;
-        cg::this_cluster().sync();
+        if (threadIdx.x == 0) {
+            for (int i = 0; i < 2; ++i)
+                asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(shared_address(&x.arrived[i])) : "memory");
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        }
+        cooperative_groups::this_cluster().sync();  // every block runs, its barriers ready, before it is sent anything
+    }
+}
+// A block leaves only when nothing is on its way to it.
+template <int TEAM>
+__device__ __forceinline__ void close_exchange() {
+    if constexpr (TEAM == kCluster) cooperative_groups::this_cluster().sync();
+}
+
+// Sends the warp's values (value n in lanes 32 / N n and on) and waits for those
+// of all the team's warps. A cluster's blocks send straight into each other's
+// shared memory, where a barrier counts the bytes: unlike a barrier of the
+// cluster, this does not wait for the stores of the row before. False when the
+// wait gave up (never, unless a block of the cluster failed).
+template <typename W, int N, int TEAM, int V, int K>
+__device__ __forceinline__ bool exchange(Exchange<W, N, TEAM> &x, uint32_t round, const Place<TEAM, V, K> &at, W value) {
+    const int n = at.wlane / (32 / N), sub = at.wlane % (32 / N), flip = round & 1;
+    if constexpr (TEAM == kCluster) {
+        const uint32_t barrier = shared_address(&x.arrived[flip]);
+        if (threadIdx.x == 0)
+            asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(barrier),
+                         "r"((uint32_t)(at.entries * N * (int)sizeof(W)))
+                         : "memory");
+        if (sub < at.ranks) {
+            uint32_t to, there;
+            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"
+                         : "=r"(to)
+                         : "r"(shared_address(&x.values[flip][n][at.warp])), "r"(sub));
+            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(barrier), "r"(sub));
+            if constexpr (sizeof(W) == 8)
+                asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.b64 [%0], %1, [%2];" ::"r"(to),
+                             "l"(__double_as_longlong(value)), "r"(there)
+                             : "memory");
+            else
+                asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];" ::"r"(to),
+                             "r"(__float_as_uint(value)), "r"(there)
+                             : "memory");
+        }
+        uint32_t done = 0;
+        for (uint32_t poll = 0; poll < kWaitPolls && !done; ++poll)
+            asm volatile(
+                "{\n.reg .pred p;\nmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
+                "selp.u32 %0, 1, 0, p;\n}"
+                : "=r"(done)
+                : "r"(barrier), "r"((round >> 1) & 1u)
+                : "memory");
+        return done != 0;
     } else {
-        if (sub == 0) sums[n][at.warp] = value;
-        __syncthreads();
+        if (sub == 0) x.values[flip][n][at.first_entry + at.warp] = value;
+        if constexpr (TEAM == kPart)
+            asm volatile("bar.sync %0, %1;" ::"r"(1 + at.team), "r"(at.threads) : "memory");
+        else
+            __syncthreads();
+        return true;
     }
 }
 
@@ -477,6 +545,7 @@ cudaError_t by_shape(const Shape &s, F &&f) {
     using std::integral_constant;
     auto team = [&](auto shift, auto full) {
         if (s.team() == kWarp) return f(integral_constant<int, kWarp>{}, shift, full);
+        if (s.team() == kPart) return f(integral_constant<int, kPart>{}, shift, full);
         if (s.team() == kBlock) return f(integral_constant<int, kBlock>{}, shift, full);
         return f(integral_constant<int, kCluster>{}, shift, full);
     };

@@ -15,18 +15,16 @@ namespace {
 
 // One pass over x and y_bar (and z_bar): x_bar row by row, and the column sums
 // of y_bar xh and y_bar in the registers of the thread that owns the column; at
-// the end partial[team][0: weight, 1: bias][col] (teams that are parts of a warp:
-// one partial for their block).
+// the end partial[block or cluster][0: weight, 1: bias][col], the teams of a
+// block added up in shared memory.
 template <typename T, bool DROP, int TEAM, bool SHIFT, bool FULL>
 __global__ void __launch_bounds__(TEAM == kWarp ? kWarpBlock : kTeamThreads, TEAM == kWarp ? 4 : 2)
     vjp_kernel(const BackwardArgs a, int lanes, bool float_parameters, int stages, Wide<T> *partial) {
     using W = Wide<T>;
     constexpr int V = 16 / (int)sizeof(T), K = values_per_thread(sizeof(T)) / V, Q = K * V / 2;
     constexpr int R = rows_at_once(sizeof(T), SHIFT, TEAM);
-    constexpr int kColumns = TEAM == kWarp ? 32 * K * V : 1;
-    extern __shared__ __align__(16) unsigned char memory[];
-    __shared__ W sums[2][2 * R][kSums<TEAM>];
-    __shared__ W columns[2][kColumns];
+    extern __shared__ __align__(128) unsigned char memory[];  // a row of copies or reads is whole 128-byte lines
+    __shared__ Exchange<W, 2 * R, TEAM> sums;
     __shared__ unsigned char drop_bytes[SHIFT && DROP ? kDropBytes : 1];
     const Place<TEAM, V, K> at(lanes);
     const bool has_dz = DROP && a.dz != nullptr;
@@ -58,9 +56,9 @@ __global__ void __launch_bounds__(TEAM == kWarp ? kWarpBlock : kTeamThreads, TEA
         }
     };
     statistics(at.begin);
-    if constexpr (TEAM == kCluster) cooperative_groups::this_cluster().sync();  // every block runs before it is written to
-    int flip = 0;
-    for (size_t first = at.begin; first < a.rows; first += R * at.step, flip ^= 1) {
+    open_exchange(sums);
+    uint32_t round = 0;
+    for (size_t first = at.begin; first < a.rows; first += R * at.step, ++round) {
         W mean[R], rstd[R], part[2 * R];
 #pragma unroll
         for (int u = 0; u < R; ++u) mean[u] = next_mean[u], rstd[u] = next_rstd[u];
@@ -103,15 +101,16 @@ __global__ void __launch_bounds__(TEAM == kWarp ? kWarpBlock : kTeamThreads, TEA
             part[0] = team_sum(part[0], at.threads) * over;
             part[1] = team_sum(part[1], at.threads) * over;
         } else {
-            publish<2 * R>(sums[flip], at, folded_sums(part));
+            const bool complete = exchange(sums, round, at, folded_sums(part));
             constexpr int kJoin = 32 / (2 * R);  // lanes that add one value up
             W total = 0;
 #pragma unroll
             for (int j = 0; j < (TEAM == kCluster ? 64 / kJoin : 1); ++j) {
                 const int e = at.wlane % kJoin + j * kJoin;
-                if (e < at.entries) total += sums[flip][at.wlane / kJoin][e];
+                if (e < at.entries) total += sums.values[round & 1][at.wlane / kJoin][at.first_entry + e];
             }
             total = team_sum(total, kJoin) * over;
+            if (!complete) total = (W)NAN;
 #pragma unroll
             for (int n = 0; n < 2 * R; ++n) part[n] = __shfl_sync(0xffffffffu, total, n * kJoin);
         }
@@ -151,10 +150,11 @@ __global__ void __launch_bounds__(TEAM == kWarp ? kWarpBlock : kTeamThreads, TEA
         }
         ring.done();
     }
+    close_exchange<TEAM>();
     if (partial == nullptr) return;
-    W *mine = partial + at.team * 2 * a.cols;
+    W *mine = partial + at.slice * 2 * a.cols;
     auto value = [&](const Pair<W> (&p)[Q], int e) { return e & 1 ? p[e / 2].y : p[e / 2].x; };
-    if constexpr (TEAM != kWarp) {
+    if constexpr (TEAM >= kBlock) {
 #pragma unroll
         for (int e = 0; e < K * V; ++e) {
             const int c = at.column(e / V) + e % V;
@@ -164,20 +164,27 @@ __global__ void __launch_bounds__(TEAM == kWarp ? kWarpBlock : kTeamThreads, TEA
             }
         }
     } else {
-        // The block's teams in order.
-        for (int team = 0; team < kWarpBlock / lanes; ++team) {
-            if ((int)threadIdx.x / lanes == team)
+        // The block's teams in order, where the ring was (two rows of it hold two
+        // sums of a row); value e of lane l at e threads + (l ^ e): no bank twice.
+        W *columns = (W *)memory, *bias_columns = columns + at.threads * K * V;
+        auto place = [&](int e, int lane) { return e * at.threads + (at.threads >= 32 ? lane ^ e : lane); };
+        wait_async<0>();
+        __syncthreads();
+        for (int team = 0; team < at.teams; ++team) {
+            if (at.team == team)
 #pragma unroll
                 for (int e = 0; e < K * V; ++e) {
-                    const int c = at.column(e / V) + e % V;
-                    columns[0][c] = value(dw, e) + (team > 0 ? columns[0][c] : W(0));
-                    columns[1][c] = value(db, e) + (team > 0 ? columns[1][c] : W(0));
+                    const int to = place(e, at.lane);
+                    columns[to] = value(dw, e) + (team > 0 ? columns[to] : W(0));
+                    bias_columns[to] = value(db, e) + (team > 0 ? bias_columns[to] : W(0));
                 }
             __syncthreads();
         }
-        for (int c = threadIdx.x; c < a.cols; c += kWarpBlock) {
-            mine[c] = columns[0][c];
-            mine[a.cols + c] = columns[1][c];
+        for (int c = threadIdx.x; c < a.cols; c += blockDim.x) {
+            const int vector = c / V % (at.unit_lanes * K), unit = c / (at.unit_lanes * K * V);
+            const int from = place(vector / at.unit_lanes * V + c % V, unit * 32 + vector % at.unit_lanes);
+            mine[c] = columns[from];
+            mine[a.cols + c] = bias_columns[from];
         }
     }
 }

@@ -43,7 +43,10 @@ bool make_drop(const geo_b200_dropout_config_t &config, const uint64_t *device_o
         config.cols > GEO_B200_LAYER_MAX_COLS || (config.cols & (((size_t)1 << config.dimension) - 1)) != 0)
         return false;
     const double threshold = std::nearbyint(config.rate * 65536.0);
-    out->seed = config.seed;
+    for (uint32_t round = 0; round < 10; ++round) {
+        out->key[round][0] = (uint32_t)config.seed + round * 0x9E3779B9u;
+        out->key[round][1] = (uint32_t)(config.seed >> 32) + round * 0xBB67AE85u;
+    }
     out->offset = config.offset;
     out->device_offset = device_offset;
     out->threshold = (uint32_t)threshold;

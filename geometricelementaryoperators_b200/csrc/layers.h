@@ -235,7 +235,7 @@ inline geo_b200_status_t status_of(cudaError_t e) {
 
 // What a kernel needs of a geo_b200_dropout_config_t.
 struct Drop {
-    uint64_t seed;
+    uint32_t key[10][2];  // the seed's two words, advanced for each round
     uint64_t offset;
     const uint64_t *device_offset;
     double scale;        // 65536 / (65536 - threshold); 0 when everything is dropped
@@ -252,20 +252,18 @@ struct Block {
 };
 
 // Philox4x32-10: ten rounds of two 32 x 32 -> 64 bit products whose high halves
-// are mixed with the key (Salmon et al., SC 2011).
-__device__ __forceinline__ Block philox(uint64_t index, uint64_t offset, uint64_t seed) {
+// are mixed with the key (Salmon et al., SC 2011). The keys of the rounds come
+// from the host: as kernel parameters they cost the kernel no instruction.
+__device__ __forceinline__ Block philox(uint64_t index, uint64_t offset, const uint32_t (&key)[10][2]) {
     uint32_t c0 = (uint32_t)index, c1 = (uint32_t)(index >> 32);
     uint32_t c2 = (uint32_t)offset, c3 = (uint32_t)(offset >> 32);
-    uint32_t k0 = (uint32_t)seed, k1 = (uint32_t)(seed >> 32);
 #pragma unroll
     for (int round = 0; round < 10; ++round) {
         const uint64_t p0 = (uint64_t)c0 * 0xD2511F53u, p1 = (uint64_t)c2 * 0xCD9E8D57u;
-        c0 = (uint32_t)(p1 >> 32) ^ c1 ^ k0;
+        c0 = (uint32_t)(p1 >> 32) ^ c1 ^ key[round][0];
         c1 = (uint32_t)p1;
-        c2 = (uint32_t)(p0 >> 32) ^ c3 ^ k1;
+        c2 = (uint32_t)(p0 >> 32) ^ c3 ^ key[round][1];
         c3 = (uint32_t)p0;
-        k0 += 0x9E3779B9u;
-        k1 += 0xBB67AE85u;
     }
     return {{c0, c1, c2, c3}};
 }
@@ -276,7 +274,7 @@ __device__ __forceinline__ uint64_t drop_offset(const Drop &drop) {
 
 // Bit i: whether draw i of the block is kept.
 __device__ __forceinline__ uint32_t kept_of_block(const Drop &drop, uint64_t offset, uint64_t index) {
-    const Block b = philox(index, offset, drop.seed);
+    const Block b = philox(index, offset, drop.key);
     uint32_t bits = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -304,7 +302,7 @@ __device__ __forceinline__ uint32_t kept_of_eight(const Drop &drop, uint64_t off
 template <int V>
 __device__ __forceinline__ void draws_of_pairs(const Drop &drop, uint64_t offset, uint64_t e, uint32_t (&out)[V / 2]) {
     const uint64_t unit = e >> drop.shift;
-    const Block b = philox(unit >> 3, offset, drop.seed);
+    const Block b = philox(unit >> 3, offset, drop.key);
     if (drop.shift == 0) {
 #pragma unroll
         for (int q = 0; q < V / 2; ++q) {
@@ -358,7 +356,7 @@ __device__ __forceinline__ uint32_t kept_by_warp(const Drop &drop, uint64_t offs
 
 // Whether the unit is kept; for callers that look at one unit at a time.
 __device__ __forceinline__ bool unit_kept(const Drop &drop, uint64_t offset, uint64_t unit) {
-    const Block b = philox(unit >> 3, offset, drop.seed);
+    const Block b = philox(unit >> 3, offset, drop.key);
     const uint32_t word = (unit & 4) ? ((unit & 2) ? b.word[3] : b.word[2]) : ((unit & 2) ? b.word[1] : b.word[0]);
     return ((unit & 1) ? word : word << 16) > drop.bound;
 }
