@@ -43,9 +43,9 @@ bool aligned16(size_t cols, size_t bytes, size_t parameter_bytes, std::initializ
 namespace {
 
 // Threads that a multiprocessor holds: 80 registers a thread, 128 where two
-// rows are held at a time or vectors are put together from two.
+// rows are held at a time.
 constexpr int resident_threads(size_t bytes, bool shift, int team) {
-    return shift || rows_at_once(bytes, shift, team) == 2 ? 512 : 768;
+    return rows_at_once(bytes, shift, team) == 2 ? 512 : 768;
 }
 
 template <typename T, bool DROP, int TEAM, bool SHIFT, bool FULL>

@@ -466,10 +466,10 @@ __device__ __forceinline__ void drop_row(const Drop &drop, uint64_t offset, uint
     if constexpr (SHIFT) {
         const uint64_t first = row_start + at.unit_first;
         const uint32_t in_block = (uint32_t)first & 7u;
-        const int blocks = at.unit_lanes * K * V / 8 + 1;
+        const int blocks = at.unit_lanes * K * V / 8 + 1, left = cols - at.unit_first;
         unsigned char *mine = bytes + at.unit * blocks;
         __syncwarp();
-        for (int n = at.unit_lane; n < blocks; n += at.unit_lanes)
+        for (int n = at.unit_lane; n < blocks && 8 * n < left + (int)in_block; n += at.unit_lanes)
             mine[n] = (unsigned char)kept_of_eight(drop, offset, (first & ~(uint64_t)7) + 8 * n);
         __syncwarp();
 #pragma unroll

@@ -164,27 +164,29 @@ __global__ void __launch_bounds__(TEAM == kWarp ? kWarpBlock : kTeamThreads, TEA
             }
         }
     } else {
-        // The block's teams in order, where the ring was (two rows of it hold two
-        // sums of a row); value e of lane l at e threads + (l ^ e): no bank twice.
-        W *columns = (W *)memory, *bias_columns = columns + at.threads * K * V;
-        auto place = [&](int e, int lane) { return e * at.threads + (at.threads >= 32 ? lane ^ e : lane); };
+        // Every thread's sums to where the ring was (two rows of it hold two sums
+        // of a row; value e of thread t at e threads + (t ^ e): no bank twice),
+        // then a column's, the block's teams in order.
+        const int each = blockDim.x;
+        W *found = (W *)memory;
+        auto place = [&](int e, int thread) { return e * each + (thread ^ (e & 31)); };
         wait_async<0>();
         __syncthreads();
-        for (int team = 0; team < at.teams; ++team) {
-            if (at.team == team)
 #pragma unroll
-                for (int e = 0; e < K * V; ++e) {
-                    const int to = place(e, at.lane);
-                    columns[to] = value(dw, e) + (team > 0 ? columns[to] : W(0));
-                    bias_columns[to] = value(db, e) + (team > 0 ? bias_columns[to] : W(0));
-                }
-            __syncthreads();
+        for (int e = 0; e < K * V; ++e) {
+            found[place(e, threadIdx.x)] = value(dw, e);
+            found[each * K * V + place(e, threadIdx.x)] = value(db, e);
         }
-        for (int c = threadIdx.x; c < a.cols; c += blockDim.x) {
+        __syncthreads();
+        for (int n = threadIdx.x; n < 2 * a.cols; n += each) {
+            const bool bias = n >= a.cols;
+            const int c = bias ? n - a.cols : n;
             const int vector = c / V % (at.unit_lanes * K), unit = c / (at.unit_lanes * K * V);
-            const int from = place(vector / at.unit_lanes * V + c % V, unit * 32 + vector % at.unit_lanes);
-            mine[c] = columns[from];
-            mine[a.cols + c] = bias_columns[from];
+            const int e = vector / at.unit_lanes * V + c % V, lane = unit * 32 + vector % at.unit_lanes;
+            W sum = 0;
+            for (int team = 0; team < at.teams; ++team)
+                sum += found[(bias ? each * K * V : 0) + place(e, team * lanes + lane)];
+            mine[n] = sum;
         }
     }
 }
