@@ -230,17 +230,6 @@ __device__ __forceinline__ void set_past(Pair<W> (&v)[K * V / 2], const Place<TE
     }
 }
 
-__device__ __forceinline__ uint32_t shared_address(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
-
-__device__ __forceinline__ void copy_async(uint32_t to, const void *from, bool live) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(live ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void commit_async() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int LEFT>
-__device__ __forceinline__ void wait_async() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
-}
-
 // Bytes [shift, shift + 16) of 32, shift a multiple of the value size below 16.
 template <typename T, int V>
 __device__ __forceinline__ Vec<T, V> shifted(const Vec<T, V> &low, const Vec<T, V> &high, uint32_t shift) {

@@ -231,6 +231,21 @@ inline geo_b200_status_t status_of(cudaError_t e) {
     return GEO_B200_RUNTIME_FAILURE;
 }
 
+#ifdef __CUDACC__
+// ---- asynchronous copies into shared memory -----------------------------------
+
+__device__ __forceinline__ uint32_t shared_address(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+__device__ __forceinline__ void copy_async(uint32_t to, const void *from, bool live = true) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(live ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void commit_async() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT>
+__device__ __forceinline__ void wait_async() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
+}
+#endif
+
 // ---- dropout's draws ---------------------------------------------------------
 
 // What a kernel needs of a geo_b200_dropout_config_t.

@@ -1,11 +1,13 @@
 // rotary.cu -- rotary positions and their VJP (geo/geo_b200.h section 5).
 //
 // Pair i of a head at position p is turned by t = p f_i. The angle is taken in
-// turns, p (hi + lo), with the rounding error of p hi recovered by a fused
-// multiply-add, and its whole quarter turns are dropped in float64 before the
-// sine and cosine are taken in the arithmetic type: what is left is at most an
-// eighth of a turn, so its conversion to float32 costs 2^-28 turns and far
-// positions lose nothing.
+// quarter turns, p (hi + lo), in float64: adding 1.5 2^52 to p hi in a fused
+// multiply-add rounds it to whole quarters, whose last two bits are the quadrant,
+// and a second one leaves p hi - quarters with a single rounding. What is left is
+// at most half a quarter turn, so its conversion to float32 costs 2^-26 quarters
+// and far positions lose nothing. Its sine and cosine are polynomials
+// (interpolated at Chebyshev nodes, within 2^-28), two pairs at a time in packed
+// float32 arithmetic.
 #include <cmath>
 
 #include "geo_runtime.h"
@@ -23,25 +25,51 @@ struct RotaryArgs {
     size_t batch, tokens, heads, head_dim;
     size_t xb, xt, xh, yb, yt, yh, pb;
     int64_t first_position;
-    size_t groups, share;  // heads are split into `groups` of `share`
+    size_t share;  // heads of a block: its row of the grid says which
     int narrow_positions;
 };
 
+// What is left of p (hi + lo) quarter turns after `quadrant` whole ones.
+__device__ __forceinline__ double split_quarters(double p, double2 quarters, uint32_t &quadrant) {
+    const double magic = 6755399441055744.0;  // 1.5 2^52: the sum's last bit is worth 1
+    const double rounded = ::fma(p, quarters.x, magic);
+    quadrant = (uint32_t)__double2loint(rounded);
+    return ::fma(p, quarters.y, ::fma(p, quarters.x, -(rounded - magic)));
+}
+
+// Sine and cosine of x quarter turns, |x| <= 1/2.
+__device__ __forceinline__ void sine_cosine(Pair<float> x, Pair<float> &sine, Pair<float> &cosine) {
+    const Pair<float> u = x * x;
+    Pair<float> p = fma(both(-0.00460214913748f), u, both(0.0796802176242f));
+    p = fma(p, u, both(-0.645963477663f));
+    p = fma(p, u, both(1.57079632195f));
+    sine = x * p;
+    Pair<float> c = fma(both(0.00090673988654f), u, both(-0.0208615283385f));
+    c = fma(c, u, both(0.253669410357f));
+    c = fma(c, u, both(-1.23370054937f));
+    cosine = fma(c, u, both(1.0f));
+}
+__device__ __forceinline__ void sine_cosine(Pair<double> x, Pair<double> &sine, Pair<double> &cosine) {
+    sincospi(0.5 * x.x, &sine.x, &cosine.x);
+    sincospi(0.5 * x.y, &sine.y, &cosine.y);
+}
+
+__device__ __forceinline__ float signed_by(float v, uint32_t bit1) {
+    return __uint_as_float(__float_as_uint(v) ^ (bit1 & 2u) << 30);
+}
+__device__ __forceinline__ double signed_by(double v, uint32_t bit1) { return bit1 & 2u ? -v : v; }
+
+// amplitude times cosine and sine of p times two pairs' quarter turns per position.
 template <typename W>
-__device__ __forceinline__ void rotor(int64_t position, double hi, double lo, W amplitude, W &c, W &s) {
-    const double p = (double)position;
-    const double turns = p * hi;
-    const double rest = fma(p, lo, fma(p, hi, -turns));
-    const double quarters = rint(turns * 4.0);
-    const double left = (turns - quarters * 0.25) + rest;
-    W sine, cosine;
-    if constexpr (std::is_same_v<W, double>)
-        sincospi(2.0 * left, &sine, &cosine);
-    else
-        sincospif((float)(2.0 * left), &sine, &cosine);
-    const int q = (int)((long long)quarters & 3);
-    c = amplitude * ((q & 1) ? (q == 1 ? -sine : sine) : (q == 0 ? cosine : -cosine));
-    s = amplitude * ((q & 1) ? (q == 1 ? cosine : -cosine) : (q == 0 ? sine : -sine));
+__device__ __forceinline__ void rotors(double p, double2 a, double2 b, W amplitude, Pair<W> &c, Pair<W> &s) {
+    uint32_t qa, qb;
+    const double xa = split_quarters(p, a, qa), xb = split_quarters(p, b, qb);
+    Pair<W> sine, cosine;
+    sine_cosine(Pair<W>{(W)xa, (W)xb}, sine, cosine);
+    c = {signed_by(qa & 1 ? sine.x : cosine.x, qa + 1), signed_by(qb & 1 ? sine.y : cosine.y, qb + 1)};
+    s = {signed_by(qa & 1 ? cosine.x : sine.x, qa), signed_by(qb & 1 ? cosine.y : sine.y, qb)};
+    c = c * both(amplitude);
+    s = s * both(amplitude);
 }
 
 // SPLIT: pair j is value j of p and of q; else pair j is values 2j, 2j + 1 of p.
@@ -72,65 +100,102 @@ __device__ __forceinline__ void turn(Vec<T, V> &p, Vec<T, V> &q, const Pair<Wide
 
 // A thread takes the pairs that one vector (INTERLEAVED: V / 2 pairs) or two
 // vectors half a head apart (HALF: V pairs) hold of one token, works their rotors
-// out once, and turns them in `share` heads, kHeads loads ahead; the coordinates
-// past rotary_dim go the same way as vectors that are only copied. Where nothing
-// wider than a value is aligned, a pair is two values.
-constexpr int kHeads = 4;
+// out once, and turns them in `share` heads; the coordinates past rotary_dim go
+// the same way as vectors that are only copied. Heads come through slots of the
+// thread's own in shared memory, kAhead asynchronous copies ahead, so that few
+// registers keep the bytes in flight that HBM wants; the first ones are on their
+// way while the rotors are worked out. Where nothing wider than a value is
+// aligned, a pair is two values; vectors below 16 bytes are loaded directly.
+constexpr int kAhead = 5;
 template <typename T, int V, bool HALF>
-__global__ void __launch_bounds__(kThreads)
+constexpr int kSlots = V * sizeof(T) == 16 ? (kAhead + 1) * (HALF ? 2 : 1) : 0;  // vectors a thread
+template <typename T, int V, bool HALF>
+__global__ void __launch_bounds__(kThreads, 4)
     rotary_kernel(const RotaryArgs a, const __grid_constant__ geo_b200_rotary_plan_t plan, int backward) {
     using W = Wide<T>;
     constexpr bool SPLIT = HALF || V == 1;     // a pair's coordinates are in two vectors
     constexpr int N = SPLIT ? 2 : 1;           // vectors a head
     constexpr int PAIRS = SPLIT ? V : V / 2;   // pairs a thread
+    constexpr bool RING = kSlots<T, V, HALF> > 0;
     const uint32_t half = plan.rotary_dim / 2, second = HALF ? half : 1;
     const uint32_t turned = plan.rotary_dim / (N * V);
     const uint32_t units = turned + ((uint32_t)a.head_dim - plan.rotary_dim) / V;
-    const size_t count = a.batch * a.tokens * a.groups * units;
-    for (size_t id = blockIdx.x * (size_t)kThreads + threadIdx.x; id < count; id += (size_t)gridDim.x * kThreads) {
-        size_t rest = id / units;
-        const uint32_t unit = (uint32_t)(id - rest * units);
-        const size_t bt = rest / a.groups, group = rest - bt * a.groups;
-        const size_t b = bt / a.tokens, t = bt - b * a.tokens;
-        const size_t from = group * a.share, left = a.heads - from;
-        const size_t heads = left < a.share ? left : a.share;
+    const size_t count = a.tokens * units;
+    const size_t from = blockIdx.y * a.share, left = a.heads - from;
+    const uint32_t heads = (uint32_t)(left < a.share ? left : a.share);
+    extern __shared__ __align__(128) unsigned char memory[];
+    __shared__ double2 quarters[GEO_B200_ROTARY_MAX_DIM / 2];
+    // Out of the parameters, where lanes that read different pairs wait for one another.
+    for (uint32_t i = threadIdx.x; i < half; i += kThreads)
+        quarters[i] = make_double2(4.0 * plan.turns[i], 4.0 * plan.turns_low[i]);
+    __syncthreads();
+    for (size_t id = blockIdx.x * (size_t)kThreads + threadIdx.x; id < a.batch * count;
+         id += (size_t)gridDim.x * kThreads) {
+        size_t b = 0, in_batch = id;
+        if (a.batch > 1) {
+            b = a.batch * count <= 0xFFFFFFFFu ? (uint32_t)id / (uint32_t)count : id / count;
+            in_batch = id - b * count;
+        }
+        const size_t t = count <= 0xFFFFFFFFu ? (uint32_t)in_batch / units : in_batch / units;
+        const uint32_t unit = (uint32_t)(in_batch - t * units);
         const bool copied = unit >= turned;
         if (copied && a.x == a.y) continue;
         const size_t at = copied ? plan.rotary_dim + (size_t)(unit - turned) * V : (size_t)unit * (HALF ? V : N * V);
         const T *x = (const T *)a.x + b * a.xb + t * a.xt + from * a.xh + at;
         T *y = (T *)a.y + b * a.yb + t * a.yt + from * a.yh + at;
+        const uint32_t both_vectors = SPLIT && !copied;
+
+        const unsigned char *slot = memory + threadIdx.x * 16;
+        uint32_t write = 0, read = 0, fetched = 0;
+        auto fetch = [&] {
+            if (fetched < heads) {
+                const uint32_t to = shared_address(slot) + write * (N * kThreads * 16);
+                copy_async(to, x);
+                if (both_vectors) copy_async(to + kThreads * 16, x + second);
+                x += a.xh;
+                ++fetched;
+                write = write == kAhead ? 0 : write + 1;
+            }
+            commit_async();
+        };
+        if constexpr (RING)
+            for (int k = 0; k < kAhead; ++k) fetch();
+
         Pair<W> c[(PAIRS + 1) / 2], s[(PAIRS + 1) / 2];
         if (!copied) {
             const size_t where = b * a.pb + t;
             const int64_t position = a.positions == nullptr ? a.first_position + (int64_t)t
                                      : a.narrow_positions   ? (int64_t)((const int32_t *)a.positions)[where]
                                                             : ((const int64_t *)a.positions)[where];
+            const W amplitude = (W)plan.amplitude;
 #pragma unroll
-            for (int j = 0; j < PAIRS; ++j) {
+            for (int j = 0; j < PAIRS; j += 2) {
                 const uint32_t pair = unit * PAIRS + j;
-                W cosine, sine;
-                rotor<W>(position, plan.turns[pair], plan.turns_low[pair], (W)plan.amplitude, cosine, sine);
-                if (backward) sine = -sine;
-                (j & 1 ? c[j / 2].y : c[j / 2].x) = cosine;
-                (j & 1 ? s[j / 2].y : s[j / 2].x) = sine;
+                rotors<W>((double)position, quarters[pair], quarters[PAIRS > 1 ? pair + 1 : pair], amplitude, c[j / 2],
+                          s[j / 2]);
+                if (backward) s[j / 2] = s[j / 2] * both(W(-1));
             }
         }
-        for (size_t h = 0; h < heads; h += kHeads) {
-            Vec<T, V> v[kHeads][N];
-#pragma unroll
-            for (int k = 0; k < kHeads; ++k)
-                if (h + k < heads) {
-                    v[k][0] = load<T, V>(x + (h + k) * a.xh);
-                    if (SPLIT && !copied) v[k][N - 1] = load<T, V>(x + (h + k) * a.xh + second);
-                }
-#pragma unroll
-            for (int k = 0; k < kHeads; ++k)
-                if (h + k < heads) {
-                    if (!copied) turn<T, V, SPLIT>(v[k][0], v[k][N - 1], c, s);
-                    store<T, V>(y + (h + k) * a.yh, v[k][0]);
-                    if (SPLIT && !copied) store<T, V>(y + (h + k) * a.yh + second, v[k][N - 1]);
-                }
+        for (uint32_t h = 0; h < heads; ++h) {
+            Vec<T, V> v[N];
+            if constexpr (RING) {
+                fetch();
+                wait_async<kAhead>();
+                const unsigned char *got = slot + read * (N * kThreads * 16);
+                v[0] = load<T, V>((const T *)got);
+                if (both_vectors) v[N - 1] = load<T, V>((const T *)(got + kThreads * 16));
+                read = read == kAhead ? 0 : read + 1;
+            } else {
+                v[0] = load<T, V>(x);
+                if (both_vectors) v[N - 1] = load<T, V>(x + second);
+                x += a.xh;
+            }
+            if (!copied) turn<T, V, SPLIT>(v[0], v[N - 1], c, s);
+            store<T, V>(y, v[0]);
+            if (both_vectors) store<T, V>(y + second, v[N - 1]);
+            y += a.yh;
         }
+        if constexpr (RING) wait_async<0>();
     }
 }
 
@@ -228,33 +293,37 @@ geo_b200_status_t rotary(const geo_b200_rotary_plan_t *plan, const geo_b200_rota
     a.first_position = s.first_position;
     a.narrow_positions = s.position_type == GEO_B200_I32;
     // A rotor costs about as much as turning four heads: heads are shared out
-    // only as far as it takes to give every multiprocessor 1024 threads.
+    // only as far as it takes to give every multiprocessor 2048 threads.
     const int v = vector_width(a, *plan, b);
     const bool half = plan->layout == GEO_B200_ROTARY_HALF;
     const size_t units = plan->rotary_dim / (half || v == 1 ? 2 * v : v) + (s.head_dim - plan->rotary_dim) / v;
-    const size_t wanted = (size_t)geo::device_sm_count() * 1024, threads = tokens * units;
+    const size_t wanted = (size_t)geo::device_sm_count() * 2048, threads = tokens * units;
     size_t groups = threads < wanted ? (wanted + threads - 1) / threads : 1;
     if (groups > s.heads) groups = s.heads;
+    if (groups > 65535) groups = 65535;
     a.share = (s.heads + groups - 1) / groups;
-    a.groups = (s.heads + a.share - 1) / a.share;
-    const size_t blocks = (threads * a.groups + kThreads - 1) / kThreads;
-    const unsigned grid = (unsigned)(blocks < 0x7fffffff ? blocks : 0x7fffffff);
+    if (a.share > 0xFFFFFFFFu) return GEO_B200_INVALID_ARGUMENT;
+    const size_t blocks = (threads + kThreads - 1) / kThreads;
+    const dim3 grid((unsigned)(blocks < 0x7fffffff ? blocks : 0x7fffffff), (unsigned)((s.heads + a.share - 1) / a.share));
     return status_of(by_type(s.type, [&](auto t) {
         using T = decltype(t);
         auto go = [&](auto width) {
             constexpr int V = decltype(width)::value;
-            if (half)
-                rotary_kernel<T, V, true><<<grid, kThreads, 0, stream>>>(a, *plan, backward);
-            else
-                rotary_kernel<T, V, false><<<grid, kThreads, 0, stream>>>(a, *plan, backward);
+            const size_t ring = (size_t)(half ? kSlots<T, V, true> : kSlots<T, V, false>) * kThreads * 16;
+            auto kernel = half ? rotary_kernel<T, V, true> : rotary_kernel<T, V, false>;
+            if (ring > 40 * 1024) {
+                const cudaError_t e =
+                    cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)ring);
+                if (e != cudaSuccess) return e;
+            }
+            kernel<<<grid, kThreads, ring, stream>>>(a, *plan, backward);
+            return cudaGetLastError();
         };
-        if (v == 1) go(std::integral_constant<int, 1>{});
-        if (v == 2) go(std::integral_constant<int, 2>{});
-        if constexpr (sizeof(T) <= 4)
-            if (v == 4) go(std::integral_constant<int, 4>{});
         if constexpr (sizeof(T) == 2)
-            if (v == 8) go(std::integral_constant<int, 8>{});
-        return cudaGetLastError();
+            if (v == 8) return go(std::integral_constant<int, 8>{});
+        if constexpr (sizeof(T) <= 4)
+            if (v == 4) return go(std::integral_constant<int, 4>{});
+        return v == 2 ? go(std::integral_constant<int, 2>{}) : go(std::integral_constant<int, 1>{});
     }));
 }
 
