@@ -113,8 +113,101 @@ __global__ void __launch_bounds__(kThreads) drop_vectors_kernel(const Rows a, co
     }
 }
 
-// Rows that do not start on 16 bytes, or are not made of whole eights: a warp
-// takes 256 values of one row, lane by lane.
+// 16-bit rows that do not start on 16 bytes, or are not made of whole eights:
+// `lanes` lanes (a power of two) put together lanes - 1 aligned chunks of eight
+// values of y. Each loads the aligned chunk of x (and of the residual) in which
+// its values start and takes the rest from its neighbour's; so it does with the
+// draws, whose blocks lie as they like too. The last lane only lends. Chunks that
+// reach over a row's ends are written, and those over the array's ends read,
+// value by value.
+template <typename T>
+__device__ __forceinline__ Vec<T, 8> load_chunk(const T *base, const T *whole_end, const T *start, int cols, int column) {
+    const int shift = (int)((((uintptr_t)start >> 1) + column) & 7), first = column - shift;
+    Vec<T, 8> own = Vec<T, 8>::zero();
+    if (first + 8 > 0 && first < cols) {
+        const T *from = start + first;
+        if ((first >= 0 && first + 8 <= cols) || (from >= base && from + 8 <= whole_end)) {
+            own = load<T, 8>(from);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (first + j >= 0 && first + j < cols)
+                    own.w[j / 2] |= (uint32_t) * (const unsigned short *)(from + j) << (j % 2 * 16);
+        }
+    }
+    return own;
+}
+template <typename T>
+__device__ __forceinline__ Vec<T, 8> join_chunk(const Vec<T, 8> &own, const T *start, int column) {
+    Vec<T, 8> next;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) next.w[k] = __shfl_down_sync(0xffffffffu, own.w[k], 1);
+    return shifted(own, next, (uint32_t)((((uintptr_t)start >> 1) + column) & 7) * 2);
+}
+template <typename T, bool RESIDUAL>
+__global__ void __launch_bounds__(kThreads) drop_chunks_kernel(const Rows a, const Drop drop, uint32_t lane_bits, uint32_t pieces) {
+    const uint64_t offset = drop_offset(drop);
+    const float scale = (float)drop.scale;
+    const uint32_t lanes = 1u << lane_bits, lane = threadIdx.x & (lanes - 1);
+    const int cols = (int)a.cols;
+    const size_t count = a.rows * pieces, step = (size_t)gridDim.x * (kThreads >> lane_bits);
+    const T *x_end = (const T *)a.x + (a.rows - 1) * a.x_stride + cols;
+    const T *residual_end = (const T *)a.residual + (a.rows - 1) * a.residual_stride + cols;
+    // A piece's row and first column, and its chunks, on their way while the piece before is worked on.
+    struct Piece {
+        size_t row;
+        int c;
+        Vec<T, 8> x, residual;
+    };
+    auto fetch = [&](size_t first) {
+        const size_t piece = first + ((threadIdx.x & 31) >> lane_bits);
+        const bool live = piece < count;
+        Piece p;
+        p.row = live ? piece : 0;
+        if (pieces > 1) p.row = count <= 0xFFFFFFFFu ? (uint32_t)p.row / pieces : p.row / pieces;
+        const int back = (int)((uintptr_t)((T *)a.y + p.row * a.y_stride) >> 1 & 7);
+        p.c = live ? (int)((uint32_t)(piece - p.row * pieces) * (lanes - 1) + lane) * 8 - back : cols;
+        p.x = load_chunk((const T *)a.x, x_end, (const T *)a.x + p.row * a.x_stride, cols, p.c);
+        if constexpr (RESIDUAL)
+            p.residual = load_chunk((const T *)a.residual, residual_end,
+                                    (const T *)a.residual + p.row * a.residual_stride, cols, p.c);
+        return p;
+    };
+    // The bound is the warp's first piece, so that all its lanes stay for the shuffles.
+    const size_t begin = blockIdx.x * (size_t)(kThreads >> lane_bits) + (threadIdx.x >> 5 << (5 - lane_bits));
+    Piece next = fetch(begin);
+    for (size_t first = begin; first < count; first += step) {
+        const Piece p = next;
+        if (first + step < count) next = fetch(first + step);
+        const size_t row = p.row;
+        const int c = p.c;
+        T *y = (T *)a.y + row * a.y_stride;
+        const Vec<T, 8> x = join_chunk(p.x, (const T *)a.x + row * a.x_stride, c);
+        Vec<T, 8> residual = x;
+        if constexpr (RESIDUAL) residual = join_chunk(p.residual, (const T *)a.residual + row * a.residual_stride, c);
+        const uint64_t e = row * (uint64_t)cols + (int64_t)c;
+        const uint32_t mine = kept_of_eight(drop, offset, e & ~(uint64_t)7);
+        const uint32_t kept = (mine | __shfl_down_sync(0xffffffffu, mine, 1) << 8) >> ((uint32_t)e & 7u);
+        Vec<T, 8> out;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            Pair<float> v = x.pair(q);
+            v.x = (kept >> (2 * q)) & 1 ? v.x : 0.0f;
+            v.y = (kept >> (2 * q + 1)) & 1 ? v.y : 0.0f;
+            out.set(q, RESIDUAL ? fma(v, both(scale), residual.pair(q)) : v * both(scale));
+        }
+        if (lane == lanes - 1 || c >= cols || c + 8 <= 0) continue;
+        if (c >= 0 && c + 8 <= cols) {
+            store<T, 8>(y + c, out);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (c + j >= 0 && c + j < cols) store_value<T, 8>(y + c + j, out, j);
+        }
+    }
+}
+
+// Wider values off 16 bytes: a warp takes 256 values of one row, lane by lane.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) drop_values_kernel(const Rows a, const Drop drop) {
     using W = Wide<T>;
@@ -166,6 +259,18 @@ cudaError_t launch(uint32_t type, const void *x, size_t x_stride, const void *re
                 drop_vectors_kernel<T, false, true><<<(unsigned)grid, kThreads, 0, stream>>>(a, drop);
             else
                 drop_vectors_kernel<T, false, false><<<(unsigned)grid, kThreads, 0, stream>>>(a, drop);
+        } else if constexpr (sizeof(T) == 2) {
+            a.rows = rows, a.cols = cols;  // row by row, packed or not: a row's columns fit 32 bits
+            uint32_t lane_bits = 1;
+            while (lane_bits < 5 && (1u << lane_bits) - 1 < (cols + 14) / 8) ++lane_bits;
+            const uint32_t whole = (1u << lane_bits) - 1, pieces = ((uint32_t)(cols + 14) / 8 + whole - 1) / whole;
+            const size_t each = kThreads >> lane_bits, blocks = (rows * pieces + each - 1) / each;
+            const size_t most = (size_t)geo::device_sm_count() * 12;  // twice the resident ones
+            const unsigned grid = (unsigned)(blocks < most ? blocks : most);
+            if (residual != nullptr)
+                drop_chunks_kernel<T, true><<<grid, kThreads, 0, stream>>>(a, drop, lane_bits, pieces);
+            else
+                drop_chunks_kernel<T, false><<<grid, kThreads, 0, stream>>>(a, drop, lane_bits, pieces);
         } else {
             const size_t pieces = a.rows * ((a.cols + 255) / 256), blocks = (pieces + kThreads / 32 - 1) / (kThreads / 32);
             drop_values_kernel<T><<<(unsigned)(blocks < 0x7fffffff ? blocks : 0x7fffffff), kThreads, 0, stream>>>(a, drop);

@@ -264,7 +264,7 @@ cudaError_t launch(NormTypes n, const ForwardArgs &a, cudaStream_t stream) {
             constexpr int resident = resident_threads(sizeof(T), S, G), at_once = rows_at_once(sizeof(T), S, G);
             const size_t stage = (DROP ? 2 : 1) * s.part(sizeof(T));
             const int stages = ring_stages(stage, at_once, s.threads(), resident);
-            const size_t wanted = (a.rows + s.teams() - 1) / s.teams();
+            const size_t each = s.teams() * at_once, wanted = (a.rows + each - 1) / each;
             const size_t most = (size_t)geo::device_sm_count() * (resident / s.threads()) / s.blocks;
             return launch_team(norm_kernel<T, DROP, G, S, F>, s, wanted < most ? wanted : most, stages * stage, stream,
                                a, s.lanes, float_parameters, stages);

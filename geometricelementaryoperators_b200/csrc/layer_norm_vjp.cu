@@ -152,6 +152,8 @@ __global__ void __launch_bounds__(TEAM == kWarp ? kWarpBlock : kTeamThreads, TEA
     }
     close_exchange<TEAM>();
     if (partial == nullptr) return;
+    // The kernel that joins the partial sums may be set up from here on.
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     W *mine = partial + at.slice * 2 * a.cols;
     auto value = [&](const Pair<W> (&p)[Q], int e) { return e & 1 ? p[e / 2].y : p[e / 2].x; };
     if constexpr (TEAM >= kBlock) {
@@ -192,17 +194,17 @@ __global__ void __launch_bounds__(TEAM == kWarp ? kWarpBlock : kTeamThreads, TEA
 }
 
 // out[c] = sum over the blocks of partial[block][which][c]. `wide` columns a
-// block of threads, 1024 / wide threads a column, each over every so many
-// blocks in order, then those in order.
+// block of threads, blockDim / wide threads a column, each over every so many
+// blocks in order, then those as a tree.
 template <typename W, typename P>
 __global__ void __launch_bounds__(1024) join_columns_kernel(const W *partial, int blocks, int cols, int wide,
                                                             void *dweight, void *dbias) {
     __shared__ W sums[1024];
     P *out = (P *)(blockIdx.y == 0 ? dweight : dbias);
-    if (out == nullptr) return;
-    const int column = threadIdx.x & (wide - 1), part = threadIdx.x / wide, parts = 1024 / wide;
+    const int column = threadIdx.x & (wide - 1), part = threadIdx.x / wide, parts = blockDim.x / wide;
     const int c = (int)blockIdx.x * wide + column;
     W sum = 0;
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // for the kernel before to end
     if (c < cols) {
 #pragma unroll 8
         for (int i = part; i < blocks; i += parts) sum += partial[((size_t)i * 2 + blockIdx.y) * cols + c];
@@ -212,9 +214,8 @@ __global__ void __launch_bounds__(1024) join_columns_kernel(const W *partial, in
         __syncthreads();
         if (part < n) sums[threadIdx.x] += sums[threadIdx.x + n * wide];
     }
-    if (part == 0 && c < cols) out[c] = narrow<P>((Wide<P>)sums[threadIdx.x]);
+    if (part == 0 && c < cols && out != nullptr) out[c] = narrow<P>((Wide<P>)sums[threadIdx.x]);
 }
-
 
 // ---- rows of any length --------------------------------------------------------
 
@@ -296,8 +297,8 @@ size_t column_blocks(size_t rows, size_t cols) {
 
 // Teams (blocks of teams, kWarp) of the pass: as many as 512 threads a
 // multiprocessor make, each with a partial sum of the columns.
-size_t team_grid(const Shape &s, size_t rows) {
-    const size_t wanted = (rows + s.teams() - 1) / s.teams();
+size_t team_grid(const Shape &s, size_t bytes, size_t rows) {
+    const size_t each = s.teams() * rows_at_once(bytes, s.shift, s.team()), wanted = (rows + each - 1) / each;
     const size_t most = (size_t)geo::device_sm_count() * (512 / s.threads()) / s.blocks;
     return wanted < most ? wanted : most;
 }
@@ -319,7 +320,7 @@ cudaError_t launch(NormTypes n, const BackwardArgs &a, void *workspace, cudaStre
         size_t blocks = 0;
         cudaError_t e = cudaSuccess;
         if (s.lanes != 0) {
-            blocks = team_grid(s, a.rows);
+            blocks = team_grid(s, bytes, a.rows);
             W *partial = sums ? (W *)workspace : nullptr;
             e = by_shape(s, [&](auto team, auto shift, auto full) {
                 constexpr int G = decltype(team)::value;
@@ -343,11 +344,22 @@ cudaError_t launch(NormTypes n, const BackwardArgs &a, void *workspace, cudaStre
             e = cudaGetLastError();
         }
         if (e != cudaSuccess || !sums) return e;
+        // Launched while the pass still runs: its start-up is over when the sums are there.
+        // Whole 128-byte lines where there are enough columns for that; about eight partial sums a thread.
         const int wide = a.cols >= 2048 ? 32 : 8;
-        const dim3 join((unsigned)((a.cols + wide - 1) / wide), 2);
-        join_columns_kernel<W, P><<<join, 1024, 0, stream>>>((const W *)workspace, (int)blocks, a.cols, wide,
-                                                             a.dweight, a.dbias);
-        return cudaGetLastError();
+        int parts = 8;
+        while (parts < 1024 / wide && (size_t)parts * 8 < blocks) parts *= 2;
+        cudaLaunchConfig_t config = {};
+        config.gridDim = dim3((unsigned)((a.cols + wide - 1) / wide), 2);
+        config.blockDim = dim3((unsigned)(wide * parts));
+        config.stream = stream;
+        cudaLaunchAttribute attribute = {};
+        attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attribute.val.programmaticStreamSerializationAllowed = 1;
+        config.attrs = &attribute;
+        config.numAttrs = 1;
+        return cudaLaunchKernelEx(&config, join_columns_kernel<W, P>, (const W *)workspace, (int)blocks, a.cols, wide,
+                                  a.dweight, a.dbias);
     });
 }
 
@@ -360,7 +372,7 @@ size_t vjp_workspace(NormTypes t, size_t rows, size_t cols) {
     for (const bool aligned : {false, true}) {
         if (aligned && cols * bytes % 16 != 0) continue;
         const Shape s = shape_of(cols, bytes, aligned);
-        const size_t n = s.lanes != 0 ? team_grid(s, rows) : column_blocks(rows, cols);
+        const size_t n = s.lanes != 0 ? team_grid(s, bytes, rows) : column_blocks(rows, cols);
         if (n > blocks) blocks = n;
     }
     return blocks * 2 * cols * wide_bytes(t.type);

@@ -178,6 +178,37 @@ __device__ __forceinline__ void store(T *p, const Vec<T, V> &v) {
     else
         *reinterpret_cast<unsigned short *>(p) = (unsigned short)v.w[0];
 }
+
+// Bytes [shift, shift + 16) of 32, shift a multiple of the value size below 16.
+template <typename T, int V>
+__device__ __forceinline__ Vec<T, V> shifted(const Vec<T, V> &low, const Vec<T, V> &high, uint32_t shift) {
+    uint32_t w[8] = {low.w[0], low.w[1], low.w[2], low.w[3], high.w[0], high.w[1], high.w[2], high.w[3]};
+#pragma unroll
+    for (int k = 0; k < 6; ++k) w[k] = (shift & 8) ? w[k + 2] : w[k];
+    if constexpr (sizeof(T) <= 4) {
+#pragma unroll
+        for (int k = 0; k < 5; ++k) w[k] = (shift & 4) ? w[k + 1] : w[k];
+    }
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) w[k] = __funnelshift_r(w[k], w[k + 1], (shift & 2) * 8);
+    }
+    Vec<T, V> r;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) r.w[k] = w[k];
+    return r;
+}
+
+// Value j of a vector, as it is stored.
+template <typename T, int V>
+__device__ __forceinline__ void store_value(T *p, const Vec<T, V> &v, int j) {
+    if constexpr (sizeof(T) == 8)
+        *reinterpret_cast<uint2 *>(p) = make_uint2(v.w[2 * j], v.w[2 * j + 1]);
+    else if constexpr (sizeof(T) == 4)
+        *reinterpret_cast<uint32_t *>(p) = v.w[j];
+    else
+        *reinterpret_cast<unsigned short *>(p) = (unsigned short)(v.w[j / 2] >> (j % 2 * 16));
+}
 #endif
 
 inline size_t type_bytes(uint32_t type) {
