@@ -191,6 +191,7 @@ __global__ void __launch_bounds__(TEAM == kWarp ? kWarpBlock : kTeamThreads,
             store_row<T, V, K, SHIFT, FULL>((T *)a.y + row * a.y_stride, at, live, a.cols, out);
         }
     }
+    wait_async<0>();
     close_exchange<TEAM>();
 }
 

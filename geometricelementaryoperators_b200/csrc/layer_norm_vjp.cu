@@ -150,6 +150,7 @@ __global__ void __launch_bounds__(TEAM == kWarp ? kWarpBlock : kTeamThreads, TEA
         }
         ring.done();
     }
+    wait_async<0>();
     close_exchange<TEAM>();
     if (partial == nullptr) return;
     // The kernel that joins the partial sums may be set up from here on.
@@ -172,7 +173,6 @@ __global__ void __launch_bounds__(TEAM == kWarp ? kWarpBlock : kTeamThreads, TEA
         const int each = blockDim.x;
         W *found = (W *)memory;
         auto place = [&](int e, int thread) { return e * each + (thread ^ (e & 31)); };
-        wait_async<0>();
         __syncthreads();
 #pragma unroll
         for (int e = 0; e < K * V; ++e) {

@@ -99,10 +99,13 @@ KINDS = [("f64", "f64"), ("f32", "f32"), ("bf16", "bf16"), ("bf16", "f32"), ("f1
 SHAPES = [(1, 1, 0), (3, 1, 0), (5, 7, 0), (1, 64, 0), (130, 64, 0), (1, 1024, 0), (33, 96, 1), (9, 333, 0), (7, 1000, 8),
           (300, 128, 0), (17, 2056, 0), (40, 1003, 1), (3, 5120, 0), (2, 8192, 0), (5, 16384, 0), (2, 16381, 3),
           (2000, 40, 0), (4100, 16, 0), (6, 20008, 0), (700, 257, 0)]
+# Many rows for every team of threads, so that each takes several: part of a block, a block, clusters of 2 to 8 blocks.
+LONG = [(4100, 520, 0), (3001, 1003, 1), (1500, 4096, 0), (1300, 4001, 1), (1000, 5120, 0), (701, 16384, 0), (900, 8193, 1),
+        (333, 32768, 0)]
 
 
 @pytest.mark.parametrize("kind,pkind", KINDS)
-@pytest.mark.parametrize("rows,cols,pad", SHAPES)
+@pytest.mark.parametrize("rows,cols,pad", SHAPES + LONG)
 def test_layer_norm(kind, pkind, rows, cols, pad):
     dtype, ptype = ref.torch_type(kind), ref.torch_type(pkind)
     x = make(rows, cols, dtype, pad, seed=cols, shift=0.5)
@@ -122,7 +125,7 @@ def test_layer_norm(kind, pkind, rows, cols, pad):
 
 
 @pytest.mark.parametrize("kind,pkind", KINDS)
-@pytest.mark.parametrize("rows,cols,pad", SHAPES)
+@pytest.mark.parametrize("rows,cols,pad", SHAPES + LONG)
 def test_layer_norm_vjp(kind, pkind, rows, cols, pad):
     t = torch()
     dtype, ptype = ref.torch_type(kind), ref.torch_type(pkind)
@@ -195,6 +198,84 @@ def test_layer_norm_in_place_and_without_parameters(kind, cols, pad):
         outs.append((o.clone(), dw, db))
     for o in outs[1:]:
         assert all(torch().equal(p, q) for p, q in zip(outs[0], o))
+
+
+@pytest.mark.parametrize("kind,pkind", KINDS)
+@pytest.mark.parametrize("cols", [8, 72, 1000, 5120])
+def test_layer_norm_parameters_off_16_bytes(kind, pkind, cols):
+    """Weight, bias and their cotangents start one value into their arrays: the values of aligned ones, in the bounds."""
+    t = torch()
+    dtype, ptype = ref.torch_type(kind), ref.torch_type(pkind)
+    x, dy = make(37, cols, dtype, seed=1), make(37, cols, dtype, seed=2)
+    w, b = (v[1:] for v in parameters(cols + 1, ptype))
+    y, _ = like(x)
+    mean, rstd = stats_like(x)
+    c = norm_config(x, ptype)
+    call("geo_b200_layer_norm", ctypes.byref(c), P(x), P(w), P(b), P(y), P(mean), P(rstd))
+    want = ref.norm(x.double(), w.double(), b.double(), EPS)
+    ref.assert_within(y, want[0], ref.norm_bound(x.double(), w.double(), b.double(), want[2], want[0], dtype)[0])
+    space, size = workspace(c)
+    whole = t.full((2, cols + 2), 7.0, device="cuda", dtype=ptype)
+    dw, db = whole[0, 1:-1], whole[1, 1:-1]
+    dx, _ = like(x)
+    call("geo_b200_layer_norm_vjp", ctypes.byref(c), P(x), P(w), P(mean), P(rstd), P(dy), P(dx), P(dw), P(db), P(space),
+         size)
+    wide = [v.double() for v in (x, w, mean, rstd, dy)]
+    want = ref.norm_vjp(*wide)
+    bounds = ref.norm_vjp_bound(*wide, want[0], dtype)
+    u = ref.half_step(ptype)
+    ref.assert_within(dx, want[0], bounds[0], "dx")
+    ref.assert_within(dw, want[1], bounds[1] + u * want[1].abs() + ref.least(ptype), "dweight")
+    ref.assert_within(db, want[2], bounds[2] + u * want[2].abs() + ref.least(ptype), "dbias")
+    assert (whole[:, 0] == 7).all() and (whole[:, -1] == 7).all()
+
+
+@pytest.mark.parametrize("kind", ["f64", "f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows,cols,pads", [(50, 100, (1, 0, 3, 2)), (9, 1003, (0, 5, 1, 2)), (40, 64, (8, 1, 0, 4)),
+                                            (7, 5001, (2, 3, 0, 1)), (130, 13, (0, 1, 2, 3))])
+def test_arrays_of_unlike_alignment(kind, rows, cols, pads):
+    """Each array with a stride and an alignment of its own: the bits of packed arrays' dropout, the fused call and its
+    VJP within their bounds, and nothing written beside the rows."""
+    t = torch()
+    dtype = ref.torch_type(kind)
+    x, res, dy, dz = (make(rows, cols, dtype, p, seed=i) for i, p in enumerate(pads))
+    packed = [v.contiguous() for v in (x, res, dy, dz)]
+    w, b = parameters(cols, dtype)
+    strides = [v.stride(0) for v in (x, res, dy, dz)]
+    outs = [like(v) for v in (res, dy, dz, x)]  # z, y, dresidual, dx
+    so = [strides[1], strides[2], strides[3], strides[0]]
+    d = drop_config(x, 0.3, x_stride=strides[0], residual_stride=strides[1], y_stride=so[0],
+                    y_cotangent_stride=strides[3], x_cotangent_stride=so[3])
+    n = norm_config(x, dtype, x_stride=so[0], y_stride=so[1], y_cotangent_stride=strides[2], x_cotangent_stride=so[2])
+    dp, np_ = drop_config(packed[0], 0.3), norm_config(packed[0], dtype)
+    z, _ = like(packed[0])
+    call("geo_b200_dropout", ctypes.byref(d), P(x), P(res), None, P(outs[0][0]))
+    call("geo_b200_dropout", ctypes.byref(dp), P(packed[0]), P(packed[1]), None, P(z))
+    assert t.equal(outs[0][0], z)
+    mean, rstd = stats_like(x)
+    call("geo_b200_residual_dropout_layer_norm", ctypes.byref(n), ctypes.byref(d), P(x), P(res), None, P(w), P(b),
+         P(outs[0][0]), P(outs[1][0]), P(mean), P(rstd))
+    assert t.equal(outs[0][0], z)
+    keep = mask(dp)
+    exact_z = drop_reference(packed[0].double(), packed[1].double(), keep, 0.3)
+    want = ref.norm(exact_z, w.double(), b.double(), EPS)
+    bound = ref.norm_bound(exact_z, w.double(), b.double(), want[2], want[0], dtype, 2 * ref.PATH)[0]
+    ref.assert_within(outs[1][0], want[0], bound, "y")
+    space, size = workspace(n)
+    dw, db = t.empty_like(w), t.empty_like(b)
+    call("geo_b200_residual_dropout_layer_norm_vjp", ctypes.byref(n), ctypes.byref(d), None, P(outs[0][0]), P(w), P(mean),
+         P(rstd), P(dy), P(dz), P(outs[2][0]), P(outs[3][0]), P(dw), P(db), P(space), size)
+    wide = [v.double() for v in (z, w, mean, rstd, packed[2])]
+    norm_dx, want_dw, want_db = ref.norm_vjp(*wide)
+    total = norm_dx + packed[3].double()
+    bounds = ref.norm_vjp_bound(*wide, total, dtype)
+    ref.assert_within(outs[2][0], total, bounds[0] + ref.u_wide(dtype) * total.abs(), "dresidual")
+    assert bool((outs[3][0][~keep] == 0).all())
+    u = ref.half_step(dtype)
+    ref.assert_within(dw, want_dw, bounds[1] + u * want_dw.abs() + ref.least(dtype), "dweight")
+    ref.assert_within(db, want_db, bounds[2] + u * want_db.abs() + ref.least(dtype), "dbias")
+    for _, whole in outs:
+        assert untouched(whole, cols)
 
 
 @pytest.mark.parametrize("cols", [16, 100, 1024, 5000, 20000])
@@ -360,7 +441,8 @@ def test_dropout_units_past_32_bits():
 
 FUSED = [(1, 1, 0, 0), (3, 7, 0, 0), (1, 1024, 0, 0), (130, 64, 0, 6), (33, 96, 1, 3), (9, 333, 0, 0), (7, 1000, 8, 2),
          (300, 128, 0, 5), (40, 1003, 1, 0), (3, 5120, 0, 0), (5, 16384, 0, 1), (2, 16381, 3, 0), (6, 20008, 0, 3),
-         (2000, 40, 0, 1), (700, 258, 0, 1)]
+         (2000, 40, 0, 1), (700, 258, 0, 1), (4100, 520, 0, 3), (3001, 1003, 1, 0), (1500, 4096, 0, 0), (1000, 5120, 0, 6),
+         (701, 16384, 0, 0), (900, 8193, 1, 0)]
 
 
 @pytest.mark.parametrize("kind,pkind", KINDS)
