@@ -117,7 +117,6 @@ __global__ void __launch_bounds__(TEAM == kWarp ? kWarpBlock : kTeamThreads,
             for (int q = 0; q < Q; ++q) two = two + v[u][q];
             sum[u] = two.x + two.y;
         }
-        ring.done();
         // Two sweeps over registers: the mean of what the warp (or its team)
         // holds, then the squares about it. Values past the row are 0 in the
         // first, the mean itself in the second.
@@ -183,13 +182,14 @@ __global__ void __launch_bounds__(TEAM == kWarp ? kWarpBlock : kTeamThreads,
             if constexpr (DROP) {
 #pragma unroll
                 for (int q = 0; q < Q; ++q) set_pair(out, q, v[u][q]);
-                store_row<T, V, K, SHIFT, FULL>((T *)a.z + row * a.z_stride, at, live, a.cols, out);
+                ring.put((T *)a.z + row * a.z_stride, live, u, 0, out);
             }
 #pragma unroll
             for (int q = 0; q < Q; ++q)
                 set_pair(out, q, fma((v[u][q] + both(-mean[u])) * both(rstd[u]), w[q], b[q]));
-            store_row<T, V, K, SHIFT, FULL>((T *)a.y + row * a.y_stride, at, live, a.cols, out);
+            ring.put((T *)a.y + row * a.y_stride, live, u, DROP ? 1 : 0, out);
         }
+        ring.done();
     }
     wait_async<0>();
     close_exchange<TEAM>();

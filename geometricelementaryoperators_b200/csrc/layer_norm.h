@@ -17,13 +17,12 @@
 // take two rows of 16-bit values at a time: one barrier for both, two chains of
 // additions side by side.
 //
-// Rows that do not start on 16 bytes (SHIFT) are moved in the aligned 16-byte
-// chunks that they lie in, by the warp whose part they hold, one more than the
-// part has vectors; a thread takes its vector out of two neighbouring chunks by
-// shifting, and puts one together for storing from its own and its neighbour's
-// vector. A chunk that is shared with another warp's part or another row is
-// written value by value. The first and last chunk of an array, which may reach
-// over its ends, are read value by value.
+// Rows that do not start on 16 bytes (SHIFT) are moved in words of 4 bytes (8 in
+// float64), neighbouring lanes neighbouring words, into and out of shared memory,
+// where a unit's part starts on 16 bytes and threads find their vectors. Only a
+// 16-bit row that starts in the middle of a word needs shifting, by one value;
+// the half of a word that belongs to someone else is not written, and a word that
+// reaches over an end of the array is read value by value.
 #pragma once
 
 #include <cooperative_groups.h>
@@ -230,6 +229,17 @@ __device__ __forceinline__ void set_past(Pair<W> (&v)[K * V / 2], const Place<TE
     }
 }
 
+// SHIFT: the word that moves values, how many a thread moves (one more where a
+// row of 16-bit values starts in the middle of a word), and whether it does.
+template <typename T>
+using Word = std::conditional_t<sizeof(T) == 8, uint64_t, uint32_t>;
+template <typename T, int V, int K>
+constexpr int kWords = K * V * (int)sizeof(T) / (int)sizeof(Word<T>) + (sizeof(T) == 2 ? 1 : 0);
+template <typename T>
+__device__ __forceinline__ int half_word(const T *p) {
+    return sizeof(T) == 2 ? (int)((uintptr_t)p >> 1 & 1) : 0;
+}
+
 // The slots of one thread, for `arrays` arrays of rows.
 template <typename T, int V, int K, int TEAM, bool SHIFT, bool FULL, int R>
 struct Ring {
@@ -257,21 +267,34 @@ struct Ring {
         const bool live = row < rows;
         const uint32_t slot = shared_address(slots) + write * next_stage + array * next_array;
         if constexpr (SHIFT) {
-            if (!live) return;
-            const T *start = base + row * stride, *first = start + at.unit_first, *end = start + cols;
-            const T *chunk = (const T *)((uintptr_t)first & ~(uintptr_t)15) + at.unit_lane * V;
-            const T *whole_end = base + (rows - 1) * stride + cols;
+            const int left = cols - at.unit_first;
+            if (!live || left <= 0) return;
+            constexpr int kPerWord = (int)(sizeof(Word<T>) / sizeof(T)), kBytes = (int)sizeof(Word<T>);
+            const T *first = base + row * stride + at.unit_first;
+            const int part = at.unit_lanes * K * V, held = left < part ? left : part, half = half_word(first);
+            const int words = (held + half + kPerWord - 1) / kPerWord, gap = TEAM == kWarp ? at.unit_lanes : 32;
+            const Word<T> *from = (const Word<T> *)(first - half) + at.unit_lane;
+            const uint32_t to = slot + at.unit_lane * (kBytes - 16);
+            // The array's first and last word may reach over its ends.
+            const bool ends = sizeof(T) == 2 && (row == 0 || row == rows - 1);
+            if (!ends) {
 #pragma unroll
-            for (int i = 0; i <= K; ++i) {
-                const T *from = chunk + i * (int)(vector_gap() / sizeof(T));
-                if ((i == K && at.unit_lane != 0) || from >= end) continue;
-                if (from < base || from + V > whole_end) {
-                    unsigned char *to = const_cast<unsigned char *>(slots) + write * next_stage + array * next_array +
-                                        i * vector_gap();
-                    for (int j = 0; j < V; ++j)
-                        if (from + j >= start && from + j < end) ((T *)to)[j] = from[j];
-                } else {
-                    copy_async(slot + i * vector_gap(), from, true);
+                for (int k = 0; k < kWords<T, V, K>; ++k)
+                    if (k * gap + at.unit_lane < words) copy_async<kBytes>(to + k * gap * kBytes, from + k * gap);
+            } else {
+                const T *whole_end = base + (rows - 1) * stride + cols;
+#pragma unroll 1
+                for (int w = 0; w + at.unit_lane < words; w += gap) {
+                    const T *word = (const T *)(from + w);
+                    if (word >= base && word + kPerWord <= whole_end) {
+                        copy_async<kBytes>(to + w * kBytes, word);
+                    } else {
+                        for (int j = 0; j < kPerWord; ++j)
+                            if (word + j >= base && word + j < whole_end)
+                                asm volatile("st.shared.u16 [%0], %1;" ::"r"(to + w * kBytes + j * (int)sizeof(T)),
+                                             "h"(*(const unsigned short *)(word + j))
+                                             : "memory");
+                    }
                 }
             }
         } else {
@@ -303,11 +326,57 @@ struct Ring {
     // global memory. SHIFT: what is past the row's end is anything.
     __device__ __forceinline__ void get(Vec<T, V> (&out)[K], int u, int array, const T *row_start) const {
         const unsigned char *from = slots + (read + u) * next_stage + array * next_array;
-        const uint32_t shift = SHIFT ? (uint32_t)(uintptr_t)(row_start + at.unit_first) & 15 : 0;
+        const uint32_t shift = SHIFT ? 16u * half_word(row_start + at.unit_first) : 0;
 #pragma unroll
         for (int i = 0; i < K; ++i) {
             out[i] = load<T, V>((const T *)(from + i * vector_gap()));
-            if constexpr (SHIFT) out[i] = shifted(out[i], load<T, V>((const T *)(from + i * vector_gap() + 16)), shift);
+            if constexpr (SHIFT && sizeof(T) == 2) {
+                const uint32_t next = *(const uint32_t *)(from + i * vector_gap() + 16);
+#pragma unroll
+                for (int w = 0; w < 4; ++w)
+                    out[i].w[w] = __funnelshift_r(out[i].w[w], w < 3 ? out[i].w[w + 1] : next, shift);
+            }
+        }
+    }
+    // The thread's part of a row to global memory; SHIFT: through the place of
+    // array `array` of row u, which has been read (every lane of the warp takes part).
+    __device__ __forceinline__ void put(T *row_start, bool live, int u, int array, const Vec<T, V> (&v)[K]) const {
+        if constexpr (SHIFT) {
+            constexpr int kPerWord = (int)(sizeof(Word<T>) / sizeof(T));
+            unsigned char *vectors = const_cast<unsigned char *>(slots) + (read + u) * next_stage + array * next_array;
+            __syncwarp();  // the neighbours have read their vectors
+#pragma unroll
+            for (int i = 0; i < K; ++i) store<T, V>((T *)(vectors + i * vector_gap()), v[i]);
+            __syncwarp();
+            const int part = at.unit_lanes * K * V, left = cols - at.unit_first, held = left < part ? left : part;
+            if (!live || held <= 0) return;
+            T *first = row_start + at.unit_first;
+            const int half = half_word(first), gap = TEAM == kWarp ? at.unit_lanes : 32;
+            const Word<T> *words = (const Word<T> *)(vectors - at.unit_lane * 16) + at.unit_lane;
+            Word<T> *to = (Word<T> *)(first - half) + at.unit_lane;
+            // Word w of the row holds values w kPerWord - half and on: with half, the
+            // upper half of word w - 1 here and the lower half of word w. Whole ones:
+            const int begin = half, end = (held + half) / kPerWord;
+#pragma unroll
+            for (int k = 0; k < kWords<T, V, K>; ++k) {
+                const int w = k * gap + at.unit_lane;
+                if (w >= end || (k == 0 && w < begin)) continue;
+                if constexpr (sizeof(T) == 2)
+                    to[k * gap] = __funnelshift_r(words[k * gap - half], words[k * gap], 16 * half);
+                else
+                    to[k * gap] = words[k * gap];
+            }
+            if constexpr (sizeof(T) == 2) {  // and the halves at both ends
+                const unsigned short *values = (const unsigned short *)(words - at.unit_lane);
+                if (half && at.unit_lane == 0) *(unsigned short *)first = values[0];
+                if (((held + half) & 1) && at.unit_lane == at.unit_lanes - 1)
+                    *(unsigned short *)(first + held - 1) = values[held - 1];
+            }
+        } else {
+            T *to = row_start + at.column(0);
+#pragma unroll
+            for (int i = 0; i < K; ++i)
+                if (live && (FULL || at.column(i) < cols)) store<T, V>(to + (at.column(i) - at.column(0)), v[i]);
         }
     }
     __device__ __forceinline__ void done() {
@@ -452,48 +521,6 @@ __device__ __forceinline__ void drop_row(const Drop &drop, uint64_t offset, uint
 #pragma unroll
             for (int q = 0; q < V / 2; ++q) v[i * V / 2 + q] = drop_pair(v[i * V / 2 + q], draws[q], drop.bound);
         }
-    }
-}
-
-// The thread's part of a row to global memory (every lane of the warp takes part).
-template <typename T, int V, int K, bool SHIFT, bool FULL, int TEAM>
-__device__ __forceinline__ void store_row(T *row_start, const Place<TEAM, V, K> &at, bool live, int cols,
-                                          const Vec<T, V> (&v)[K]) {
-    if constexpr (SHIFT) {
-        // Chunk (i, lane) begins `back` values before the thread's vector i: the
-        // end of the vector before it, then its own beginning.
-        const uint32_t shift = (uint32_t)(uintptr_t)(row_start + at.unit_first) & 15;
-        const int back = (int)(shift / sizeof(T));
-        const int from = at.unit_first, last = at.unit_first + at.unit_lanes * K * V;
-        const int to = last < cols ? last : cols;  // the unit's columns are [from, to)
-        const int before = ((int)threadIdx.x & 31 & ~(at.unit_lanes - 1)) + ((at.unit_lane - 1) & (at.unit_lanes - 1));
-#pragma unroll
-        for (int i = 0; i <= K; ++i) {
-            Vec<T, V> previous, out;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                // Lane 0's previous vector is the last lane's of the round before.
-                const uint32_t other = i > 0 ? v[i > 0 ? i - 1 : 0].w[k] : 0u, own = i < K ? v[i < K ? i : 0].w[k] : 0u;
-                previous.w[k] =
-                    __shfl_sync(0xffffffffu, at.unit_lane == at.unit_lanes - 1 ? other : own, before);
-                out.w[k] = own;
-            }
-            if (shift != 0) out = shifted(previous, out, 16 - shift);
-            const int start = from + (i * at.unit_lanes + at.unit_lane) * V - back;
-            if (!live || (i == K && at.unit_lane != 0) || start >= to) continue;
-            if (start >= from && start + V <= to) {
-                store<T, V>(row_start + start, out);
-            } else {
-#pragma unroll
-                for (int j = 0; j < V; ++j)
-                    if (start + j >= from && start + j < to) store_value<T, V>(row_start + start + j, out, j);
-            }
-        }
-    } else {
-        T *to = row_start + at.column(0);
-#pragma unroll
-        for (int i = 0; i < K; ++i)
-            if (live && (FULL || at.column(i) < cols)) store<T, V>(to + (at.column(i) - at.column(0)), v[i]);
     }
 }
 

@@ -137,14 +137,14 @@ __global__ void __launch_bounds__(TEAM == kWarp ? kWarpBlock : kTeamThreads, TEA
             if (a.dsum != nullptr) {
 #pragma unroll
                 for (int q = 0; q < Q; ++q) set_pair(x, q, v[q]);
-                store_row<T, V, K, SHIFT, FULL>((T *)a.dsum + row * a.dsum_stride, at, live, a.cols, x);
+                ring.put((T *)a.dsum + row * a.dsum_stride, live, u, 0, x);
             }
             if constexpr (DROP) {
                 if (a.dx != nullptr) {
                     drop_row<T, V, K, SHIFT, FULL>(a.drop, offset, row * (size_t)a.cols, at, a.cols, drop_bytes, v);
 #pragma unroll
                     for (int q = 0; q < Q; ++q) set_pair(x, q, v[q] * both(scale));
-                    store_row<T, V, K, SHIFT, FULL>((T *)a.dx + row * a.dx_stride, at, live, a.cols, x);
+                    ring.put((T *)a.dx + row * a.dx_stride, live, u, 1, x);
                 }
             }
         }

@@ -267,8 +267,13 @@ inline geo_b200_status_t status_of(cudaError_t e) {
 
 __device__ __forceinline__ uint32_t shared_address(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
+// 16 bytes (zeros when not `live`), or a word of 4 or 8.
+template <int BYTES = 16>
 __device__ __forceinline__ void copy_async(uint32_t to, const void *from, bool live = true) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(live ? 16 : 0) : "memory");
+    if constexpr (BYTES == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(live ? 16 : 0) : "memory");
+    else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(from), "n"(BYTES) : "memory");
 }
 __device__ __forceinline__ void commit_async() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int LEFT>
