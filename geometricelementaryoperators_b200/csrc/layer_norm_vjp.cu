@@ -155,42 +155,31 @@ __global__ void __launch_bounds__(TEAM == kWarp ? kWarpBlock : kTeamThreads, TEA
     if (partial == nullptr) return;
     // The kernel that joins the partial sums may be set up from here on.
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    W *mine = partial + at.slice * 2 * a.cols;
     auto value = [&](const Pair<W> (&p)[Q], int e) { return e & 1 ? p[e / 2].y : p[e / 2].x; };
-    if constexpr (TEAM >= kBlock) {
+    // Every thread's sums to where the ring was (two rows of it hold two sums of a
+    // row; value e of thread t at e threads + (t ^ e): no bank twice), then a
+    // column's, the block's teams in order, in whole lines to global memory.
+    const int each = blockDim.x, first_column = at.rank * lanes * K * V;
+    const int columns = a.cols - first_column < lanes * K * V ? a.cols - first_column : lanes * K * V;
+    W *found = (W *)memory, *mine = partial + at.slice * 2 * a.cols + first_column;
+    auto place = [&](int e, int thread) { return e * each + (thread ^ (e & 31)); };
+    __syncthreads();
 #pragma unroll
-        for (int e = 0; e < K * V; ++e) {
-            const int c = at.column(e / V) + e % V;
-            if (c < a.cols) {
-                mine[c] = value(dw, e);
-                mine[a.cols + c] = value(db, e);
-            }
-        }
-    } else {
-        // Every thread's sums to where the ring was (two rows of it hold two sums
-        // of a row; value e of thread t at e threads + (t ^ e): no bank twice),
-        // then a column's, the block's teams in order.
-        const int each = blockDim.x;
-        W *found = (W *)memory;
-        auto place = [&](int e, int thread) { return e * each + (thread ^ (e & 31)); };
-        __syncthreads();
-#pragma unroll
-        for (int e = 0; e < K * V; ++e) {
-            found[place(e, threadIdx.x)] = value(dw, e);
-            found[each * K * V + place(e, threadIdx.x)] = value(db, e);
-        }
-        __syncthreads();
-        for (int n = threadIdx.x; n < 2 * a.cols; n += each) {
-            const bool bias = n >= a.cols;
-            const int c = bias ? n - a.cols : n;
-            const int vector = c / V % (at.unit_lanes * K), unit = c / (at.unit_lanes * K * V);
-            const int e = vector / at.unit_lanes * V + c % V, lane = unit * 32 + vector % at.unit_lanes;
+    for (int e = 0; e < K * V; ++e) {
+        found[place(e, threadIdx.x)] = value(dw, e);
+        found[each * K * V + place(e, threadIdx.x)] = value(db, e);
+    }
+    __syncthreads();
+    for (int which = 0; which < 2; ++which)
+        for (int c = threadIdx.x; c < columns; c += each) {
+            const int vector = c / V, unit = TEAM == kWarp ? 0 : vector / (32 * K), in_unit = vector - unit * 32 * K;
+            const int round = TEAM == kWarp ? in_unit / at.unit_lanes : in_unit / 32;
+            const int e = round * V + c % V, lane = unit * 32 + in_unit - round * at.unit_lanes;
             W sum = 0;
             for (int team = 0; team < at.teams; ++team)
-                sum += found[(bias ? each * K * V : 0) + place(e, team * lanes + lane)];
-            mine[n] = sum;
+                sum += found[which * each * K * V + place(e, team * lanes + lane)];
+            mine[(size_t)which * a.cols + c] = sum;
         }
-    }
 }
 
 // out[c] = sum over the blocks of partial[block][which][c]. `wide` columns a
