@@ -3,7 +3,13 @@
 // ones are in layer_norm_vjp.cu, what they share in layer_norm.h.
 //
 // Per row of C values: m = sum x / C, v = sum (x - m)^2 / C,
-// y = (x - m) rsqrt(v + epsilon) w + b. A few multiply-adds a value: HBM bounds it.
+// y = (x - m) rsqrt(v + epsilon) w + b. A few multiply-adds a value, so HBM bounds
+// it; but a 16-bit value comes and goes in four bytes, and at 6.5 TB/s a
+// multiprocessor has 22 instructions for each, hence the packed arithmetic, the
+// parameters in registers and the few exchanges between threads. Measured, calls
+// in turn over several sets of arrays: 8192 x 4096 bfloat16 25 us (5.4 TB/s, 83% of
+// the copy bandwidth), with residual and dropout 16384 x 4096 100 us (5.4 TB/s, 82%;
+// Philox is a quarter of its instructions).
 #include "layer_norm.h"
 
 #include <cmath>
@@ -198,6 +204,7 @@ __global__ void __launch_bounds__(TEAM == kWarp ? kWarpBlock : kTeamThreads,
 
 // ---- rows of any length --------------------------------------------------------
 
+// For rows beyond eight blocks of threads (32768 values, 16384 in float64).
 // One CTA per row, three sweeps over it (the second and third hit L2).
 template <typename T, typename P, bool DROP>
 __global__ void __launch_bounds__(kThreads) norm_any_kernel(const ForwardArgs a) {

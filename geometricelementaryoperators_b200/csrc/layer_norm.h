@@ -5,17 +5,22 @@
 // threads holds it: part of a warp (a power of two up to 32 lanes, several rows a
 // warp), several warps of a block (up to 256 threads; smaller teams share a
 // block, each with a barrier of its own), or a cluster of up to eight blocks that
-// exchange their warps' sums through distributed shared memory. Thread
-// `lane` of the team holds K vectors of V values
-// (16 bytes; a warp's vectors are adjacent: lane, lane + 32, ... of its part), 16
-// values in all (8 in float64), so that a column belongs to one thread: weight, bias and the column
-// sums of the backward pass stay in its registers over all its rows. Rows come
-// through a ring in shared memory filled by asynchronous copies, each thread
-// copying and waiting for its own vectors only (no barrier), one to four rows
-// ahead: with few warps (registers) that keeps enough bytes in flight. What is
-// left to wait for is the sums' way across the team, so teams of several warps
+// send each other their warps' sums through distributed shared memory. A thread
+// holds K vectors of V values, 16 bytes each, 16 values in all (8 in float64), so
+// that a column belongs to one thread: weight, bias and the column sums of the
+// backward pass stay in its registers over all its rows. A warp's vectors lie side
+// by side (lane, lane + 32, ...), which leaves constant offsets between them. (Half
+// as many values a thread and twice the threads: 16384 x 4096 bfloat16 fused VJP
+// 176 instead of 166 us at the time, the sums across threads being a fixed cost.)
+//
+// Rows come through a ring in shared memory filled by asynchronous copies, each
+// thread copying and waiting for its own vectors only (no barrier), one to four
+// rows ahead: with few warps (registers) that keeps enough bytes in flight. What
+// is left to wait for is the sums' way across the team, so teams of several warps
 // take two rows of 16-bit values at a time: one barrier for both, two chains of
-// additions side by side.
+// additions side by side (the same VJP: 166 us a row at a time, 127 two). Within a
+// warp there is no barrier to share and the second row's registers cost more than
+// it gives (65536 x 256 bfloat16 VJP: 25 us a row at a time, 44 two).
 //
 // Rows that do not start on 16 bytes (SHIFT) are moved in words of 4 bytes (8 in
 // float64), neighbouring lanes neighbouring words, into and out of shared memory,
@@ -49,7 +54,6 @@ struct BackwardArgs {
     Drop drop;
 };
 
-
 // Launches (layer_norm.cu, layer_norm_vjp.cu). `partial` is the workspace of
 // vjp_workspace() bytes, or null without column sums.
 struct NormTypes {
@@ -60,6 +64,7 @@ cudaError_t launch_norm_vjp(NormTypes t, const BackwardArgs &a, bool drop, void 
 size_t vjp_workspace(NormTypes t, size_t rows, size_t cols);
 
 // How a row is held.
+constexpr int values_per_thread(size_t bytes) { return bytes == 8 ? 8 : 16; }
 enum Team : int { kWarp = 0, kPart = 1, kBlock = 2, kCluster = 3 };  // part of a warp, of a block; a block; several
 constexpr int kTeamThreads = 256;  // of a block, at most
 constexpr int kWarpBlock = 128;    // threads of a block of kWarp teams
@@ -75,13 +80,12 @@ struct Shape {
     // Bytes of one array's part of a row in a block's ring.
     size_t part(size_t bytes) const {
         const size_t units = team() == kWarp ? teams() : threads() / 32;
-        return (size_t)threads() * (bytes == 8 ? 8 : 16) * bytes + (shift ? units * 16 : 0);
+        return (size_t)threads() * values_per_thread(bytes) * bytes + (shift ? units * 16 : 0);
     }
     size_t teams() const {  // of a block
         return team() == kWarp ? kWarpBlock / lanes : (team() == kPart ? kTeamThreads / lanes : 1);
     }
 };
-constexpr int values_per_thread(size_t bytes) { return bytes == 8 ? 8 : 16; }
 Shape shape_of(size_t cols, size_t bytes, bool aligned);
 
 // Whether every array starts on, and every row is a multiple of, 16 bytes.
@@ -120,7 +124,6 @@ __device__ W block_sum(W v, W *scratch) {
     __syncthreads();
     return sum;
 }
-
 
 // Sum over 2, 4, ... `lanes` adjacent lanes, the same on each.
 template <typename W>

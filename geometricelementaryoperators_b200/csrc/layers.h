@@ -178,37 +178,6 @@ __device__ __forceinline__ void store(T *p, const Vec<T, V> &v) {
     else
         *reinterpret_cast<unsigned short *>(p) = (unsigned short)v.w[0];
 }
-
-// Bytes [shift, shift + 16) of 32, shift a multiple of the value size below 16.
-template <typename T, int V>
-__device__ __forceinline__ Vec<T, V> shifted(const Vec<T, V> &low, const Vec<T, V> &high, uint32_t shift) {
-    uint32_t w[8] = {low.w[0], low.w[1], low.w[2], low.w[3], high.w[0], high.w[1], high.w[2], high.w[3]};
-#pragma unroll
-    for (int k = 0; k < 6; ++k) w[k] = (shift & 8) ? w[k + 2] : w[k];
-    if constexpr (sizeof(T) <= 4) {
-#pragma unroll
-        for (int k = 0; k < 5; ++k) w[k] = (shift & 4) ? w[k + 1] : w[k];
-    }
-    if constexpr (sizeof(T) == 2) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) w[k] = __funnelshift_r(w[k], w[k + 1], (shift & 2) * 8);
-    }
-    Vec<T, V> r;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) r.w[k] = w[k];
-    return r;
-}
-
-// Value j of a vector, as it is stored.
-template <typename T, int V>
-__device__ __forceinline__ void store_value(T *p, const Vec<T, V> &v, int j) {
-    if constexpr (sizeof(T) == 8)
-        *reinterpret_cast<uint2 *>(p) = make_uint2(v.w[2 * j], v.w[2 * j + 1]);
-    else if constexpr (sizeof(T) == 4)
-        *reinterpret_cast<uint32_t *>(p) = v.w[j];
-    else
-        *reinterpret_cast<unsigned short *>(p) = (unsigned short)(v.w[j / 2] >> (j % 2 * 16));
-}
 #endif
 
 inline size_t type_bytes(uint32_t type) {
@@ -233,7 +202,6 @@ cudaError_t by_type(uint32_t type, F &&f) {
         default: return f(__half{});
     }
 }
-
 #endif
 
 // ---- argument checks ---------------------------------------------------------
@@ -247,8 +215,8 @@ struct Array {
 // pointer of another device or of pageable memory would fault in the kernel.
 bool arrays_usable(std::initializer_list<Array> arrays);
 
-// Row length and strides (0 = packed, replaced by cols) of up to `count` arrays;
-// false when a stride is below cols or an offset would not fit 63 bits.
+// Strides of rows x cols arrays, 0 (packed) replaced by cols; false when one is
+// below cols or an offset in bytes would not fit 63 bits.
 bool resolve_strides(size_t rows, size_t cols, std::initializer_list<size_t *> strides);
 
 // An output may be an input only with the same stride.
@@ -378,7 +346,7 @@ __device__ __forceinline__ Pair<W> drop_pair(Pair<W> v, uint32_t draws, uint32_t
     return {(draws << 16) > bound ? v.x : W(0), draws > bound ? v.y : W(0)};
 }
 
-// Rows that are not made of whole vectors: bit i of the result is whether value
+// For values spread over a warp: bit i of the result is whether value
 // base + i step + lane is kept (i < K), lane = thread of the warp, the same base
 // and step on every lane, all lanes taking part. The 32 values of one i lie in at
 // most five blocks, so each lane works one block out for six i at a time and

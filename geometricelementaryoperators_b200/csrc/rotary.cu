@@ -7,7 +7,10 @@
 // at most half a quarter turn, so its conversion to float32 costs 2^-26 quarters
 // and far positions lose nothing. Its sine and cosine are polynomials
 // (interpolated at Chebyshev nodes, within 2^-28), two pairs at a time in packed
-// float32 arithmetic.
+// float32 arithmetic. HBM bounds it: a rotor is shared by the heads of a token.
+// Measured, calls in turn over several sets of arrays: 16384 tokens of 40 heads of
+// 128 bfloat16 values 58.6 us (5.7 TB/s, 88% of the copy bandwidth); eight tokens of
+// a decoding step 2.7 us on the device.
 #include <cmath>
 
 #include "geo_runtime.h"
@@ -292,8 +295,8 @@ geo_b200_status_t rotary(const geo_b200_rotary_plan_t *plan, const geo_b200_rota
     a.pb = s.position_batch_stride;
     a.first_position = s.first_position;
     a.narrow_positions = s.position_type == GEO_B200_I32;
-    // A rotor costs about as much as turning four heads: heads are shared out
-    // only as far as it takes to give every multiprocessor 2048 threads.
+    // Heads are shared out, and rotors worked out more than once, as far as it takes to give every multiprocessor
+    // 2048 threads (8192 tokens of 32 heads of 64 float16 values: 13.0 us, 13.9 with 1024).
     const int v = vector_width(a, *plan, b);
     const bool half = plan->layout == GEO_B200_ROTARY_HALF;
     const size_t units = plan->rotary_dim / (half || v == 1 ? 2 * v : v) + (s.head_dim - plan->rotary_dim) / v;
