@@ -275,8 +275,8 @@ cudaError_t launch(NormTypes n, const ForwardArgs &a, cudaStream_t stream) {
             const int stages = ring_stages(stage, at_once, s.threads(), resident);
             const size_t each = s.teams() * at_once, wanted = (a.rows + each - 1) / each;
             const size_t most = (size_t)geo::device_sm_count() * (resident / s.threads()) / s.blocks;
-            return launch_team(norm_kernel<T, DROP, G, S, F>, s, wanted < most ? wanted : most, stages * stage, stream,
-                               a, s.lanes, float_parameters, stages);
+            return launch_team(norm_kernel<T, DROP, G, S, F>, s, wanted < most ? wanted : most, s.blocks, stages * stage,
+                               stream, a, s.lanes, float_parameters, stages);
         });
     });
 }

@@ -553,10 +553,11 @@ cudaError_t by_types(NormTypes n, F &&f) {
     });
 }
 
-// Launches a team kernel: shared memory above the default allowance, clusters.
+// Launches `grid` teams' worth of blocks of a team kernel, in clusters of
+// `cluster`; shared memory above the default allowance is asked for.
 template <typename... A>
-cudaError_t launch_team(void (*kernel)(A...), const Shape &s, size_t grid, size_t ring, cudaStream_t stream,
-                        const A &...args) {
+cudaError_t launch_team(void (*kernel)(A...), const Shape &s, size_t grid, size_t cluster, size_t ring,
+                        cudaStream_t stream, const A &...args) {
     if (ring > 40 * 1024) {
         const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)ring);
         if (e != cudaSuccess) return e;
@@ -568,10 +569,10 @@ cudaError_t launch_team(void (*kernel)(A...), const Shape &s, size_t grid, size_
     config.stream = stream;
     cudaLaunchAttribute attribute = {};
     attribute.id = cudaLaunchAttributeClusterDimension;
-    attribute.val.clusterDim.x = (unsigned)s.blocks;
+    attribute.val.clusterDim.x = (unsigned)cluster;
     attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
     config.attrs = &attribute;
-    config.numAttrs = s.blocks > 1 ? 1 : 0;
+    config.numAttrs = cluster > 1 ? 1 : 0;
     return cudaLaunchKernelEx(&config, kernel, args...);
 }
 

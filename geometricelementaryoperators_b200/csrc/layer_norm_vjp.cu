@@ -24,10 +24,12 @@ namespace {
 // One pass over x and y_bar (and z_bar): x_bar row by row, and the column sums
 // of y_bar xh and y_bar in the registers of the thread that owns the column; at
 // the end partial[block or cluster][0: weight, 1: bias][col], the teams of a
-// block added up in shared memory.
+// block added up in shared memory. `alone`: the grid is one cluster, whose blocks
+// add the partial sums up themselves, and no second kernel is needed.
+constexpr int kAloneBlocks = 8;
 template <typename T, bool DROP, int TEAM, bool SHIFT, bool FULL>
 __global__ void __launch_bounds__(TEAM == kWarp ? kWarpBlock : kTeamThreads, TEAM == kWarp ? 4 : 2)
-    vjp_kernel(const BackwardArgs a, int lanes, bool float_parameters, int stages, Wide<T> *partial) {
+    vjp_kernel(const BackwardArgs a, int lanes, bool float_parameters, int stages, Wide<T> *partial, bool alone) {
     using W = Wide<T>;
     constexpr int V = 16 / (int)sizeof(T), K = values_per_thread(sizeof(T)) / V, Q = K * V / 2;
     constexpr int R = rows_at_once(sizeof(T), SHIFT, TEAM);
@@ -162,7 +164,7 @@ __global__ void __launch_bounds__(TEAM == kWarp ? kWarpBlock : kTeamThreads, TEA
     close_exchange<TEAM>();
     if (partial == nullptr) return;
     // The kernel that joins the partial sums may be set up from here on.
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (!alone) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     auto value = [&](const Pair<W> (&p)[Q], int e) { return e & 1 ? p[e / 2].y : p[e / 2].x; };
     // Every thread's sums to where the ring was (two rows of it hold two sums of a
     // row; value e of thread t at e threads + (t ^ e): no bank twice), then a
@@ -188,6 +190,23 @@ __global__ void __launch_bounds__(TEAM == kWarp ? kWarpBlock : kTeamThreads, TEA
                 sum += found[which * each * K * V + place(e, team * lanes + lane)];
             mine[(size_t)which * a.cols + c] = sum;
         }
+    if constexpr (TEAM != kCluster) {
+        if (!alone) return;
+        cooperative_groups::this_cluster().sync();  // makes the blocks' sums visible to one another
+        for (int n = blockIdx.x * each + threadIdx.x; n < 2 * a.cols; n += gridDim.x * each) {
+            W sum = 0;
+#pragma unroll
+            for (int block = 0; block < kAloneBlocks; ++block)
+                if (block < (int)gridDim.x) sum += partial[(size_t)block * 2 * a.cols + n];
+            const int c = n < a.cols ? n : n - a.cols;
+            void *out = n < a.cols ? a.dweight : a.dbias;
+            if (out == nullptr) continue;
+            if (sizeof(T) == 2 && float_parameters)
+                ((float *)out)[c] = (float)sum;
+            else
+                ((T *)out)[c] = narrow<T>(sum);
+        }
+    }
 }
 
 // out[c] = sum over the blocks of partial[block][which][c]: 32 columns a block of
@@ -318,17 +337,21 @@ cudaError_t launch(NormTypes n, const BackwardArgs &a, void *workspace, cudaStre
         using P = decltype(p);
         using W = Wide<T>;
         size_t blocks = 0;
+        bool alone = false;
         cudaError_t e = cudaSuccess;
         if (s.lanes != 0) {
             blocks = team_grid(s, bytes, a.rows);
+            // A grid of at most eight blocks is one cluster (64 x 1024 bfloat16: 5.6 us on the device and one launch, 6.0
+            // us and two with a second kernel).
+            alone = sums && s.team() != kCluster && blocks <= kAloneBlocks;
             W *partial = sums ? (W *)workspace : nullptr;
             e = by_shape(s, [&](auto team, auto shift, auto full) {
                 constexpr int G = decltype(team)::value;
                 constexpr bool S = decltype(shift)::value, F = decltype(full)::value;
                 const size_t stage = (a.dz != nullptr ? 3 : 2) * s.part(sizeof(T));
                 const int stages = ring_stages(stage, rows_at_once(sizeof(T), S, G), s.threads(), 512);
-                return launch_team(vjp_kernel<T, DROP, G, S, F>, s, blocks, stages * stage, stream, a, s.lanes,
-                                   float_parameters, stages, partial);
+                return launch_team(vjp_kernel<T, DROP, G, S, F>, s, blocks, alone ? blocks : s.blocks, stages * stage,
+                                   stream, a, s.lanes, float_parameters, stages, partial, alone);
             });
         } else {
             // Columns first: the row kernel may overwrite x or y_bar.
@@ -343,7 +366,7 @@ cudaError_t launch(NormTypes n, const BackwardArgs &a, void *workspace, cudaStre
                 vjp_rows_any_kernel<T, P, DROP><<<grid, kThreads, 0, stream>>>(a);
             e = cudaGetLastError();
         }
-        if (e != cudaSuccess || !sums) return e;
+        if (e != cudaSuccess || !sums || alone) return e;
         // Launched while the pass still runs: its start-up is over when the sums are there.
         // About eight partial sums a thread.
         int parts = 8;
