@@ -49,8 +49,8 @@ bool aligned16(size_t cols, size_t bytes, size_t parameter_bytes, std::initializ
 namespace {
 
 // Threads that a multiprocessor holds: 80 registers a thread, 128 where two
-// rows are held at a time, and where 80 spill (1102 x 10123 float16 off 16 bytes,
-// fused: 59 us with 512 threads, 67 us with 768).
+// rows are held at a time, and where 80 spill (off 16 bytes, fused: 8192 x 4001
+// float16 96 us with 512 threads, 105 with 768; 1102 x 10123 42 and 50).
 constexpr int resident_threads(size_t bytes, bool shift, int team) {
     return rows_at_once(bytes, shift, team) == 2 || (shift && team != kWarp) ? 512 : 768;
 }
@@ -275,8 +275,9 @@ cudaError_t launch(NormTypes n, const ForwardArgs &a, cudaStream_t stream) {
             const int stages = ring_stages(stage, at_once, s.threads(), resident);
             const size_t each = s.teams() * at_once, wanted = (a.rows + each - 1) / each;
             const size_t most = (size_t)geo::device_sm_count() * (resident / s.threads()) / s.blocks;
-            return launch_team(norm_kernel<T, DROP, G, S, F>, s, wanted < most ? wanted : most, s.blocks, stages * stage,
-                               stream, a, s.lanes, float_parameters, stages);
+            size_t grid = wanted < most ? wanted : most;
+            return launch_team(norm_kernel<T, DROP, G, S, F>, s, grid, s.blocks, stages * stage, stream, a, s.lanes,
+                               float_parameters, stages);
         });
     });
 }

@@ -554,9 +554,14 @@ cudaError_t by_types(NormTypes n, F &&f) {
 }
 
 // Launches `grid` teams' worth of blocks of a team kernel, in clusters of
-// `cluster`; shared memory above the default allowance is asked for.
+// `cluster`; shared memory above the default allowance is asked for. A cluster
+// lies within one group of multiprocessors, so fewer clusters may be resident
+// than the multiprocessors' total allows (of four blocks, two a multiprocessor: 71
+// of 74): `grid` is cut to those, or the rest would start when the first have
+// taken all their rows (4096 x 16384 bfloat16: forward 81 us with 74 clusters, 53
+// with 71; VJP 117 and 91). The question costs 0.4 us on the host.
 template <typename... A>
-cudaError_t launch_team(void (*kernel)(A...), const Shape &s, size_t grid, size_t cluster, size_t ring,
+cudaError_t launch_team(void (*kernel)(A...), const Shape &s, size_t &grid, size_t cluster, size_t ring,
                         cudaStream_t stream, const A &...args) {
     if (ring > 40 * 1024) {
         const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)ring);
@@ -573,6 +578,13 @@ cudaError_t launch_team(void (*kernel)(A...), const Shape &s, size_t grid, size_
     attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
     config.attrs = &attribute;
     config.numAttrs = cluster > 1 ? 1 : 0;
+    if (s.team() == kCluster) {
+        int resident = 0;
+        const cudaError_t e = cudaOccupancyMaxActiveClusters(&resident, kernel, &config);
+        if (e != cudaSuccess) return e;
+        if (resident > 0 && grid > (size_t)resident) grid = (size_t)resident;
+        config.gridDim.x = (unsigned)(grid * s.blocks);
+    }
     return cudaLaunchKernelEx(&config, kernel, args...);
 }
 
