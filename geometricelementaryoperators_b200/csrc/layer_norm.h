@@ -559,7 +559,7 @@ cudaError_t by_types(NormTypes n, F &&f) {
 // than the multiprocessors' total allows (of four blocks, two a multiprocessor: 71
 // of 74): `grid` is cut to those, or the rest would start when the first have
 // taken all their rows (4096 x 16384 bfloat16: forward 81 us with 74 clusters, 53
-// with 71; VJP 117 and 91). The question costs 0.4 us on the host.
+// with 71; VJP 117 and 90). The question costs 0.4 us on the host.
 template <typename... A>
 cudaError_t launch_team(void (*kernel)(A...), const Shape &s, size_t &grid, size_t cluster, size_t ring,
                         cudaStream_t stream, const A &...args) {
