@@ -107,6 +107,9 @@ inline int ring_stages(size_t row_bytes, int at_once, int threads, int resident)
     const int n = (int)((size_t)220 * 1024 * threads / resident / row_bytes) / at_once * at_once;
     return n >= most ? most : (n > 2 * at_once ? n : 2 * at_once);
 }
+// No ring is larger: half of a multiprocessor's 220 KB for the largest blocks (256 of 512 threads), and the fewest rows,
+// 2 at_once, of three arrays take 96 KB and the 16 bytes a unit of rows off 16 bytes.
+constexpr int kRingMost = 110 * 1024;
 
 #ifdef __CUDACC__
 
@@ -554,17 +557,19 @@ cudaError_t by_types(NormTypes n, F &&f) {
 }
 
 // Launches `grid` teams' worth of blocks of a team kernel, in clusters of
-// `cluster`; shared memory above the default allowance is asked for. A cluster
-// lies within one group of multiprocessors, so fewer clusters may be resident
-// than the multiprocessors' total allows (of four blocks, two a multiprocessor: 71
-// of 74): `grid` is cut to those, or the rest would start when the first have
-// taken all their rows (4096 x 16384 bfloat16: forward 81 us with 74 clusters, 53
-// with 71; VJP 117 and 90). The question costs 0.4 us on the host.
+// `cluster`. Shared memory above the default allowance is a property of the kernel,
+// not of the launch, and other host threads launch the same kernel with rings of
+// their own: what is allowed is the same for all, kRingMost. A cluster lies within
+// one group of multiprocessors, so fewer clusters may be resident than the
+// multiprocessors' total allows (of four blocks, two a multiprocessor: 71 of 74):
+// `grid` is cut to those, or the rest would start when the first have taken all
+// their rows (4096 x 16384 bfloat16: forward 81 us with 74 clusters, 53 with 71;
+// VJP 117 and 90). The question costs 0.4 us on the host.
 template <typename... A>
 cudaError_t launch_team(void (*kernel)(A...), const Shape &s, size_t &grid, size_t cluster, size_t ring,
                         cudaStream_t stream, const A &...args) {
     if (ring > 40 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)ring);
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingMost);
         if (e != cudaSuccess) return e;
     }
     cudaLaunchConfig_t config = {};
