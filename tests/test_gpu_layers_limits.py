@@ -78,3 +78,40 @@ def test_two_host_threads_of_unlike_widths(kind, widths, layer_loops):
         assert all(t.equal(o, v) for o, v in zip(out, want))
 
 
+@pytest.mark.parametrize("kind", ["bf16", "f32", "f64"])
+@pytest.mark.parametrize("cols", [8, 24, 32, 25, 72, 1000, 1024, 1003, 3000, 4096, 5128, 8192, 40000])
+@pytest.mark.parametrize("fused", [False, True])
+def test_vjp_of_constant_rows_near_the_end_of_the_range(kind, cols, fused):
+    """Rows of one value v, whose own (v - mean) rstd is 0 while v rstd overflows: the formula's finite x_bar, at widths
+    that fill a team of threads and at those that do not."""
+    t = torch()
+    dtype = ref.torch_type(kind)
+    x, dy, dz = (make(9, cols, dtype, seed=s) for s in range(3))
+    w, b = parameters(cols, dtype)
+    _, mean, rstd = ref.norm(x.double(), None, None, EPS)
+    for row in (0, 4, 8):
+        x[row] = 1e306 if kind == "f64" else 2e36
+        mean[row], rstd[row] = x[row, 0].double(), EPS ** -0.5
+    x[4] *= -1
+    mean[4] *= -1
+    mean, rstd = mean.to(ref.wide_type(dtype)), rstd.to(ref.wide_type(dtype))
+    n, d = norm_config(x, dtype), drop_config(x, 0.0)
+    space, size = workspace(n)
+    dx = t.empty_like(x)
+    dw, db = t.empty_like(w), t.empty_like(b)
+    if fused:
+        call("geo_b200_residual_dropout_layer_norm_vjp", ctypes.byref(n), ctypes.byref(d), None, P(x), P(w), P(mean),
+             P(rstd), P(dy), P(dz), P(dx), None, P(dw), P(db), P(space), size)
+    else:
+        call("geo_b200_layer_norm_vjp", ctypes.byref(n), P(x), P(w), P(mean), P(rstd), P(dy), P(dx), P(dw), P(db), P(space),
+             size)
+    wide = [v.double() for v in (x, w, mean, rstd, dy)]
+    want = ref.norm_vjp(*wide)
+    total = want[0] + dz.double() if fused else want[0]
+    bounds = ref.norm_vjp_bound(*wide, total, dtype, max(ref.PATH, cols // 100))
+    u = ref.half_step(dtype)
+    ref.assert_within(dx, total, bounds[0] + ref.u_wide(dtype) * total.abs(), "dx")
+    ref.assert_within(dw, want[1], bounds[1] + u * want[1].abs() + ref.least(dtype), "dweight")
+    ref.assert_within(db, want[2], bounds[2] + u * want[2].abs() + ref.least(dtype), "dbias")
+
+
