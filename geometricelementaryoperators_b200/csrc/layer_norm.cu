@@ -205,9 +205,11 @@ __global__ void __launch_bounds__(TEAM == kWarp ? kWarpBlock : kTeamThreads,
 // ---- rows of any length --------------------------------------------------------
 
 // For rows beyond eight blocks of threads (32768 values, 16384 in float64).
-// One CTA per row, three sweeps over it (the second and third hit L2).
+// One CTA per row, three sweeps over it (the second and third hit L2). Eight CTAs a
+// multiprocessor (256 x 65536 bfloat16 116 us, 128 without that bound); with dropout
+// they would spill (fused 355 us, 325 without).
 template <typename T, typename P, bool DROP>
-__global__ void __launch_bounds__(kThreads) norm_any_kernel(const ForwardArgs a) {
+__global__ void __launch_bounds__(kThreads, DROP ? 4 : 8) norm_any_kernel(const ForwardArgs a) {
     using W = Wide<T>;
     __shared__ W scratch[kThreads / 32];
     const uint64_t offset = DROP ? drop_offset(a.drop) : 0;
@@ -226,14 +228,12 @@ __global__ void __launch_bounds__(kThreads) norm_any_kernel(const ForwardArgs a)
                 return widen(x[c]);
             }
         };
-        W sum = 0;
-        for (int c = threadIdx.x; c < a.cols; c += kThreads) sum += value(c);
+        const W sum = long_sum<W>((int)threadIdx.x, a.cols, kThreads, [&](W &s, int c) { s += value(c); });
         const W mean = block_sum(sum, scratch) / (W)a.cols;
-        W squares = 0;
-        for (int c = threadIdx.x; c < a.cols; c += kThreads) {
+        const W squares = long_sum<W>((int)threadIdx.x, a.cols, kThreads, [&](W &s, int c) {
             const W d = value(c) - mean;
-            squares += d * d;
-        }
+            s += d * d;
+        });
         const W rstd = W(1) / sqrt(block_sum(squares, scratch) / (W)a.cols + (W)a.epsilon);
         for (int c = threadIdx.x; c < a.cols; c += kThreads) {
             const W v = value(c);

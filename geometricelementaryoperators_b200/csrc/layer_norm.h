@@ -128,6 +128,33 @@ __device__ W block_sum(W v, W *scratch) {
     return sum;
 }
 
+// What add(sum, i) adds up over i = first, first + step, ... below last: 64 values
+// one after another, then 64 of those sums, then the rest. In one chain of float32
+// additions the errors of equal values add up too: the mean of a row of 2^22 times
+// 0.1 was 2590 roundings off. float64 has the bits for one chain. Unrolled by eight,
+// since no loads are in flight at the end of a chain (256 x 65536 float32 VJP 245 us,
+// 308 by four, 279 as one chain).
+template <typename V, typename I, typename F>
+__device__ __forceinline__ V long_sum(I first, I last, I step, F &&add) {
+    V sum = {};
+    if constexpr (std::is_same_v<V, double> || std::is_same_v<V, Pair<double>>) {
+        for (; first < last; first += step) add(sum, first);
+        return sum;
+    }
+    while (first < last) {
+        V middle = {};
+        for (int j = 0; j < 64 && first < last; ++j) {
+            const I end = last - first > 64 * step ? first + 64 * step : last;
+            V inner = {};
+#pragma unroll 8
+            for (; first < end; first += step) add(inner, first);
+            middle = middle + inner;
+        }
+        sum = sum + middle;
+    }
+    return sum;
+}
+
 // Sum over 2, 4, ... `lanes` adjacent lanes, the same on each.
 template <typename W>
 __device__ __forceinline__ W team_sum(W v, int lanes) {

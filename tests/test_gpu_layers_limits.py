@@ -115,3 +115,67 @@ def test_vjp_of_constant_rows_near_the_end_of_the_range(kind, cols, fused):
     ref.assert_within(db, want[2], bounds[2] + u * want[2].abs() + ref.least(dtype), "dbias")
 
 
+#: Additions along the longest path of a row's or a column's sum in the kernels for rows of any length: 64 values one
+#: after another in a thread, 64 of those sums, the rest (cols / 2^20, rows / 2^15), a warp's 5 steps, 8 warps or groups,
+#: and 3 for the division and the result.
+LONG_PATH = 64 + 64 + 16 + 5 + 8 + 3
+
+
+@pytest.mark.parametrize("cols", [(1 << 20) + 3, 1 << 22, 1 << 24])
+@pytest.mark.parametrize("value", [0.1, 1.1])
+def test_statistics_of_long_rows_of_one_value(cols, value):
+    """Equal values round the same way at every addition: the error of a long chain of them grows with its length, that
+    of sums of sums does not."""
+    t = torch()
+    x = t.full((2, cols), value, device="cuda")
+    zero = t.zeros_like(x)
+    y, z = t.empty_like(x), t.empty_like(x)
+    mean, rstd = stats_like(x)
+    n, d = norm_config(x, t.float32), drop_config(x, 0.0)
+    want = [torch().tensor(v, device="cuda", dtype=t.float64) for v in (0.0, float(x[0, 0]), EPS ** -0.5)]
+    bounds = [float(v.max()) for v in ref.norm_bound(x[:, :8].double(), None, None, want[2].expand(2), want[0], t.float32,
+                                                     LONG_PATH)]
+    for fused in (False, True):
+        if fused:
+            call("geo_b200_residual_dropout_layer_norm", ctypes.byref(n), ctypes.byref(d), P(x), P(zero), None, None, None,
+                 P(z), P(y), P(mean), P(rstd))
+            assert t.equal(z, x)
+        else:
+            call("geo_b200_layer_norm", ctypes.byref(n), P(x), None, None, P(y), P(mean), P(rstd))
+        for got, v, bound, what in zip((y, mean, rstd), want, bounds, ("y", "mean", "rstd")):
+            assert float((got.double() - v).abs().max()) <= bound, (what, fused)
+
+
+@pytest.mark.parametrize("value", [0.1, 1.1])
+def test_vjp_of_long_rows_of_one_cotangent(value):
+    t = torch()
+    cols = 1 << 22
+    x = make(2, cols, t.float32, seed=3)
+    dy = t.full_like(x, value)
+    _, mean, rstd = ref.norm(x.double(), None, None, EPS)
+    mean, rstd = mean.float(), rstd.float()
+    dx = t.empty_like(x)
+    call("geo_b200_layer_norm_vjp", ctypes.byref(norm_config(x, t.float32)), P(x), None, P(mean), P(rstd), P(dy), P(dx),
+         None, None, None, 0)
+    wide = [x.double(), None, mean.double(), rstd.double(), dy.double()]
+    want = ref.norm_vjp(*wide)[0]
+    ref.assert_within(dx, want, ref.norm_vjp_bound(*wide, want, t.float32, LONG_PATH)[0], "dx")
+
+
+@pytest.mark.parametrize("value", [0.1, 1.1])
+def test_column_sums_over_many_long_rows(value):
+    """32776 columns, 32768 rows of one cotangent: bias_bar is rows times it."""
+    t = torch()
+    rows, cols = 1 << 15, 32776
+    x = t.zeros(rows, cols, device="cuda")
+    dy = t.full_like(x, value)
+    mean, rstd = t.full((rows,), -1.0, device="cuda"), t.full((rows,), 1.0, device="cuda")
+    n = norm_config(x, t.float32)
+    space, size = workspace(n)
+    dw, db = (t.empty(cols, device="cuda") for _ in range(2))
+    call("geo_b200_layer_norm_vjp", ctypes.byref(n), P(x), None, P(mean), P(rstd), P(dy), None, P(dw), P(db), P(space), size)
+    want = rows * float(dy[0, 0])
+    for got in (dw, db):  # xh = 1: the same sum
+        assert float((got.double() - want).abs().max()) <= LONG_PATH * 2.0 ** -24 * want
+
+
