@@ -273,6 +273,8 @@ SIGNATURES: dict[str, tuple] = {
     "geo_b200_layer_norm_vjp_workspace": (_SZ, [ctypes.POINTER(LayerNormConfig)]),
     "geo_b200_layer_norm_vjp": (
         _I, [ctypes.POINTER(LayerNormConfig), _P, _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P]),
+    "geo_b200_layer_norm_wait_selftest": (
+        _I, [ctypes.POINTER(LayerNormConfig), _P, _P, _P, _P, _P, _P, _P, _P, _SZ, ctypes.c_uint32, ctypes.c_uint32, _P]),
     "geo_b200_dropout": (_I, [ctypes.POINTER(DropoutConfig), _P, _P, _P, _P, _P]),
     "geo_b200_dropout_vjp": (_I, [ctypes.POINTER(DropoutConfig), _P, _P, _P, _P]),
     "geo_b200_residual_dropout_layer_norm": (

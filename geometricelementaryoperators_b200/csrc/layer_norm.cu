@@ -55,7 +55,7 @@ constexpr int resident_threads(size_t bytes, bool shift, int team) {
     return rows_at_once(bytes, shift, team) == 2 || (shift && team != kWarp) ? 512 : 768;
 }
 
-template <typename T, bool DROP, int TEAM, bool SHIFT, bool FULL>
+template <typename T, bool DROP, int TEAM, bool SHIFT, bool FULL, bool STARVE = false>
 __global__ void __launch_bounds__(TEAM == kWarp ? kWarpBlock : kTeamThreads,
                                   resident_threads(sizeof(T), SHIFT, TEAM) / (TEAM == kWarp ? kWarpBlock : kTeamThreads))
     norm_kernel(const ForwardArgs a, int lanes, bool float_parameters, int stages) {
@@ -100,6 +100,7 @@ __global__ void __launch_bounds__(TEAM == kWarp ? kWarpBlock : kTeamThreads,
     open_exchange(sums);
 
     uint32_t round = 0;
+    bool complete = true;  // no wait for the cluster gave up
     for (size_t first = at.begin; first < a.rows; first += R * at.step, ++round) {
         for (int u = 0; u < R; ++u) next();
         ring.wait();
@@ -152,7 +153,9 @@ __global__ void __launch_bounds__(TEAM == kWarp ? kWarpBlock : kTeamThreads,
         } else {
             squares[0] = R == 2 ? folded_sums(squares) : team_sum(squares[0], 32);
             // Values 2 u: sum of row u, 2 u + 1: its squares.
-            const bool complete = exchange(sums, round, at, at.wlane / (16 / R) % 2 ? squares[0] : sum[0]);
+            complete = exchange(sums, round, at, at.wlane / (16 / R) % 2 ? squares[0] : sum[0], complete,
+                                STARVE ? a.starve.polls : kWaitPolls,
+                                STARVE && round == a.starve.round && at.rank == at.ranks - 1);
             auto found = [&](int n, int j) { return sums.values[round & 1][n][at.first_entry + joiner + j * kJoin]; };
             // Warps joined about the row's mean: squares + held (warp's mean - mean)^2.
             W total = 0, other[kEach];
@@ -250,6 +253,19 @@ __global__ void __launch_bounds__(kThreads, DROP ? 4 : 8) norm_any_kernel(const 
     }
 }
 
+// `stages` rows of `stage` bytes in the ring, and the grid, of a team kernel.
+template <typename T, bool DROP, int TEAM, bool SHIFT, bool FULL, bool STARVE = false>
+cudaError_t launch_shape(const Shape &s, const ForwardArgs &a, bool float_parameters, cudaStream_t stream) {
+    constexpr int resident = resident_threads(sizeof(T), SHIFT, TEAM), at_once = rows_at_once(sizeof(T), SHIFT, TEAM);
+    const size_t stage = (DROP ? 2 : 1) * s.part(sizeof(T));
+    const int stages = ring_stages(stage, at_once, s.threads(), resident);
+    const size_t each = s.teams() * at_once, wanted = (a.rows + each - 1) / each;
+    const size_t most = (size_t)geo::device_sm_count() * (resident / s.threads()) / s.blocks;
+    size_t grid = wanted < most ? wanted : most;
+    return launch_team(norm_kernel<T, DROP, TEAM, SHIFT, FULL, STARVE>, s, grid, s.blocks, stages * stage, stream, a,
+                       s.lanes, float_parameters, stages);
+}
+
 template <bool DROP>
 cudaError_t launch(NormTypes n, const ForwardArgs &a, cudaStream_t stream) {
     const size_t bytes = type_bytes(n.type);
@@ -268,16 +284,8 @@ cudaError_t launch(NormTypes n, const ForwardArgs &a, cudaStream_t stream) {
     return by_type(n.type, [&](auto t) {
         using T = decltype(t);
         return by_shape(s, [&](auto team, auto shift, auto full) {
-            constexpr int G = decltype(team)::value;
-            constexpr bool S = decltype(shift)::value, F = decltype(full)::value;
-            constexpr int resident = resident_threads(sizeof(T), S, G), at_once = rows_at_once(sizeof(T), S, G);
-            const size_t stage = (DROP ? 2 : 1) * s.part(sizeof(T));
-            const int stages = ring_stages(stage, at_once, s.threads(), resident);
-            const size_t each = s.teams() * at_once, wanted = (a.rows + each - 1) / each;
-            const size_t most = (size_t)geo::device_sm_count() * (resident / s.threads()) / s.blocks;
-            size_t grid = wanted < most ? wanted : most;
-            return launch_team(norm_kernel<T, DROP, G, S, F>, s, grid, s.blocks, stages * stage, stream, a, s.lanes,
-                               float_parameters, stages);
+            return launch_shape<T, DROP, decltype(team)::value, decltype(shift)::value, decltype(full)::value>(
+                s, a, float_parameters, stream);
         });
     });
 }
@@ -286,6 +294,10 @@ cudaError_t launch(NormTypes n, const ForwardArgs &a, cudaStream_t stream) {
 
 cudaError_t launch_norm(NormTypes t, const ForwardArgs &a, bool drop, cudaStream_t stream) {
     return drop ? launch<true>(t, a, stream) : launch<false>(t, a, stream);
+}
+
+cudaError_t launch_norm_starved(const ForwardArgs &a, cudaStream_t stream) {
+    return launch_shape<float, false, kCluster, false, true, true>(shape_of(a.cols, 4, true), a, true, stream);
 }
 
 }  // namespace layers
@@ -485,4 +497,49 @@ extern "C" geo_b200_status_t geo_b200_residual_dropout_layer_norm_vjp(
     a.dsum_stride = c.x_cotangent_stride;
     a.dx_stride = d.x_cotangent_stride;
     return status_of(launch_norm_vjp({c.type, c.parameter_type}, a, true, device_workspace, stream));
+}
+
+extern "C" geo_b200_status_t geo_b200_layer_norm_wait_selftest(
+    const geo_b200_layer_norm_config_t *config, const void *device_x, const void *device_y_cotangent, void *device_out,
+    void *device_mean, void *device_rstd, void *device_weight_cotangent, void *device_bias_cotangent,
+    void *device_workspace, size_t workspace_bytes, uint32_t round, uint32_t wait_limit, cudaStream_t stream) {
+    geo::NvtxRange range("geo_b200.layer_norm_wait_selftest");
+    if (!config_valid(config) || config->type != GEO_B200_F32 || config->x_stride != 0 || config->y_stride != 0 ||
+        config->y_cotangent_stride != 0 || config->x_cotangent_stride != 0 || wait_limit == 0 || device_x == nullptr ||
+        device_out == nullptr || device_mean == nullptr || device_rstd == nullptr)
+        return GEO_B200_INVALID_ARGUMENT;
+    const Shape s = shape_of(config->cols, 4, true);
+    if (s.team() != kCluster || s.lanes == 0 || !s.full ||
+        !arrays_usable({{device_x, 16}, {device_y_cotangent, 16}, {device_out, 16}, {device_mean, 4}, {device_rstd, 4},
+                        {device_weight_cotangent, 4}, {device_bias_cotangent, 4}}))
+        return GEO_B200_INVALID_ARGUMENT;
+    if (device_y_cotangent == nullptr) {
+        ForwardArgs a = {};
+        a.x = device_x;
+        a.y = device_out;
+        a.mean = device_mean;
+        a.rstd = device_rstd;
+        a.rows = config->rows;
+        a.cols = (int)config->cols;
+        a.x_stride = a.y_stride = config->cols;
+        a.epsilon = config->epsilon;
+        a.starve = {round, wait_limit};
+        return status_of(launch_norm_starved(a, stream));
+    }
+    if (device_weight_cotangent == nullptr || device_bias_cotangent == nullptr ||
+        !workspace_usable(*config, device_workspace, workspace_bytes))
+        return GEO_B200_INVALID_ARGUMENT;
+    BackwardArgs a = {};
+    a.x = device_x;
+    a.mean = device_mean;
+    a.rstd = device_rstd;
+    a.dy = device_y_cotangent;
+    a.dsum = device_out;
+    a.dweight = device_weight_cotangent;
+    a.dbias = device_bias_cotangent;
+    a.rows = config->rows;
+    a.cols = (int)config->cols;
+    a.x_stride = a.dy_stride = a.dsum_stride = config->cols;
+    a.starve = {round, wait_limit};
+    return status_of(launch_norm_vjp_starved(a, device_workspace, stream));
 }

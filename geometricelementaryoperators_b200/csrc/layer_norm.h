@@ -37,6 +37,12 @@
 namespace geo {
 namespace layers {
 
+// For the self-test of the clusters' waits alone: the round in which the last block
+// of every cluster sends nothing, and how often a wait looks.
+struct Starve {
+    uint32_t round, polls;
+};
+
 struct ForwardArgs {
     const void *x, *residual, *weight, *bias;
     void *z, *y, *mean, *rstd;
@@ -44,6 +50,7 @@ struct ForwardArgs {
     int cols;
     double epsilon;
     Drop drop;
+    Starve starve;
 };
 
 struct BackwardArgs {
@@ -52,6 +59,7 @@ struct BackwardArgs {
     size_t rows, x_stride, dy_stride, dz_stride, dsum_stride, dx_stride;
     int cols;
     Drop drop;
+    Starve starve;
 };
 
 // Launches (layer_norm.cu, layer_norm_vjp.cu). `partial` is the workspace of
@@ -61,6 +69,9 @@ struct NormTypes {
 };
 cudaError_t launch_norm(NormTypes t, const ForwardArgs &a, bool drop, cudaStream_t stream);
 cudaError_t launch_norm_vjp(NormTypes t, const BackwardArgs &a, bool drop, void *partial, cudaStream_t stream);
+// float32 rows that fill a cluster of blocks, with a.starve.
+cudaError_t launch_norm_starved(const ForwardArgs &a, cudaStream_t stream);
+cudaError_t launch_norm_vjp_starved(const BackwardArgs &a, void *partial, cudaStream_t stream);
 size_t vjp_workspace(NormTypes t, size_t rows, size_t cols);
 
 // How a row is held.
@@ -139,18 +150,18 @@ __device__ __forceinline__ V long_sum(I first, I last, I step, F &&add) {
     V sum = {};
     if constexpr (std::is_same_v<V, double> || std::is_same_v<V, Pair<double>>) {
         for (; first < last; first += step) add(sum, first);
-        return sum;
-    }
-    while (first < last) {
-        V middle = {};
-        for (int j = 0; j < 64 && first < last; ++j) {
-            const I end = last - first > 64 * step ? first + 64 * step : last;
-            V inner = {};
+    } else {
+        while (first < last) {
+            V middle = {};
+            for (int j = 0; j < 64 && first < last; ++j) {
+                const I end = last - first > 64 * step ? first + 64 * step : last;
+                V inner = {};
 #pragma unroll 8
-            for (; first < end; first += step) add(inner, first);
-            middle = middle + inner;
+                for (; first < end; first += step) add(inner, first);
+                middle = middle + inner;
+            }
+            sum = sum + middle;
         }
-        sum = sum + middle;
     }
     return sum;
 }
@@ -469,18 +480,26 @@ __device__ __forceinline__ void close_exchange() {
 // Sends the warp's values (value n in lanes 32 / N n and on) and waits for those
 // of all the team's warps. A cluster's blocks send straight into each other's
 // shared memory, where a barrier counts the bytes: unlike a barrier of the
-// cluster, this does not wait for the stores of the row before. False when the
-// wait gave up (never, unless a block of the cluster failed).
+// cluster, this does not wait for the stores of the row before.
+// `complete`: what the round before returned. False, for the whole warp, when this
+// wait or one before gave up (never, unless a block of the cluster failed). Such a
+// warp sends and waits no more: its barriers' phases are no longer those of its
+// rounds. The other warps of the cluster miss its values in the next round and give
+// up in turn. Nothing is on its way to a block that leaves: after what it sent last
+// every warp waited for that round to be complete, or a wait's whole length.
+// `silent`: sends nothing (the self-test).
 template <typename W, int N, int TEAM, int V, int K>
-__device__ __forceinline__ bool exchange(Exchange<W, N, TEAM> &x, uint32_t round, const Place<TEAM, V, K> &at, W value) {
+__device__ __forceinline__ bool exchange(Exchange<W, N, TEAM> &x, uint32_t round, const Place<TEAM, V, K> &at, W value,
+                                         bool complete, uint32_t polls = kWaitPolls, bool silent = false) {
     const int n = at.wlane / (32 / N), sub = at.wlane % (32 / N), flip = round & 1;
     if constexpr (TEAM == kCluster) {
+        if (!complete) return false;
         const uint32_t barrier = shared_address(&x.arrived[flip]);
         if (threadIdx.x == 0)
             asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(barrier),
                          "r"((uint32_t)(at.entries * N * (int)sizeof(W)))
                          : "memory");
-        if (sub < at.ranks) {
+        if (sub < at.ranks && !silent) {
             uint32_t to, there;
             asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"
                          : "=r"(to)
@@ -496,14 +515,14 @@ __device__ __forceinline__ bool exchange(Exchange<W, N, TEAM> &x, uint32_t round
                              : "memory");
         }
         uint32_t done = 0;
-        for (uint32_t poll = 0; poll < kWaitPolls && !done; ++poll)
+        for (uint32_t poll = 0; poll < polls && !done; ++poll)
             asm volatile(
                 "{\n.reg .pred p;\nmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
                 "selp.u32 %0, 1, 0, p;\n}"
                 : "=r"(done)
                 : "r"(barrier), "r"((round >> 1) & 1u)
                 : "memory");
-        return done != 0;
+        return __all_sync(0xffffffffu, done);
     } else {
         if (sub == 0) x.values[flip][n][at.first_entry + at.warp] = value;
         if constexpr (TEAM == kPart)

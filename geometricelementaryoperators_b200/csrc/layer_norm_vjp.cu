@@ -27,7 +27,7 @@ namespace {
 // block added up in shared memory. `alone`: the grid is one cluster, whose blocks
 // add the partial sums up themselves, and no second kernel is needed.
 constexpr int kAloneBlocks = 8;
-template <typename T, bool DROP, int TEAM, bool SHIFT, bool FULL>
+template <typename T, bool DROP, int TEAM, bool SHIFT, bool FULL, bool STARVE = false>
 __global__ void __launch_bounds__(TEAM == kWarp ? kWarpBlock : kTeamThreads, TEAM == kWarp ? 4 : 2)
     vjp_kernel(const BackwardArgs a, int lanes, bool float_parameters, int stages, Wide<T> *partial, bool alone) {
     using W = Wide<T>;
@@ -68,6 +68,7 @@ __global__ void __launch_bounds__(TEAM == kWarp ? kWarpBlock : kTeamThreads, TEA
     statistics(at.begin);
     open_exchange(sums);
     uint32_t round = 0;
+    bool complete = true;  // no wait for the cluster gave up
     for (size_t first = at.begin; first < a.rows; first += R * at.step, ++round) {
         W mean[R], rstd[R], part[2 * R];
 #pragma unroll
@@ -121,7 +122,8 @@ __global__ void __launch_bounds__(TEAM == kWarp ? kWarpBlock : kTeamThreads, TEA
             part[0] = team_sum(part[0], at.threads) * over;
             part[1] = team_sum(part[1], at.threads) * over;
         } else {
-            const bool complete = exchange(sums, round, at, folded_sums(part));
+            complete = exchange(sums, round, at, folded_sums(part), complete, STARVE ? a.starve.polls : kWaitPolls,
+                                STARVE && round == a.starve.round && at.rank == at.ranks - 1);
             constexpr int kJoin = 32 / (2 * R);  // lanes that add one value up
             W total = 0;
 #pragma unroll
@@ -173,6 +175,10 @@ __global__ void __launch_bounds__(TEAM == kWarp ? kWarpBlock : kTeamThreads, TEA
     wait_async<0>();
     close_exchange<TEAM>();
     if (partial == nullptr) return;
+    if (!complete) {
+#pragma unroll
+        for (int q = 0; q < Q; ++q) dw[q] = db[q] = both((W)NAN);
+    }
     // The kernel that joins the partial sums may be set up from here on.
     if (!alone) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     auto value = [&](const Pair<W> (&p)[Q], int e) { return e & 1 ? p[e / 2].y : p[e / 2].x; };
@@ -332,6 +338,37 @@ size_t team_grid(const Shape &s, size_t bytes, size_t rows) {
     return wanted < most ? wanted : most;
 }
 
+// The pass of a team kernel; `blocks`: the partial sums it leaves.
+template <typename T, bool DROP, int TEAM, bool SHIFT, bool FULL, bool STARVE = false>
+cudaError_t launch_shape(const Shape &s, const BackwardArgs &a, bool float_parameters, Wide<T> *partial, bool alone,
+                         size_t &blocks, cudaStream_t stream) {
+    const size_t stage = (a.dz != nullptr ? 3 : 2) * s.part(sizeof(T));
+    const int stages = ring_stages(stage, rows_at_once(sizeof(T), SHIFT, TEAM), s.threads(), 512);
+    return launch_team(vjp_kernel<T, DROP, TEAM, SHIFT, FULL, STARVE>, s, blocks, alone ? blocks : s.blocks,
+                       stages * stage, stream, a, s.lanes, float_parameters, stages, partial, alone);
+}
+
+// Launched while the pass still runs: its start-up is over when the sums are there.
+// About eight partial sums a thread, more where 1024 threads a multiprocessor do not reach: with 32 threads a
+// column always 8192 x 5120 bfloat16 60.0 us, so 57.1; 300 x 4096 10.8, so 9.9; with 8 always 8192 x 2048 27.4,
+// so 26.0.
+template <typename W, typename P>
+cudaError_t launch_join(const BackwardArgs &a, const W *partial, size_t blocks, cudaStream_t stream) {
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3((unsigned)((a.cols + kJoinColumns - 1) / kJoinColumns), 2);
+    const size_t columns = (size_t)config.gridDim.x * 2 * kJoinColumns, threads = (size_t)geo::device_sm_count() * 1024;
+    int parts = 8;
+    while (parts < 1024 / kJoinColumns && (size_t)parts * 8 < blocks && columns * parts * 2 <= threads) parts *= 2;
+    config.blockDim = dim3((unsigned)(kJoinColumns * parts));
+    config.stream = stream;
+    cudaLaunchAttribute attribute = {};
+    attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attribute.val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = &attribute;
+    config.numAttrs = 1;
+    return cudaLaunchKernelEx(&config, join_columns_kernel<W, P>, partial, (int)blocks, a.cols, a.dweight, a.dbias);
+}
+
 template <bool DROP>
 cudaError_t launch(NormTypes n, const BackwardArgs &a, void *workspace, cudaStream_t stream) {
     const bool sums = a.dweight != nullptr || a.dbias != nullptr;
@@ -346,6 +383,7 @@ cudaError_t launch(NormTypes n, const BackwardArgs &a, void *workspace, cudaStre
         using T = decltype(t);
         using P = decltype(p);
         using W = Wide<T>;
+        W *partial = sums ? (W *)workspace : nullptr;
         size_t blocks = 0;
         bool alone = false;
         cudaError_t e = cudaSuccess;
@@ -354,22 +392,16 @@ cudaError_t launch(NormTypes n, const BackwardArgs &a, void *workspace, cudaStre
             // A grid of at most eight blocks is one cluster (64 x 1024 bfloat16: 5.6 us on the device and one launch, 6.0
             // us and two with a second kernel).
             alone = sums && s.team() != kCluster && blocks <= kAloneBlocks;
-            W *partial = sums ? (W *)workspace : nullptr;
             e = by_shape(s, [&](auto team, auto shift, auto full) {
-                constexpr int G = decltype(team)::value;
-                constexpr bool S = decltype(shift)::value, F = decltype(full)::value;
-                const size_t stage = (a.dz != nullptr ? 3 : 2) * s.part(sizeof(T));
-                const int stages = ring_stages(stage, rows_at_once(sizeof(T), S, G), s.threads(), 512);
-                return launch_team(vjp_kernel<T, DROP, G, S, F>, s, blocks, alone ? blocks : s.blocks, stages * stage,
-                                   stream, a, s.lanes, float_parameters, stages, partial, alone);
+                return launch_shape<T, DROP, decltype(team)::value, decltype(shift)::value, decltype(full)::value>(
+                    s, a, float_parameters, partial, alone, blocks, stream);
             });
         } else {
             // Columns first: the row kernel may overwrite x or y_bar.
             if (sums) {
                 blocks = column_blocks(a.rows, a.cols);
                 const dim3 grid((unsigned)((a.cols + 31) / 32), (unsigned)blocks);
-                vjp_columns_any_kernel<T>
-                    <<<grid, kThreads, 0, stream>>>(a, (W *)workspace, (a.rows + blocks - 1) / blocks);
+                vjp_columns_any_kernel<T><<<grid, kThreads, 0, stream>>>(a, partial, (a.rows + blocks - 1) / blocks);
             }
             const unsigned grid = (unsigned)(a.rows < (1u << 20) ? a.rows : (1u << 20));
             if (a.dsum != nullptr || a.dx != nullptr)
@@ -377,24 +409,7 @@ cudaError_t launch(NormTypes n, const BackwardArgs &a, void *workspace, cudaStre
             e = cudaGetLastError();
         }
         if (e != cudaSuccess || !sums || alone) return e;
-        // Launched while the pass still runs: its start-up is over when the sums are there.
-        // About eight partial sums a thread, more where 1024 threads a multiprocessor do not reach: with 32 threads a
-        // column always 8192 x 5120 bfloat16 60.0 us, so 57.1; 300 x 4096 10.8, so 9.9; with 8 always 8192 x 2048 27.4,
-        // so 26.0.
-        cudaLaunchConfig_t config = {};
-        config.gridDim = dim3((unsigned)((a.cols + kJoinColumns - 1) / kJoinColumns), 2);
-        const size_t columns = (size_t)config.gridDim.x * 2 * kJoinColumns, threads = (size_t)geo::device_sm_count() * 1024;
-        int parts = 8;
-        while (parts < 1024 / kJoinColumns && (size_t)parts * 8 < blocks && columns * parts * 2 <= threads) parts *= 2;
-        config.blockDim = dim3((unsigned)(kJoinColumns * parts));
-        config.stream = stream;
-        cudaLaunchAttribute attribute = {};
-        attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attribute.val.programmaticStreamSerializationAllowed = 1;
-        config.attrs = &attribute;
-        config.numAttrs = 1;
-        return cudaLaunchKernelEx(&config, join_columns_kernel<W, P>, (const W *)workspace, (int)blocks, a.cols,
-                                  a.dweight, a.dbias);
+        return launch_join<W, P>(a, partial, blocks, stream);
     });
 }
 
@@ -415,6 +430,14 @@ size_t vjp_workspace(NormTypes t, size_t rows, size_t cols) {
 
 cudaError_t launch_norm_vjp(NormTypes t, const BackwardArgs &a, bool drop, void *partial, cudaStream_t stream) {
     return drop ? launch<true>(t, a, partial, stream) : launch<false>(t, a, partial, stream);
+}
+
+cudaError_t launch_norm_vjp_starved(const BackwardArgs &a, void *partial, cudaStream_t stream) {
+    const Shape s = shape_of(a.cols, 4, true);
+    size_t blocks = team_grid(s, 4, a.rows);
+    const cudaError_t e = launch_shape<float, false, kCluster, false, true, true>(s, a, true, (float *)partial, false,
+                                                                                 blocks, stream);
+    return e != cudaSuccess ? e : launch_join<float, float>(a, (float *)partial, blocks, stream);
 }
 
 }  // namespace layers

@@ -410,6 +410,25 @@ geo_b200_status_t geo_b200_layer_norm_vjp(const geo_b200_layer_norm_config_t *co
                                           void *device_bias_cotangent, void *device_workspace,
                                           size_t workspace_bytes, cudaStream_t stream);
 
+/* Rows of more than 4096 values, up to 32768 (half of that in float64) lie in a
+ * cluster of thread blocks that send one another their sums. Every wait for those
+ * gives up after a fixed number of polls (seconds, where a row takes microseconds;
+ * it cannot happen unless a block of the cluster failed). A warp whose wait gave up
+ * waits and sends no more: what it writes from then on is NaN (its part of the rows,
+ * their statistics, its columns of weight_bar and bias_bar), and so it is for the
+ * cluster's other warps from their next row on. The call ends and the context stays
+ * usable.
+ * Self-test of that path, float32, packed and 16-byte aligned rows that fill their
+ * cluster (cols a multiple of 8192 that is a power of two), without a weight: layer
+ * norm of device_x into device_out (device_y_cotangent NULL, mean and rstd
+ * written), or its VJP (device_out: x_bar; mean and rstd read). In round `round` of
+ * the rows that a cluster takes one after another, its last block sends nothing;
+ * waits give up after wait_limit polls. Later rows, and the column sums, are NaN. */
+geo_b200_status_t geo_b200_layer_norm_wait_selftest(
+    const geo_b200_layer_norm_config_t *config, const void *device_x, const void *device_y_cotangent, void *device_out,
+    void *device_mean, void *device_rstd, void *device_weight_cotangent, void *device_bias_cotangent,
+    void *device_workspace, size_t workspace_bytes, uint32_t round, uint32_t wait_limit, cudaStream_t stream);
+
 /* Dropout, y = [residual +] keep x / (1 - rate), whose mask is computed from a
  * counter and never stored. What is kept or dropped as one is a unit of
  * 2^dimension consecutive values of a row: a single value (dimension 0), or a

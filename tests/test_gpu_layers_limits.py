@@ -179,3 +179,60 @@ def test_column_sums_over_many_long_rows(value):
         assert float((got.double() - want).abs().max()) <= LONG_PATH * 2.0 ** -24 * want
 
 
+@pytest.mark.parametrize("cols", [8192, 16384, 32768])
+@pytest.mark.parametrize("backward", [False, True])
+def test_wait_of_a_cluster_that_gives_up(cols, backward):
+    """A block that sends nothing in one round: rows before it are right; that one and all later ones, their statistics
+    and the column sums are NaN; the context stays usable. A round that does not come changes nothing."""
+    t = torch()
+    L = abi.lib()
+    rows = 1200
+    x, dy = make(rows, cols, t.float32, seed=1, shift=0.5), make(rows, cols, t.float32, seed=2)
+    _, m, r = ref.norm(x.double(), None, None, EPS)
+    n = norm_config(x, t.float32, x_stride=0, y_stride=0, y_cotangent_stride=0, x_cotangent_stride=0)
+    space, size = workspace(n)
+    out, want = t.full_like(x, 7.0), t.empty_like(x)
+    stats = [m.float(), r.float()] if backward else stats_like(x)
+    sums = [t.full((cols,), 7.0, device="cuda") for _ in range(2)]
+
+    def usual():
+        """The ordinary call's results."""
+        s, v = [p.clone() for p in stats], [t.empty_like(p) for p in sums]
+        if backward:
+            call("geo_b200_layer_norm_vjp", ctypes.byref(n), P(x), None, P(s[0]), P(s[1]), P(dy), P(want), P(v[0]), P(v[1]),
+                 P(space), size)
+        else:
+            call("geo_b200_layer_norm", ctypes.byref(n), P(x), None, None, P(want), P(s[0]), P(s[1]))
+        return [want] + (v if backward else s)
+
+    def starved(round, polls):
+        call("geo_b200_layer_norm_wait_selftest", ctypes.byref(n), P(x), P(dy) if backward else None, P(out), P(stats[0]),
+             P(stats[1]), P(sums[0]), P(sums[1]), P(space), size, round, polls)
+        t.cuda.synchronize()
+        return [out] + (sums if backward else stats)
+
+    for round in (1, 2):
+        clean = [v.clone() for v in usual()]
+        got = starved(round, 1 << 14)
+        bad = t.isnan(out).any(1)
+        first = int(bad.int().argmax())
+        assert 0 < first <= rows // 2 and first % round == 0
+        assert t.isnan(out[first:]).all() and t.equal(out[:first], clean[0][:first])
+        for v, w in zip(got[1:], clean[1:]):
+            if backward:
+                assert t.isnan(v).all()
+            else:
+                assert t.isnan(v[first:]).all() and t.equal(v[:first], w[:first])
+        again = usual()
+        assert all(t.equal(v, w) for v, w in zip(again, clean))
+    assert all(t.equal(v, w) for v, w in zip(starved(1 << 20, 1 << 14), clean))
+    refused = [dict(type=abi.F64, parameter_type=abi.F64), dict(cols=4096), dict(cols=cols - 4), dict(x_stride=cols),
+               dict(epsilon=-1.0)]
+    for bad in refused:
+        c = norm_config(x, t.float32, **{**dict(x_stride=0, y_stride=0, y_cotangent_stride=0, x_cotangent_stride=0), **bad})
+        assert L.geo_b200_layer_norm_wait_selftest(ctypes.byref(c), P(x), None, P(out), P(stats[0]), P(stats[1]), None, None,
+                                                   None, 0, 1, 64, stream()) == INVALID
+    assert L.geo_b200_layer_norm_wait_selftest(ctypes.byref(n), P(x), None, P(out), P(stats[0]), P(stats[1]), None, None,
+                                               None, 0, 1, 0, stream()) == INVALID
+
+
