@@ -358,7 +358,11 @@ extern "C" geo_b200_status_t geo_b200_layer_norm(const geo_b200_layer_norm_confi
 }
 
 extern "C" size_t geo_b200_layer_norm_vjp_workspace(const geo_b200_layer_norm_config_t *config) {
-    return config_valid(config) ? workspace_bytes_of(*config) : 0;
+    if (!config_valid(config)) return 0;
+    geo_b200_layer_norm_config_t c = *config;
+    return resolve_strides(c.rows, c.cols, {&c.x_stride, &c.y_cotangent_stride, &c.x_cotangent_stride})
+               ? workspace_bytes_of(c)
+               : 0;
 }
 
 extern "C" geo_b200_status_t geo_b200_layer_norm_vjp(const geo_b200_layer_norm_config_t *config, const void *device_x,

@@ -242,3 +242,18 @@ def test_rotary_null_and_bad_plans():
         assert call(ctypes.byref(abi.RotaryPlan()), q, SOME, None, SOME, None) == INVALID  # never initialised
         moved = rotary_shape(x_head_stride=64, y_head_stride=72)
         assert call(p, ctypes.byref(moved), SOME, None, SOME, None) == INVALID  # in place, another stride
+
+
+@pytest.mark.parametrize("name", ["x_stride", "y_cotangent_stride", "x_cotangent_stride"])
+@pytest.mark.parametrize("stride", [63, 1 << 60])
+def test_vjp_workspace_of_refused_strides(name, stride):
+    """0 bytes for whatever the VJP refuses, its strides among it; the forward's own stride does not matter."""
+    L = abi.lib()
+    c = norm_config(**{name: stride})
+    assert L.geo_b200_layer_norm_vjp(ctypes.byref(c), SOME, None, SOME, SOME, SOME, SOME, SOME, SOME, SOME, 1 << 30,
+                                     None) == INVALID
+    assert L.geo_b200_layer_norm_vjp_workspace(ctypes.byref(c)) == 0
+    packed = L.geo_b200_layer_norm_vjp_workspace(ctypes.byref(norm_config()))
+    assert packed > 0
+    assert L.geo_b200_layer_norm_vjp_workspace(ctypes.byref(norm_config(**{name: 72}))) == packed
+    assert L.geo_b200_layer_norm_vjp_workspace(ctypes.byref(norm_config(y_stride=stride))) == packed
