@@ -12,8 +12,14 @@ import pytest
 import layer_reference as ref
 from geometricelementaryoperators_b200 import abi
 from gpu_helpers import stream, torch
-from test_gpu_layers import (EPS, INVALID, P, call, drop_config, like, make, norm_config, parameters, rotary_case,
-                             rotary_shape, stats_like, workspace)
+from test_gpu_layers import (EPS, INVALID, KINDS, P, call, drop_bound, drop_config, like, make, mask, norm_config,
+                             parameters, rotary_case, rotary_shape, stats_like, untouched, workspace)
+from test_gpu_layers import test_layer_norm as check_layer_norm
+from test_gpu_layers import test_layer_norm_in_place_and_without_parameters as check_in_place
+from test_gpu_layers import test_layer_norm_non_finite_rows_stay_apart as check_non_finite
+from test_gpu_layers import test_layer_norm_vjp as check_layer_norm_vjp
+from test_gpu_layers import test_residual_dropout_layer_norm as check_fused
+from test_gpu_layers import test_residual_dropout_layer_norm_vjp as check_fused_vjp
 
 pytestmark = pytest.mark.gpu
 
@@ -234,5 +240,77 @@ def test_wait_of_a_cluster_that_gives_up(cols, backward):
                                                    None, 0, 1, 64, stream()) == INVALID
     assert L.geo_b200_layer_norm_wait_selftest(ctypes.byref(n), P(x), None, P(out), P(stats[0]), P(stats[1]), None, None,
                                                None, 0, 1, 0, stream()) == INVALID
+
+
+# Rows beyond the clusters' length (32768 values, 16384 in float64), for every type: packed, many, off 16 bytes.
+@pytest.mark.parametrize("kind,pkind", KINDS)
+@pytest.mark.parametrize("rows,cols,pad", [(3, 32769, 0), (70, 40000, 0), (2, 100003, 1), (200, 33000, 8)])
+def test_layer_norm_of_rows_of_any_length(kind, pkind, rows, cols, pad):
+    check_layer_norm(kind, pkind, rows, cols, pad)
+    check_layer_norm_vjp(kind, pkind, rows, cols, pad)
+
+
+@pytest.mark.parametrize("kind,pkind", KINDS)
+@pytest.mark.parametrize("rows,cols,pad,dimension", [(3, 32769, 0, 0), (70, 40000, 0, 6), (2, 100003, 1, 0), (200, 33000, 8, 3)])
+def test_residual_dropout_layer_norm_of_rows_of_any_length(kind, pkind, rows, cols, pad, dimension):
+    check_fused(kind, pkind, rows, cols, pad, dimension)
+    check_fused_vjp(kind, pkind, rows, cols, pad, dimension)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("cols,pad", [(32776, 0), (40001, 1)])
+def test_rows_of_any_length_in_place_and_non_finite(kind, cols, pad):
+    check_in_place(kind, cols, pad)
+    check_non_finite(kind, cols)
+
+
+@pytest.mark.parametrize("kind", ["f64", "f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows,cols,pads", [(50, 100, (1, 0, 3, 2)), (9, 1003, (0, 5, 1, 2)), (7, 5001, (2, 3, 0, 1)),
+                                            (130, 13, (0, 1, 2, 3)), (3, 33001, (1, 2, 0, 3))])
+def test_dropped_cotangent_of_arrays_of_unlike_alignment(kind, rows, cols, pads):
+    """x_bar of the fused VJP, every array with a stride and an alignment of its own: kept values scaled, dropped ones 0."""
+    t = torch()
+    dtype = ref.torch_type(kind)
+    z, dy, dz, other = (make(rows, cols, dtype, p, seed=i, shift=0.2) for i, p in enumerate(pads))
+    w, b = parameters(cols, dtype)
+    _, mean, rstd = ref.norm(z.double(), None, None, EPS)
+    mean, rstd = mean.to(ref.wide_type(dtype)), rstd.to(ref.wide_type(dtype))
+    (dres, rw), (dx, xw) = like(dy), like(other)
+    rate = 0.3
+    n = norm_config(z, dtype, y_cotangent_stride=dy.stride(0), x_cotangent_stride=dres.stride(0))
+    d = drop_config(z, rate, y_stride=z.stride(0), y_cotangent_stride=dz.stride(0), x_cotangent_stride=dx.stride(0))
+    keep = mask(d)
+    call("geo_b200_residual_dropout_layer_norm_vjp", ctypes.byref(n), ctypes.byref(d), None, P(z), P(w), P(mean), P(rstd),
+         P(dy), P(dz), P(dres), P(dx), None, None, None, 0)
+    wide = [v.double() for v in (z, w, mean, rstd, dy)]
+    want = ref.norm_vjp(*wide)[0] + dz.double()
+    bounds = ref.norm_vjp_bound(*wide, want, dtype, max(ref.PATH, cols // 100))
+    inner = bounds[0] - ref.half_step(dtype) * want.abs() + ref.u_wide(dtype) * want.abs()
+    ref.assert_within(dres, want, bounds[0] + ref.u_wide(dtype) * want.abs(), "dresidual")
+    want_dx = t.where(keep, want * ref.scale(rate), t.zeros_like(want))
+    ref.assert_within(dx, want_dx, drop_bound(want, keep, rate, want_dx, dtype) + ref.scale(rate) * inner, "dx")
+    assert untouched(rw, cols) and untouched(xw, cols)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f64", "bf16"])
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+def test_rotary_at_the_highest_frequencies(kind, layout):
+    """A base below 1 makes frequencies up to the largest that a plan takes (2^18 turns a position): at far positions the
+    angle's own error, 2^-63 |position| turns times the turns a position, is what the result is off by."""
+    t = torch()
+    x = rotary_case(kind, 1, 6, 3, 64)
+    positions = np.array([[-(1 << 31), (1 << 31) - 1, 1 << 31, 1234567891, -2147483647, 77]])
+    c = abi.RotaryConfig(layout=abi.ROTARY_HALF if layout == "half" else abi.ROTARY_INTERLEAVED, rotary_dim=64, base=4e-7,
+                         scaling=abi.ROTARY_SCALING_NONE, amplitude=1.0)
+    plan = abi.RotaryPlan()
+    assert abi.lib().geo_b200_rotary_plan_init(ctypes.byref(plan), ctypes.byref(c)) == 0
+    turns = ref.rotary_turns(64, 4e-7)
+    assert 2 ** 17 < turns[-1] <= 2 ** 18
+    for name, backward in (("geo_b200_rotary", False), ("geo_b200_rotary_vjp", True)):
+        y = t.empty_like(x)
+        call(name, ctypes.byref(plan), ctypes.byref(rotary_shape(x, y, position_batch_stride=6)), P(x),
+             P(t.tensor(positions, device="cuda")), P(y))
+        want = ref.rotary(x.double(), positions, turns, layout, 1.0, backward)
+        ref.assert_within(y, want, ref.rotary_bound(x.double(), want, turns, layout, 1.0, x.dtype, 1 << 31), name)
 
 
