@@ -314,3 +314,40 @@ def test_rotary_at_the_highest_frequencies(kind, layout):
         ref.assert_within(y, want, ref.rotary_bound(x.double(), want, turns, layout, 1.0, x.dtype, 1 << 31), name)
 
 
+@pytest.mark.parametrize("kind,cols", [("f32", 8192), ("bf16", 5120), ("bf16", 4096), ("f16", 8001), ("f32", 33000)])
+def test_captured_graph_of_wide_rows(kind, cols):
+    """Forward and VJP of rows in blocks, in clusters and of any length, captured and replayed on other inputs: the bits
+    of eager calls, while eager calls with a workspace of their own run on another stream."""
+    t = torch()
+    dtype = ref.torch_type(kind)
+    x, res, dy, dz = (make(300, cols, dtype, seed=s) for s in range(4))
+    w, b = parameters(cols, dtype)
+    n, d = norm_config(x, dtype), drop_config(x, 0.4)
+    outs, spaces = [], []
+    for _ in range(2):
+        outs.append([t.empty_like(x) for _ in range(4)] + stats_like(x) + [t.empty_like(w), t.empty_like(b)])
+        spaces.append(workspace(n))
+
+    def step(k):
+        z, y, dres, dx, mean, rstd, dw, db = outs[k]
+        call("geo_b200_residual_dropout_layer_norm", ctypes.byref(n), ctypes.byref(d), P(x), P(res), None, P(w), P(b), P(z),
+             P(y), P(mean), P(rstd))
+        call("geo_b200_residual_dropout_layer_norm_vjp", ctypes.byref(n), ctypes.byref(d), None, P(z), P(w), P(mean),
+             P(rstd), P(dy), P(dz), P(dres), P(dx), P(dw), P(db), P(spaces[k][0]), spaces[k][1])
+
+    side, graph = t.cuda.Stream(), t.cuda.CUDAGraph()
+    side.wait_stream(t.cuda.current_stream())
+    with t.cuda.graph(graph, stream=side):
+        step(0)
+    for s in range(3):
+        for k, v in enumerate((x, res, dy, dz)):
+            v.copy_(make(300, cols, dtype, seed=100 + 10 * s + k))
+        t.cuda.synchronize()
+        for _ in range(3):
+            with t.cuda.stream(side):
+                graph.replay()
+            step(1)
+        t.cuda.synchronize()
+        assert all(t.equal(p, q) for p, q in zip(*outs))
+
+
