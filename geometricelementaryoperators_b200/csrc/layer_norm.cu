@@ -48,16 +48,21 @@ bool aligned16(size_t cols, size_t bytes, size_t parameter_bytes, std::initializ
 
 namespace {
 
-// Threads that a multiprocessor holds: 80 registers a thread, 128 where two
-// rows are held at a time, and where 80 spill (off 16 bytes, fused: 8192 x 4001
-// float16 96 us with 512 threads, 105 with 768; 1102 x 10123 42 and 50).
-constexpr int resident_threads(size_t bytes, bool shift, int team) {
-    return rows_at_once(bytes, shift, team) == 2 || (shift && team != kWarp) ? 512 : 768;
+// Threads that a multiprocessor holds: 512 of up to 128 registers each. With 768 of
+// 80 most kernels spill, and the deeper ring that 512 leave room for feeds them as
+// well: 65536 x 200 float64 37.0 us with 512, 46.7 with 768; 2^18 x 65 float64 fused
+// 146, 180; 2^19 x 64 bfloat16 fused 50.3, 62.4; 16384 x 3000 float32 68.0, 78.2; 4096
+// x 8192 float64 101, 113; 8192 x 4001 float16 fused 96, 105. float32 rows in clusters
+// wait for the exchange and want the warps: 4096 x 8192 52.1 us with 512, 48.8 with
+// 768; 2048 x 32768 113, 105; with dropout to work on meanwhile they do not (96.5,
+// 100.7).
+constexpr int resident_threads(size_t bytes, bool drop, bool shift, int team) {
+    return bytes == 4 && team == kCluster && !drop && !shift ? 768 : 512;
 }
 
 template <typename T, bool DROP, int TEAM, bool SHIFT, bool FULL, bool STARVE = false>
 __global__ void __launch_bounds__(TEAM == kWarp ? kWarpBlock : kTeamThreads,
-                                  resident_threads(sizeof(T), SHIFT, TEAM) / (TEAM == kWarp ? kWarpBlock : kTeamThreads))
+                                  resident_threads(sizeof(T), DROP, SHIFT, TEAM) / (TEAM == kWarp ? kWarpBlock : kTeamThreads))
     norm_kernel(const ForwardArgs a, int lanes, bool float_parameters, int stages) {
     using W = Wide<T>;
     constexpr int V = 16 / (int)sizeof(T), K = values_per_thread(sizeof(T)) / V, Q = K * V / 2;
@@ -256,7 +261,7 @@ __global__ void __launch_bounds__(kThreads, DROP ? 4 : 8) norm_any_kernel(const 
 // `stages` rows of `stage` bytes in the ring, and the grid, of a team kernel.
 template <typename T, bool DROP, int TEAM, bool SHIFT, bool FULL, bool STARVE = false>
 cudaError_t launch_shape(const Shape &s, const ForwardArgs &a, bool float_parameters, cudaStream_t stream) {
-    constexpr int resident = resident_threads(sizeof(T), SHIFT, TEAM), at_once = rows_at_once(sizeof(T), SHIFT, TEAM);
+    constexpr int resident = resident_threads(sizeof(T), DROP, SHIFT, TEAM), at_once = rows_at_once(sizeof(T), SHIFT, TEAM);
     const size_t stage = (DROP ? 2 : 1) * s.part(sizeof(T));
     const int stages = ring_stages(stage, at_once, s.threads(), resident);
     const size_t each = s.teams() * at_once, wanted = (a.rows + each - 1) / each;

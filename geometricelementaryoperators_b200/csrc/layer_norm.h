@@ -458,7 +458,7 @@ struct Exchange {
     W values[2][N][kEntries<TEAM>];
     uint64_t arrived[2];  // kCluster: mbarriers that count the bytes which other blocks send
 };
-constexpr uint32_t kWaitPolls = 1u << 22;  // seconds; a round takes microseconds
+constexpr uint32_t kWaitPolls = 1u << 22;  // 16 seconds (3.9 us each); a round takes microseconds
 
 template <typename W, int N, int TEAM>
 __device__ __forceinline__ void open_exchange(Exchange<W, N, TEAM> &x) {
