@@ -3,11 +3,11 @@
 //
 // y = [residual +] keep x / (1 - rate): one multiply-add a value and an eighth of a
 // Philox block (forty instructions), so HBM bounds it as long as a block is worked
-// out once for its eight values. Measured, calls in turn over several sets of
-// arrays: 8192^2 bfloat16 with a residual 62 us (6.5 TB/s, 99% of the copy
-// bandwidth), 2^18 x 64 float64 by whole multivectors 44 us (6.1 TB/s, 93%);
-// 8192 x 2001 bfloat16 off 16 bytes 34 us (2.9 TB/s: instructions, 330 for eight
-// values).
+// out once for its eight values. Measured on two boards, calls in turn over three sets
+// of arrays, host included: 8192^2 bfloat16 with a residual 62 and 66 us (6.1 TB/s, 94%
+// of the copy bandwidth on the slower one), 2^18 x 64 float64 by whole multivectors 44
+// and 45 us (6.0 TB/s, 92%); 8192 x 2001 bfloat16 with a residual, rows off 16 bytes,
+// 34 us (2.9 TB/s: 420 instructions for eight values, on 72% of the issue slots).
 #include "geo_runtime.h"
 #include "layers.h"
 

@@ -7,9 +7,11 @@
 // it; but a 16-bit value comes and goes in four bytes, and at 6.5 TB/s a
 // multiprocessor has 22 instructions for each, hence the packed arithmetic, the
 // parameters in registers and the few exchanges between threads (11 instructions a
-// value, 25 with residual and dropout). Measured, calls in turn over several sets of
-// arrays: 8192 x 4096 bfloat16 25 us (5.4 TB/s, 83% of the copy bandwidth), with
-// residual and dropout 16384 x 4096 94 us (5.7 TB/s, 87%).
+// value, 25 with residual and dropout). What is left to wait for are shared memory
+// and fixed latencies, at 16 warps a multiprocessor (half the issue slots are used).
+// Measured on two boards, calls in turn over three sets of arrays, host included:
+// 8192 x 4096 bfloat16 25 us (5.3 TB/s, 82% of the copy bandwidth), with residual
+// and dropout 16384 x 4096 94 and 101 us (5.3 TB/s, 81% on the slower one).
 #include "layer_norm.h"
 
 #include <cmath>

@@ -7,11 +7,12 @@
 // One pass reads x and y_bar once and writes x_bar once: HBM bounds it. The column
 // sums stay with the thread that owns the column over all rows of its team, so
 // what is added up at the end is one partial sum a block, in a fixed order.
-// Measured, calls in turn over several sets of arrays: 2^19 x 64 float64 136 us
-// (6.0 TB/s, 91% of the copy bandwidth), 16384 x 4096 bfloat16 behind residual +
-// dropout 120 us (5.6 TB/s, 85%: 35 instructions a value, a third of them
-// dropout's), 3001 x 1003 float32 off 16 bytes 20 us (two and a half rows a team:
-// start-up and joining are half of it).
+// Measured on two boards, calls in turn over three sets of arrays, host included:
+// 2^19 x 64 float64 136 and 140 us (5.8 TB/s, 89% of the copy bandwidth on the slower
+// one), 16384 x 4096 bfloat16 behind residual + dropout 120 and 129 us (5.2 TB/s, 80%:
+// 35 instructions a value, a third of them dropout's, on 61% of the issue slots),
+// 3001 x 1003 float32 off 16 bytes 20 us (two and a half rows a team: start-up and
+// joining are half of it).
 #include "layer_norm.h"
 
 #include "geo_runtime.h"
@@ -226,9 +227,9 @@ __global__ void __launch_bounds__(TEAM == kWarp ? kWarpBlock : kTeamThreads, TEA
 }
 
 // out[c] = sum over the blocks of partial[block][which][c]: 32 columns a block of
-// threads, so that whole 128-byte lines are read (16384 x 4096 bfloat16 VJP: 114 us;
-// with 16 columns 118), blockDim / 32 threads a column, each over every so many
-// blocks in order, then those as a tree.
+// threads, so that whole 128-byte lines are read, blockDim / 32 threads a column, each
+// over every so many blocks in order, then those as a tree. (With 16 columns 16384 x
+// 4096 bfloat16 takes as long, 74.0 and 74.5 us.)
 constexpr int kJoinColumns = 32;
 template <typename W, typename P>
 __global__ void __launch_bounds__(1024) join_columns_kernel(const W *partial, int blocks, int cols, void *dweight,

@@ -4,13 +4,19 @@
 // quarter turns, p (hi + lo), in float64: adding 1.5 2^52 to p hi in a fused
 // multiply-add rounds it to whole quarters, whose last two bits are the quadrant,
 // and a second one leaves p hi - quarters with a single rounding. What is left is
-// at most half a quarter turn, so its conversion to float32 costs 2^-26 quarters
-// and far positions lose nothing. Its sine and cosine are polynomials
-// (interpolated at Chebyshev nodes, within 2^-28), two pairs at a time in packed
-// float32 arithmetic. HBM bounds it: a rotor is shared by the heads of a token.
-// Measured, calls in turn over several sets of arrays: 16384 tokens of 40 heads of
-// 128 bfloat16 values 58 us (5.8 TB/s, 88% of the copy bandwidth); eight tokens of
-// a decoding step 2.9 us on the device.
+// at most half a quarter turn and p lo, so its conversion to float32 costs 2^-26
+// quarters and far positions lose nothing. Its sine and cosine are polynomials
+// (interpolated at Chebyshev nodes, within 2^-28 up to half a quarter), two pairs at a
+// time in packed float32 arithmetic. At positions of 2^31, p lo is at most 2^-21
+// quarters for a pair of one turn a position; for one of 2^18, the most that a plan
+// takes, it is 1/8 and the polynomials are within 2^-21, where the frequency's own
+// last place is worth 2^-13.
+// HBM bounds it where a token has heads enough: a rotor is worked out once for the
+// heads that a thread turns, all of a token's where that leaves every multiprocessor
+// 2048 threads, else a group of them (5777 tokens of nine: three groups, each rotor
+// three times). Measured, calls in turn over three sets of arrays, host included: 16384
+// tokens of 40 heads of 128 bfloat16 values 58 to 59 us (5.7 TB/s, 87% of the copy
+// bandwidth); eight tokens of a decoding step 2.9 us on the device.
 #include <cmath>
 
 #include "geo_runtime.h"

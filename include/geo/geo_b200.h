@@ -353,15 +353,18 @@ geo_b200_status_t geo_b200_sparse_apply_parametric_vjp_f64(const geo_operator_pl
  *     other pointers are refused with GEO_B200_INVALID_ARGUMENT, as is an array
  *     that is not aligned to its value type, before anything is launched. Only
  *     argument and launch errors are reported. Nothing is allocated and nothing
- *     is kept between calls; calls may be captured into a CUDA graph.
+ *     is kept between calls; calls may be captured into a CUDA graph, and made by
+ *     several host threads at once.
  *   - strides are in values; 0 means packed rows, otherwise stride >= cols.
  *     Nothing is written between the rows; what lies there may be read along
  *     with its neighbours and has no effect.
  *   - an output may be the same array (pointer and stride) as an input of the
  *     call that it overwrites; arrays must not overlap otherwise.
- *   - arithmetic and sums are float64 for GEO_B200_F64 and float32 otherwise,
- *     rounded once (to nearest, ties to even) to the array's type. Sums are
- *     taken in a fixed order: the same call gives the same bits.
+ *   - arithmetic and sums are float64 for GEO_B200_F64 and float32 otherwise
+ *     (epsilon, the scale of dropout and the amplitude of rotary positions are
+ *     rounded to it, and what leaves its range is infinite), rounded once (to
+ *     nearest, ties to even) to the array's type. Sums are taken in a fixed
+ *     order: the same call gives the same bits.
  *   - infinities and NaN reach every output that depends on them. */
 typedef enum {
     GEO_B200_F64 = 1,
@@ -374,7 +377,9 @@ typedef enum {
 #define GEO_B200_LAYER_MAX_ROWS 4294967296ull
 
 /* Layer norm over each row: with mean m and variance v (divided by cols),
- *   rstd = 1 / sqrt(v + epsilon),  y = (x - m) rstd weight + bias. */
+ *   rstd = 1 / sqrt(v + epsilon),  y = (x - m) rstd weight + bias.
+ * The mean over a multivector's coefficients, and a weight and bias for each, do
+ * not commute with rotors: on rows of multivectors this is a norm of channels. */
 typedef struct {
     uint32_t type;              /* geo_b200_type_t of x, y and their cotangents */
     uint32_t parameter_type;    /* of weight, bias and their cotangents: `type`, or F32 for the 16-bit types */
