@@ -516,7 +516,7 @@ extern "C" geo_b200_status_t geo_b200_layer_norm_wait_selftest(
     void *device_workspace, size_t workspace_bytes, uint32_t round, uint32_t wait_limit, cudaStream_t stream) {
     geo::NvtxRange range("geo_b200.layer_norm_wait_selftest");
     if (!config_valid(config) || config->type != GEO_B200_F32 || config->x_stride != 0 || config->y_stride != 0 ||
-        config->y_cotangent_stride != 0 || config->x_cotangent_stride != 0 || wait_limit == 0 || device_x == nullptr ||
+        config->y_cotangent_stride != 0 || config->x_cotangent_stride != 0 || wait_limit == 0 || wait_limit > kWaitPolls || device_x == nullptr ||
         device_out == nullptr || device_mean == nullptr || device_rstd == nullptr)
         return GEO_B200_INVALID_ARGUMENT;
     const Shape s = shape_of(config->cols, 4, true);

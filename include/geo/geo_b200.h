@@ -428,7 +428,8 @@ geo_b200_status_t geo_b200_layer_norm_vjp(const geo_b200_layer_norm_config_t *co
  * norm of device_x into device_out (device_y_cotangent NULL, mean and rstd
  * written), or its VJP (device_out: x_bar; mean and rstd read). In round `round` of
  * the rows that a cluster takes one after another, its last block sends nothing;
- * waits give up after wait_limit polls. Later rows, and the column sums, are NaN. */
+ * waits give up after wait_limit polls, 1 .. 2^22. Later rows, and the column sums,
+ * are NaN. */
 geo_b200_status_t geo_b200_layer_norm_wait_selftest(
     const geo_b200_layer_norm_config_t *config, const void *device_x, const void *device_y_cotangent, void *device_out,
     void *device_mean, void *device_rstd, void *device_weight_cotangent, void *device_bias_cotangent,

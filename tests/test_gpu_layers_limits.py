@@ -351,3 +351,12 @@ def test_captured_graph_of_wide_rows(kind, cols):
         assert all(t.equal(p, q) for p, q in zip(*outs))
 
 
+def test_wait_selftest_refuses_longer_waits():
+    t = torch()
+    x = make(4, 8192, t.float32)
+    y, _ = like(x)
+    mean, rstd = stats_like(x)
+    n = norm_config(x, t.float32, x_stride=0, y_stride=0, y_cotangent_stride=0, x_cotangent_stride=0)
+    for polls, status in ((1 << 22, 0), ((1 << 22) + 1, INVALID), ((1 << 32) - 1, INVALID)):
+        assert abi.lib().geo_b200_layer_norm_wait_selftest(ctypes.byref(n), P(x), None, P(y), P(mean), P(rstd), None, None,
+                                                           None, 0, 1000, polls, stream()) == status  # no such round
