@@ -110,6 +110,71 @@ class LayerNormConfig(ctypes.Structure):
     ]
 
 
+GATE_NONE, GATE_LINEAR, GATE_SIGMOID, GATE_TANH = 0, 1, 2, 3  # geo_b200_gate_t
+ACTIVATION_SILU, ACTIVATION_GELU, ACTIVATION_SIGMOID, ACTIVATION_RELU = 1, 2, 3, 4  # geo_b200_activation_t
+
+
+class BlockNormConfig(ctypes.Structure):
+    """geo_b200_block_norm_config_t: strides in values, 0 for packed rows."""
+
+    _fields_ = [
+        ("type", ctypes.c_uint32),
+        ("parameter_type", ctypes.c_uint32),
+        ("gate", ctypes.c_uint32),
+        ("reserved", ctypes.c_uint32),
+        ("rows", ctypes.c_size_t),
+        ("cols", ctypes.c_size_t),
+        ("x_stride", ctypes.c_size_t),
+        ("residual_stride", ctypes.c_size_t),
+        ("gate_stride", ctypes.c_size_t),
+        ("z_stride", ctypes.c_size_t),
+        ("y_stride", ctypes.c_size_t),
+        ("y_cotangent_stride", ctypes.c_size_t),
+        ("z_cotangent_stride", ctypes.c_size_t),
+        ("residual_cotangent_stride", ctypes.c_size_t),
+        ("x_cotangent_stride", ctypes.c_size_t),
+        ("gate_cotangent_stride", ctypes.c_size_t),
+        ("epsilon", ctypes.c_double),
+        ("residual_scale", ctypes.c_double),
+        ("block_scale", ctypes.c_double),
+    ]
+
+
+class FeedForwardConfig(ctypes.Structure):
+    """geo_b200_feed_forward_config_t: strides in values, 0 for packed rows."""
+
+    _fields_ = [
+        ("type", ctypes.c_uint32),
+        ("gradient_type", ctypes.c_uint32),
+        ("activation", ctypes.c_uint32),
+        ("reserved", ctypes.c_uint32),
+        ("rows", ctypes.c_size_t),
+        ("cols", ctypes.c_size_t),
+        ("hidden", ctypes.c_size_t),
+        ("x_stride", ctypes.c_size_t),
+        ("y_stride", ctypes.c_size_t),
+        ("y_cotangent_stride", ctypes.c_size_t),
+        ("x_cotangent_stride", ctypes.c_size_t),
+        ("gate_weight_stride", ctypes.c_size_t),
+        ("up_weight_stride", ctypes.c_size_t),
+        ("down_weight_stride", ctypes.c_size_t),
+        ("gate_stride", ctypes.c_size_t),
+        ("up_stride", ctypes.c_size_t),
+    ]
+
+
+class Gradient(ctypes.Structure):
+    """geo_b200_gradient_t: one array of a model's gradients, and where its clipped values go."""
+
+    _fields_ = [
+        ("type", ctypes.c_uint32),
+        ("reserved", ctypes.c_uint32),
+        ("count", ctypes.c_size_t),
+        ("gradient", ctypes.c_void_p),
+        ("clipped", ctypes.c_void_p),
+    ]
+
+
 class DropoutConfig(ctypes.Structure):
     """geo_b200_dropout_config_t: units of 2^dimension values are kept or dropped as one."""
 
@@ -285,6 +350,18 @@ SIGNATURES: dict[str, tuple] = {
     "geo_b200_rotary_plan_init": (_I, [ctypes.POINTER(RotaryPlan), ctypes.POINTER(RotaryConfig)]),
     "geo_b200_rotary": (_I, [ctypes.POINTER(RotaryPlan), ctypes.POINTER(RotaryShape), _P, _P, _P, _P]),
     "geo_b200_rotary_vjp": (_I, [ctypes.POINTER(RotaryPlan), ctypes.POINTER(RotaryShape), _P, _P, _P, _P]),
+    "geo_b200_rms_norm": (_I, [ctypes.POINTER(LayerNormConfig), _P, _P, _P, _P, _P]),
+    "geo_b200_rms_norm_vjp_workspace": (_SZ, [ctypes.POINTER(LayerNormConfig)]),
+    "geo_b200_rms_norm_vjp": (_I, [ctypes.POINTER(LayerNormConfig), _P, _P, _P, _P, _P, _P, _P, _SZ, _P]),
+    "geo_b200_block_norm": (_I, [ctypes.POINTER(BlockNormConfig), *[_P] * 10]),
+    "geo_b200_block_norm_vjp_workspace": (_SZ, [ctypes.POINTER(BlockNormConfig)]),
+    "geo_b200_block_norm_vjp": (_I, [ctypes.POINTER(BlockNormConfig), *[_P] * 15, _SZ, _P]),
+    "geo_b200_feed_forward_workspace": (_SZ, [ctypes.POINTER(FeedForwardConfig)]),
+    "geo_b200_feed_forward_vjp_workspace": (_SZ, [ctypes.POINTER(FeedForwardConfig)]),
+    "geo_b200_feed_forward": (_I, [ctypes.POINTER(FeedForwardConfig), *[_P] * 8, _SZ, _P]),
+    "geo_b200_feed_forward_vjp": (_I, [ctypes.POINTER(FeedForwardConfig), *[_P] * 12, _SZ, _P]),
+    "geo_b200_gradient_clip_workspace": (_SZ, [ctypes.POINTER(Gradient), _SZ]),
+    "geo_b200_gradient_clip": (_I, [ctypes.POINTER(Gradient), _SZ, _D, _P, _P, _P, _SZ, _P]),
 }
 
 

@@ -1,0 +1,279 @@
+// feed_forward.cu -- the gated feed-forward block (geo/geo_b200.h section 5): entry
+// points, which kernels a call takes, and its workspace.
+//
+// Forward, two products: gate and up with the activation and their product (h), then
+// h down_weight^T. VJP, three: y_bar down_weight with the activation's derivative
+// behind it, x_bar, and the weights' cotangents (one launch: with down_weight's turned,
+// all three are [hidden][cols] sums over the rows).
+// h and the cotangents of gate and up pass between them in the workspace, rounded to
+// the arrays' type (the tensor cores' operands): a product of 16-bit values sums
+// thousands of them in float32, so their roundings average out against the result's
+// own. A float32 result has no rounding to hide them (2.3e-3 of its size off, where its
+// sums are 2e-6): on their way to one, what was lost is kept as a second array of the
+// type and multiplied as well.
+#include "feed_forward.h"
+
+#include <algorithm>
+
+#include "geo_runtime.h"
+
+namespace {
+
+using namespace geo::layers;
+
+constexpr size_t kAlign = 256;
+
+// The config with its strides resolved; false for what the call would refuse.
+bool resolve(const geo_b200_feed_forward_config_t *config, bool vjp, geo_b200_feed_forward_config_t *out) {
+    if (config == nullptr || type_bytes(config->type) == 0 || config->reserved != 0) return false;
+    geo_b200_feed_forward_config_t c = *config;
+    if (c.gradient_type != c.type && !(type_bytes(c.type) == 2 && c.gradient_type == GEO_B200_F32)) return false;
+    if (c.activation < GEO_B200_ACTIVATION_SILU || c.activation > GEO_B200_ACTIVATION_RELU) return false;
+    if (c.rows == 0 || c.cols == 0 || c.hidden == 0 || c.rows > GEO_B200_FEED_FORWARD_MAX_ROWS ||
+        c.cols > GEO_B200_FEED_FORWARD_MAX_WIDTH || c.hidden > GEO_B200_FEED_FORWARD_MAX_WIDTH)
+        return false;
+    if (!resolve_strides(c.hidden, c.cols, {&c.gate_weight_stride, &c.up_weight_stride}) ||
+        !resolve_strides(c.cols, c.hidden, {&c.down_weight_stride}) ||
+        !resolve_strides(c.rows, c.hidden, {&c.gate_stride, &c.up_stride}) ||
+        !resolve_strides(c.rows, c.cols, {&c.x_stride}))
+        return false;
+    if (vjp ? !resolve_strides(c.rows, c.cols, {&c.y_cotangent_stride, &c.x_cotangent_stride})
+            : !resolve_strides(c.rows, c.cols, {&c.y_stride}))
+        return false;
+    *out = c;
+    return true;
+}
+
+size_t round8(size_t n) { return (n + 7) / 8 * 8; }
+bool off16(size_t stride) { return stride % 8 != 0; }
+
+// Where things lie in the workspace. `take` returns the place of rows x stride values.
+struct Space {
+    unsigned char *base;
+    size_t used = 0;
+    void *take(size_t rows, size_t stride, size_t bytes) {
+        void *p = base == nullptr ? nullptr : base + used;
+        used += (rows * stride * bytes + kAlign - 1) / kAlign * kAlign;
+        return p;
+    }
+};
+
+// Few rows are the weights' way through memory: one warp a column (feed_forward_plain.cu).
+bool few_rows(const geo_b200_feed_forward_config_t &c) {
+    return c.rows <= (size_t)(type_bytes(c.type) == 2 ? kFewRows / 2 : kFewRows);
+}
+
+// The arrays of a call that TMA would read, by rows of `stride` values; those off 16
+// bytes by their stride are copied to the workspace.
+struct Operand {
+    Matrix m;
+    size_t rows, cols;
+};
+size_t packed_bytes(const Operand &o) {
+    return off16(o.m.stride) ? (o.rows * round8(o.cols) * 2 + kAlign - 1) / kAlign * kAlign : 0;
+}
+cudaError_t pack(Operand &o, Space &space, cudaStream_t stream) {
+    if (!off16(o.m.stride)) return cudaSuccess;
+    void *to = space.take(o.rows, round8(o.cols), 2);
+    const cudaError_t e = launch_pack_rows(o.m, o.rows, o.cols, to, round8(o.cols), stream);
+    o.m = {to, round8(o.cols)};
+    return e;
+}
+// Whether the tensor-core kernels take these arrays, once those off 16 bytes by their stride are copied.
+bool tensor_call(const geo_b200_feed_forward_config_t &c, std::initializer_list<const Operand *> arrays) {
+    if (type_bytes(c.type) != 2 || !tensor_products_available()) return false;
+    // A tensor map's strides end at 2^40 bytes.
+    for (const Operand *o : arrays)
+        if (!off16(o->m.stride) && ((uintptr_t)o->m.p % 16 != 0 || o->m.stride >= (size_t)1 << 39)) return false;
+    return true;
+}
+
+// Outputs apart from the inputs and from each other, as far as their starts tell.
+bool apart(std::initializer_list<const void *> outs, std::initializer_list<const void *> ins) {
+    for (auto o = outs.begin(); o != outs.end(); ++o) {
+        if (*o == nullptr) continue;
+        for (const void *i : ins)
+            if (*o == i) return false;
+        for (auto other = o + 1; other != outs.end(); ++other)
+            if (*o == *other) return false;
+    }
+    return true;
+}
+
+}  // namespace
+
+extern "C" size_t geo_b200_feed_forward_workspace(const geo_b200_feed_forward_config_t *config) {
+    geo_b200_feed_forward_config_t c;
+    if (!resolve(config, false, &c)) return 0;
+    Space space = {nullptr};
+    const size_t b = type_bytes(c.type);
+    space.take(c.rows, round8(c.hidden), b);
+    if (b == 2 && !few_rows(c))
+        for (const Operand &o : {Operand{{nullptr, c.x_stride}, c.rows, c.cols},
+                                 Operand{{nullptr, c.gate_weight_stride}, c.hidden, c.cols},
+                                 Operand{{nullptr, c.up_weight_stride}, c.hidden, c.cols},
+                                 Operand{{nullptr, c.down_weight_stride}, c.cols, c.hidden}})
+            space.used += packed_bytes(o);
+    return space.used;
+}
+
+extern "C" size_t geo_b200_feed_forward_vjp_workspace(const geo_b200_feed_forward_config_t *config) {
+    geo_b200_feed_forward_config_t c;
+    if (!resolve(config, true, &c)) return 0;
+    Space space = {nullptr};
+    const size_t b = type_bytes(c.type);
+    for (int i = 0; i < (c.gradient_type != c.type ? 6 : 3); ++i) space.take(c.rows, round8(c.hidden), b);
+    if (b == 2)
+        for (const Operand &o : {Operand{{nullptr, c.x_stride}, c.rows, c.cols},
+                                 Operand{{nullptr, c.y_cotangent_stride}, c.rows, c.cols},
+                                 Operand{{nullptr, c.gate_weight_stride}, c.hidden, c.cols},
+                                 Operand{{nullptr, c.up_weight_stride}, c.hidden, c.cols},
+                                 Operand{{nullptr, c.down_weight_stride}, c.cols, c.hidden}})
+            space.used += packed_bytes(o);
+    // Parts of the weights' cotangents, whichever kernels take the call.
+    int splits = weight_splits_plain(c.type, c.hidden, c.cols, c.rows);
+    if (b == 2) splits = std::max(splits, weight_splits_tensor(c.hidden, c.cols, c.rows));
+    if (splits > 1) space.take(3 * splits * c.hidden, partial_stride(c.cols), wide_bytes(c.type));
+    return space.used;
+}
+
+extern "C" geo_b200_status_t geo_b200_feed_forward(const geo_b200_feed_forward_config_t *config, const void *device_x,
+                                                   const void *device_gate_weight, const void *device_up_weight,
+                                                   const void *device_down_weight, void *device_gate, void *device_up,
+                                                   void *device_y, void *device_workspace, size_t workspace_bytes,
+                                                   cudaStream_t stream) {
+    geo::NvtxRange range("geo_b200.feed_forward");
+    geo_b200_feed_forward_config_t c;
+    if (!resolve(config, false, &c) || device_x == nullptr || device_gate_weight == nullptr ||
+        device_up_weight == nullptr || device_down_weight == nullptr || device_y == nullptr ||
+        (device_gate == nullptr) != (device_up == nullptr) || device_workspace == nullptr ||
+        workspace_bytes < geo_b200_feed_forward_workspace(config) ||
+        !apart({device_gate, device_up, device_y, device_workspace},
+               {device_x, device_gate_weight, device_up_weight, device_down_weight}))
+        return GEO_B200_INVALID_ARGUMENT;
+    const size_t b = type_bytes(c.type);
+    if (!arrays_usable({{device_x, b}, {device_gate_weight, b}, {device_up_weight, b}, {device_down_weight, b},
+                        {device_gate, b}, {device_up, b}, {device_y, b}, {device_workspace, kAlign}}))
+        return GEO_B200_INVALID_ARGUMENT;
+    Space space = {(unsigned char *)device_workspace};
+    const size_t hidden_stride = round8(c.hidden);
+    void *h = space.take(c.rows, hidden_stride, b);
+    Operand x = {{device_x, c.x_stride}, c.rows, c.cols}, wg = {{device_gate_weight, c.gate_weight_stride}, c.hidden, c.cols},
+            wu = {{device_up_weight, c.up_weight_stride}, c.hidden, c.cols},
+            wd = {{device_down_weight, c.down_weight_stride}, c.cols, c.hidden};
+    const bool few = few_rows(c), tensor = !few && tensor_call(c, {&x, &wg, &wu, &wd});
+    if (tensor)
+        for (Operand *o : {&x, &wg, &wu, &wd}) {
+            const cudaError_t e = pack(*o, space, stream);
+            if (e != cudaSuccess) return status_of(e);
+        }
+    Product gated = {};
+    gated.m = (int)c.rows, gated.n = (int)c.hidden, gated.k = (int)c.cols, gated.problems = gated.splits = 1;
+    gated.activation = (int)c.activation;
+    gated.a[0] = x.m;
+    gated.b[0] = wg.m;
+    gated.b[1] = wu.m;
+    gated.out[0] = {device_gate, c.gate_stride};
+    gated.out[1] = {device_up, c.up_stride};
+    gated.out[2] = {h, hidden_stride};
+    Product down = {};
+    down.m = (int)c.rows, down.n = (int)c.cols, down.k = (int)c.hidden, down.problems = down.splits = 1;
+    down.a[0] = {h, hidden_stride};
+    down.b[0] = wd.m;
+    down.out[0] = {device_y, c.y_stride};
+    auto launch = [&](ProductKind kind, const Product &p) {
+        if (few) return launch_product_few(kind, c.type, p, stream);
+        return tensor ? launch_product_tensor(kind, c.type, c.type, p, {UINT32_MAX, kPipelinePolls}, stream)
+                      : launch_product_plain(kind, c.type, c.type, p, stream);
+    };
+    const cudaError_t e = launch(kGated, gated);
+    return status_of(e != cudaSuccess ? e : launch(kDown, down));
+}
+
+extern "C" geo_b200_status_t geo_b200_feed_forward_vjp(
+    const geo_b200_feed_forward_config_t *config, const void *device_x, const void *device_gate_weight,
+    const void *device_up_weight, const void *device_down_weight, const void *device_gate, const void *device_up,
+    const void *device_y_cotangent, void *device_x_cotangent, void *device_gate_weight_cotangent,
+    void *device_up_weight_cotangent, void *device_down_weight_cotangent, void *device_workspace,
+    size_t workspace_bytes, cudaStream_t stream) {
+    geo::NvtxRange range("geo_b200.feed_forward_vjp");
+    geo_b200_feed_forward_config_t c;
+    const bool weights = device_gate_weight_cotangent != nullptr || device_up_weight_cotangent != nullptr;
+    const bool inner = weights || device_x_cotangent != nullptr;  // needs the cotangents of gate and up
+    if (!resolve(config, true, &c) || (!inner && device_down_weight_cotangent == nullptr) ||
+        (weights && device_x == nullptr) ||
+        (device_x_cotangent != nullptr && (device_gate_weight == nullptr || device_up_weight == nullptr)) ||
+        device_down_weight == nullptr || device_gate == nullptr || device_up == nullptr ||
+        device_y_cotangent == nullptr || device_workspace == nullptr ||
+        workspace_bytes < geo_b200_feed_forward_vjp_workspace(config) ||
+        !apart({device_x_cotangent, device_gate_weight_cotangent, device_up_weight_cotangent,
+                device_down_weight_cotangent, device_workspace},
+               {device_x, device_gate_weight, device_up_weight, device_down_weight, device_gate, device_up,
+                device_y_cotangent}))
+        return GEO_B200_INVALID_ARGUMENT;
+    const size_t b = type_bytes(c.type), g = type_bytes(c.gradient_type);
+    if (!arrays_usable({{device_x, b}, {device_gate_weight, b}, {device_up_weight, b}, {device_down_weight, b},
+                        {device_gate, b}, {device_up, b}, {device_y_cotangent, b}, {device_x_cotangent, b},
+                        {device_gate_weight_cotangent, g}, {device_up_weight_cotangent, g},
+                        {device_down_weight_cotangent, g}, {device_workspace, kAlign}}))
+        return GEO_B200_INVALID_ARGUMENT;
+    Space space = {(unsigned char *)device_workspace};
+    const size_t hidden_stride = round8(c.hidden);
+    void *inside[3], *low[3] = {};  // cotangents of gate and up, h; what they lost to rounding
+    for (void *&p : inside) p = space.take(c.rows, hidden_stride, b);
+    if (c.gradient_type != c.type)
+        for (void *&p : low) p = space.take(c.rows, hidden_stride, b);
+    Operand x = {{device_x, c.x_stride}, c.rows, c.cols}, wg = {{device_gate_weight, c.gate_weight_stride}, c.hidden, c.cols},
+            wu = {{device_up_weight, c.up_weight_stride}, c.hidden, c.cols},
+            wd = {{device_down_weight, c.down_weight_stride}, c.cols, c.hidden},
+            dy = {{device_y_cotangent, c.y_cotangent_stride}, c.rows, c.cols};
+    const bool tensor = tensor_call(c, {&x, &wg, &wu, &wd, &dy});
+    if (tensor)
+        for (Operand *o : {&x, &wg, &wu, &wd, &dy}) {
+            const cudaError_t e = o->m.p == nullptr ? cudaSuccess : pack(*o, space, stream);
+            if (e != cudaSuccess) return status_of(e);
+        }
+    auto launch = [&](ProductKind kind, const Product &p) {
+        return tensor ? launch_product_tensor(kind, c.type, c.gradient_type, p, {UINT32_MAX, kPipelinePolls}, stream)
+                      : launch_product_plain(kind, c.type, c.gradient_type, p, stream);
+    };
+    Product hidden = {};
+    hidden.m = (int)c.rows, hidden.n = (int)c.hidden, hidden.k = (int)c.cols, hidden.problems = hidden.splits = 1;
+    hidden.activation = (int)c.activation;
+    hidden.a[0] = dy.m;
+    hidden.b[0] = wd.m;
+    hidden.saved[0] = {device_gate, c.gate_stride};
+    hidden.saved[1] = {device_up, c.up_stride};
+    for (int i = 0; i < 3; ++i) {
+        const bool wanted = i == 2 ? device_down_weight_cotangent != nullptr : inner;
+        if (wanted) hidden.out[i] = {inside[i], hidden_stride};
+        if (wanted && (i == 2 || weights)) hidden.out_low[i] = {low[i], hidden_stride};
+    }
+    cudaError_t e = launch(kHidden, hidden);
+    if (e == cudaSuccess && device_x_cotangent != nullptr) {
+        Product input = {};
+        input.m = (int)c.rows, input.n = (int)c.cols, input.k = (int)c.hidden, input.problems = input.splits = 1;
+        for (int i = 0; i < 2; ++i) input.a[i] = {inside[i], hidden_stride};
+        input.b[0] = wg.m;
+        input.b[1] = wu.m;
+        input.out[0] = {device_x_cotangent, c.x_cotangent_stride};
+        e = launch(kInput, input);
+    }
+    Product w = {};
+    w.m = (int)c.hidden, w.n = (int)c.cols, w.k = (int)c.rows;
+    w.splits = tensor ? weight_splits_tensor(c.hidden, c.cols, c.rows) : weight_splits_plain(c.type, c.hidden, c.cols, c.rows);
+    w.partial = space.take(0, 0, 1);  // the rest
+    const OutMatrix outs[3] = {{device_gate_weight_cotangent, c.gate_weight_stride},
+                               {device_up_weight_cotangent, c.up_weight_stride},
+                               {device_down_weight_cotangent, c.down_weight_stride}};
+    for (int i = 0; i < 3; ++i)
+        if (outs[i].p != nullptr) {
+            w.a[w.problems] = {inside[i], hidden_stride};
+            w.low[w.problems] = {low[i], hidden_stride};
+            w.b[w.problems] = i == 2 ? dy.m : x.m;
+            w.transposed[w.problems] = i == 2;
+            w.out[w.problems++] = outs[i];
+        }
+    if (e == cudaSuccess && w.problems > 0) e = launch(kWeights, w);
+    return status_of(e);
+}

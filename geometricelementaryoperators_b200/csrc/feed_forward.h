@@ -1,0 +1,117 @@
+// feed_forward.h -- what the gated feed-forward block's entry points
+// (feed_forward.cu) and products (feed_forward_tensor.cu: 16-bit types on the
+// tensor cores; feed_forward_plain.cu: the others, and few rows) share.
+#pragma once
+
+#include "layers.h"
+
+namespace geo {
+namespace layers {
+
+// A row-major array; stride in values.
+struct Matrix {
+    const void *p;
+    size_t stride;
+};
+struct OutMatrix {
+    void *p;
+    size_t stride;
+};
+
+// The products of the block. M x N results, sums over K:
+enum ProductKind : int {
+    kGated = 0,   // gate = x Wg^T, up = x Wu^T, h = act(gate) up:   a[0] [M][K], b[0], b[1] [N][K]
+    kDown = 1,    // y = h Wd^T:                                     a[0] [M][K], b[0] [N][K]
+    kHidden = 2,  // h_bar = y_bar Wd, from it the cotangents of gate and up, and h: a[0] [M][K], b[0] [K][N]
+    kInput = 3,   // x_bar = gate_bar Wg + up_bar Wu:                a[0], a[1] [M][K], b[0], b[1] [K][N]
+    kWeights = 4  // up to three results of one size, a[z]^T b[z]:   a[z] [K][M], b[z] [K][N]
+};
+
+struct Product {
+    int m, n, k;
+    int activation;    // geo_b200_activation_t
+    int problems;      // kWeights: how many results; else 1
+    int splits;        // kWeights: parts of K, each with results of its own in `partial`, which are then added up; else 1
+    Matrix a[3], b[3];
+    Matrix low[3];     // kWeights to float32 from 16-bit types: what a[z] lost to rounding
+    Matrix saved[2];   // kHidden: gate, up
+    OutMatrix out[3];  // kGated: gate, up (may be null), h; kHidden: cotangents of gate and up, h; kWeights: [M][N], or
+    bool transposed[3];     // ... [N][M]
+    OutMatrix out_low[3];  // kHidden: what those lost to rounding, or null
+    void *partial;     // splits > 1: [problem][split][M][partial_stride(N)] of the arithmetic type
+};
+inline size_t partial_stride(size_t n) { return (n + 3) / 4 * 4; }
+
+// How many parts K is cut into for kWeights: where the results are too small to give
+// every multiprocessor a tile (rows of tile_m by tile_n), as many as do, but none under
+// `least` of K. Counts all three results, whichever are asked for.
+int weight_splits(size_t m, size_t n, size_t k, int tile_m, int tile_n, size_t least);
+constexpr int kSplitMost = 64;
+// The tensor-core and the plain kernels' own.
+int weight_splits_tensor(size_t m, size_t n, size_t k);
+int weight_splits_plain(uint32_t type, size_t m, size_t n, size_t k);
+// Adds the parts up, in their order, into the results.
+cudaError_t launch_join_splits(uint32_t type, uint32_t out_type, const Product &p, cudaStream_t stream);
+
+// For the self-test of the pipeline's waits alone: the block of K at which the
+// producer of every CTA stops (never: UINT32_MAX), and how often a wait looks.
+struct PipelineStarve {
+    uint32_t block, polls;
+};
+constexpr uint32_t kPipelinePolls = 1u << 22;  // seconds, where a stage takes microseconds
+
+// `type`: of the operands; `out_type`: of kWeights' results. A stream-ordered launch.
+cudaError_t launch_product_tensor(ProductKind kind, uint32_t type, uint32_t out_type, const Product &p,
+                                  PipelineStarve starve, cudaStream_t stream);
+cudaError_t launch_product_plain(ProductKind kind, uint32_t type, uint32_t out_type, const Product &p,
+                                 cudaStream_t stream);
+// kGated, kDown with at most kFewRows rows.
+constexpr int kFewRows = 8;
+cudaError_t launch_product_few(ProductKind kind, uint32_t type, const Product &p, cudaStream_t stream);
+// Copies rows x cols values of 16 bits to rows of `to_stride` (a multiple of 8), zeros behind each row's end.
+cudaError_t launch_pack_rows(const Matrix &from, size_t rows, size_t cols, void *to, size_t to_stride,
+                             cudaStream_t stream);
+// Whether the tensor-core products can run at all (the driver's tensor map encoder).
+bool tensor_products_available();
+
+#ifdef __CUDACC__
+// What v loses to its rounding to T, itself to be rounded to T: together they hold
+// twice T's digits. Nothing where T has no finite value for v.
+template <typename T>
+__device__ __forceinline__ float lost_to(float v) {
+    const float left = v - widen(narrow<T>(v));
+    return fabsf(left) < INFINITY ? left : 0.0f;
+}
+
+// ---- the activation ------------------------------------------------------------
+
+// act(a) and, where `slope` is asked for, act'(a). FAST: logistic()'s, next to the
+// 16-bit rounding of what it enters.
+template <bool FAST, typename W>
+__device__ __forceinline__ W activation(int kind, W a, W *slope) {
+    switch (kind) {
+        case GEO_B200_ACTIVATION_RELU:
+            if (slope != nullptr) *slope = a > W(0) ? W(1) : (a == a ? W(0) : a);  // NaN stays
+            return a > W(0) ? a : (a == a ? W(0) : a);
+        case GEO_B200_ACTIVATION_GELU: {
+            // Phi by the complementary error function, whose far tail keeps its relative accuracy.
+            const W below = W(0.5) * erfc(a * W(-0.70710678118654752440));
+            if (slope != nullptr) *slope = below + a * (exp(W(-0.5) * a * a) * W(0.39894228040143267794));
+            return a * below;
+        }
+        default: {
+            W s, rest;
+            logistic<FAST>(a, s, rest);
+            if (kind == GEO_B200_ACTIVATION_SIGMOID) {
+                if (slope != nullptr) *slope = s * rest;
+                return s;
+            }
+            if (slope != nullptr) *slope = s * (W(1) + a * rest);
+            return a * s;
+        }
+    }
+}
+#endif
+
+}  // namespace layers
+}  // namespace geo

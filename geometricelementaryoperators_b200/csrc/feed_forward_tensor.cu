@@ -1,0 +1,548 @@
+// feed_forward_tensor.cu -- the feed-forward block's products of 16-bit types on
+// the tensor cores (geo/geo_b200.h section 5).
+//
+// All products are C = A B over tiles of 128 rows by BN columns, K in steps of 64.
+// One block a multiprocessor, persistent over its tiles, six warps:
+//   warp 0   one thread copies tiles of A and B into a ring of stages (TMA,
+//            128-byte swizzle, completion on the stage's `full` mbarrier);
+//   warp 1   one thread issues the matrix instructions of a stage (tcgen05.mma,
+//            128 x BN x 16) and commits them to the stage's `empty` mbarrier, a
+//            tile's last to `ready`; the float32 sums stand in tensor memory, two
+//            tiles of BN columns in turn;
+//   warps 2-5 take a finished tile out of tensor memory (32 rows a warp), do what
+//            belongs to the product (activation, its derivative), round once and
+//            write it through shared memory in whole 64-byte pieces, while the next
+//            tile is multiplied.
+// Operands whose sum index is not the adjacent one (weights in the VJP, both sides
+// of the weights' cotangents) are copied as they lie, [64 of K][64 values] boxes,
+// and read by the matrix instruction as "MN-major": nothing is transposed.
+// kGated puts BN / 2 rows of each weight side by side in one B tile, so that gate and
+// up of the same hidden values are in one tile of sums; kInput adds both its products
+// into one tile, K running through the first pair of operands, then the second.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include "feed_forward.h"
+#include "geo_runtime.h"
+
+namespace geo {
+namespace layers {
+
+namespace {
+
+constexpr int kBM = 128, kBK = 64, kThreads = 192, kEpilogueWarps = 4;
+constexpr uint32_t bytes_a(bool twice) { return (twice ? 2 : 1) * kBM * kBK * 2; }
+constexpr uint32_t bytes_b(int bn) { return (uint32_t)bn * kBK * 2; }
+constexpr uint32_t kStagingPitch = 144;  // bytes of a row of 32 values of up to 4 bytes; 16 more keep banks apart
+constexpr uint32_t kStaging = 32 * kStagingPitch;
+constexpr uint32_t kSharedMost = 227 * 1024;
+constexpr int stages_of(int bn, bool twice) {
+    const int n = (int)((kSharedMost - 1024 - kEpilogueWarps * kStaging - 512) / (bytes_a(twice) + bytes_b(bn)));
+    return n > 8 ? 8 : n;
+}
+constexpr uint32_t shared_bytes(int bn, bool twice) {
+    return 1024 + stages_of(bn, twice) * (bytes_a(twice) + bytes_b(bn)) + kEpilogueWarps * kStaging;
+}
+struct Maps {
+    CUtensorMap a[3], b[3], low[3];
+};
+
+__device__ __forceinline__ void barrier_init(uint32_t barrier, uint32_t count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(barrier), "r"(count) : "memory");
+}
+__device__ __forceinline__ void barrier_expect(uint32_t barrier, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(barrier), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void barrier_arrive(uint32_t barrier) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(barrier) : "memory");
+}
+__device__ __forceinline__ bool barrier_try(uint32_t barrier, uint32_t parity) {
+    uint32_t done;
+    asm volatile(
+        "{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}"
+        : "=r"(done)
+        : "r"(barrier), "r"(parity)
+        : "memory");
+    return done != 0;
+}
+// Waits for the phase, at most `polls` looks; false when it gave up or another warp did.
+__device__ __forceinline__ bool barrier_wait(uint32_t barrier, uint32_t parity, uint32_t polls, volatile int *gave_up) {
+    for (uint32_t i = 0; i < polls; ++i) {
+        if (barrier_try(barrier, parity)) return true;
+        if (gave_up != nullptr && *gave_up) return false;
+    }
+    if (gave_up != nullptr) *gave_up = 1;
+    return false;
+}
+
+__device__ __forceinline__ void tma_load(uint32_t to, const CUtensorMap *map, int x, int y, uint32_t barrier) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(to),
+        "l"(map), "r"(x), "r"(y), "r"(barrier)
+        : "memory");
+}
+
+// Shared-memory descriptor of a 128-byte-swizzled operand. Its eight-row groups are
+// 1024 bytes apart; `leading`: bytes between blocks of 64 values (MN-major only).
+__device__ __forceinline__ uint64_t operand(uint32_t address, uint32_t leading) {
+    return (uint64_t)((address & 0x3FFFF) >> 4) | (uint64_t)((leading >> 4) & 0x3FFF) << 16 |
+           (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+// 16-bit operands, float32 sums, 128 x n.
+template <typename T>
+__device__ __forceinline__ constexpr uint32_t instruction(bool a_mn, bool b_mn, int n) {
+    const uint32_t format = std::is_same_v<T, __nv_bfloat16> ? 1 : 0;
+    return 1u << 4 | format << 7 | format << 10 | (uint32_t)a_mn << 15 | (uint32_t)b_mn << 16 |
+           (uint32_t)(n / 8) << 17 | (uint32_t)(kBM / 16) << 24;
+}
+__device__ __forceinline__ void multiply(uint32_t sums, uint64_t a, uint64_t b, uint32_t instruction, bool add) {
+    asm volatile(
+        "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(sums),
+        "l"(a), "l"(b), "r"(instruction), "r"((uint32_t)add)
+        : "memory");
+}
+__device__ __forceinline__ void commit_to(uint32_t barrier) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(barrier) : "memory");
+}
+
+// 32 columns of this thread's row of the warp's 32 rows of tensor memory.
+__device__ __forceinline__ void take_columns(uint32_t address, float (&v)[32]) {
+    uint32_t r[32];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(address));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+__device__ __forceinline__ size_t partial_width(int n) { return ((size_t)n + 3) / 4 * 4; }
+
+// Whether rows of this array can be read and written by 16 bytes.
+template <typename T>
+__device__ __forceinline__ bool by_16(const void *p, size_t stride) {
+    return ((uintptr_t)p % 16 | stride * sizeof(T) % 16) == 0;
+}
+
+// Writes this thread's 32 columns of its row (rows row0 + lane, columns col0 ...) of
+// an m x n array, through the warp's staging.
+template <typename O>
+__device__ __forceinline__ void put_columns(unsigned char *staging, const float (&v)[32], const OutMatrix &out, int row0,
+                                            int col0, int m, int n) {
+    constexpr int kVector = 16 / (int)sizeof(O), kPitch = 32 * (int)sizeof(O) + 16;
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int j = 0; j < 32 / kVector; ++j) {
+        Vec<O, kVector> piece;
+#pragma unroll
+        for (int q = 0; q < kVector / 2; ++q) piece.set(q, {v[j * kVector + 2 * q], v[j * kVector + 2 * q + 1]});
+        store<O, kVector>((O *)(staging + lane * kPitch) + j * kVector, piece);
+    }
+    __syncwarp();
+    if (by_16<O>(out.p, out.stride)) {
+        constexpr int kPieces = 32 / kVector, kRows = 32 / kPieces;
+        const int piece = lane % kPieces, c = col0 + piece * kVector;
+#pragma unroll
+        for (int r0 = 0; r0 < 32; r0 += kRows) {
+            const int r = r0 + lane / kPieces;
+            if (row0 + r >= m || c >= n) continue;
+            const O *from = (const O *)(staging + r * kPitch) + piece * kVector;
+            O *to = (O *)out.p + (size_t)(row0 + r) * out.stride + c;
+            if (c + kVector <= n) {
+                store<O, kVector>(to, load<O, kVector>(from));
+            } else {
+                for (int j = 0; c + j < n; ++j) to[j] = from[j];
+            }
+        }
+    } else {
+        for (int r = 0; r < 32 && row0 + r < m; ++r)
+            if (col0 + lane < n)
+                ((O *)out.p)[(size_t)(row0 + r) * out.stride + col0 + lane] = ((const O *)(staging + r * kPitch))[lane];
+    }
+    __syncwarp();
+}
+
+// 32 columns of a row of an m x n array; zeros outside.
+template <typename T>
+__device__ __forceinline__ void get_columns(const Matrix &in, int row, int col0, int m, int n, float (&v)[32]) {
+    if (row < m && col0 + 32 <= n && by_16<T>(in.p, in.stride)) {
+        const T *from = (const T *)in.p + (size_t)row * in.stride + col0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const Vec<T, 8> piece = load<T, 8>(from + 8 * j);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const Pair<float> p = piece.pair(q);
+                v[8 * j + 2 * q] = p.x;
+                v[8 * j + 2 * q + 1] = p.y;
+            }
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+            v[j] = row < m && col0 + j < n ? widen(((const T *)in.p)[(size_t)row * in.stride + col0 + j]) : 0.0f;
+    }
+}
+
+// Which tile is worked on n-th: panels of `kPanel` tiles down, all columns of tiles
+// across, so that the tiles in work at one time (one a multiprocessor) share rows
+// of A and columns of B in L2.
+constexpr int kPanel = 16;
+struct Tile {
+    int problem, split, row, column;
+};
+__device__ __forceinline__ Tile tile_of(int index, int down, int across, int splits) {
+    Tile t;
+    const int each = down * across, part = index / each;
+    t.problem = part / splits;
+    t.split = part - t.problem * splits;
+    index -= part * each;
+    const int panel = index / (kPanel * across), first = panel * kPanel;
+    const int height = down - first < kPanel ? down - first : kPanel;
+    index -= panel * kPanel * across;
+    t.row = first + index % height;
+    t.column = index / height;
+    return t;
+}
+
+// TWICE: A comes as the sum of two arrays, each multiplied with the same tile of B. O: of what is written.
+template <typename T, typename O, bool TWICE, int KIND, int BN>
+__global__ void __launch_bounds__(kThreads, 1)
+    product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Product p, int down, int across, int tiles,
+                   PipelineStarve starve) {
+    constexpr bool kAMn = KIND == kWeights, kBMn = KIND == kHidden || KIND == kInput || KIND == kWeights;
+    constexpr int kStages = stages_of(BN, TWICE), kColumns = KIND == kGated ? BN / 2 : BN;  // of the result, a tile
+    constexpr uint32_t kBytesA = bytes_a(TWICE), kStageBytes = kBytesA + bytes_b(BN), kSumColumns = 2 * BN < 32 ? 32 : 2 * BN;
+    extern __shared__ unsigned char memory[];
+    __shared__ __align__(8) uint64_t barriers[2 * kStages + 5];
+    __shared__ uint32_t sums_address;
+    __shared__ volatile int gave_up;
+    const uint32_t base = (shared_address(memory) + 1023) & ~1023u;
+    unsigned char *staging = memory + (base - shared_address(memory)) + kStages * kStageBytes;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t full = shared_address(barriers), empty = full + 8 * kStages, ready = empty + 8 * kStages,
+                   taken = ready + 16, drained = taken + 16;
+    if (threadIdx.x == 0) {
+        gave_up = 0;
+        for (int s = 0; s < kStages; ++s) barrier_init(full + 8 * s, 1), barrier_init(empty + 8 * s, 1);
+        for (int i = 0; i < 2; ++i) barrier_init(ready + 8 * i, 1), barrier_init(taken + 8 * i, kEpilogueWarps);
+        barrier_init(drained, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                         shared_address(&sums_address)),
+                     "r"(kSumColumns)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t sums = sums_address;
+    const int blocks_k = (p.k + kBK - 1) / kBK;
+    // A tile's blocks of K: kInput goes through K twice, kWeights' splits each through a part.
+    auto first_of = [&](const Tile &t) { return KIND == kWeights ? (int)((long long)blocks_k * t.split / p.splits) : 0; };
+    auto last_of = [&](const Tile &t) {
+        return KIND == kWeights ? (int)((long long)blocks_k * (t.split + 1) / p.splits)
+                                : (KIND == kInput ? 2 : 1) * blocks_k;
+    };
+
+    if (warp == 0 && lane == 0) {
+        uint32_t step = 0;  // of all tiles, one after another
+        bool good = true;
+        for (int index = blockIdx.x; index < tiles && good; index += gridDim.x) {
+            const Tile t = tile_of(index, down, across, p.splits);
+            const int last = last_of(t);
+            for (int i = first_of(t); i < last; ++i, ++step) {
+                const uint32_t s = step % kStages, round = step / kStages;
+                if (step >= starve.block || !barrier_wait(empty + 8 * s, (round & 1) ^ 1, starve.polls, &gave_up)) {
+                    good = false;
+                    break;
+                }
+                const uint32_t to = base + s * kStageBytes, barrier = full + 8 * s;
+                barrier_expect(barrier, kStageBytes);
+                const int second = KIND == kInput && i >= blocks_k ? 1 : 0, k = (i - second * blocks_k) * kBK;
+                const CUtensorMap *a = &maps.a[KIND == kWeights ? t.problem : second], *b = &maps.b[KIND == kWeights ? t.problem : second];
+                if constexpr (kAMn) {
+                    for (int j = 0; j < kBM / 64; ++j) tma_load(to + j * 8192, a, t.row * kBM + j * 64, k, barrier);
+                    if constexpr (TWICE)
+                        for (int j = 0; j < kBM / 64; ++j)
+                            tma_load(to + (kBM / 64 + j) * 8192, &maps.low[t.problem], t.row * kBM + j * 64, k, barrier);
+                } else {
+                    tma_load(to, a, k, t.row * kBM, barrier);
+                }
+                if constexpr (kBMn) {
+                    for (int j = 0; j < BN / 64; ++j)
+                        tma_load(to + kBytesA + j * 8192, b, t.column * BN + j * 64, k, barrier);
+                } else if constexpr (KIND == kGated) {
+                    tma_load(to + kBytesA, &maps.b[0], k, t.column * kColumns, barrier);
+                    tma_load(to + kBytesA + bytes_b(kColumns), &maps.b[1], k, t.column * kColumns, barrier);
+                } else {
+                    tma_load(to + kBytesA, b, k, t.column * BN, barrier);
+                }
+            }
+        }
+        if (!good) {
+            // Copies in flight land before the block ends. A stage's last copies were of its last round begun.
+            for (uint32_t n = step < (uint32_t)kStages ? step : kStages; n > 0; --n) {
+                const uint32_t last = step - n;
+                barrier_wait(full + 8 * (last % kStages), (last / kStages) & 1, starve.polls, nullptr);
+            }
+        }
+    } else if (warp == 1 && lane == 0) {
+        constexpr uint32_t kInstruction = instruction<T>(kAMn, kBMn, BN);
+        uint32_t step = 0, round = 0;
+        bool good = true;
+        for (int index = blockIdx.x; index < tiles && good; index += gridDim.x, ++round) {
+            const uint32_t to = round & 1, use = round >> 1;
+            const Tile t = tile_of(index, down, across, p.splits);
+            const int first = first_of(t), last = last_of(t);
+            if (!barrier_wait(taken + 8 * to, (use & 1) ^ 1, starve.polls, &gave_up)) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            for (int i = first; i < last; ++i, ++step) {
+                const uint32_t s = step % kStages;
+                if (!barrier_wait(full + 8 * s, (step / kStages) & 1, starve.polls, &gave_up)) {
+                    good = false;
+                    break;
+                }
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint32_t at = base + s * kStageBytes;
+                const uint64_t a = operand(at, kAMn ? 8192 : 16), b = operand(at + kBytesA, kBMn ? 8192 : 16);
+#pragma unroll
+                for (int k = 0; k < kBK / 16; ++k)  // 16 of K: 32 bytes along a row, or 16 rows of 128 bytes
+                    multiply(sums + to * BN, a + (uint64_t)k * (kAMn ? 128 : 2), b + (uint64_t)k * (kBMn ? 128 : 2),
+                             kInstruction, i > first || k > 0);
+                if constexpr (TWICE) {
+#pragma unroll
+                    for (int k = 0; k < kBK / 16; ++k)
+                        multiply(sums + to * BN, a + (uint64_t)(bytes_a(false) / 16 + k * 128), b + (uint64_t)k * 128,
+                                 kInstruction, true);
+                }
+                commit_to(empty + 8 * s);
+            }
+            if (good) commit_to(ready + 8 * to);
+        }
+        // Matrix instructions in flight end before tensor memory is given back.
+        commit_to(drained);
+        barrier_wait(drained, 0, starve.polls, nullptr);
+    } else if (warp >= 2) {
+        unsigned char *mine = staging + (warp - 2) * kStaging;
+        const int quarter = warp & 3;  // the rows of tensor memory that this warp may read
+        uint32_t round = 0;
+        bool good = true;
+        for (int index = blockIdx.x; index < tiles; index += gridDim.x, ++round) {
+            const Tile t = tile_of(index, down, across, p.splits);
+            const uint32_t from = round & 1, use = round >> 1;
+            if (good) good = barrier_wait(ready + 8 * from, use & 1, starve.polls, &gave_up);
+            good = __all_sync(0xffffffffu, good);
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const uint32_t at = sums + from * BN + ((uint32_t)quarter << 21);
+            const int row0 = t.row * kBM + quarter * 32, row = row0 + lane;
+            // What gave up is NaN from here on.
+            auto take = [&](int c, float (&v)[32]) {
+                if (good) {
+                    take_columns(at + c, v);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) v[j] = __int_as_float(0x7FC00000);
+                }
+            };
+            if (row0 < p.m) {
+#pragma unroll 1
+                for (int c = 0; c < kColumns; c += 32) {
+                    const int col0 = t.column * kColumns + c;
+                    if (col0 >= p.n) break;
+                    float v[32];
+                    take(c, v);
+                    if constexpr (KIND == kGated) {
+                        if (p.out[0].p != nullptr) put_columns<T>(mine, v, p.out[0], row0, col0, p.m, p.n);
+                        float u[32];
+                        take(kColumns + c, u);
+                        if (p.out[1].p != nullptr) put_columns<T>(mine, u, p.out[1], row0, col0, p.m, p.n);
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) v[j] = activation<true>(p.activation, v[j], (float *)nullptr) * u[j];
+                        put_columns<T>(mine, v, p.out[2], row0, col0, p.m, p.n);
+                    } else if constexpr (KIND == kHidden) {
+                        float g[32], u[32];
+                        get_columns<T>(p.saved[0], row, col0, p.m, p.n, g);
+                        get_columns<T>(p.saved[1], row, col0, p.m, p.n, u);
+                        float h[32];
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) {
+                            float slope;
+                            const float f = activation<true>(p.activation, g[j], &slope);
+                            h[j] = f * u[j];
+                            g[j] = v[j] * u[j] * slope;
+                            u[j] = v[j] * f;
+                        }
+                        auto put = [&](float (&x)[32], int n) {
+                            if (p.out[n].p != nullptr) put_columns<T>(mine, x, p.out[n], row0, col0, p.m, p.n);
+                            if (p.out_low[n].p != nullptr) {
+#pragma unroll
+                                for (int j = 0; j < 32; ++j) x[j] = lost_to<T>(x[j]);
+                                put_columns<T>(mine, x, p.out_low[n], row0, col0, p.m, p.n);
+                            }
+                        };
+                        put(g, 0);
+                        put(u, 1);
+                        put(h, 2);
+                    } else {
+                        if constexpr (KIND == kWeights) {
+                            if (p.splits > 1) {
+                                if constexpr (sizeof(O) == 4) {
+                                    const size_t stride = partial_width(p.n), part = t.problem * p.splits + t.split;
+                                    put_columns<O>(mine, v, {(O *)p.partial + part * p.m * stride, stride}, row0, col0,
+                                                   p.m, p.n);
+                                }
+                                continue;
+                            }
+                            if (p.transposed[t.problem]) {
+                                // A column of the tile is a row of the result: lanes are neighbours there.
+#pragma unroll
+                                for (int j = 0; j < 32; ++j)
+                                    if (row < p.m && col0 + j < p.n)
+                                        ((O *)p.out[t.problem].p)[(size_t)(col0 + j) * p.out[t.problem].stride + row] =
+                                            narrow<O>(v[j]);
+                                continue;
+                            }
+                        }
+                        put_columns<O>(mine, v, p.out[KIND == kWeights ? t.problem : 0], row0, col0, p.m, p.n);
+                    }
+                }
+            }
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) barrier_arrive(taken + 8 * from);
+        }
+    }
+    __syncwarp();
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    if (warp == 1)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(sums), "r"(kSumColumns) : "memory");
+}
+
+// ---- launches --------------------------------------------------------------------
+
+PFN_cuTensorMapEncodeTiled_v12000 map_encoder() {
+    static PFN_cuTensorMapEncodeTiled_v12000 fn = []() -> PFN_cuTensorMapEncodeTiled_v12000 {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
+            q != cudaDriverEntryPointSuccess) {
+            (void)cudaGetLastError();
+            return nullptr;
+        }
+        return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+    }();
+    return fn;
+}
+
+// [rows][cols] in boxes of box_rows rows by 64 values (128 bytes, swizzled); zeros outside.
+bool encode(CUtensorMap *map, bool bfloat, const Matrix &x, int rows, int cols, int box_rows) {
+    const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)x.stride * 2};
+    const cuuint32_t box[2] = {64, (cuuint32_t)box_rows};
+    const cuuint32_t each[2] = {1, 1};
+    return map_encoder()(map, bfloat ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
+                         const_cast<void *>(x.p), dims, strides, box, each, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, typename O, bool TWICE, int KIND, int BN>
+cudaError_t launch_tiles(const Product &p, PipelineStarve starve, cudaStream_t stream) {
+    constexpr bool kAMn = KIND == kWeights, kBMn = KIND == kHidden || KIND == kInput || KIND == kWeights;
+    constexpr int kColumns = KIND == kGated ? BN / 2 : BN;
+    constexpr bool kBfloat = std::is_same_v<T, __nv_bfloat16>;
+    constexpr uint32_t kShared = shared_bytes(BN, TWICE);
+    Maps maps = {};
+    const int pairs_a = KIND == kInput ? 2 : p.problems, pairs_b = KIND == kInput || KIND == kGated ? 2 : p.problems;
+    bool good = true;
+    for (int i = 0; i < pairs_a; ++i) {
+        good = good && (kAMn ? encode(&maps.a[i], kBfloat, p.a[i], p.k, p.m, kBK)
+                             : encode(&maps.a[i], kBfloat, p.a[i], p.m, p.k, kBM));
+        if (TWICE) good = good && encode(&maps.low[i], kBfloat, p.low[i], p.k, p.m, kBK);
+    }
+    for (int i = 0; i < pairs_b; ++i)
+        good = good && (kBMn ? encode(&maps.b[i], kBfloat, p.b[i], p.k, p.n, kBK)
+                             : encode(&maps.b[i], kBfloat, p.b[i], p.n, p.k, kColumns));
+    if (!good) return cudaErrorInvalidValue;
+    const int down = (p.m + kBM - 1) / kBM, across = (p.n + kColumns - 1) / kColumns;
+    const long long tiles = (long long)down * across * p.problems * p.splits;
+    if (tiles > INT32_MAX) return cudaErrorInvalidValue;
+    const int most = geo::device_sm_count(), grid = tiles < most ? (int)tiles : most;
+    const auto kernel = product_kernel<T, O, TWICE, KIND, BN>;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kShared);
+    if (e != cudaSuccess) return e;
+    kernel<<<grid, kThreads, kShared, stream>>>(maps, p, down, across, (int)tiles, starve);
+    return cudaGetLastError();
+}
+
+// The widest tile that still gives every multiprocessor about one: wide tiles move
+// fewer bytes a multiplication, narrow ones share few tiles more evenly.
+template <typename T, typename O, bool TWICE, int KIND>
+cudaError_t launch_kind(const Product &p, PipelineStarve starve, cudaStream_t stream) {
+    const long long down = (p.m + kBM - 1) / kBM, sms = geo::device_sm_count();
+    auto waves_cost = [&](int bn) {
+        const int columns = KIND == kGated ? bn / 2 : bn;
+        const long long tiles = down * ((p.n + columns - 1) / columns) * p.problems * p.splits;
+        return (tiles + sms - 1) / sms * (bn + 32);
+    };
+    constexpr int kLeast = KIND == kDown ? 32 : 64;  // a tile of kGated is half as wide, rows of boxes are 64
+    int best = 256;
+    for (int bn = 128; bn >= kLeast; bn /= 2)
+        if (waves_cost(bn) < waves_cost(best)) best = bn;
+    switch (best) {
+        case 256: return launch_tiles<T, O, TWICE, KIND, 256>(p, starve, stream);
+        case 128: return launch_tiles<T, O, TWICE, KIND, 128>(p, starve, stream);
+        case 64: return launch_tiles<T, O, TWICE, KIND, 64>(p, starve, stream);
+        default:
+            if constexpr (kLeast == 32) return launch_tiles<T, O, TWICE, KIND, 32>(p, starve, stream);
+            return cudaErrorInvalidValue;
+    }
+}
+
+template <typename T>
+cudaError_t launch_type(ProductKind kind, uint32_t type, uint32_t out_type, const Product &p, PipelineStarve starve,
+                        cudaStream_t stream) {
+    switch (kind) {
+        case kGated: return launch_kind<T, T, false, kGated>(p, starve, stream);
+        case kDown: return launch_kind<T, T, false, kDown>(p, starve, stream);
+        case kHidden: return launch_kind<T, T, false, kHidden>(p, starve, stream);
+        case kInput: return launch_kind<T, T, false, kInput>(p, starve, stream);
+        default: break;
+    }
+    cudaError_t e;
+    if (out_type == GEO_B200_F32)
+        e = launch_kind<T, float, true, kWeights>(p, starve, stream);
+    else if (p.splits > 1)
+        e = launch_kind<T, float, false, kWeights>(p, starve, stream);
+    else
+        e = launch_kind<T, T, false, kWeights>(p, starve, stream);
+    return e != cudaSuccess || p.splits == 1 ? e : launch_join_splits(type, out_type, p, stream);
+}
+
+}  // namespace
+
+bool tensor_products_available() { return map_encoder() != nullptr; }
+
+int weight_splits_tensor(size_t m, size_t n, size_t k) { return weight_splits(m, n, k, kBM, 128, 8 * kBK); }
+
+cudaError_t launch_product_tensor(ProductKind kind, uint32_t type, uint32_t out_type, const Product &p,
+                                  PipelineStarve starve, cudaStream_t stream) {
+    return type == GEO_B200_BF16 ? launch_type<__nv_bfloat16>(kind, type, out_type, p, starve, stream)
+                                 : launch_type<__half>(kind, type, out_type, p, starve, stream);
+}
+
+}  // namespace layers
+}  // namespace geo

@@ -359,6 +359,7 @@ struct Ring {
     // All but the newest stages - R rows have arrived.
     __device__ __forceinline__ void wait() const {
         switch (stages - R) {
+            case 0: wait_async<0>(); break;
             case 1: wait_async<1>(); break;
             case 2: wait_async<2>(); break;
             case 3: wait_async<3>(); break;
@@ -381,6 +382,17 @@ struct Ring {
                     out[i].w[w] = __funnelshift_r(out[i].w[w], w < 3 ? out[i].w[w + 1] : next, shift);
             }
         }
+    }
+    // Vector i alone.
+    __device__ __forceinline__ Vec<T, V> get_one(int i, int u, int array, const T *row_start) const {
+        const unsigned char *from = slots + (read + u) * next_stage + array * next_array + i * vector_gap();
+        Vec<T, V> out = load<T, V>((const T *)from);
+        if constexpr (SHIFT && sizeof(T) == 2) {
+            const uint32_t shift = 16u * half_word(row_start + at.unit_first), next = *(const uint32_t *)(from + 16);
+#pragma unroll
+            for (int w = 0; w < 4; ++w) out.w[w] = __funnelshift_r(out.w[w], w < 3 ? out.w[w + 1] : next, shift);
+        }
+        return out;
     }
     // The thread's part of a row to global memory; SHIFT: through the place of
     // array `array` of row u, which has been read (every lane of the warp takes part).
@@ -576,6 +588,91 @@ __device__ __forceinline__ void drop_row(const Drop &drop, uint64_t offset, uint
     }
 }
 
+// The end of a VJP's pass: the two column sums of every thread, in the registers of the
+// thread that owns the column, to partial[block or cluster][0, 1][col], the teams of a
+// block added up in `memory` (where the ring was). `alone`: the grid is one cluster,
+// whose blocks add the partial sums up themselves, and no second kernel is needed.
+constexpr int kAloneBlocks = 8;
+template <typename T, int TEAM, int V, int K>
+__device__ __forceinline__ void leave_column_sums(const Place<TEAM, V, K> &at, const Pair<Wide<T>> (&dw)[K * V / 2],
+                                                  const Pair<Wide<T>> (&db)[K * V / 2], Wide<T> *memory,
+                                                  Wide<T> *partial, bool alone, int lanes, int cols, void *dweight,
+                                                  void *dbias, bool float_parameters) {
+    using W = Wide<T>;
+    constexpr int Q = K * V / 2;
+    // The kernel that joins the partial sums may be set up from here on.
+    if (!alone) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    auto value = [&](const Pair<W> (&p)[Q], int e) { return e & 1 ? p[e / 2].y : p[e / 2].x; };
+    // Every thread's sums to where the ring was (two rows of it hold two sums of a
+    // row; value e of thread t at e threads + (t ^ e): no bank twice), then a
+    // column's, the block's teams in order, in whole lines to global memory.
+    const int each = blockDim.x, first_column = at.rank * lanes * K * V;
+    const int columns = cols - first_column < lanes * K * V ? cols - first_column : lanes * K * V;
+    W *found = memory, *mine = partial + at.slice * 2 * cols + first_column;
+    auto place = [&](int e, int thread) { return e * each + (thread ^ (e & 31)); };
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < K * V; ++e) {
+        found[place(e, threadIdx.x)] = value(dw, e);
+        found[each * K * V + place(e, threadIdx.x)] = value(db, e);
+    }
+    __syncthreads();
+    const int kinds = dbias != nullptr ? 2 : 1;
+    for (int which = 0; which < kinds; ++which)
+        for (int c = threadIdx.x; c < columns; c += each) {
+            const int vector = c / V, unit = TEAM == kWarp ? 0 : vector / (32 * K), in_unit = vector - unit * 32 * K;
+            const int round = TEAM == kWarp ? in_unit / at.unit_lanes : in_unit / 32;
+            const int e = round * V + c % V, lane = unit * 32 + in_unit - round * at.unit_lanes;
+            W sum = 0;
+            for (int team = 0; team < at.teams; ++team)
+                sum += found[which * each * K * V + place(e, team * lanes + lane)];
+            mine[(size_t)which * cols + c] = sum;
+        }
+    if constexpr (TEAM != kCluster) {
+        if (!alone) return;
+        cooperative_groups::this_cluster().sync();  // makes the blocks' sums visible to one another
+        for (int n = blockIdx.x * each + threadIdx.x; n < kinds * cols; n += gridDim.x * each) {
+            W sum = 0;
+#pragma unroll
+            for (int block = 0; block < kAloneBlocks; ++block)
+                if (block < (int)gridDim.x) sum += partial[(size_t)block * 2 * cols + n];
+            const int c = n < cols ? n : n - cols;
+            void *out = n < cols ? dweight : dbias;
+            if (out == nullptr) continue;
+            if (sizeof(T) == 2 && float_parameters)
+                ((float *)out)[c] = (float)sum;
+            else
+                ((T *)out)[c] = narrow<T>(sum);
+        }
+    }
+}
+
+// out[c] = sum over the blocks of partial[block][which][c]: 32 columns a block of
+// threads, so that whole 128-byte lines are read, blockDim / 32 threads a column, each
+// over every so many blocks in order, then those as a tree. (With 16 columns 16384 x
+// 4096 bfloat16 takes as long, 74.0 and 74.5 us.)
+constexpr int kJoinColumns = 32;
+template <typename W, typename P>
+__global__ void __launch_bounds__(1024) join_columns_kernel(const W *partial, int blocks, int cols, void *dweight,
+                                                            void *dbias) {
+    __shared__ W sums[1024];
+    P *out = (P *)(blockIdx.y == 0 ? dweight : dbias);
+    const int column = threadIdx.x % kJoinColumns, part = threadIdx.x / kJoinColumns, parts = blockDim.x / kJoinColumns;
+    const int c = (int)blockIdx.x * kJoinColumns + column;
+    W sum = 0;
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // for the kernel before to end
+    if (c < cols) {
+#pragma unroll 8
+        for (int i = part; i < blocks; i += parts) sum += partial[((size_t)i * 2 + blockIdx.y) * cols + c];
+    }
+    sums[threadIdx.x] = sum;
+    for (int n = parts / 2; n > 0; n /= 2) {
+        __syncthreads();
+        if (part < n) sums[threadIdx.x] += sums[threadIdx.x + n * kJoinColumns];
+    }
+    if (part == 0 && c < cols && out != nullptr) out[c] = narrow<P>((Wide<P>)sums[threadIdx.x]);
+}
+
 // f(TEAM, SHIFT, FULL) of a shape as compile-time constants, as far as they occur.
 template <typename F>
 cudaError_t by_shape(const Shape &s, F &&f) {
@@ -637,6 +734,28 @@ cudaError_t launch_team(void (*kernel)(A...), const Shape &s, size_t &grid, size
         config.gridDim.x = (unsigned)(grid * s.blocks);
     }
     return cudaLaunchKernelEx(&config, kernel, args...);
+}
+
+// Launched while the pass still runs: its start-up is over when the sums are there.
+// About eight partial sums a thread, more where 1024 threads a multiprocessor do not reach: with 32 threads a
+// column always 8192 x 5120 bfloat16 60.0 us, so 57.1; 300 x 4096 10.8, so 9.9; with 8 always 8192 x 2048 27.4,
+// so 26.0.
+template <typename W, typename P>
+cudaError_t launch_join(const W *partial, size_t blocks, int cols, void *dweight, void *dbias, int sms,
+                        cudaStream_t stream) {
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3((unsigned)((cols + kJoinColumns - 1) / kJoinColumns), dbias != nullptr ? 2 : 1);
+    const size_t columns = (size_t)config.gridDim.x * config.gridDim.y * kJoinColumns, threads = (size_t)sms * 1024;
+    int parts = 8;
+    while (parts < 1024 / kJoinColumns && (size_t)parts * 8 < blocks && columns * parts * 2 <= threads) parts *= 2;
+    config.blockDim = dim3((unsigned)(kJoinColumns * parts));
+    config.stream = stream;
+    cudaLaunchAttribute attribute = {};
+    attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attribute.val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = &attribute;
+    config.numAttrs = 1;
+    return cudaLaunchKernelEx(&config, join_columns_kernel<W, P>, partial, (int)blocks, cols, dweight, dbias);
 }
 
 #endif

@@ -27,7 +27,6 @@ namespace {
 // the end partial[block or cluster][0: weight, 1: bias][col], the teams of a
 // block added up in shared memory. `alone`: the grid is one cluster, whose blocks
 // add the partial sums up themselves, and no second kernel is needed.
-constexpr int kAloneBlocks = 8;
 template <typename T, bool DROP, int TEAM, bool SHIFT, bool FULL, bool STARVE = false>
 __global__ void __launch_bounds__(TEAM == kWarp ? kWarpBlock : kTeamThreads, TEAM == kWarp ? 4 : 2)
     vjp_kernel(const BackwardArgs a, int lanes, bool float_parameters, int stages, Wide<T> *partial, bool alone) {
@@ -180,76 +179,8 @@ __global__ void __launch_bounds__(TEAM == kWarp ? kWarpBlock : kTeamThreads, TEA
 #pragma unroll
         for (int q = 0; q < Q; ++q) dw[q] = db[q] = both((W)NAN);
     }
-    // The kernel that joins the partial sums may be set up from here on.
-    if (!alone) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    auto value = [&](const Pair<W> (&p)[Q], int e) { return e & 1 ? p[e / 2].y : p[e / 2].x; };
-    // Every thread's sums to where the ring was (two rows of it hold two sums of a
-    // row; value e of thread t at e threads + (t ^ e): no bank twice), then a
-    // column's, the block's teams in order, in whole lines to global memory.
-    const int each = blockDim.x, first_column = at.rank * lanes * K * V;
-    const int columns = a.cols - first_column < lanes * K * V ? a.cols - first_column : lanes * K * V;
-    W *found = (W *)memory, *mine = partial + at.slice * 2 * a.cols + first_column;
-    auto place = [&](int e, int thread) { return e * each + (thread ^ (e & 31)); };
-    __syncthreads();
-#pragma unroll
-    for (int e = 0; e < K * V; ++e) {
-        found[place(e, threadIdx.x)] = value(dw, e);
-        found[each * K * V + place(e, threadIdx.x)] = value(db, e);
-    }
-    __syncthreads();
-    for (int which = 0; which < 2; ++which)
-        for (int c = threadIdx.x; c < columns; c += each) {
-            const int vector = c / V, unit = TEAM == kWarp ? 0 : vector / (32 * K), in_unit = vector - unit * 32 * K;
-            const int round = TEAM == kWarp ? in_unit / at.unit_lanes : in_unit / 32;
-            const int e = round * V + c % V, lane = unit * 32 + in_unit - round * at.unit_lanes;
-            W sum = 0;
-            for (int team = 0; team < at.teams; ++team)
-                sum += found[which * each * K * V + place(e, team * lanes + lane)];
-            mine[(size_t)which * a.cols + c] = sum;
-        }
-    if constexpr (TEAM != kCluster) {
-        if (!alone) return;
-        cooperative_groups::this_cluster().sync();  // makes the blocks' sums visible to one another
-        for (int n = blockIdx.x * each + threadIdx.x; n < 2 * a.cols; n += gridDim.x * each) {
-            W sum = 0;
-#pragma unroll
-            for (int block = 0; block < kAloneBlocks; ++block)
-                if (block < (int)gridDim.x) sum += partial[(size_t)block * 2 * a.cols + n];
-            const int c = n < a.cols ? n : n - a.cols;
-            void *out = n < a.cols ? a.dweight : a.dbias;
-            if (out == nullptr) continue;
-            if (sizeof(T) == 2 && float_parameters)
-                ((float *)out)[c] = (float)sum;
-            else
-                ((T *)out)[c] = narrow<T>(sum);
-        }
-    }
-}
-
-// out[c] = sum over the blocks of partial[block][which][c]: 32 columns a block of
-// threads, so that whole 128-byte lines are read, blockDim / 32 threads a column, each
-// over every so many blocks in order, then those as a tree. (With 16 columns 16384 x
-// 4096 bfloat16 takes as long, 74.0 and 74.5 us.)
-constexpr int kJoinColumns = 32;
-template <typename W, typename P>
-__global__ void __launch_bounds__(1024) join_columns_kernel(const W *partial, int blocks, int cols, void *dweight,
-                                                            void *dbias) {
-    __shared__ W sums[1024];
-    P *out = (P *)(blockIdx.y == 0 ? dweight : dbias);
-    const int column = threadIdx.x % kJoinColumns, part = threadIdx.x / kJoinColumns, parts = blockDim.x / kJoinColumns;
-    const int c = (int)blockIdx.x * kJoinColumns + column;
-    W sum = 0;
-    asm volatile("griddepcontrol.wait;" ::: "memory");  // for the kernel before to end
-    if (c < cols) {
-#pragma unroll 8
-        for (int i = part; i < blocks; i += parts) sum += partial[((size_t)i * 2 + blockIdx.y) * cols + c];
-    }
-    sums[threadIdx.x] = sum;
-    for (int n = parts / 2; n > 0; n /= 2) {
-        __syncthreads();
-        if (part < n) sums[threadIdx.x] += sums[threadIdx.x + n * kJoinColumns];
-    }
-    if (part == 0 && c < cols && out != nullptr) out[c] = narrow<P>((Wide<P>)sums[threadIdx.x]);
+    leave_column_sums<T, TEAM, V, K>(at, dw, db, (W *)memory, partial, alone, lanes, a.cols, a.dweight, a.dbias,
+                                     float_parameters);
 }
 
 // ---- rows of any length --------------------------------------------------------
@@ -349,27 +280,6 @@ cudaError_t launch_shape(const Shape &s, const BackwardArgs &a, bool float_param
                        stages * stage, stream, a, s.lanes, float_parameters, stages, partial, alone);
 }
 
-// Launched while the pass still runs: its start-up is over when the sums are there.
-// About eight partial sums a thread, more where 1024 threads a multiprocessor do not reach: with 32 threads a
-// column always 8192 x 5120 bfloat16 60.0 us, so 57.1; 300 x 4096 10.8, so 9.9; with 8 always 8192 x 2048 27.4,
-// so 26.0.
-template <typename W, typename P>
-cudaError_t launch_join(const BackwardArgs &a, const W *partial, size_t blocks, cudaStream_t stream) {
-    cudaLaunchConfig_t config = {};
-    config.gridDim = dim3((unsigned)((a.cols + kJoinColumns - 1) / kJoinColumns), 2);
-    const size_t columns = (size_t)config.gridDim.x * 2 * kJoinColumns, threads = (size_t)geo::device_sm_count() * 1024;
-    int parts = 8;
-    while (parts < 1024 / kJoinColumns && (size_t)parts * 8 < blocks && columns * parts * 2 <= threads) parts *= 2;
-    config.blockDim = dim3((unsigned)(kJoinColumns * parts));
-    config.stream = stream;
-    cudaLaunchAttribute attribute = {};
-    attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attribute.val.programmaticStreamSerializationAllowed = 1;
-    config.attrs = &attribute;
-    config.numAttrs = 1;
-    return cudaLaunchKernelEx(&config, join_columns_kernel<W, P>, partial, (int)blocks, a.cols, a.dweight, a.dbias);
-}
-
 template <bool DROP>
 cudaError_t launch(NormTypes n, const BackwardArgs &a, void *workspace, cudaStream_t stream) {
     const bool sums = a.dweight != nullptr || a.dbias != nullptr;
@@ -410,7 +320,7 @@ cudaError_t launch(NormTypes n, const BackwardArgs &a, void *workspace, cudaStre
             e = cudaGetLastError();
         }
         if (e != cudaSuccess || !sums || alone) return e;
-        return launch_join<W, P>(a, partial, blocks, stream);
+        return launch_join<W, P>(partial, blocks, a.cols, a.dweight, a.dbias, geo::device_sm_count(), stream);
     });
 }
 
@@ -438,7 +348,8 @@ cudaError_t launch_norm_vjp_starved(const BackwardArgs &a, void *partial, cudaSt
     size_t blocks = team_grid(s, 4, a.rows);
     const cudaError_t e = launch_shape<float, false, kCluster, false, true, true>(s, a, true, (float *)partial, false,
                                                                                  blocks, stream);
-    return e != cudaSuccess ? e : launch_join<float, float>(a, (float *)partial, blocks, stream);
+    return e != cudaSuccess ? e : launch_join<float, float>((float *)partial, blocks, a.cols, a.dweight, a.dbias,
+                                                             geo::device_sm_count(), stream);
 }
 
 }  // namespace layers

@@ -180,6 +180,25 @@ __device__ __forceinline__ void store(T *p, const Vec<T, V> &v) {
 }
 #endif
 
+#ifdef __CUDACC__
+// s = 1 / (1 + e^-a) and rest = 1 - s, each to its own relative accuracy: both from
+// e^-|a|. FAST: float32's fast exponential and division (a few 2^-22 relative for
+// |a| of a few units, |a| 2^-23 beyond), for results that are rounded to 16 bits.
+template <bool FAST, typename W>
+__device__ __forceinline__ void logistic(W a, W &s, W &rest) {
+    W e, d;
+    if constexpr (FAST && sizeof(W) == 4) {
+        e = __expf(-fabsf(a));
+        d = __fdividef(1.0f, 1.0f + e);
+    } else {
+        e = exp(-fabs(a));
+        d = W(1) / (W(1) + e);
+    }
+    s = a < W(0) ? e * d : d;
+    rest = a < W(0) ? d : e * d;
+}
+#endif
+
 inline size_t type_bytes(uint32_t type) {
     switch (type) {
         case GEO_B200_F64: return 8;

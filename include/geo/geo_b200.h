@@ -571,6 +571,166 @@ geo_b200_status_t geo_b200_rotary_vjp(const geo_b200_rotary_plan_t *plan, const 
                                       const void *device_y_cotangent, const void *device_positions,
                                       void *device_x_cotangent, cudaStream_t stream);
 
+/* RMS norm over each row: rstd = 1 / sqrt(mean(x^2) + epsilon), y = x rstd weight.
+ * No mean is taken off: where the rotors of an algebra leave the sum of squares of a
+ * multivector's coefficients alone (every Cl(n,0)) and the weight is the same for all
+ * of them, this norm commutes with rotors. config as for layer norm, weight and rstd
+ * likewise (either may be NULL). */
+geo_b200_status_t geo_b200_rms_norm(const geo_b200_layer_norm_config_t *config, const void *device_x,
+                                    const void *device_weight, void *device_y, void *device_rstd,
+                                    cudaStream_t stream);
+/* Bytes of device workspace of its VJP on the current device; 0 for a config that the VJP would refuse. */
+size_t geo_b200_rms_norm_vjp_workspace(const geo_b200_layer_norm_config_t *config);
+/* VJP: with xh = x rstd, g = y_bar weight (means over the row),
+ *   x_bar = rstd (g - xh mean(g xh)),  weight_bar = sum over the rows of y_bar xh.
+ * Either output may be NULL, not both. The workspace (16-byte aligned; for weight_bar
+ * alone) as for layer norm. */
+geo_b200_status_t geo_b200_rms_norm_vjp(const geo_b200_layer_norm_config_t *config, const void *device_x,
+                                        const void *device_weight, const void *device_rstd,
+                                        const void *device_y_cotangent, void *device_x_cotangent,
+                                        void *device_weight_cotangent, void *device_workspace, size_t workspace_bytes,
+                                        cudaStream_t stream);
+
+/* Between two blocks of a model: the norm after the block that gave x, its gate, the
+ * residual stream, and the norm before the next block, in one pass:
+ *   z = residual_scale residual + block_scale act(gate) rms_norm(x; post_weight),
+ *   y = rms_norm(z; pre_weight),
+ * act by config->gate: 1 (NONE, no gate array), the gate itself, its sigmoid or its
+ * tanh. The statistics of z and y are taken from z before it is rounded to its type. */
+typedef enum {
+    GEO_B200_GATE_NONE = 0,
+    GEO_B200_GATE_LINEAR = 1,
+    GEO_B200_GATE_SIGMOID = 2,
+    GEO_B200_GATE_TANH = 3
+} geo_b200_gate_t;
+
+typedef struct {
+    uint32_t type;              /* geo_b200_type_t of all rows */
+    uint32_t parameter_type;    /* of the weights and their cotangents: `type`, or F32 for the 16-bit types */
+    uint32_t gate;              /* geo_b200_gate_t */
+    uint32_t reserved;          /* 0 */
+    size_t rows, cols;          /* 1 .. GEO_B200_LAYER_MAX_ROWS, 1 .. GEO_B200_LAYER_MAX_COLS */
+    size_t x_stride, residual_stride, gate_stride, z_stride, y_stride;
+    size_t y_cotangent_stride, z_cotangent_stride;
+    size_t residual_cotangent_stride, x_cotangent_stride, gate_cotangent_stride;
+    double epsilon;             /* finite, >= 0; of both norms */
+    double residual_scale, block_scale;  /* finite */
+} geo_b200_block_norm_config_t;
+
+/* device_gate: NULL for NONE, else [rows][cols]. Weights may be NULL (1). rstd of x
+ * and of z (what the VJP needs) may be NULL. */
+geo_b200_status_t geo_b200_block_norm(const geo_b200_block_norm_config_t *config, const void *device_x,
+                                      const void *device_residual, const void *device_gate,
+                                      const void *device_post_weight, const void *device_pre_weight, void *device_z,
+                                      void *device_y, void *device_x_rstd, void *device_z_rstd, cudaStream_t stream);
+/* Bytes of device workspace of its VJP on the current device; 0 for a config that the VJP would refuse. */
+size_t geo_b200_block_norm_vjp_workspace(const geo_b200_block_norm_config_t *config);
+/* VJP from y_bar and, where z is used further on, its own cotangent z_bar (may be NULL):
+ *   dz = rms_norm_vjp(z; y_bar) + z_bar,  residual_bar = residual_scale dz,
+ *   n = x x_rstd post_weight,  gate_bar = block_scale act'(gate) n dz,
+ *   x_bar = rms_norm_vjp(x; block_scale act(gate) dz), and the weights' cotangents.
+ * Any output may be NULL, not all; gate_bar is NULL without a gate. Workspace (16-byte
+ * aligned; for the weights' cotangents alone) as for layer norm. */
+geo_b200_status_t geo_b200_block_norm_vjp(
+    const geo_b200_block_norm_config_t *config, const void *device_x, const void *device_gate, const void *device_z,
+    const void *device_post_weight, const void *device_pre_weight, const void *device_x_rstd,
+    const void *device_z_rstd, const void *device_y_cotangent, const void *device_z_cotangent,
+    void *device_residual_cotangent, void *device_x_cotangent, void *device_gate_cotangent,
+    void *device_post_weight_cotangent, void *device_pre_weight_cotangent, void *device_workspace,
+    size_t workspace_bytes, cudaStream_t stream);
+
+/* Gated feed-forward block of rows of cols values through hidden values:
+ *   gate = x gate_weight^T,  up = x up_weight^T,  h = act(gate) up,  y = h down_weight^T,
+ * gate_weight and up_weight [hidden][cols], down_weight [cols][hidden].
+ * act(a): a sigmoid(a) (SILU), a Phi(a) with the normal distribution function (GELU),
+ * sigmoid(a), or max(a, 0) (RELU, whose derivative at 0 is 0). The 16-bit types are
+ * multiplied exactly and summed in float32; h, and the VJP's cotangents of gate and
+ * up, are rounded to `type` on their way to the next product, but to the sum of two
+ * values of it on their way to float32 cotangents of weights, which costs that product
+ * twice. An infinity may come out as NaN. */
+typedef enum {
+    GEO_B200_ACTIVATION_SILU = 1,
+    GEO_B200_ACTIVATION_GELU = 2,
+    GEO_B200_ACTIVATION_SIGMOID = 3,
+    GEO_B200_ACTIVATION_RELU = 4
+} geo_b200_activation_t;
+
+#define GEO_B200_FEED_FORWARD_MAX_WIDTH 1048576u    /* 2^20 values: cols, hidden */
+#define GEO_B200_FEED_FORWARD_MAX_ROWS 16777216u    /* 2^24 */
+
+typedef struct {
+    uint32_t type;              /* geo_b200_type_t of all arrays but the weights' cotangents */
+    uint32_t gradient_type;     /* of the weights' cotangents: `type`, or F32 for the 16-bit types */
+    uint32_t activation;        /* geo_b200_activation_t */
+    uint32_t reserved;          /* 0 */
+    size_t rows, cols, hidden;
+    size_t x_stride, y_stride, y_cotangent_stride, x_cotangent_stride;
+    size_t gate_weight_stride, up_weight_stride, down_weight_stride;  /* of the weights and of their cotangents */
+    size_t gate_stride, up_stride;
+} geo_b200_feed_forward_config_t;
+
+/* Bytes of device workspace of the forward and of the VJP on the current device; 0
+ * for a config that the call would refuse. Where the type has 16 bits, rows that do
+ * not start on 16 bytes (by their stride) are copied there first. Arrays that do not
+ * start on 16 bytes although their rows would allow it are taken as well, and are
+ * slow. Calls that may overlap on the GPU, captured graphs among them, need a
+ * workspace each. */
+size_t geo_b200_feed_forward_workspace(const geo_b200_feed_forward_config_t *config);
+size_t geo_b200_feed_forward_vjp_workspace(const geo_b200_feed_forward_config_t *config);
+
+/* device_gate and device_up (before the activation; what the VJP needs): both NULL, or
+ * both [rows][hidden] outputs. workspace: 256-byte aligned. No output may overlap an input. */
+geo_b200_status_t geo_b200_feed_forward(const geo_b200_feed_forward_config_t *config, const void *device_x,
+                                        const void *device_gate_weight, const void *device_up_weight,
+                                        const void *device_down_weight, void *device_gate, void *device_up,
+                                        void *device_y, void *device_workspace, size_t workspace_bytes,
+                                        cudaStream_t stream);
+/* VJP: with h_bar = y_bar down_weight, gate_bar = h_bar up act'(gate), up_bar = h_bar act(gate),
+ *   x_bar = gate_bar gate_weight + up_bar up_weight,
+ *   gate_weight_bar = gate_bar^T x,  up_weight_bar = up_bar^T x,  down_weight_bar = y_bar^T h.
+ * Any output may be NULL, not all (what no output needs may be NULL too: x without
+ * gate_weight_bar and up_weight_bar); outputs are overwritten. */
+geo_b200_status_t geo_b200_feed_forward_vjp(const geo_b200_feed_forward_config_t *config, const void *device_x,
+                                            const void *device_gate_weight, const void *device_up_weight,
+                                            const void *device_down_weight, const void *device_gate,
+                                            const void *device_up, const void *device_y_cotangent,
+                                            void *device_x_cotangent, void *device_gate_weight_cotangent,
+                                            void *device_up_weight_cotangent, void *device_down_weight_cotangent,
+                                            void *device_workspace, size_t workspace_bytes, cudaStream_t stream);
+
+/* ---- 6. gradients of a training step ------------------------------------ */
+
+/* Norm over all gradients of a model, and clipping before the update:
+ *   norm = sqrt(sum of squares of every value of every gradient),
+ *   scale = min(1, max_norm / norm)  (1 for a norm of 0),  clipped = scale gradient,
+ * each value rounded once to its type. Squares are summed in float64, in a fixed order:
+ * the same call gives the same bits. A norm that is infinite or NaN (a gradient is) makes
+ * scale NaN; the clipped values are then scale times gradient, NaN as well: the
+ * update must not be made. Asynchronous and allocating nothing as section 5. */
+typedef struct {
+    uint32_t type;              /* geo_b200_type_t */
+    uint32_t reserved;          /* 0 */
+    size_t count;               /* 0 .. 2^40 adjacent values */
+    const void *gradient;       /* device memory; may be NULL for count 0 */
+    void *clipped;              /* NULL: this one is not written; the gradient itself; or another array */
+} geo_b200_gradient_t;
+
+#define GEO_B200_GRADIENT_MAX_TENSORS 65536u
+
+/* Bytes of device workspace of the call below on the current device; 0 for gradients
+ * that it would refuse by their types or counts. */
+size_t geo_b200_gradient_clip_workspace(const geo_b200_gradient_t *gradients, size_t count);
+
+/* gradients: a host array of 1 .. GEO_B200_GRADIENT_MAX_TENSORS entries, read before
+ * the call returns (a captured graph keeps what it held). An array that is written must
+ * not overlap any other of the call, its own gradient apart; the same gradient may be
+ * listed twice where it is only read, and counts twice. max_norm: > 0, infinite for no
+ * bound. device_norm and device_scale (a float64 each) may be NULL. workspace: 16-byte
+ * aligned. Calls that may overlap on the GPU, captured graphs among them, need one each. */
+geo_b200_status_t geo_b200_gradient_clip(const geo_b200_gradient_t *gradients, size_t count, double max_norm,
+                                         double *device_norm, double *device_scale, void *device_workspace,
+                                         size_t workspace_bytes, cudaStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
