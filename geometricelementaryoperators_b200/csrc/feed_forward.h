@@ -76,11 +76,10 @@ bool tensor_products_available();
 
 #ifdef __CUDACC__
 // What v loses to its rounding to T, itself to be rounded to T: together they hold
-// twice T's digits. Nothing where T has no finite value for v.
+// twice T's digits. (What T has no finite value for loses an infinity or NaN.)
 template <typename T>
 __device__ __forceinline__ float lost_to(float v) {
-    const float left = v - widen(narrow<T>(v));
-    return fabsf(left) < INFINITY ? left : 0.0f;
+    return v - widen(narrow<T>(v));
 }
 
 // ---- the activation ------------------------------------------------------------
@@ -109,6 +108,18 @@ __device__ __forceinline__ W activation(int kind, W a, W *slope) {
             if (slope != nullptr) *slope = s * (W(1) + a * rest);
             return a * s;
         }
+    }
+}
+// f(kind as a compile-time constant): chosen once for many values, whose functions can
+// then be worked out side by side.
+template <typename F>
+__device__ __forceinline__ void by_activation(int kind, F &&f) {
+    using std::integral_constant;
+    switch (kind) {
+        case GEO_B200_ACTIVATION_SILU: f(integral_constant<int, GEO_B200_ACTIVATION_SILU>{}); break;
+        case GEO_B200_ACTIVATION_GELU: f(integral_constant<int, GEO_B200_ACTIVATION_GELU>{}); break;
+        case GEO_B200_ACTIVATION_SIGMOID: f(integral_constant<int, GEO_B200_ACTIVATION_SIGMOID>{}); break;
+        default: f(integral_constant<int, GEO_B200_ACTIVATION_RELU>{}); break;
     }
 }
 #endif

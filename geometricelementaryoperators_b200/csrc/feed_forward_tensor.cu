@@ -9,10 +9,10 @@
 //            128 x BN x 16) and commits them to the stage's `empty` mbarrier, a
 //            tile's last to `ready`; the float32 sums stand in tensor memory, two
 //            tiles of BN columns in turn;
-//   warps 2-5 take a finished tile out of tensor memory (32 rows a warp), do what
-//            belongs to the product (activation, its derivative), round once and
-//            write it through shared memory in whole 64-byte pieces, while the next
-//            tile is multiplied.
+//   warps 2-5 (2-9 where there is more to do) take a finished tile out of tensor
+//            memory (32 rows a warp), do what belongs to the product (activation, its
+//            derivative), round once and write it through shared memory in whole
+//            64-byte pieces, while the next tile is multiplied.
 // Operands whose sum index is not the adjacent one (weights in the VJP, both sides
 // of the weights' cotangents) are copied as they lie, [64 of K][64 values] boxes,
 // and read by the matrix instruction as "MN-major": nothing is transposed.
@@ -30,19 +30,27 @@ namespace layers {
 
 namespace {
 
-constexpr int kBM = 128, kBK = 64, kThreads = 192, kEpilogueWarps = 4;
+constexpr int kBM = 128, kBK = 64;
+// Warps that take the sums out. The VJP's first product reads two more arrays and
+// writes up to six; float32 results of two-term operands are summed up in registers.
+constexpr int epilogue_warps(int kind, bool twice) { return kind == kHidden || twice ? 8 : 4; }
+// Blocks of K that are summed in tensor memory in one go, where the result is float32:
+// the tensor cores cut where float32 arithmetic rounds, which takes 1.8e-5 off the
+// size of sums over 8192 rows. The parts are added up in registers, rounded to nearest.
+constexpr int kChunk = 16;
 constexpr uint32_t bytes_a(bool twice) { return (twice ? 2 : 1) * kBM * kBK * 2; }
 constexpr uint32_t bytes_b(int bn) { return (uint32_t)bn * kBK * 2; }
-constexpr uint32_t kStagingPitch = 144;  // bytes of a row of 32 values of up to 4 bytes; 16 more keep banks apart
-constexpr uint32_t kStaging = 32 * kStagingPitch;
+constexpr uint32_t kRows = 32 * 80;  // a warp's 32 rows of 64 bytes; 16 more keep banks apart
+constexpr uint32_t staging_of(int kind) { return kind == kHidden ? 3 * kRows : kRows; }  // of a warp
 constexpr uint32_t kSharedMost = 227 * 1024;
-constexpr int stages_of(int bn, bool twice) {
-    const int n = (int)((kSharedMost - 1024 - kEpilogueWarps * kStaging - 512) / (bytes_a(twice) + bytes_b(bn)));
+constexpr int stages_of(int kind, int bn, bool twice) {
+    const int n = (int)((kSharedMost - 1024 - epilogue_warps(kind, twice) * staging_of(kind) - 512) / (bytes_a(twice) + bytes_b(bn)));
     return n > 8 ? 8 : n;
 }
-constexpr uint32_t shared_bytes(int bn, bool twice) {
-    return 1024 + stages_of(bn, twice) * (bytes_a(twice) + bytes_b(bn)) + kEpilogueWarps * kStaging;
+constexpr uint32_t shared_bytes(int kind, int bn, bool twice) {
+    return 1024 + stages_of(kind, bn, twice) * (bytes_a(twice) + bytes_b(bn)) + epilogue_warps(kind, twice) * staging_of(kind);
 }
+
 struct Maps {
     CUtensorMap a[3], b[3], low[3];
 };
@@ -131,63 +139,99 @@ __device__ __forceinline__ bool by_16(const void *p, size_t stride) {
     return ((uintptr_t)p % 16 | stride * sizeof(T) % 16) == 0;
 }
 
-// Writes this thread's 32 columns of its row (rows row0 + lane, columns col0 ...) of
-// an m x n array, through the warp's staging.
+// Writes 64 bytes of this thread's row (rows row0 + lane, columns col0 ...) of an m x n
+// array, through the warp's staging.
 template <typename O>
-__device__ __forceinline__ void put_columns(unsigned char *staging, const float (&v)[32], const OutMatrix &out, int row0,
-                                            int col0, int m, int n) {
-    constexpr int kVector = 16 / (int)sizeof(O), kPitch = 32 * (int)sizeof(O) + 16;
+__device__ __forceinline__ void put_words(unsigned char *staging, const uint32_t (&words)[16], const OutMatrix &out,
+                                          int row0, int col0, int m, int n) {
+    constexpr int kVector = 16 / (int)sizeof(O), kWidth = 64 / (int)sizeof(O), kPitch = 80;
     const int lane = threadIdx.x & 31;
 #pragma unroll
-    for (int j = 0; j < 32 / kVector; ++j) {
-        Vec<O, kVector> piece;
-#pragma unroll
-        for (int q = 0; q < kVector / 2; ++q) piece.set(q, {v[j * kVector + 2 * q], v[j * kVector + 2 * q + 1]});
-        store<O, kVector>((O *)(staging + lane * kPitch) + j * kVector, piece);
-    }
+    for (int j = 0; j < 4; ++j)
+        *(uint4 *)(staging + lane * kPitch + 16 * j) =
+            make_uint4(words[4 * j], words[4 * j + 1], words[4 * j + 2], words[4 * j + 3]);
     __syncwarp();
     if (by_16<O>(out.p, out.stride)) {
-        constexpr int kPieces = 32 / kVector, kRows = 32 / kPieces;
-        const int piece = lane % kPieces, c = col0 + piece * kVector;
+        const int c = col0 + lane % 4 * kVector;
 #pragma unroll
-        for (int r0 = 0; r0 < 32; r0 += kRows) {
-            const int r = r0 + lane / kPieces;
+        for (int r0 = 0; r0 < 32; r0 += 8) {
+            const int r = r0 + lane / 4;
             if (row0 + r >= m || c >= n) continue;
-            const O *from = (const O *)(staging + r * kPitch) + piece * kVector;
+            const O *piece = (const O *)(staging + r * kPitch) + lane % 4 * kVector;
             O *to = (O *)out.p + (size_t)(row0 + r) * out.stride + c;
             if (c + kVector <= n) {
-                store<O, kVector>(to, load<O, kVector>(from));
+                store<O, kVector>(to, load<O, kVector>(piece));
             } else {
-                for (int j = 0; c + j < n; ++j) to[j] = from[j];
+                for (int j = 0; c + j < n; ++j) to[j] = piece[j];
             }
         }
     } else {
-        for (int r = 0; r < 32 && row0 + r < m; ++r)
-            if (col0 + lane < n)
-                ((O *)out.p)[(size_t)(row0 + r) * out.stride + col0 + lane] = ((const O *)(staging + r * kPitch))[lane];
+        for (int r = lane / kWidth; r < 32 && row0 + r < m; r += 32 / kWidth)
+            if (col0 + lane % kWidth < n)
+                ((O *)out.p)[(size_t)(row0 + r) * out.stride + col0 + lane % kWidth] =
+                    ((const O *)(staging + r * kPitch))[lane % kWidth];
     }
     __syncwarp();
 }
-
-// 32 columns of a row of an m x n array; zeros outside.
+// Two neighbours as a word of 16-bit values.
 template <typename T>
-__device__ __forceinline__ void get_columns(const Matrix &in, int row, int col0, int m, int n, float (&v)[32]) {
-    if (row < m && col0 + 32 <= n && by_16<T>(in.p, in.stride)) {
-        const T *from = (const T *)in.p + (size_t)row * in.stride + col0;
+__device__ __forceinline__ uint32_t word_of(float x, float y) {
+    Vec<T, 2> v;
+    v.set(0, {x, y});
+    return v.w[0];
+}
+// 32 columns, v[from ...].
+template <typename O, int COUNT>
+__device__ __forceinline__ void put_columns(unsigned char *staging, const float (&v)[COUNT], int from,
+                                            const OutMatrix &out, int row0, int col0, int m, int n) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const Vec<T, 8> piece = load<T, 8>(from + 8 * j);
+    for (int part = 0; part < (int)sizeof(O) / 2; ++part) {
+        if (part > 0 && col0 + 16 >= n) break;
+        uint32_t words[16];
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const Pair<float> p = piece.pair(q);
-                v[8 * j + 2 * q] = p.x;
-                v[8 * j + 2 * q + 1] = p.y;
-            }
+        for (int i = 0; i < 16; ++i) {
+            if constexpr (sizeof(O) == 4)
+                words[i] = __float_as_uint(v[from + part * 16 + i]);
+            else
+                words[i] = word_of<O>(v[from + 2 * i], v[from + 2 * i + 1]);
         }
-    } else {
+        put_words<O>(staging, words, out, row0, col0 + part * 16, m, n);
+    }
+}
+
+// Starts to copy 32 columns of 32 rows of an m x n array of 16-bit values (rows row0 ...,
+// columns col0 ...) into the warp's shared memory, zeros for what is outside, four lanes
+// a row.
+template <typename T>
+__device__ __forceinline__ void fetch_columns(unsigned char *to, const Matrix &in, int row0, int col0, int m, int n) {
+    const int lane = threadIdx.x & 31, c = col0 + lane % 4 * 8;
+    const bool whole = by_16<T>(in.p, in.stride) && c + 8 <= n;
 #pragma unroll
-        for (int j = 0; j < 32; ++j)
-            v[j] = row < m && col0 + j < n ? widen(((const T *)in.p)[(size_t)row * in.stride + col0 + j]) : 0.0f;
+    for (int i = 0; i < 4; ++i) {
+        const int r = row0 + i * 8 + lane / 4;
+        const unsigned short *from = (const unsigned short *)in.p + (size_t)r * in.stride + c;
+        unsigned char *place = to + (i * 8 + lane / 4) * 80 + lane % 4 * 16;
+        if (c >= n || r >= m) {
+            *(uint4 *)place = make_uint4(0, 0, 0, 0);
+        } else if (whole) {
+            copy_async(shared_address(place), from);
+        } else {
+            for (int j = 0; j < 8; ++j) ((unsigned short *)place)[j] = c + j < n ? from[j] : 0;
+        }
+    }
+}
+// This thread's row of them.
+template <typename T>
+__device__ __forceinline__ void get_columns(const unsigned char *from, float (&v)[32]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const Vec<T, 8> piece = load<T, 8>((const T *)(from + (threadIdx.x & 31) * 80) + 8 * j);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const Pair<float> two = piece.pair(q);
+            v[8 * j + 2 * q] = two.x;
+            v[8 * j + 2 * q + 1] = two.y;
+        }
     }
 }
 
@@ -214,11 +258,12 @@ __device__ __forceinline__ Tile tile_of(int index, int down, int across, int spl
 
 // TWICE: A comes as the sum of two arrays, each multiplied with the same tile of B. O: of what is written.
 template <typename T, typename O, bool TWICE, int KIND, int BN>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(64 + 32 * epilogue_warps(KIND, TWICE), 1)
     product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Product p, int down, int across, int tiles,
                    PipelineStarve starve) {
     constexpr bool kAMn = KIND == kWeights, kBMn = KIND == kHidden || KIND == kInput || KIND == kWeights;
-    constexpr int kStages = stages_of(BN, TWICE), kColumns = KIND == kGated ? BN / 2 : BN;  // of the result, a tile
+    constexpr int kWarps = epilogue_warps(KIND, TWICE);
+    constexpr int kStages = stages_of(KIND, BN, TWICE), kColumns = KIND == kGated ? BN / 2 : BN;  // of the result, a tile
     constexpr uint32_t kBytesA = bytes_a(TWICE), kStageBytes = kBytesA + bytes_b(BN), kSumColumns = 2 * BN < 32 ? 32 : 2 * BN;
     extern __shared__ unsigned char memory[];
     __shared__ __align__(8) uint64_t barriers[2 * kStages + 5];
@@ -232,7 +277,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (threadIdx.x == 0) {
         gave_up = 0;
         for (int s = 0; s < kStages; ++s) barrier_init(full + 8 * s, 1), barrier_init(empty + 8 * s, 1);
-        for (int i = 0; i < 2; ++i) barrier_init(ready + 8 * i, 1), barrier_init(taken + 8 * i, kEpilogueWarps);
+        for (int i = 0; i < 2; ++i) barrier_init(ready + 8 * i, 1), barrier_init(taken + 8 * i, kWarps);
         barrier_init(drained, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -299,53 +344,67 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     } else if (warp == 1 && lane == 0) {
         constexpr uint32_t kInstruction = instruction<T>(kAMn, kBMn, BN);
-        uint32_t step = 0, round = 0;
+        uint32_t step = 0, round = 0;  // round: of the two places for sums
         bool good = true;
-        for (int index = blockIdx.x; index < tiles && good; index += gridDim.x, ++round) {
-            const uint32_t to = round & 1, use = round >> 1;
+        for (int index = blockIdx.x; index < tiles && good; index += gridDim.x) {
             const Tile t = tile_of(index, down, across, p.splits);
-            const int first = first_of(t), last = last_of(t);
-            if (!barrier_wait(taken + 8 * to, (use & 1) ^ 1, starve.polls, &gave_up)) break;
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            for (int i = first; i < last; ++i, ++step) {
-                const uint32_t s = step % kStages;
-                if (!barrier_wait(full + 8 * s, (step / kStages) & 1, starve.polls, &gave_up)) {
-                    good = false;
-                    break;
-                }
+            const int last = last_of(t);
+            for (int i = first_of(t); i < last && good; ++round) {
+                const uint32_t to = round & 1, use = round >> 1;
+                const int first = i, end = TWICE && last - i > kChunk ? i + kChunk : last;
+                good = barrier_wait(taken + 8 * to, (use & 1) ^ 1, starve.polls, &gave_up);
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint32_t at = base + s * kStageBytes;
-                const uint64_t a = operand(at, kAMn ? 8192 : 16), b = operand(at + kBytesA, kBMn ? 8192 : 16);
+                for (; i < end && good; ++i, ++step) {
+                    const uint32_t s = step % kStages;
+                    if (!barrier_wait(full + 8 * s, (step / kStages) & 1, starve.polls, &gave_up)) {
+                        good = false;
+                        break;
+                    }
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const uint32_t at = base + s * kStageBytes;
+                    const uint64_t a = operand(at, kAMn ? 8192 : 16), b = operand(at + kBytesA, kBMn ? 8192 : 16);
 #pragma unroll
-                for (int k = 0; k < kBK / 16; ++k)  // 16 of K: 32 bytes along a row, or 16 rows of 128 bytes
-                    multiply(sums + to * BN, a + (uint64_t)k * (kAMn ? 128 : 2), b + (uint64_t)k * (kBMn ? 128 : 2),
-                             kInstruction, i > first || k > 0);
-                if constexpr (TWICE) {
+                    for (int k = 0; k < kBK / 16; ++k)  // 16 of K: 32 bytes along a row, or 16 rows of 128 bytes
+                        multiply(sums + to * BN, a + (uint64_t)k * (kAMn ? 128 : 2), b + (uint64_t)k * (kBMn ? 128 : 2),
+                                 kInstruction, i > first || k > 0);
+                    if constexpr (TWICE) {
 #pragma unroll
-                    for (int k = 0; k < kBK / 16; ++k)
-                        multiply(sums + to * BN, a + (uint64_t)(bytes_a(false) / 16 + k * 128), b + (uint64_t)k * 128,
-                                 kInstruction, true);
+                        for (int k = 0; k < kBK / 16; ++k)
+                            multiply(sums + to * BN, a + (uint64_t)(bytes_a(false) / 16 + k * 128),
+                                     b + (uint64_t)k * 128, kInstruction, true);
+                    }
+                    commit_to(empty + 8 * s);
                 }
-                commit_to(empty + 8 * s);
+                if (good) commit_to(ready + 8 * to);
             }
-            if (good) commit_to(ready + 8 * to);
         }
         // Matrix instructions in flight end before tensor memory is given back.
         commit_to(drained);
         barrier_wait(drained, 0, starve.polls, nullptr);
     } else if (warp >= 2) {
-        unsigned char *mine = staging + (warp - 2) * kStaging;
+        unsigned char *mine = staging + (warp - 2) * staging_of(KIND);
         const int quarter = warp & 3;  // the rows of tensor memory that this warp may read
+        constexpr int kPart = kColumns / (kWarps / 4);  // its columns, from `begin` on
+        const int begin = (warp - 2) / 4 * kPart;
         uint32_t round = 0;
         bool good = true;
-        for (int index = blockIdx.x; index < tiles; index += gridDim.x, ++round) {
+        for (int index = blockIdx.x; index < tiles; index += gridDim.x) {
             const Tile t = tile_of(index, down, across, p.splits);
-            const uint32_t from = round & 1, use = round >> 1;
-            if (good) good = barrier_wait(ready + 8 * from, use & 1, starve.polls, &gave_up);
-            good = __all_sync(0xffffffffu, good);
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const uint32_t at = sums + from * BN + ((uint32_t)quarter << 21);
             const int row0 = t.row * kBM + quarter * 32, row = row0 + lane;
+            uint32_t at = 0;
+            auto wait = [&] {  // for the next sums
+                const uint32_t from = round & 1, use = round >> 1;
+                if (good) good = barrier_wait(ready + 8 * from, use & 1, starve.polls, &gave_up);
+                good = __all_sync(0xffffffffu, good);
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                at = sums + from * BN + ((uint32_t)quarter << 21);
+            };
+            auto release = [&] {
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) barrier_arrive(taken + 8 * (round & 1));
+                ++round;
+            };
             // What gave up is NaN from here on.
             auto take = [&](int c, float (&v)[32]) {
                 if (good) {
@@ -355,72 +414,125 @@ __global__ void __launch_bounds__(kThreads, 1)
                     for (int j = 0; j < 32; ++j) v[j] = __int_as_float(0x7FC00000);
                 }
             };
-            if (row0 < p.m) {
-#pragma unroll 1
-                for (int c = 0; c < kColumns; c += 32) {
-                    const int col0 = t.column * kColumns + c;
-                    if (col0 >= p.n) break;
-                    float v[32];
-                    take(c, v);
-                    if constexpr (KIND == kGated) {
-                        if (p.out[0].p != nullptr) put_columns<T>(mine, v, p.out[0], row0, col0, p.m, p.n);
-                        float u[32];
-                        take(kColumns + c, u);
-                        if (p.out[1].p != nullptr) put_columns<T>(mine, u, p.out[1], row0, col0, p.m, p.n);
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) v[j] = activation<true>(p.activation, v[j], (float *)nullptr) * u[j];
-                        put_columns<T>(mine, v, p.out[2], row0, col0, p.m, p.n);
-                    } else if constexpr (KIND == kHidden) {
-                        float g[32], u[32];
-                        get_columns<T>(p.saved[0], row, col0, p.m, p.n, g);
-                        get_columns<T>(p.saved[1], row, col0, p.m, p.n, u);
-                        float h[32];
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) {
-                            float slope;
-                            const float f = activation<true>(p.activation, g[j], &slope);
-                            h[j] = f * u[j];
-                            g[j] = v[j] * u[j] * slope;
-                            u[j] = v[j] * f;
+            // 32 columns of a result of kWeights, kDown, kInput.
+            auto put = [&](const auto &v, int from, int col0) {
+                if constexpr (KIND == kWeights) {
+                    if (p.splits > 1) {
+                        if constexpr (sizeof(O) == 4) {
+                            const size_t stride = partial_width(p.n), part = t.problem * p.splits + t.split;
+                            put_columns<O>(mine, v, from, {(O *)p.partial + part * p.m * stride, stride}, row0, col0, p.m,
+                                           p.n);
                         }
-                        auto put = [&](float (&x)[32], int n) {
-                            if (p.out[n].p != nullptr) put_columns<T>(mine, x, p.out[n], row0, col0, p.m, p.n);
-                            if (p.out_low[n].p != nullptr) {
+                        return;
+                    }
+                    if (p.transposed[t.problem]) {
+                        // A column of the tile is a row of the result: lanes are neighbours there.
+                        const OutMatrix &out = p.out[t.problem];
 #pragma unroll
-                                for (int j = 0; j < 32; ++j) x[j] = lost_to<T>(x[j]);
-                                put_columns<T>(mine, x, p.out_low[n], row0, col0, p.m, p.n);
-                            }
-                        };
-                        put(g, 0);
-                        put(u, 1);
-                        put(h, 2);
-                    } else {
-                        if constexpr (KIND == kWeights) {
-                            if (p.splits > 1) {
-                                if constexpr (sizeof(O) == 4) {
-                                    const size_t stride = partial_width(p.n), part = t.problem * p.splits + t.split;
-                                    put_columns<O>(mine, v, {(O *)p.partial + part * p.m * stride, stride}, row0, col0,
-                                                   p.m, p.n);
-                                }
-                                continue;
-                            }
-                            if (p.transposed[t.problem]) {
-                                // A column of the tile is a row of the result: lanes are neighbours there.
-#pragma unroll
-                                for (int j = 0; j < 32; ++j)
-                                    if (row < p.m && col0 + j < p.n)
-                                        ((O *)p.out[t.problem].p)[(size_t)(col0 + j) * p.out[t.problem].stride + row] =
-                                            narrow<O>(v[j]);
-                                continue;
-                            }
-                        }
-                        put_columns<O>(mine, v, p.out[KIND == kWeights ? t.problem : 0], row0, col0, p.m, p.n);
+                        for (int j = 0; j < 32; ++j)
+                            if (row < p.m && col0 + j < p.n)
+                                ((O *)out.p)[(size_t)(col0 + j) * out.stride + row] = narrow<O>(v[from + j]);
+                        return;
                     }
                 }
+                put_columns<O>(mine, v, from, p.out[KIND == kWeights ? t.problem : 0], row0, col0, p.m, p.n);
+            };
+            if constexpr (TWICE) {
+                float sum[kPart];
+#pragma unroll
+                for (int j = 0; j < kPart; ++j) sum[j] = 0.0f;
+                const int last = last_of(t);
+                for (int i = first_of(t); i < last; i += kChunk) {
+                    wait();
+#pragma unroll
+                    for (int c = 0; c < kPart; c += 32) {
+                        float v[32];
+                        take(begin + c, v);
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) sum[c + j] += v[j];
+                    }
+                    release();
+                }
+                if (row0 < p.m) {
+#pragma unroll
+                    for (int c = 0; c < kPart; c += 32) {
+                        const int col0 = t.column * kColumns + begin + c;
+                        if (col0 < p.n) put(sum, c, col0);
+                    }
+                }
+            } else {
+                auto fetch = [&](int c) {
+                    const int col0 = t.column * kColumns + c;
+                    fetch_columns<T>(mine + kRows, p.saved[0], row0, col0, p.m, p.n);
+                    fetch_columns<T>(mine + 2 * kRows, p.saved[1], row0, col0, p.m, p.n);
+                    commit_async();
+                };
+                if constexpr (KIND == kHidden) fetch(begin);
+                wait();
+                if (row0 < p.m) {
+#pragma unroll 1
+                    for (int c = begin; c < begin + kPart; c += 32) {
+                        const int col0 = t.column * kColumns + c;
+                        if (col0 >= p.n) break;
+                        float v[32];
+                        take(c, v);
+                        if constexpr (KIND == kGated) {
+                            if (p.out[0].p != nullptr) put_columns<T>(mine, v, 0, p.out[0], row0, col0, p.m, p.n);
+                            float u[32];
+                            take(kColumns + c, u);
+                            if (p.out[1].p != nullptr) put_columns<T>(mine, u, 0, p.out[1], row0, col0, p.m, p.n);
+                            by_activation(p.activation, [&](auto kind) {
+#pragma unroll
+                                for (int j = 0; j < 32; ++j)
+                                    v[j] = activation<true>(decltype(kind)::value, v[j], (float *)nullptr) * u[j];
+                            });
+                            put_columns<T>(mine, v, 0, p.out[2], row0, col0, p.m, p.n);
+                        } else if constexpr (KIND == kHidden) {
+                            // O float: with what the 16-bit values lose.
+                            constexpr int kTerms = std::is_same_v<O, float> ? 2 : 1;
+                            float g[32], u[32];
+                            wait_async<0>();
+                            __syncwarp();
+                            get_columns<T>(mine + kRows, g);
+                            get_columns<T>(mine + 2 * kRows, u);
+                            __syncwarp();
+                            if (c + 32 < begin + kPart) fetch(c + 32);  // on its way meanwhile
+                            uint32_t words[3][kTerms][16];
+                            by_activation(p.activation, [&](auto kind) {
+#pragma unroll
+                                for (int q = 0; q < 16; ++q) {
+                                    Pair<float> f, slope;
+                                    f.x = activation<true>(decltype(kind)::value, g[2 * q], &slope.x);
+                                    f.y = activation<true>(decltype(kind)::value, g[2 * q + 1], &slope.y);
+                                    const Pair<float> hb = {v[2 * q], v[2 * q + 1]}, up2 = {u[2 * q], u[2 * q + 1]};
+                                    const Pair<float> results[3] = {hb * up2 * slope, hb * f, f * up2};
+#pragma unroll
+                                    for (int n = 0; n < 3; ++n) {
+                                        words[n][0][q] = word_of<T>(results[n].x, results[n].y);
+                                        if constexpr (kTerms == 2) {
+                                            Vec<T, 2> high;
+                                            high.w[0] = words[n][0][q];
+                                            const Pair<float> left = results[n] + high.pair(0) * both(-1.0f);
+                                            words[n][1][q] = word_of<T>(left.x, left.y);
+                                        }
+                                    }
+                                }
+                            });
+#pragma unroll
+                            for (int n = 0; n < 3; ++n) {
+                                if (p.out[n].p != nullptr)
+                                    put_words<T>(mine, words[n][0], p.out[n], row0, col0, p.m, p.n);
+                                if constexpr (kTerms == 2)
+                                    if (p.out_low[n].p != nullptr)
+                                        put_words<T>(mine, words[n][1], p.out_low[n], row0, col0, p.m, p.n);
+                            }
+                        } else {
+                            put(v, 0, col0);
+                        }
+                    }
+                }
+                release();
             }
-            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) barrier_arrive(taken + 8 * from);
         }
     }
     __syncwarp();
@@ -464,7 +576,8 @@ cudaError_t launch_tiles(const Product &p, PipelineStarve starve, cudaStream_t s
     constexpr bool kAMn = KIND == kWeights, kBMn = KIND == kHidden || KIND == kInput || KIND == kWeights;
     constexpr int kColumns = KIND == kGated ? BN / 2 : BN;
     constexpr bool kBfloat = std::is_same_v<T, __nv_bfloat16>;
-    constexpr uint32_t kShared = shared_bytes(BN, TWICE);
+    constexpr uint32_t kShared = shared_bytes(KIND, BN, TWICE);
+    constexpr int kThreads = 64 + 32 * epilogue_warps(KIND, TWICE);
     Maps maps = {};
     const int pairs_a = KIND == kInput ? 2 : p.problems, pairs_b = KIND == kInput || KIND == kGated ? 2 : p.problems;
     bool good = true;
@@ -518,7 +631,9 @@ cudaError_t launch_type(ProductKind kind, uint32_t type, uint32_t out_type, cons
     switch (kind) {
         case kGated: return launch_kind<T, T, false, kGated>(p, starve, stream);
         case kDown: return launch_kind<T, T, false, kDown>(p, starve, stream);
-        case kHidden: return launch_kind<T, T, false, kHidden>(p, starve, stream);
+        case kHidden:
+            return out_type == GEO_B200_F32 ? launch_kind<T, float, false, kHidden>(p, starve, stream)
+                                            : launch_kind<T, T, false, kHidden>(p, starve, stream);
         case kInput: return launch_kind<T, T, false, kInput>(p, starve, stream);
         default: break;
     }
