@@ -58,7 +58,7 @@ cudaError_t launch_join_splits(uint32_t type, uint32_t out_type, const Product &
 struct PipelineStarve {
     uint32_t block, polls;
 };
-constexpr uint32_t kPipelinePolls = 1u << 22;  // seconds, where a stage takes microseconds
+constexpr uint32_t kPipelinePolls = 1u << 20;  // seconds, where a stage takes microseconds
 
 // `type`: of the operands; `out_type`: of kWeights' results. A stream-ordered launch.
 cudaError_t launch_product_tensor(ProductKind kind, uint32_t type, uint32_t out_type, const Product &p,

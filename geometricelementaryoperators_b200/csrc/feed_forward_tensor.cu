@@ -16,9 +16,15 @@
 // Operands whose sum index is not the adjacent one (weights in the VJP, both sides
 // of the weights' cotangents) are copied as they lie, [64 of K][64 values] boxes,
 // and read by the matrix instruction as "MN-major": nothing is transposed.
+// PAIR: two blocks on neighbouring multiprocessors work on one tile of 256 rows
+// (tcgen05 cta_group::2). Each copies its own 128 rows of A and half of the columns of
+// B, and the first block's instructions multiply for both: 32 KB copied a block of K
+// instead of 48. What bounds a single block is the way from L2 into its shared memory:
+// the instructions of the VJP's products waited 28 to 59% of their time for data.
 // kGated puts BN / 2 rows of each weight side by side in one B tile, so that gate and
 // up of the same hidden values are in one tile of sums; kInput adds both its products
 // into one tile, K running through the first pair of operands, then the second.
+#include <cooperative_groups.h>
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -43,12 +49,16 @@ constexpr uint32_t bytes_b(int bn) { return (uint32_t)bn * kBK * 2; }
 constexpr uint32_t kRows = 32 * 80;  // a warp's 32 rows of 64 bytes; 16 more keep banks apart
 constexpr uint32_t staging_of(int kind) { return kind == kHidden ? 3 * kRows : kRows; }  // of a warp
 constexpr uint32_t kSharedMost = 227 * 1024;
-constexpr int stages_of(int kind, int bn, bool twice) {
-    const int n = (int)((kSharedMost - 1024 - epilogue_warps(kind, twice) * staging_of(kind) - 512) / (bytes_a(twice) + bytes_b(bn)));
+// A block's part of a stage.
+constexpr uint32_t stage_bytes(int bn, bool twice, bool pair) { return bytes_a(twice) + bytes_b(bn) / (pair ? 2 : 1); }
+constexpr int stages_of(int kind, int bn, bool twice, bool pair) {
+    const int n = (int)((kSharedMost - 1024 - epilogue_warps(kind, twice) * staging_of(kind) - 512) /
+                        stage_bytes(bn, twice, pair));
     return n > 8 ? 8 : n;
 }
-constexpr uint32_t shared_bytes(int kind, int bn, bool twice) {
-    return 1024 + stages_of(kind, bn, twice) * (bytes_a(twice) + bytes_b(bn)) + epilogue_warps(kind, twice) * staging_of(kind);
+constexpr uint32_t shared_bytes(int kind, int bn, bool twice, bool pair) {
+    return 1024 + stages_of(kind, bn, twice, pair) * stage_bytes(bn, twice, pair) +
+           epilogue_warps(kind, twice) * staging_of(kind);
 }
 
 struct Maps {
@@ -64,10 +74,19 @@ __device__ __forceinline__ void barrier_expect(uint32_t barrier, uint32_t bytes)
 __device__ __forceinline__ void barrier_arrive(uint32_t barrier) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(barrier) : "memory");
 }
+// The same barrier of the pair's block `rank`.
+__device__ __forceinline__ uint32_t barrier_of(uint32_t barrier, uint32_t rank) {
+    uint32_t there;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(barrier), "r"(rank));
+    return there;
+}
+__device__ __forceinline__ void barrier_arrive_cluster(uint32_t there) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(there) : "memory");
+}
 __device__ __forceinline__ bool barrier_try(uint32_t barrier, uint32_t parity) {
     uint32_t done;
     asm volatile(
-        "{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}"
+        "{\n.reg .pred p;\nmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}"
         : "=r"(done)
         : "r"(barrier), "r"(parity)
         : "memory");
@@ -83,11 +102,21 @@ __device__ __forceinline__ bool barrier_wait(uint32_t barrier, uint32_t parity, 
     return false;
 }
 
+// A box of the tensor to this block's shared memory; `barrier` may be of the pair's first block.
+template <bool PAIR>
 __device__ __forceinline__ void tma_load(uint32_t to, const CUtensorMap *map, int x, int y, uint32_t barrier) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(to),
-        "l"(map), "r"(x), "r"(y), "r"(barrier)
-        : "memory");
+    if constexpr (PAIR)
+        asm volatile(
+            "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 "
+            "[%0], [%1, {%2, %3}], [%4];" ::"r"(to),
+            "l"(map), "r"(x), "r"(y), "r"(barrier)
+            : "memory");
+    else
+        asm volatile(
+            "cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
+                to),
+            "l"(map), "r"(x), "r"(y), "r"(barrier)
+            : "memory");
 }
 
 // Shared-memory descriptor of a 128-byte-swizzled operand. Its eight-row groups are
@@ -96,22 +125,40 @@ __device__ __forceinline__ uint64_t operand(uint32_t address, uint32_t leading) 
     return (uint64_t)((address & 0x3FFFF) >> 4) | (uint64_t)((leading >> 4) & 0x3FFF) << 16 |
            (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
 }
-// 16-bit operands, float32 sums, 128 x n.
+// 16-bit operands, float32 sums, m x n.
 template <typename T>
-__device__ __forceinline__ constexpr uint32_t instruction(bool a_mn, bool b_mn, int n) {
+__device__ __forceinline__ constexpr uint32_t instruction(bool a_mn, bool b_mn, int m, int n) {
     const uint32_t format = std::is_same_v<T, __nv_bfloat16> ? 1 : 0;
     return 1u << 4 | format << 7 | format << 10 | (uint32_t)a_mn << 15 | (uint32_t)b_mn << 16 |
-           (uint32_t)(n / 8) << 17 | (uint32_t)(kBM / 16) << 24;
+           (uint32_t)(n / 8) << 17 | (uint32_t)(m / 16) << 24;
 }
+template <bool PAIR>
 __device__ __forceinline__ void multiply(uint32_t sums, uint64_t a, uint64_t b, uint32_t instruction, bool add) {
-    asm volatile(
-        "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(sums),
-        "l"(a), "l"(b), "r"(instruction), "r"((uint32_t)add)
-        : "memory");
+    if constexpr (PAIR)
+        asm volatile(
+            "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+            "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(sums),
+            "l"(a), "l"(b), "r"(instruction), "r"((uint32_t)add)
+            : "memory");
+    else
+        asm volatile(
+            "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+            "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(sums),
+            "l"(a), "l"(b), "r"(instruction), "r"((uint32_t)add)
+            : "memory");
 }
+// Arrives at the barrier (PAIR: of both blocks) once the matrix instructions so far have ended.
+template <bool PAIR>
 __device__ __forceinline__ void commit_to(uint32_t barrier) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(barrier) : "memory");
+    if constexpr (PAIR)
+        asm volatile(
+            "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+                barrier),
+            "h"((unsigned short)3)
+            : "memory");
+    else
+        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(barrier)
+                     : "memory");
 }
 
 // 32 columns of this thread's row of the warp's 32 rows of tensor memory.
@@ -257,14 +304,14 @@ __device__ __forceinline__ Tile tile_of(int index, int down, int across, int spl
 }
 
 // TWICE: A comes as the sum of two arrays, each multiplied with the same tile of B. O: of what is written.
-template <typename T, typename O, bool TWICE, int KIND, int BN>
+template <typename T, typename O, bool TWICE, int KIND, int BN, bool PAIR>
 __global__ void __launch_bounds__(64 + 32 * epilogue_warps(KIND, TWICE), 1)
     product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Product p, int down, int across, int tiles,
                    PipelineStarve starve) {
     constexpr bool kAMn = KIND == kWeights, kBMn = KIND == kHidden || KIND == kInput || KIND == kWeights;
     constexpr int kWarps = epilogue_warps(KIND, TWICE);
-    constexpr int kStages = stages_of(KIND, BN, TWICE), kColumns = KIND == kGated ? BN / 2 : BN;  // of the result, a tile
-    constexpr uint32_t kBytesA = bytes_a(TWICE), kStageBytes = kBytesA + bytes_b(BN), kSumColumns = 2 * BN < 32 ? 32 : 2 * BN;
+    constexpr int kStages = stages_of(KIND, BN, TWICE, PAIR), kColumns = KIND == kGated ? BN / 2 : BN;  // of the result, a tile
+    constexpr uint32_t kBytesA = bytes_a(TWICE), kStageBytes = stage_bytes(BN, TWICE, PAIR), kSumColumns = 2 * BN < 32 ? 32 : 2 * BN;
     extern __shared__ unsigned char memory[];
     __shared__ __align__(8) uint64_t barriers[2 * kStages + 5];
     __shared__ uint32_t sums_address;
@@ -272,25 +319,40 @@ __global__ void __launch_bounds__(64 + 32 * epilogue_warps(KIND, TWICE), 1)
     const uint32_t base = (shared_address(memory) + 1023) & ~1023u;
     unsigned char *staging = memory + (base - shared_address(memory)) + kStages * kStageBytes;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // Of the pair; tiles are taken by pairs.
+    const int rank = PAIR ? (int)cooperative_groups::this_cluster().block_rank() : 0;
+    const int team = PAIR ? (int)blockIdx.x / 2 : (int)blockIdx.x, teams = PAIR ? (int)gridDim.x / 2 : (int)gridDim.x;
     const uint32_t full = shared_address(barriers), empty = full + 8 * kStages, ready = empty + 8 * kStages,
                    taken = ready + 16, drained = taken + 16;
     if (threadIdx.x == 0) {
         gave_up = 0;
         for (int s = 0; s < kStages; ++s) barrier_init(full + 8 * s, 1), barrier_init(empty + 8 * s, 1);
-        for (int i = 0; i < 2; ++i) barrier_init(ready + 8 * i, 1), barrier_init(taken + 8 * i, kWarps);
+        for (int i = 0; i < 2; ++i) barrier_init(ready + 8 * i, 1), barrier_init(taken + 8 * i, (PAIR ? 2 : 1) * kWarps);
         barrier_init(drained, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
-                         shared_address(&sums_address)),
-                     "r"(kSumColumns)
-                     : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        if constexpr (PAIR) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                             shared_address(&sums_address)),
+                         "r"(kSumColumns)
+                         : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                             shared_address(&sums_address)),
+                         "r"(kSumColumns)
+                         : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        }
     }
-    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-    __syncthreads();
-    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    auto everyone = [&] {
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        __syncthreads();
+        if constexpr (PAIR) cooperative_groups::this_cluster().sync();
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    };
+    everyone();
     const uint32_t sums = sums_address;
     const int blocks_k = (p.k + kBK - 1) / kBK;
     // A tile's blocks of K: kInput goes through K twice, kWeights' splits each through a part.
@@ -303,7 +365,7 @@ __global__ void __launch_bounds__(64 + 32 * epilogue_warps(KIND, TWICE), 1)
     if (warp == 0 && lane == 0) {
         uint32_t step = 0;  // of all tiles, one after another
         bool good = true;
-        for (int index = blockIdx.x; index < tiles && good; index += gridDim.x) {
+        for (int index = team; index < tiles && good; index += teams) {
             const Tile t = tile_of(index, down, across, p.splits);
             const int last = last_of(t);
             for (int i = first_of(t); i < last; ++i, ++step) {
@@ -312,41 +374,50 @@ __global__ void __launch_bounds__(64 + 32 * epilogue_warps(KIND, TWICE), 1)
                     good = false;
                     break;
                 }
-                const uint32_t to = base + s * kStageBytes, barrier = full + 8 * s;
-                barrier_expect(barrier, kStageBytes);
+                const uint32_t to = base + s * kStageBytes;
+                const uint32_t barrier = PAIR ? barrier_of(full + 8 * s, 0) : full + 8 * s;
+                if (rank == 0) barrier_expect(full + 8 * s, (PAIR ? 2 : 1) * kStageBytes);
                 const int second = KIND == kInput && i >= blocks_k ? 1 : 0, k = (i - second * blocks_k) * kBK;
-                const CUtensorMap *a = &maps.a[KIND == kWeights ? t.problem : second], *b = &maps.b[KIND == kWeights ? t.problem : second];
+                const int row0 = (PAIR ? t.row * 2 + rank : t.row) * kBM;
+                // This block's rows of B.
+                constexpr int kHeld = PAIR ? BN / 2 : BN;
+                const int col0 = t.column * (KIND == kGated ? kColumns : BN) + (KIND == kGated ? 0 : rank * kHeld);
+                const CUtensorMap *a = &maps.a[KIND == kWeights ? t.problem : second];
+                const CUtensorMap *b = &maps.b[KIND == kWeights ? t.problem : second];
                 if constexpr (kAMn) {
-                    for (int j = 0; j < kBM / 64; ++j) tma_load(to + j * 8192, a, t.row * kBM + j * 64, k, barrier);
+                    for (int j = 0; j < kBM / 64; ++j) tma_load<PAIR>(to + j * 8192, a, row0 + j * 64, k, barrier);
                     if constexpr (TWICE)
                         for (int j = 0; j < kBM / 64; ++j)
-                            tma_load(to + (kBM / 64 + j) * 8192, &maps.low[t.problem], t.row * kBM + j * 64, k, barrier);
+                            tma_load<PAIR>(to + (kBM / 64 + j) * 8192, &maps.low[t.problem], row0 + j * 64, k, barrier);
                 } else {
-                    tma_load(to, a, k, t.row * kBM, barrier);
+                    tma_load<PAIR>(to, a, k, row0, barrier);
                 }
                 if constexpr (kBMn) {
-                    for (int j = 0; j < BN / 64; ++j)
-                        tma_load(to + kBytesA + j * 8192, b, t.column * BN + j * 64, k, barrier);
+                    for (int j = 0; j < kHeld / 64; ++j)
+                        tma_load<PAIR>(to + kBytesA + j * 8192, b, col0 + j * 64, k, barrier);
+                } else if constexpr (KIND == kGated && PAIR) {  // gate's rows in one block, up's in the other
+                    tma_load<PAIR>(to + kBytesA, &maps.b[rank], k, col0, barrier);
                 } else if constexpr (KIND == kGated) {
-                    tma_load(to + kBytesA, &maps.b[0], k, t.column * kColumns, barrier);
-                    tma_load(to + kBytesA + bytes_b(kColumns), &maps.b[1], k, t.column * kColumns, barrier);
+                    tma_load<PAIR>(to + kBytesA, &maps.b[0], k, col0, barrier);
+                    tma_load<PAIR>(to + kBytesA + bytes_b(kColumns), &maps.b[1], k, col0, barrier);
                 } else {
-                    tma_load(to + kBytesA, b, k, t.column * BN, barrier);
+                    tma_load<PAIR>(to + kBytesA, b, k, col0, barrier);
                 }
             }
         }
         if (!good) {
-            // Copies in flight land before the block ends. A stage's last copies were of its last round begun.
-            for (uint32_t n = step < (uint32_t)kStages ? step : kStages; n > 0; --n) {
+            // Copies in flight land before the block ends. A stage's last copies were of its last round begun. (A
+            // pair's land at the first block's barriers, and the other one leaves no sooner than the first.)
+            for (uint32_t n = step < (uint32_t)kStages ? step : kStages; n > 0 && rank == 0; --n) {
                 const uint32_t last = step - n;
                 barrier_wait(full + 8 * (last % kStages), (last / kStages) & 1, starve.polls, nullptr);
             }
         }
-    } else if (warp == 1 && lane == 0) {
-        constexpr uint32_t kInstruction = instruction<T>(kAMn, kBMn, BN);
+    } else if (warp == 1 && lane == 0 && rank == 0) {
+        constexpr uint32_t kInstruction = instruction<T>(kAMn, kBMn, PAIR ? 2 * kBM : kBM, BN);
         uint32_t step = 0, round = 0;  // round: of the two places for sums
         bool good = true;
-        for (int index = blockIdx.x; index < tiles && good; index += gridDim.x) {
+        for (int index = team; index < tiles && good; index += teams) {
             const Tile t = tile_of(index, down, across, p.splits);
             const int last = last_of(t);
             for (int i = first_of(t); i < last && good; ++round) {
@@ -365,21 +436,21 @@ __global__ void __launch_bounds__(64 + 32 * epilogue_warps(KIND, TWICE), 1)
                     const uint64_t a = operand(at, kAMn ? 8192 : 16), b = operand(at + kBytesA, kBMn ? 8192 : 16);
 #pragma unroll
                     for (int k = 0; k < kBK / 16; ++k)  // 16 of K: 32 bytes along a row, or 16 rows of 128 bytes
-                        multiply(sums + to * BN, a + (uint64_t)k * (kAMn ? 128 : 2), b + (uint64_t)k * (kBMn ? 128 : 2),
+                        multiply<PAIR>(sums + to * BN, a + (uint64_t)k * (kAMn ? 128 : 2), b + (uint64_t)k * (kBMn ? 128 : 2),
                                  kInstruction, i > first || k > 0);
                     if constexpr (TWICE) {
 #pragma unroll
                         for (int k = 0; k < kBK / 16; ++k)
-                            multiply(sums + to * BN, a + (uint64_t)(bytes_a(false) / 16 + k * 128),
+                            multiply<PAIR>(sums + to * BN, a + (uint64_t)(bytes_a(false) / 16 + k * 128),
                                      b + (uint64_t)k * 128, kInstruction, true);
                     }
-                    commit_to(empty + 8 * s);
+                    commit_to<PAIR>(empty + 8 * s);
                 }
-                if (good) commit_to(ready + 8 * to);
+                if (good) commit_to<PAIR>(ready + 8 * to);
             }
         }
         // Matrix instructions in flight end before tensor memory is given back.
-        commit_to(drained);
+        commit_to<PAIR>(drained);
         barrier_wait(drained, 0, starve.polls, nullptr);
     } else if (warp >= 2) {
         unsigned char *mine = staging + (warp - 2) * staging_of(KIND);
@@ -388,9 +459,9 @@ __global__ void __launch_bounds__(64 + 32 * epilogue_warps(KIND, TWICE), 1)
         const int begin = (warp - 2) / 4 * kPart;
         uint32_t round = 0;
         bool good = true;
-        for (int index = blockIdx.x; index < tiles; index += gridDim.x) {
+        for (int index = team; index < tiles; index += teams) {
             const Tile t = tile_of(index, down, across, p.splits);
-            const int row0 = t.row * kBM + quarter * 32, row = row0 + lane;
+            const int row0 = (PAIR ? t.row * 2 + rank : t.row) * kBM + quarter * 32, row = row0 + lane;
             uint32_t at = 0;
             auto wait = [&] {  // for the next sums
                 const uint32_t from = round & 1, use = round >> 1;
@@ -402,7 +473,12 @@ __global__ void __launch_bounds__(64 + 32 * epilogue_warps(KIND, TWICE), 1)
             auto release = [&] {
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) barrier_arrive(taken + 8 * (round & 1));
+                if (lane == 0) {
+                    if constexpr (PAIR)
+                        barrier_arrive_cluster(barrier_of(taken + 8 * (round & 1), 0));
+                    else
+                        barrier_arrive(taken + 8 * (round & 1));
+                }
                 ++round;
             };
             // What gave up is NaN from here on.
@@ -536,11 +612,13 @@ __global__ void __launch_bounds__(64 + 32 * epilogue_warps(KIND, TWICE), 1)
         }
     }
     __syncwarp();
-    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-    __syncthreads();
-    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    if (warp == 1)
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(sums), "r"(kSumColumns) : "memory");
+    everyone();
+    if (warp == 1) {
+        if constexpr (PAIR)
+            asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(sums), "r"(kSumColumns) : "memory");
+        else
+            asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(sums), "r"(kSumColumns) : "memory");
+    }
 }
 
 // ---- launches --------------------------------------------------------------------
@@ -571,12 +649,12 @@ bool encode(CUtensorMap *map, bool bfloat, const Matrix &x, int rows, int cols, 
                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename T, typename O, bool TWICE, int KIND, int BN>
+template <typename T, typename O, bool TWICE, int KIND, int BN, bool PAIR>
 cudaError_t launch_tiles(const Product &p, PipelineStarve starve, cudaStream_t stream) {
     constexpr bool kAMn = KIND == kWeights, kBMn = KIND == kHidden || KIND == kInput || KIND == kWeights;
     constexpr int kColumns = KIND == kGated ? BN / 2 : BN;
     constexpr bool kBfloat = std::is_same_v<T, __nv_bfloat16>;
-    constexpr uint32_t kShared = shared_bytes(KIND, BN, TWICE);
+    constexpr uint32_t kShared = shared_bytes(KIND, BN, TWICE, PAIR);
     constexpr int kThreads = 64 + 32 * epilogue_warps(KIND, TWICE);
     Maps maps = {};
     const int pairs_a = KIND == kInput ? 2 : p.problems, pairs_b = KIND == kInput || KIND == kGated ? 2 : p.problems;
@@ -588,17 +666,35 @@ cudaError_t launch_tiles(const Product &p, PipelineStarve starve, cudaStream_t s
     }
     for (int i = 0; i < pairs_b; ++i)
         good = good && (kBMn ? encode(&maps.b[i], kBfloat, p.b[i], p.k, p.n, kBK)
-                             : encode(&maps.b[i], kBfloat, p.b[i], p.n, p.k, kColumns));
+                             : encode(&maps.b[i], kBfloat, p.b[i], p.n, p.k, KIND == kGated || PAIR ? BN / 2 : BN));
     if (!good) return cudaErrorInvalidValue;
-    const int down = (p.m + kBM - 1) / kBM, across = (p.n + kColumns - 1) / kColumns;
+    constexpr int kRowsAtOnce = PAIR ? 2 * kBM : kBM;
+    const int down = (p.m + kRowsAtOnce - 1) / kRowsAtOnce, across = (p.n + kColumns - 1) / kColumns;
     const long long tiles = (long long)down * across * p.problems * p.splits;
     if (tiles > INT32_MAX) return cudaErrorInvalidValue;
-    const int most = geo::device_sm_count(), grid = tiles < most ? (int)tiles : most;
-    const auto kernel = product_kernel<T, O, TWICE, KIND, BN>;
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kShared);
+    const auto kernel = product_kernel<T, O, TWICE, KIND, BN, PAIR>;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kShared);
     if (e != cudaSuccess) return e;
-    kernel<<<grid, kThreads, kShared, stream>>>(maps, p, down, across, (int)tiles, starve);
-    return cudaGetLastError();
+    cudaLaunchConfig_t config = {};
+    config.blockDim = dim3(kThreads);
+    config.dynamicSmemBytes = kShared;
+    config.stream = stream;
+    cudaLaunchAttribute attribute = {};
+    attribute.id = cudaLaunchAttributeClusterDimension;
+    attribute.val.clusterDim.x = 2;
+    attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
+    config.attrs = &attribute;
+    config.numAttrs = PAIR ? 1 : 0;
+    int most = geo::device_sm_count() / (PAIR ? 2 : 1);
+    if constexpr (PAIR) {  // a pair needs two multiprocessors side by side
+        config.gridDim = dim3((unsigned)(2 * most));
+        int resident = 0;
+        e = cudaOccupancyMaxActiveClusters(&resident, kernel, &config);
+        if (e != cudaSuccess) return e;
+        if (resident > 0 && resident < most) most = resident;
+    }
+    config.gridDim = dim3((unsigned)((tiles < most ? tiles : most) * (PAIR ? 2 : 1)));
+    return cudaLaunchKernelEx(&config, kernel, maps, p, down, across, (int)tiles, starve);
 }
 
 // The widest tile that still gives every multiprocessor about one: wide tiles move
@@ -611,16 +707,19 @@ cudaError_t launch_kind(const Product &p, PipelineStarve starve, cudaStream_t st
         const long long tiles = down * ((p.n + columns - 1) / columns) * p.problems * p.splits;
         return (tiles + sms - 1) / sms * (bn + 32);
     };
+    const int columns = KIND == kGated ? 128 : 256;
+    const long long pair_tiles = (down + 1) / 2 * ((p.n + columns - 1) / columns) * p.problems * p.splits;
     constexpr int kLeast = KIND == kDown ? 32 : 64;  // a tile of kGated is half as wide, rows of boxes are 64
     int best = 256;
     for (int bn = 128; bn >= kLeast; bn /= 2)
         if (waves_cost(bn) < waves_cost(best)) best = bn;
+    if (best == 256 && pair_tiles >= sms / 2) return launch_tiles<T, O, TWICE, KIND, 256, true>(p, starve, stream);
     switch (best) {
-        case 256: return launch_tiles<T, O, TWICE, KIND, 256>(p, starve, stream);
-        case 128: return launch_tiles<T, O, TWICE, KIND, 128>(p, starve, stream);
-        case 64: return launch_tiles<T, O, TWICE, KIND, 64>(p, starve, stream);
+        case 256: return launch_tiles<T, O, TWICE, KIND, 256, false>(p, starve, stream);
+        case 128: return launch_tiles<T, O, TWICE, KIND, 128, false>(p, starve, stream);
+        case 64: return launch_tiles<T, O, TWICE, KIND, 64, false>(p, starve, stream);
         default:
-            if constexpr (kLeast == 32) return launch_tiles<T, O, TWICE, KIND, 32>(p, starve, stream);
+            if constexpr (kLeast == 32) return launch_tiles<T, O, TWICE, KIND, 32, false>(p, starve, stream);
             return cudaErrorInvalidValue;
     }
 }
