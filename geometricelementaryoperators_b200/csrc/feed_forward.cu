@@ -47,6 +47,24 @@ bool resolve(const geo_b200_feed_forward_config_t *config, bool vjp, geo_b200_fe
 size_t round8(size_t n) { return (n + 7) / 8 * 8; }
 bool off16(size_t stride) { return stride % 8 != 0; }
 
+// The most room that the parts of sums of these products take, by whichever kernels run.
+struct Extent {
+    ProductKind kind;
+    size_t m, n, k;
+};
+size_t partial_bytes(const geo_b200_feed_forward_config_t &c, std::initializer_list<Extent> products) {
+    const size_t wide = wide_bytes(c.type);
+    size_t most = 0;
+    for (const Extent &x : products) {
+        most = std::max(most, partial_values(x.kind, cut_plain(x.kind, c.type, x.m, x.n, x.k).splits, x.m, x.n));
+        if (type_bytes(c.type) == 2) {
+            const bool twice = x.kind == kWeights && c.gradient_type != c.type;
+            most = std::max(most, partial_values(x.kind, cut_tensor(x.kind, twice, x.m, x.n, x.k).splits, x.m, x.n));
+        }
+    }
+    return most * wide;
+}
+
 // Where things lie in the workspace. `take` returns the place of rows x stride values.
 struct Space {
     unsigned char *base;
@@ -114,6 +132,7 @@ extern "C" size_t geo_b200_feed_forward_workspace(const geo_b200_feed_forward_co
                                  Operand{{nullptr, c.up_weight_stride}, c.hidden, c.cols},
                                  Operand{{nullptr, c.down_weight_stride}, c.cols, c.hidden}})
             space.used += packed_bytes(o);
+    if (!few_rows(c)) space.used += partial_bytes(c, {{kGated, c.rows, c.hidden, c.cols}, {kDown, c.rows, c.cols, c.hidden}});
     return space.used;
 }
 
@@ -130,10 +149,9 @@ extern "C" size_t geo_b200_feed_forward_vjp_workspace(const geo_b200_feed_forwar
                                  Operand{{nullptr, c.up_weight_stride}, c.hidden, c.cols},
                                  Operand{{nullptr, c.down_weight_stride}, c.cols, c.hidden}})
             space.used += packed_bytes(o);
-    // Parts of the weights' cotangents, whichever kernels take the call.
-    int splits = weight_splits_plain(c.type, c.hidden, c.cols, c.rows);
-    if (b == 2) splits = std::max(splits, weight_splits_tensor(c.hidden, c.cols, c.rows));
-    if (splits > 1) space.take(3 * splits * c.hidden, partial_stride(c.cols), wide_bytes(c.type));
+    space.used += partial_bytes(c, {{kHidden, c.rows, c.hidden, c.cols},
+                                    {kInput, c.rows, c.cols, c.hidden},
+                                    {kWeights, c.hidden, c.cols, c.rows}});
     return space.used;
 }
 
@@ -168,7 +186,7 @@ extern "C" geo_b200_status_t geo_b200_feed_forward(const geo_b200_feed_forward_c
             if (e != cudaSuccess) return status_of(e);
         }
     Product gated = {};
-    gated.m = (int)c.rows, gated.n = (int)c.hidden, gated.k = (int)c.cols, gated.problems = gated.splits = 1;
+    gated.m = (int)c.rows, gated.n = (int)c.hidden, gated.k = (int)c.cols, gated.problems = 1;
     gated.activation = (int)c.activation;
     gated.a[0] = x.m;
     gated.b[0] = wg.m;
@@ -177,12 +195,15 @@ extern "C" geo_b200_status_t geo_b200_feed_forward(const geo_b200_feed_forward_c
     gated.out[1] = {device_up, c.up_stride};
     gated.out[2] = {h, hidden_stride};
     Product down = {};
-    down.m = (int)c.rows, down.n = (int)c.cols, down.k = (int)c.hidden, down.problems = down.splits = 1;
+    down.m = (int)c.rows, down.n = (int)c.cols, down.k = (int)c.hidden, down.problems = 1;
     down.a[0] = {h, hidden_stride};
     down.b[0] = wd.m;
     down.out[0] = {device_y, c.y_stride};
-    auto launch = [&](ProductKind kind, const Product &p) {
+    void *const rest = space.take(0, 0, 1);
+    auto launch = [&](ProductKind kind, Product &p) {
         if (few) return launch_product_few(kind, c.type, p, stream);
+        p.splits = (tensor ? cut_tensor(kind, false, p.m, p.n, p.k) : cut_plain(kind, c.type, p.m, p.n, p.k)).splits;
+        p.partial = rest;
         return tensor ? launch_product_tensor(kind, c.type, c.type, p, {UINT32_MAX, kPipelinePolls}, stream)
                       : launch_product_plain(kind, c.type, c.type, p, stream);
     };
@@ -233,12 +254,16 @@ extern "C" geo_b200_status_t geo_b200_feed_forward_vjp(
             const cudaError_t e = o->m.p == nullptr ? cudaSuccess : pack(*o, space, stream);
             if (e != cudaSuccess) return status_of(e);
         }
-    auto launch = [&](ProductKind kind, const Product &p) {
+    void *const rest = space.take(0, 0, 1);
+    auto launch = [&](ProductKind kind, Product &p) {
+        const bool twice = kind == kWeights && c.gradient_type != c.type;
+        p.splits = (tensor ? cut_tensor(kind, twice, p.m, p.n, p.k) : cut_plain(kind, c.type, p.m, p.n, p.k)).splits;
+        p.partial = rest;
         return tensor ? launch_product_tensor(kind, c.type, c.gradient_type, p, {UINT32_MAX, kPipelinePolls}, stream)
                       : launch_product_plain(kind, c.type, c.gradient_type, p, stream);
     };
     Product hidden = {};
-    hidden.m = (int)c.rows, hidden.n = (int)c.hidden, hidden.k = (int)c.cols, hidden.problems = hidden.splits = 1;
+    hidden.m = (int)c.rows, hidden.n = (int)c.hidden, hidden.k = (int)c.cols, hidden.problems = 1;
     hidden.activation = (int)c.activation;
     hidden.a[0] = dy.m;
     hidden.b[0] = wd.m;
@@ -252,7 +277,7 @@ extern "C" geo_b200_status_t geo_b200_feed_forward_vjp(
     cudaError_t e = launch(kHidden, hidden);
     if (e == cudaSuccess && device_x_cotangent != nullptr) {
         Product input = {};
-        input.m = (int)c.rows, input.n = (int)c.cols, input.k = (int)c.hidden, input.problems = input.splits = 1;
+        input.m = (int)c.rows, input.n = (int)c.cols, input.k = (int)c.hidden, input.problems = 1;
         for (int i = 0; i < 2; ++i) input.a[i] = {inside[i], hidden_stride};
         input.b[0] = wg.m;
         input.b[1] = wu.m;
@@ -261,8 +286,6 @@ extern "C" geo_b200_status_t geo_b200_feed_forward_vjp(
     }
     Product w = {};
     w.m = (int)c.hidden, w.n = (int)c.cols, w.k = (int)c.rows;
-    w.splits = tensor ? weight_splits_tensor(c.hidden, c.cols, c.rows) : weight_splits_plain(c.type, c.hidden, c.cols, c.rows);
-    w.partial = space.take(0, 0, 1);  // the rest
     const OutMatrix outs[3] = {{device_gate_weight_cotangent, c.gate_weight_stride},
                                {device_up_weight_cotangent, c.up_weight_stride},
                                {device_down_weight_cotangent, c.down_weight_stride}};

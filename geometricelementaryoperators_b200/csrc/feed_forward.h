@@ -31,27 +31,35 @@ struct Product {
     int m, n, k;
     int activation;    // geo_b200_activation_t
     int problems;      // kWeights: how many results; else 1
-    int splits;        // kWeights: parts of K, each with results of its own in `partial`, which are then added up; else 1
+    int splits;        // parts of K, each with sums of its own in `partial`, which are then joined; mostly 1
     Matrix a[3], b[3];
     Matrix low[3];     // kWeights to float32 from 16-bit types: what a[z] lost to rounding
     Matrix saved[2];   // kHidden: gate, up
     OutMatrix out[3];  // kGated: gate, up (may be null), h; kHidden: cotangents of gate and up, h; kWeights: [M][N], or
     bool transposed[3];     // ... [N][M]
     OutMatrix out_low[3];  // kHidden: what those lost to rounding, or null
-    void *partial;     // splits > 1: [problem][split][M][partial_stride(N)] of the arithmetic type
+    void *partial;     // splits > 1: [sum][split][M][partial_stride(N)] of the arithmetic type
 };
-inline size_t partial_stride(size_t n) { return (n + 3) / 4 * 4; }
+__host__ __device__ inline size_t partial_stride(size_t n) { return (n + 3) / 4 * 4; }
+// How many sums a result takes (kGated: gate and up), as `problems` are asked for.
+constexpr int sums_of(ProductKind kind, int problems) { return kind == kGated ? 2 : (kind == kWeights ? problems : 1); }
 
-// How many parts K is cut into for kWeights: where the results are too small to give
-// every multiprocessor a tile (rows of tile_m by tile_n), as many as do, but none under
-// `least` of K. Counts all three results, whichever are asked for.
-int weight_splits(size_t m, size_t n, size_t k, int tile_m, int tile_n, size_t least);
-constexpr int kSplitMost = 64;
-// The tensor-core and the plain kernels' own.
-int weight_splits_tensor(size_t m, size_t n, size_t k);
-int weight_splits_plain(uint32_t type, size_t m, size_t n, size_t k);
-// Adds the parts up, in their order, into the results.
-cudaError_t launch_join_splits(uint32_t type, uint32_t out_type, const Product &p, cudaStream_t stream);
+// How a product is cut into tiles, and K into parts: by its sizes and the
+// multiprocessors alone, for the kernels that take it (`tensor`, or else the plain
+// ones). Counts all three results of kWeights, whichever are asked for.
+struct Cut {
+    int columns;  // of a tile of sums
+    bool pair;    // two blocks a tile
+    int splits;
+};
+Cut cut_tensor(ProductKind kind, bool twice, size_t m, size_t n, size_t k);
+Cut cut_plain(ProductKind kind, uint32_t type, size_t m, size_t n, size_t k);
+// Values of `partial`.
+inline size_t partial_values(ProductKind kind, int splits, size_t m, size_t n) {
+    return splits > 1 ? (size_t)sums_of(kind, 3) * splits * m * partial_stride(n) : 0;
+}
+// Adds the parts up, in their order, and does with the sums what the product's kernel does otherwise.
+cudaError_t launch_join(ProductKind kind, uint32_t type, uint32_t out_type, const Product &p, cudaStream_t stream);
 
 // For the self-test of the pipeline's waits alone: the block of K at which the
 // producer of every CTA stops (never: UINT32_MAX), and how often a wait looks.
@@ -75,6 +83,29 @@ cudaError_t launch_pack_rows(const Matrix &from, size_t rows, size_t cols, void 
 bool tensor_products_available();
 
 #ifdef __CUDACC__
+// A kernel whose start-up overlaps the end of the one before it in the stream; before
+// it reads or writes anything it waits for that one (after_previous).
+__device__ __forceinline__ void after_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+template <typename... P, typename... A>
+cudaError_t launch_after(void (*kernel)(P...), unsigned grid, unsigned threads, size_t shared, unsigned cluster,
+                         cudaStream_t stream, const A &...args) {
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(grid);
+    config.blockDim = dim3(threads);
+    config.dynamicSmemBytes = shared;
+    config.stream = stream;
+    cudaLaunchAttribute attributes[2] = {};
+    attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attributes[0].val.programmaticStreamSerializationAllowed = 1;
+    attributes[1].id = cudaLaunchAttributeClusterDimension;
+    attributes[1].val.clusterDim.x = cluster;
+    attributes[1].val.clusterDim.y = attributes[1].val.clusterDim.z = 1;
+    config.attrs = attributes;
+    config.numAttrs = cluster > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&config, kernel, args...);
+}
+
 // What v loses to its rounding to T, itself to be rounded to T: together they hold
 // twice T's digits. (What T has no finite value for loses an infinity or NaN.)
 template <typename T>

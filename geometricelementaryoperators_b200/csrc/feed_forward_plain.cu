@@ -9,6 +9,38 @@ namespace layers {
 
 namespace {
 
+// What is done with the sums of one place of a product's result: gate and up (kGated), or one.
+template <typename T, typename O, int KIND>
+__device__ __forceinline__ void finish(const Product &p, int problem, size_t row, size_t col, Wide<T> v, Wide<T> other) {
+    using W = Wide<T>;
+    constexpr bool kFast = sizeof(T) == 2;
+    auto put = [&](const OutMatrix &out, W x) {
+        if (out.p != nullptr) ((T *)out.p)[row * out.stride + col] = narrow<T>(x);
+    };
+    if constexpr (KIND == kGated) {
+        put(p.out[0], v);
+        put(p.out[1], other);
+        put(p.out[2], activation<kFast>(p.activation, v, (W *)nullptr) * other);
+    } else if constexpr (KIND == kHidden) {
+        const W g = widen(((const T *)p.saved[0].p)[row * p.saved[0].stride + col]);
+        const W u = widen(((const T *)p.saved[1].p)[row * p.saved[1].stride + col]);
+        W slope;
+        const W f = activation<kFast>(p.activation, g, &slope);
+        auto put_two = [&](int n, W x) {
+            put(p.out[n], x);
+            if constexpr (sizeof(T) == 2) put(p.out_low[n], lost_to<T>(x));
+        };
+        put_two(0, v * u * slope);
+        put_two(1, v * f);
+        put_two(2, f * u);
+    } else if constexpr (KIND == kWeights) {
+        const OutMatrix &out = p.out[problem];
+        ((O *)out.p)[p.transposed[problem] ? col * out.stride + row : row * out.stride + col] = narrow<O>((Wide<O>)v);
+    } else {
+        put(p.out[0], v);
+    }
+}
+
 // ---- tiles in registers -----------------------------------------------------------
 
 // C = A B, 256 threads a tile, TM x TN sums a thread in groups of 16 bytes along
@@ -37,12 +69,14 @@ __global__ void __launch_bounds__(kTileThreads)
     __shared__ __align__(16) W sa[kBK * kPitchA], sb[kOperands][kBK * kPitchB];
     const int ty = threadIdx.x / kSide, tx = threadIdx.x % kSide;
     const int blocks_k = (p.k + kBK - 1) / kBK;
+    after_previous();
+    let_next_start();
 
     for (int index = blockIdx.x; index < tiles; index += gridDim.x) {
         const int part = index / (down * across), rest = index % (down * across);
-        const int problem = KIND == kWeights ? part / p.splits : 0, split = KIND == kWeights ? part % p.splits : 0;
-        const int first = (int)((long long)blocks_k * split / p.splits);
-        const int last = KIND == kInput ? 2 * blocks_k : (int)((long long)blocks_k * (split + 1) / p.splits);
+        const int problem = part / p.splits, split = part - problem * p.splits;
+        const int all = (KIND == kInput ? 2 : 1) * blocks_k;
+        const int first = (int)((long long)all * split / p.splits), last = (int)((long long)all * (split + 1) / p.splits);
         const int row0 = rest % down * BM, col0 = rest / down * BN;
         Pair<W> sum[kOperands][TM][TN / 2];
 #pragma unroll
@@ -133,37 +167,13 @@ __global__ void __launch_bounds__(kTileThreads)
                 const int col = col0 + j / V * kSide * V + tx * V + j % V;
                 if (col >= p.n) continue;
                 auto value = [&](int o) { return j & 1 ? sum[o][i][j / 2].y : sum[o][i][j / 2].x; };
-                auto put = [&](const OutMatrix &out, W v) {
-                    if (out.p != nullptr) ((T *)out.p)[(size_t)row * out.stride + col] = narrow<T>(v);
-                };
-                const W v = value(0);
-                if constexpr (KIND == kGated) {
-                    const W u = value(kOperands - 1);
-                    put(p.out[0], v);
-                    put(p.out[1], u);
-                    put(p.out[2], activation<sizeof(T) == 2>(p.activation, v, (W *)nullptr) * u);
-                } else if constexpr (KIND == kHidden) {
-                    const W g = widen(((const T *)p.saved[0].p)[(size_t)row * p.saved[0].stride + col]);
-                    const W u = widen(((const T *)p.saved[1].p)[(size_t)row * p.saved[1].stride + col]);
-                    W slope;
-                    const W f = activation<sizeof(T) == 2>(p.activation, g, &slope);
-                    auto put_two = [&](int n, W x) {
-                        put(p.out[n], x);
-                        if constexpr (sizeof(T) == 2) put(p.out_low[n], lost_to<T>(x));
-                    };
-                    put_two(0, v * u * slope);
-                    put_two(1, v * f);
-                    put_two(2, f * u);
-                } else if constexpr (KIND == kWeights) {
-                    const OutMatrix &out = p.out[problem];
-                    if (p.splits > 1)
-                        ((W *)p.partial)[((size_t)part * p.m + row) * (((size_t)p.n + 3) / 4 * 4) + col] = v;
-                    else if (p.transposed[problem])
-                        ((O *)out.p)[(size_t)col * out.stride + row] = narrow<O>((Wide<O>)v);
-                    else
-                        ((O *)out.p)[(size_t)row * out.stride + col] = narrow<O>((Wide<O>)v);
+                if (p.splits > 1) {
+                    const size_t stride = partial_stride(p.n), each = (size_t)p.splits * p.m * stride;
+                    W *to = (W *)p.partial + problem * each + ((size_t)split * p.m + row) * stride + col;
+#pragma unroll
+                    for (int o = 0; o < kOperands; ++o) to[o * each] = value(o);
                 } else {
-                    put(p.out[0], v);
+                    finish<T, O, KIND>(p, problem, row, col, value(0), value(kOperands - 1));
                 }
             }
         }
@@ -177,24 +187,46 @@ cudaError_t launch_tile(const Product &p, cudaStream_t stream) {
     const int down = (p.m + BM - 1) / BM, across = (p.n + BN - 1) / BN;
     const long long tiles = (long long)down * across * p.problems * p.splits;
     if (tiles > INT32_MAX) return cudaErrorInvalidValue;
-    tile_kernel<T, O, KIND><<<(unsigned)tiles, kTileThreads, 0, stream>>>(p, down, across, (int)tiles);
-    return cudaGetLastError();
+    return launch_after(tile_kernel<T, O, KIND>, (unsigned)tiles, kTileThreads, 0, 1, stream, p, down, across, (int)tiles);
 }
 
 // ---- parts of K -----------------------------------------------------------------------
 
-template <typename W, typename O>
-__global__ void __launch_bounds__(256) join_splits_kernel(const __grid_constant__ Product p, size_t stride) {
-    const size_t each = (size_t)p.m * p.n;
+// Adds the parts of K up, in order, four columns a thread, and does with the sums what
+// the kernel that made them does where K is whole.
+template <typename T, typename O, int KIND>
+__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Product p) {
+    using W = Wide<T>;
+    constexpr int kSums = KIND == kGated ? 2 : 1, V = 16 / (int)sizeof(W);
+    after_previous();
+    let_next_start();
+    const size_t stride = partial_stride(p.n), groups = stride / 4, each = (size_t)p.m * groups;
+    const size_t part = (size_t)p.m * stride;
     for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < each * p.problems; i += (size_t)gridDim.x * 256) {
         const int problem = (int)(i / each);
-        const size_t row = (i - problem * each) / p.n, col = (i - problem * each) % p.n;
-        const W *from = (const W *)p.partial + ((size_t)problem * p.splits * p.m + row) * stride + col;
-        W sum = 0;
-#pragma unroll 8
-        for (int s = 0; s < p.splits; ++s) sum += from[(size_t)s * p.m * stride];
-        const OutMatrix &out = p.out[problem];
-        ((O *)out.p)[p.transposed[problem] ? col * out.stride + row : row * out.stride + col] = narrow<O>((Wide<O>)sum);
+        const size_t row = (i - problem * each) / groups, col = (i - problem * each) % groups * 4;
+        W sum[kSums][4];
+#pragma unroll
+        for (int z = 0; z < kSums; ++z) {
+            const W *from = (const W *)p.partial + (size_t)(KIND == kWeights ? problem : z) * p.splits * part + row * stride + col;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) sum[z][j] = W(0);
+#pragma unroll 4
+            for (int s = 0; s < p.splits; ++s, from += part)
+#pragma unroll
+                for (int v = 0; v < 4 / V; ++v) {
+                    const Vec<W, V> piece = load<W, V>(from + v * V);
+#pragma unroll
+                    for (int q = 0; q < V / 2; ++q) {
+                        sum[z][v * V + 2 * q] += piece.pair(q).x;
+                        sum[z][v * V + 2 * q + 1] += piece.pair(q).y;
+                    }
+                }
+        }
+        const int held = (size_t)p.n - col < 4 ? (int)((size_t)p.n - col) : 4;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (j < held) finish<T, O, KIND>(p, problem, row, col + j, sum[0][j], sum[kSums - 1][j]);
     }
 }
 
@@ -214,6 +246,8 @@ __global__ void __launch_bounds__(kFewThreads) few_kernel(const __grid_constant_
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int part = warp % split, columns = kFewWarps / split;
     const int col = (int)blockIdx.x * columns + warp / split;
+    after_previous();
+    let_next_start();
     W sum[kOperands][ROWS];
 #pragma unroll
     for (int o = 0; o < kOperands; ++o)
@@ -300,11 +334,8 @@ cudaError_t launch_rows(const Product &p, cudaStream_t stream) {
     while (split < kFewWarps && (long long)p.n * split < wanted && p.k > split * 512) split *= 2;
     const int columns = kFewWarps / split;
     const unsigned grid = (unsigned)((p.n + columns - 1) / columns);
-    if (aligned)
-        few_kernel<T, KIND, ROWS, true><<<grid, kFewThreads, 0, stream>>>(p, split);
-    else
-        few_kernel<T, KIND, ROWS, false><<<grid, kFewThreads, 0, stream>>>(p, split);
-    return cudaGetLastError();
+    return aligned ? launch_after(few_kernel<T, KIND, ROWS, true>, grid, kFewThreads, 0, 1, stream, p, split)
+                   : launch_after(few_kernel<T, KIND, ROWS, false>, grid, kFewThreads, 0, 1, stream, p, split);
 }
 
 template <typename T, int KIND>
@@ -319,6 +350,8 @@ cudaError_t launch_few(const Product &p, cudaStream_t stream) {
 
 __global__ void __launch_bounds__(256) pack_kernel(Matrix from, size_t rows, int cols, void *to, size_t to_stride) {
     const size_t pieces = to_stride / 8, n = rows * pieces;
+    after_previous();
+    let_next_start();
     for (size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (size_t)gridDim.x * blockDim.x) {
         const size_t row = i / pieces;
         const int col = (int)(i - row * pieces) * 8;
@@ -335,37 +368,45 @@ __global__ void __launch_bounds__(256) pack_kernel(Matrix from, size_t rows, int
 
 }  // namespace
 
-int weight_splits(size_t m, size_t n, size_t k, int tile_m, int tile_n, size_t least) {
-    const size_t tiles = 3 * ((m + tile_m - 1) / tile_m) * ((n + tile_n - 1) / tile_n), sms = geo::device_sm_count();
-    const size_t wanted = sms / tiles, most = k / least;
+// As many parts as give every multiprocessor a tile, none under 128 of K.
+Cut cut_plain(ProductKind kind, uint32_t type, size_t m, size_t n, size_t k) {
+    const bool gated = kind == kGated;
+    const size_t high = kSide * (type == GEO_B200_F64 ? (gated ? rows_of_thread<double, kGated>() : rows_of_thread<double, kDown>())
+                                                      : rows_of_thread<float, kDown>());
+    const size_t wide = kSide * (type == GEO_B200_F64 ? columns_of_thread<double, kDown>()
+                                                      : (gated ? columns_of_thread<float, kGated>() : columns_of_thread<float, kDown>()));
+    const size_t tiles = (kind == kWeights ? 3 : 1) * ((m + high - 1) / high) * ((n + wide - 1) / wide);
+    const size_t wanted = (size_t)geo::device_sm_count() / tiles, most = k * (kind == kInput ? 2 : 1) / 128;
     const size_t splits = wanted < most ? wanted : most;
-    return splits < 1 ? 1 : (splits < (size_t)kSplitMost ? (int)splits : kSplitMost);
-}
-int weight_splits_plain(uint32_t type, size_t m, size_t n, size_t k) {
-    return type == GEO_B200_F64 ? weight_splits(m, n, k, kSide * rows_of_thread<double, kWeights>(),
-                                                kSide * columns_of_thread<double, kWeights>(), 128)
-                                : weight_splits(m, n, k, kSide * rows_of_thread<float, kWeights>(),
-                                                kSide * columns_of_thread<float, kWeights>(), 128);
+    return {(int)wide, false, splits < 1 ? 1 : (splits < 64 ? (int)splits : 64)};
 }
 
-cudaError_t launch_join_splits(uint32_t type, uint32_t out_type, const Product &p, cudaStream_t stream) {
-    const size_t n = (size_t)p.m * p.n * p.problems, blocks = (n + 255) / 256, most = (size_t)geo::device_sm_count() * 8;
-    const unsigned grid = (unsigned)(blocks < most ? blocks : most);
-    return by_type(type, [&](auto t) {
+template <typename T, typename O, int KIND>
+cudaError_t launch_join_kind(const Product &p, cudaStream_t stream) {
+    const size_t n = (size_t)p.m * (partial_stride(p.n) / 4) * p.problems, blocks = (n + 255) / 256;
+    const size_t most = (size_t)geo::device_sm_count() * 8;
+    return launch_after(join_kernel<T, O, KIND>, (unsigned)(blocks < most ? blocks : most), 256, 0, 1, stream, p);
+}
+cudaError_t launch_join(ProductKind kind, uint32_t type, uint32_t out_type, const Product &p, cudaStream_t stream) {
+    return by_type(type, [&](auto t) -> cudaError_t {
         using T = decltype(t);
-        using W = Wide<T>;
-        const size_t stride = partial_stride(p.n);
-        if (sizeof(T) == 2 && out_type == GEO_B200_F32)
-            join_splits_kernel<W, W><<<grid, 256, 0, stream>>>(p, stride);
-        else
-            join_splits_kernel<W, T><<<grid, 256, 0, stream>>>(p, stride);
-        return cudaGetLastError();
+        switch (kind) {
+            case kGated: return launch_join_kind<T, T, kGated>(p, stream);
+            case kDown: return launch_join_kind<T, T, kDown>(p, stream);
+            case kHidden: return launch_join_kind<T, T, kHidden>(p, stream);
+            case kInput: return launch_join_kind<T, T, kInput>(p, stream);
+            default: break;
+        }
+        if constexpr (sizeof(T) == 2) {
+            if (out_type == GEO_B200_F32) return launch_join_kind<T, float, kWeights>(p, stream);
+        }
+        return launch_join_kind<T, T, kWeights>(p, stream);
     });
 }
 
 cudaError_t launch_product_plain(ProductKind kind, uint32_t type, uint32_t out_type, const Product &p,
                                  cudaStream_t stream) {
-    return by_type(type, [&](auto t) -> cudaError_t {
+    const cudaError_t e = by_type(type, [&](auto t) -> cudaError_t {
         using T = decltype(t);
         switch (kind) {
             case kGated: return launch_tile<T, T, kGated>(p, stream);
@@ -374,13 +415,12 @@ cudaError_t launch_product_plain(ProductKind kind, uint32_t type, uint32_t out_t
             case kInput: return launch_tile<T, T, kInput>(p, stream);
             default: break;
         }
-        cudaError_t e;
-        if constexpr (sizeof(T) == 2)
-            e = out_type == GEO_B200_F32 ? launch_tile<T, float, kWeights>(p, stream) : launch_tile<T, T, kWeights>(p, stream);
-        else
-            e = launch_tile<T, T, kWeights>(p, stream);
-        return e != cudaSuccess || p.splits == 1 ? e : launch_join_splits(type, out_type, p, stream);
+        if constexpr (sizeof(T) == 2) {
+            if (out_type == GEO_B200_F32) return launch_tile<T, float, kWeights>(p, stream);
+        }
+        return launch_tile<T, T, kWeights>(p, stream);
     });
+    return e != cudaSuccess || p.splits == 1 ? e : launch_join(kind, type, out_type, p, stream);
 }
 
 cudaError_t launch_product_few(ProductKind kind, uint32_t type, const Product &p, cudaStream_t stream) {
@@ -393,8 +433,8 @@ cudaError_t launch_product_few(ProductKind kind, uint32_t type, const Product &p
 cudaError_t launch_pack_rows(const Matrix &from, size_t rows, size_t cols, void *to, size_t to_stride,
                              cudaStream_t stream) {
     const size_t n = rows * (to_stride / 8), blocks = (n + 255) / 256, most = (size_t)geo::device_sm_count() * 32;
-    pack_kernel<<<(unsigned)(blocks < most ? blocks : most), 256, 0, stream>>>(from, rows, (int)cols, to, to_stride);
-    return cudaGetLastError();
+    return launch_after(pack_kernel, (unsigned)(blocks < most ? blocks : most), 256, 0, 1, stream, from, rows, (int)cols,
+                        to, to_stride);
 }
 
 }  // namespace layers

@@ -61,6 +61,9 @@ constexpr uint32_t shared_bytes(int kind, int bn, bool twice, bool pair) {
            epilogue_warps(kind, twice) * staging_of(kind);
 }
 
+// Rows of a box of A [M][K].
+__host__ __device__ constexpr int box_rows(int m) { return m < kBM ? (m + 7) / 8 * 8 : kBM; }
+
 struct Maps {
     CUtensorMap a[3], b[3], low[3];
 };
@@ -177,8 +180,6 @@ __device__ __forceinline__ void take_columns(uint32_t address, float (&v)[32]) {
 #pragma unroll
     for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
-
-__device__ __forceinline__ size_t partial_width(int n) { return ((size_t)n + 3) / 4 * 4; }
 
 // Whether rows of this array can be read and written by 16 bytes.
 template <typename T>
@@ -355,15 +356,17 @@ __global__ void __launch_bounds__(64 + 32 * epilogue_warps(KIND, TWICE), 1)
     everyone();
     const uint32_t sums = sums_address;
     const int blocks_k = (p.k + kBK - 1) / kBK;
-    // A tile's blocks of K: kInput goes through K twice, kWeights' splits each through a part.
-    auto first_of = [&](const Tile &t) { return KIND == kWeights ? (int)((long long)blocks_k * t.split / p.splits) : 0; };
-    auto last_of = [&](const Tile &t) {
-        return KIND == kWeights ? (int)((long long)blocks_k * (t.split + 1) / p.splits)
-                                : (KIND == kInput ? 2 : 1) * blocks_k;
-    };
+    // A tile's blocks of K: all of them (kInput: once for each pair of operands), or its split's part.
+    const int all = (KIND == kInput ? 2 : 1) * blocks_k;
+    auto first_of = [&](const Tile &t) { return (int)((long long)all * t.split / p.splits); };
+    auto last_of = [&](const Tile &t) { return (int)((long long)all * (t.split + 1) / p.splits); };
+    after_previous();
+    let_next_start();
 
     if (warp == 0 && lane == 0) {
         uint32_t step = 0;  // of all tiles, one after another
+        // The box of A is no higher than A (its other rows are multiplied as they lie, for rows that do not exist).
+        const uint32_t skipped = kAMn || PAIR ? 0 : kBytesA - box_rows(p.m) * kBK * 2;
         bool good = true;
         for (int index = team; index < tiles && good; index += teams) {
             const Tile t = tile_of(index, down, across, p.splits);
@@ -376,7 +379,7 @@ __global__ void __launch_bounds__(64 + 32 * epilogue_warps(KIND, TWICE), 1)
                 }
                 const uint32_t to = base + s * kStageBytes;
                 const uint32_t barrier = PAIR ? barrier_of(full + 8 * s, 0) : full + 8 * s;
-                if (rank == 0) barrier_expect(full + 8 * s, (PAIR ? 2 : 1) * kStageBytes);
+                if (rank == 0) barrier_expect(full + 8 * s, (PAIR ? 2 : 1) * (kStageBytes - skipped));
                 const int second = KIND == kInput && i >= blocks_k ? 1 : 0, k = (i - second * blocks_k) * kBK;
                 const int row0 = (PAIR ? t.row * 2 + rank : t.row) * kBM;
                 // This block's rows of B.
@@ -490,17 +493,14 @@ __global__ void __launch_bounds__(64 + 32 * epilogue_warps(KIND, TWICE), 1)
                     for (int j = 0; j < 32; ++j) v[j] = __int_as_float(0x7FC00000);
                 }
             };
+            // 32 columns of sum `which` of a part of K.
+            auto put_partial = [&](const auto &v, int from, int which, int col0) {
+                const size_t stride = partial_stride(p.n), part = (size_t)which * p.splits + t.split;
+                put_columns<float>(mine, v, from, {(float *)p.partial + part * p.m * stride, stride}, row0, col0, p.m, p.n);
+            };
             // 32 columns of a result of kWeights, kDown, kInput.
             auto put = [&](const auto &v, int from, int col0) {
                 if constexpr (KIND == kWeights) {
-                    if (p.splits > 1) {
-                        if constexpr (sizeof(O) == 4) {
-                            const size_t stride = partial_width(p.n), part = t.problem * p.splits + t.split;
-                            put_columns<O>(mine, v, from, {(O *)p.partial + part * p.m * stride, stride}, row0, col0, p.m,
-                                           p.n);
-                        }
-                        return;
-                    }
                     if (p.transposed[t.problem]) {
                         // A column of the tile is a row of the result: lanes are neighbours there.
                         const OutMatrix &out = p.out[t.problem];
@@ -533,7 +533,11 @@ __global__ void __launch_bounds__(64 + 32 * epilogue_warps(KIND, TWICE), 1)
 #pragma unroll
                     for (int c = 0; c < kPart; c += 32) {
                         const int col0 = t.column * kColumns + begin + c;
-                        if (col0 < p.n) put(sum, c, col0);
+                        if (col0 >= p.n) continue;
+                        if (p.splits > 1)
+                            put_partial(sum, c, t.problem, col0);
+                        else
+                            put(sum, c, col0);
                     }
                 }
             } else {
@@ -543,7 +547,8 @@ __global__ void __launch_bounds__(64 + 32 * epilogue_warps(KIND, TWICE), 1)
                     fetch_columns<T>(mine + 2 * kRows, p.saved[1], row0, col0, p.m, p.n);
                     commit_async();
                 };
-                if constexpr (KIND == kHidden) fetch(begin);
+                if constexpr (KIND == kHidden)
+                    if (p.splits == 1) fetch(begin);
                 wait();
                 if (row0 < p.m) {
 #pragma unroll 1
@@ -552,6 +557,14 @@ __global__ void __launch_bounds__(64 + 32 * epilogue_warps(KIND, TWICE), 1)
                         if (col0 >= p.n) break;
                         float v[32];
                         take(c, v);
+                        if (p.splits > 1) {
+                            put_partial(v, 0, KIND == kWeights ? t.problem : 0, col0);
+                            if constexpr (KIND == kGated) {
+                                take(kColumns + c, v);
+                                put_partial(v, 0, 1, col0);
+                            }
+                            continue;
+                        }
                         if constexpr (KIND == kGated) {
                             if (p.out[0].p != nullptr) put_columns<T>(mine, v, 0, p.out[0], row0, col0, p.m, p.n);
                             float u[32];
@@ -661,7 +674,7 @@ cudaError_t launch_tiles(const Product &p, PipelineStarve starve, cudaStream_t s
     bool good = true;
     for (int i = 0; i < pairs_a; ++i) {
         good = good && (kAMn ? encode(&maps.a[i], kBfloat, p.a[i], p.k, p.m, kBK)
-                             : encode(&maps.a[i], kBfloat, p.a[i], p.m, p.k, kBM));
+                             : encode(&maps.a[i], kBfloat, p.a[i], p.m, p.k, PAIR ? kBM : box_rows(p.m)));
         if (TWICE) good = good && encode(&maps.low[i], kBfloat, p.low[i], p.k, p.m, kBK);
     }
     for (int i = 0; i < pairs_b; ++i)
@@ -675,82 +688,93 @@ cudaError_t launch_tiles(const Product &p, PipelineStarve starve, cudaStream_t s
     const auto kernel = product_kernel<T, O, TWICE, KIND, BN, PAIR>;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kShared);
     if (e != cudaSuccess) return e;
-    cudaLaunchConfig_t config = {};
-    config.blockDim = dim3(kThreads);
-    config.dynamicSmemBytes = kShared;
-    config.stream = stream;
-    cudaLaunchAttribute attribute = {};
-    attribute.id = cudaLaunchAttributeClusterDimension;
-    attribute.val.clusterDim.x = 2;
-    attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
-    config.attrs = &attribute;
-    config.numAttrs = PAIR ? 1 : 0;
     int most = geo::device_sm_count() / (PAIR ? 2 : 1);
     if constexpr (PAIR) {  // a pair needs two multiprocessors side by side
+        cudaLaunchConfig_t config = {};
         config.gridDim = dim3((unsigned)(2 * most));
+        config.blockDim = dim3(kThreads);
+        config.dynamicSmemBytes = kShared;
+        cudaLaunchAttribute attribute = {};
+        attribute.id = cudaLaunchAttributeClusterDimension;
+        attribute.val.clusterDim.x = 2;
+        attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
+        config.attrs = &attribute;
+        config.numAttrs = 1;
         int resident = 0;
         e = cudaOccupancyMaxActiveClusters(&resident, kernel, &config);
         if (e != cudaSuccess) return e;
         if (resident > 0 && resident < most) most = resident;
     }
-    config.gridDim = dim3((unsigned)((tiles < most ? tiles : most) * (PAIR ? 2 : 1)));
-    return cudaLaunchKernelEx(&config, kernel, maps, p, down, across, (int)tiles, starve);
+    return launch_after(kernel, (unsigned)((tiles < most ? tiles : most) * (PAIR ? 2 : 1)), kThreads, kShared,
+                        PAIR ? 2 : 1, stream, maps, p, down, across, (int)tiles, starve);
 }
 
-// The widest tile that still gives every multiprocessor about one: wide tiles move
-// fewer bytes a multiplication, narrow ones share few tiles more evenly.
 template <typename T, typename O, bool TWICE, int KIND>
-cudaError_t launch_kind(const Product &p, PipelineStarve starve, cudaStream_t stream) {
-    const long long down = (p.m + kBM - 1) / kBM, sms = geo::device_sm_count();
-    auto waves_cost = [&](int bn) {
-        const int columns = KIND == kGated ? bn / 2 : bn;
-        const long long tiles = down * ((p.n + columns - 1) / columns) * p.problems * p.splits;
-        return (tiles + sms - 1) / sms * (bn + 32);
-    };
-    const int columns = KIND == kGated ? 128 : 256;
-    const long long pair_tiles = (down + 1) / 2 * ((p.n + columns - 1) / columns) * p.problems * p.splits;
-    constexpr int kLeast = KIND == kDown ? 32 : 64;  // a tile of kGated is half as wide, rows of boxes are 64
-    int best = 256;
-    for (int bn = 128; bn >= kLeast; bn /= 2)
-        if (waves_cost(bn) < waves_cost(best)) best = bn;
-    if (best == 256 && pair_tiles >= sms / 2) return launch_tiles<T, O, TWICE, KIND, 256, true>(p, starve, stream);
-    switch (best) {
+cudaError_t launch_kind(const Cut &cut, const Product &p, PipelineStarve starve, cudaStream_t stream) {
+    if (cut.pair) return launch_tiles<T, O, TWICE, KIND, 256, true>(p, starve, stream);
+    switch (cut.columns) {
         case 256: return launch_tiles<T, O, TWICE, KIND, 256, false>(p, starve, stream);
         case 128: return launch_tiles<T, O, TWICE, KIND, 128, false>(p, starve, stream);
-        case 64: return launch_tiles<T, O, TWICE, KIND, 64, false>(p, starve, stream);
-        default:
-            if constexpr (kLeast == 32) return launch_tiles<T, O, TWICE, KIND, 32, false>(p, starve, stream);
-            return cudaErrorInvalidValue;
+        default: return launch_tiles<T, O, TWICE, KIND, 64, false>(p, starve, stream);
     }
 }
 
 template <typename T>
 cudaError_t launch_type(ProductKind kind, uint32_t type, uint32_t out_type, const Product &p, PipelineStarve starve,
                         cudaStream_t stream) {
-    switch (kind) {
-        case kGated: return launch_kind<T, T, false, kGated>(p, starve, stream);
-        case kDown: return launch_kind<T, T, false, kDown>(p, starve, stream);
-        case kHidden:
-            return out_type == GEO_B200_F32 ? launch_kind<T, float, false, kHidden>(p, starve, stream)
-                                            : launch_kind<T, T, false, kHidden>(p, starve, stream);
-        case kInput: return launch_kind<T, T, false, kInput>(p, starve, stream);
-        default: break;
-    }
+    const bool to_float = out_type == GEO_B200_F32;
+    const Cut cut = cut_tensor(kind, kind == kWeights && to_float, p.m, p.n, p.k);
     cudaError_t e;
-    if (out_type == GEO_B200_F32)
-        e = launch_kind<T, float, true, kWeights>(p, starve, stream);
-    else if (p.splits > 1)
-        e = launch_kind<T, float, false, kWeights>(p, starve, stream);
-    else
-        e = launch_kind<T, T, false, kWeights>(p, starve, stream);
-    return e != cudaSuccess || p.splits == 1 ? e : launch_join_splits(type, out_type, p, stream);
+    switch (kind) {
+        case kGated: e = launch_kind<T, T, false, kGated>(cut, p, starve, stream); break;
+        case kDown: e = launch_kind<T, T, false, kDown>(cut, p, starve, stream); break;
+        case kHidden:
+            e = to_float ? launch_kind<T, float, false, kHidden>(cut, p, starve, stream)
+                         : launch_kind<T, T, false, kHidden>(cut, p, starve, stream);
+            break;
+        case kInput: e = launch_kind<T, T, false, kInput>(cut, p, starve, stream); break;
+        default:
+            e = to_float ? launch_kind<T, float, true, kWeights>(cut, p, starve, stream)
+                         : launch_kind<T, T, false, kWeights>(cut, p, starve, stream);
+            break;
+    }
+    return e != cudaSuccess || p.splits == 1 ? e : launch_join(kind, type, out_type, p, stream);
 }
 
 }  // namespace
 
 bool tensor_products_available() { return map_encoder() != nullptr; }
 
-int weight_splits_tensor(size_t m, size_t n, size_t k) { return weight_splits(m, n, k, kBM, 128, 8 * kBK); }
+// The cheapest by an estimate in cycles. A block of K costs what its matrix
+// instructions take (4096 multiply-adds a cycle) or its copies (2 cycles and a bit for
+// each row of 128 bytes: 600 cycles measured for 128 + 32 rows, 700 for 128 + 128, 670
+// for a pair's 128 + 128), whichever is more; parts of K cost the way of their sums
+// through L2 and one more launch.
+Cut cut_tensor(ProductKind kind, bool twice, size_t m, size_t n, size_t k) {
+    const long long sms = geo::device_sm_count(), problems = kind == kWeights ? 3 : 1;
+    const long long blocks = (long long)((k + kBK - 1) / kBK) * (kind == kInput ? 2 : 1);
+    const long long rows_a = kind == kWeights ? kBM : box_rows((int)(m < (size_t)kBM ? m : kBM));
+    Cut best = {256, false, 1};
+    double least = -1;
+    auto look = [&](int bn, bool pair) {
+        const long long columns = kind == kGated ? bn / 2 : bn, high = pair ? 2 * kBM : kBM;
+        const long long tiles = (long long)((m + high - 1) / high) * ((n + columns - 1) / columns) * problems;
+        const long long teams = pair ? sms / 2 : sms, terms = twice ? 2 : 1;
+        const double copies = 2.1 * (terms * rows_a + (pair ? bn / 2 : bn)) + 150, products = 2.0 * bn * terms;
+        const double block = copies > products ? copies : products;
+        for (long long splits = 1; splits <= 16 && splits * 4 <= (blocks > 4 ? blocks : 4); ++splits) {
+            const long long waves = (tiles * splits + teams - 1) / teams;
+            const double sums = (double)sums_of(kind, 3) * splits * m * n * 4;
+            if (splits > 1 && (waves > 1 || sums > (64 << 20))) break;
+            const double cost = waves * ((blocks + splits - 1) / splits * block + 800) + 4000 +
+                                (splits > 1 ? 5000 + sums / 2500 : 0);
+            if (least < 0 || cost < 0.98 * least) least = cost, best = {bn, pair, (int)splits};
+        }
+    };
+    if (m > (size_t)kBM) look(256, true);
+    for (int bn = 256; bn >= 64; bn /= 2) look(bn, false);
+    return best;
+}
 
 cudaError_t launch_product_tensor(ProductKind kind, uint32_t type, uint32_t out_type, const Product &p,
                                   PipelineStarve starve, cudaStream_t stream) {
