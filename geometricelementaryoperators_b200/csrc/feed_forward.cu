@@ -56,13 +56,31 @@ size_t partial_bytes(const geo_b200_feed_forward_config_t &c, std::initializer_l
     const size_t wide = wide_bytes(c.type);
     size_t most = 0;
     for (const Extent &x : products) {
-        most = std::max(most, partial_values(x.kind, cut_plain(x.kind, c.type, x.m, x.n, x.k).splits, x.m, x.n));
         if (type_bytes(c.type) == 2) {
             const bool twice = x.kind == kWeights && c.gradient_type != c.type;
             most = std::max(most, partial_values(x.kind, cut_tensor(x.kind, twice, x.m, x.n, x.k).splits, x.m, x.n));
+            most = std::max(most, partial_values(x.kind, cut_plain(x.kind, x.m, x.n, x.k).splits, x.m, x.n));
+        } else {
+            most = std::max(most, partial_values(x.kind, cut_wide(x.kind, c.type, x.m, x.n, x.k).splits, x.m, x.n));
         }
     }
     return most * wide;
+}
+
+// Launches a product by the kernels that take it; `rest`: room for parts of its sums.
+cudaError_t launch_product(const geo_b200_feed_forward_config_t &c, bool tensor, ProductKind kind, Product &p, void *rest,
+                           cudaStream_t stream) {
+    p.partial = rest;
+    if (type_bytes(c.type) != 2) {
+        p.splits = cut_wide(kind, c.type, p.m, p.n, p.k).splits;
+        return launch_product_wide(kind, c.type, p, stream);
+    }
+    if (tensor) {
+        p.splits = cut_tensor(kind, kind == kWeights && c.gradient_type != c.type, p.m, p.n, p.k).splits;
+        return launch_product_tensor(kind, c.type, c.gradient_type, p, {UINT32_MAX, kPipelinePolls}, stream);
+    }
+    p.splits = cut_plain(kind, p.m, p.n, p.k).splits;
+    return launch_product_plain(kind, c.type, c.gradient_type, p, stream);
 }
 
 // Where things lie in the workspace. `take` returns the place of rows x stride values.
@@ -201,11 +219,7 @@ extern "C" geo_b200_status_t geo_b200_feed_forward(const geo_b200_feed_forward_c
     down.out[0] = {device_y, c.y_stride};
     void *const rest = space.take(0, 0, 1);
     auto launch = [&](ProductKind kind, Product &p) {
-        if (few) return launch_product_few(kind, c.type, p, stream);
-        p.splits = (tensor ? cut_tensor(kind, false, p.m, p.n, p.k) : cut_plain(kind, c.type, p.m, p.n, p.k)).splits;
-        p.partial = rest;
-        return tensor ? launch_product_tensor(kind, c.type, c.type, p, {UINT32_MAX, kPipelinePolls}, stream)
-                      : launch_product_plain(kind, c.type, c.type, p, stream);
+        return few ? launch_product_few(kind, c.type, p, stream) : launch_product(c, tensor, kind, p, rest, stream);
     };
     const cudaError_t e = launch(kGated, gated);
     return status_of(e != cudaSuccess ? e : launch(kDown, down));
@@ -255,13 +269,7 @@ extern "C" geo_b200_status_t geo_b200_feed_forward_vjp(
             if (e != cudaSuccess) return status_of(e);
         }
     void *const rest = space.take(0, 0, 1);
-    auto launch = [&](ProductKind kind, Product &p) {
-        const bool twice = kind == kWeights && c.gradient_type != c.type;
-        p.splits = (tensor ? cut_tensor(kind, twice, p.m, p.n, p.k) : cut_plain(kind, c.type, p.m, p.n, p.k)).splits;
-        p.partial = rest;
-        return tensor ? launch_product_tensor(kind, c.type, c.gradient_type, p, {UINT32_MAX, kPipelinePolls}, stream)
-                      : launch_product_plain(kind, c.type, c.gradient_type, p, stream);
-    };
+    auto launch = [&](ProductKind kind, Product &p) { return launch_product(c, tensor, kind, p, rest, stream); };
     Product hidden = {};
     hidden.m = (int)c.rows, hidden.n = (int)c.hidden, hidden.k = (int)c.cols, hidden.problems = 1;
     hidden.activation = (int)c.activation;

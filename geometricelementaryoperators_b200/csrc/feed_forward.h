@@ -1,6 +1,7 @@
 // feed_forward.h -- what the gated feed-forward block's entry points
-// (feed_forward.cu) and products (feed_forward_tensor.cu: 16-bit types on the
-// tensor cores; feed_forward_plain.cu: the others, and few rows) share.
+// (feed_forward.cu) and products (feed_forward_tensor.cu: 16-bit types on the tensor
+// cores; feed_forward_wide.cu: float32 and float64; feed_forward_plain.cu: few rows, and
+// 16-bit arrays that the tensor cores cannot be given) share.
 #pragma once
 
 #include "layers.h"
@@ -45,15 +46,15 @@ __host__ __device__ inline size_t partial_stride(size_t n) { return (n + 3) / 4 
 constexpr int sums_of(ProductKind kind, int problems) { return kind == kGated ? 2 : (kind == kWeights ? problems : 1); }
 
 // How a product is cut into tiles, and K into parts: by its sizes and the
-// multiprocessors alone, for the kernels that take it (`tensor`, or else the plain
-// ones). Counts all three results of kWeights, whichever are asked for.
+// multiprocessors alone, for the kernels that take it. Counts all three results of kWeights, whichever are asked for.
 struct Cut {
     int columns;  // of a tile of sums
     bool pair;    // two blocks a tile
     int splits;
 };
 Cut cut_tensor(ProductKind kind, bool twice, size_t m, size_t n, size_t k);
-Cut cut_plain(ProductKind kind, uint32_t type, size_t m, size_t n, size_t k);
+Cut cut_wide(ProductKind kind, uint32_t type, size_t m, size_t n, size_t k);
+Cut cut_plain(ProductKind kind, size_t m, size_t n, size_t k);
 // Values of `partial`.
 inline size_t partial_values(ProductKind kind, int splits, size_t m, size_t n) {
     return splits > 1 ? (size_t)sums_of(kind, 3) * splits * m * partial_stride(n) : 0;
@@ -71,6 +72,7 @@ constexpr uint32_t kPipelinePolls = 1u << 20;  // seconds, where a stage takes m
 // `type`: of the operands; `out_type`: of kWeights' results. A stream-ordered launch.
 cudaError_t launch_product_tensor(ProductKind kind, uint32_t type, uint32_t out_type, const Product &p,
                                   PipelineStarve starve, cudaStream_t stream);
+cudaError_t launch_product_wide(ProductKind kind, uint32_t type, const Product &p, cudaStream_t stream);
 cudaError_t launch_product_plain(ProductKind kind, uint32_t type, uint32_t out_type, const Product &p,
                                  cudaStream_t stream);
 // kGated, kDown with at most kFewRows rows.
@@ -151,6 +153,38 @@ __device__ __forceinline__ void by_activation(int kind, F &&f) {
         case GEO_B200_ACTIVATION_GELU: f(integral_constant<int, GEO_B200_ACTIVATION_GELU>{}); break;
         case GEO_B200_ACTIVATION_SIGMOID: f(integral_constant<int, GEO_B200_ACTIVATION_SIGMOID>{}); break;
         default: f(integral_constant<int, GEO_B200_ACTIVATION_RELU>{}); break;
+    }
+}
+
+// What is done with the sums of one place of a product's result: gate and up (kGated), or one.
+template <typename T, typename O, int KIND>
+__device__ __forceinline__ void finish(const Product &p, int problem, size_t row, size_t col, Wide<T> v, Wide<T> other) {
+    using W = Wide<T>;
+    constexpr bool kFast = sizeof(T) == 2;
+    auto put = [&](const OutMatrix &out, W x) {
+        if (out.p != nullptr) ((T *)out.p)[row * out.stride + col] = narrow<T>(x);
+    };
+    if constexpr (KIND == kGated) {
+        put(p.out[0], v);
+        put(p.out[1], other);
+        put(p.out[2], activation<kFast>(p.activation, v, (W *)nullptr) * other);
+    } else if constexpr (KIND == kHidden) {
+        const W g = widen(((const T *)p.saved[0].p)[row * p.saved[0].stride + col]);
+        const W u = widen(((const T *)p.saved[1].p)[row * p.saved[1].stride + col]);
+        W slope;
+        const W f = activation<kFast>(p.activation, g, &slope);
+        auto put_two = [&](int n, W x) {
+            put(p.out[n], x);
+            if constexpr (sizeof(T) == 2) put(p.out_low[n], lost_to<T>(x));
+        };
+        put_two(0, v * u * slope);
+        put_two(1, v * f);
+        put_two(2, f * u);
+    } else if constexpr (KIND == kWeights) {
+        const OutMatrix &out = p.out[problem];
+        ((O *)out.p)[p.transposed[problem] ? col * out.stride + row : row * out.stride + col] = narrow<O>((Wide<O>)v);
+    } else {
+        put(p.out[0], v);
     }
 }
 #endif

@@ -1,6 +1,7 @@
-// feed_forward_plain.cu -- the feed-forward block's products that the tensor-core
-// kernels do not take (geo/geo_b200.h section 5): float32 and float64, 16-bit arrays
-// that do not start on 16 bytes, and few rows of any type.
+// feed_forward_plain.cu -- the feed-forward block's products that the other kernels do
+// not take (geo/geo_b200.h section 5): few rows of any type, and 16-bit arrays that do
+// not start on 16 bytes; the joining of sums over parts of K; copies of 16-bit rows to
+// where the tensor cores' copies can start.
 #include "feed_forward.h"
 #include "geo_runtime.h"
 
@@ -9,52 +10,20 @@ namespace layers {
 
 namespace {
 
-// What is done with the sums of one place of a product's result: gate and up (kGated), or one.
-template <typename T, typename O, int KIND>
-__device__ __forceinline__ void finish(const Product &p, int problem, size_t row, size_t col, Wide<T> v, Wide<T> other) {
-    using W = Wide<T>;
-    constexpr bool kFast = sizeof(T) == 2;
-    auto put = [&](const OutMatrix &out, W x) {
-        if (out.p != nullptr) ((T *)out.p)[row * out.stride + col] = narrow<T>(x);
-    };
-    if constexpr (KIND == kGated) {
-        put(p.out[0], v);
-        put(p.out[1], other);
-        put(p.out[2], activation<kFast>(p.activation, v, (W *)nullptr) * other);
-    } else if constexpr (KIND == kHidden) {
-        const W g = widen(((const T *)p.saved[0].p)[row * p.saved[0].stride + col]);
-        const W u = widen(((const T *)p.saved[1].p)[row * p.saved[1].stride + col]);
-        W slope;
-        const W f = activation<kFast>(p.activation, g, &slope);
-        auto put_two = [&](int n, W x) {
-            put(p.out[n], x);
-            if constexpr (sizeof(T) == 2) put(p.out_low[n], lost_to<T>(x));
-        };
-        put_two(0, v * u * slope);
-        put_two(1, v * f);
-        put_two(2, f * u);
-    } else if constexpr (KIND == kWeights) {
-        const OutMatrix &out = p.out[problem];
-        ((O *)out.p)[p.transposed[problem] ? col * out.stride + row : row * out.stride + col] = narrow<O>((Wide<O>)v);
-    } else {
-        put(p.out[0], v);
-    }
-}
-
 // ---- tiles in registers -----------------------------------------------------------
 
-// C = A B, 256 threads a tile, TM x TN sums a thread in groups of 16 bytes along
-// each side; 16 of K at a time through shared memory, the next 16 on their way in
-// registers meanwhile. Multiply-adds bound it: float32 on the packed two-wide units.
+// For 16-bit arrays of any alignment, value by value and simple: C = A B, 256 threads a
+// tile, TM x TN float32 sums a thread in groups of 16 bytes along each side; 16 of K at a
+// time through shared memory, the next 16 on their way in registers meanwhile.
 constexpr int kSide = 16, kBK = 16, kTileThreads = kSide * kSide;
 
-template <typename W, int KIND>
+template <int KIND>
 constexpr int rows_of_thread() {
-    return sizeof(W) == 8 && KIND == kGated ? 4 : 8;
+    return 8;
 }
-template <typename W, int KIND>
+template <int KIND>
 constexpr int columns_of_thread() {
-    return sizeof(W) == 8 || KIND == kGated ? 4 : 8;
+    return KIND == kGated ? 4 : 8;
 }
 
 template <typename T, typename O, int KIND>
@@ -62,7 +31,7 @@ __global__ void __launch_bounds__(kTileThreads)
     tile_kernel(const __grid_constant__ Product p, int down, int across, int tiles) {
     using W = Wide<T>;
     constexpr bool kAMn = KIND == kWeights, kBMn = KIND == kHidden || KIND == kInput || KIND == kWeights;
-    constexpr int TM = rows_of_thread<W, KIND>(), TN = columns_of_thread<W, KIND>(), V = 16 / (int)sizeof(W);
+    constexpr int TM = rows_of_thread<KIND>(), TN = columns_of_thread<KIND>(), V = 16 / (int)sizeof(W);
     constexpr int BM = kSide * TM, BN = kSide * TN, kOperands = KIND == kGated ? 2 : 1;
     constexpr int kLoadA = BM * kBK / kTileThreads, kLoadB = BN * kBK / kTileThreads;
     constexpr int kPitchA = BM + V, kPitchB = BN + V;
@@ -183,7 +152,7 @@ __global__ void __launch_bounds__(kTileThreads)
 template <typename T, typename O, int KIND>
 cudaError_t launch_tile(const Product &p, cudaStream_t stream) {
     using W = Wide<T>;
-    constexpr int BM = kSide * rows_of_thread<W, KIND>(), BN = kSide * columns_of_thread<W, KIND>();
+    constexpr int BM = kSide * rows_of_thread<KIND>(), BN = kSide * columns_of_thread<KIND>();
     const int down = (p.m + BM - 1) / BM, across = (p.n + BN - 1) / BN;
     const long long tiles = (long long)down * across * p.problems * p.splits;
     if (tiles > INT32_MAX) return cudaErrorInvalidValue;
@@ -369,12 +338,9 @@ __global__ void __launch_bounds__(256) pack_kernel(Matrix from, size_t rows, int
 }  // namespace
 
 // As many parts as give every multiprocessor a tile, none under 128 of K.
-Cut cut_plain(ProductKind kind, uint32_t type, size_t m, size_t n, size_t k) {
-    const bool gated = kind == kGated;
-    const size_t high = kSide * (type == GEO_B200_F64 ? (gated ? rows_of_thread<double, kGated>() : rows_of_thread<double, kDown>())
-                                                      : rows_of_thread<float, kDown>());
-    const size_t wide = kSide * (type == GEO_B200_F64 ? columns_of_thread<double, kDown>()
-                                                      : (gated ? columns_of_thread<float, kGated>() : columns_of_thread<float, kDown>()));
+Cut cut_plain(ProductKind kind, size_t m, size_t n, size_t k) {
+    const size_t high = kSide * rows_of_thread<kDown>();
+    const size_t wide = kSide * (kind == kGated ? columns_of_thread<kGated>() : columns_of_thread<kDown>());
     const size_t tiles = (kind == kWeights ? 3 : 1) * ((m + high - 1) / high) * ((n + wide - 1) / wide);
     const size_t wanted = (size_t)geo::device_sm_count() / tiles, most = k * (kind == kInput ? 2 : 1) / 128;
     const size_t splits = wanted < most ? wanted : most;
@@ -406,7 +372,7 @@ cudaError_t launch_join(ProductKind kind, uint32_t type, uint32_t out_type, cons
 
 cudaError_t launch_product_plain(ProductKind kind, uint32_t type, uint32_t out_type, const Product &p,
                                  cudaStream_t stream) {
-    const cudaError_t e = by_type(type, [&](auto t) -> cudaError_t {
+    auto launch = [&](auto t) -> cudaError_t {
         using T = decltype(t);
         switch (kind) {
             case kGated: return launch_tile<T, T, kGated>(p, stream);
@@ -415,11 +381,9 @@ cudaError_t launch_product_plain(ProductKind kind, uint32_t type, uint32_t out_t
             case kInput: return launch_tile<T, T, kInput>(p, stream);
             default: break;
         }
-        if constexpr (sizeof(T) == 2) {
-            if (out_type == GEO_B200_F32) return launch_tile<T, float, kWeights>(p, stream);
-        }
-        return launch_tile<T, T, kWeights>(p, stream);
-    });
+        return out_type == GEO_B200_F32 ? launch_tile<T, float, kWeights>(p, stream) : launch_tile<T, T, kWeights>(p, stream);
+    };
+    const cudaError_t e = type == GEO_B200_BF16 ? launch(__nv_bfloat16{}) : launch(__half{});
     return e != cudaSuccess || p.splits == 1 ? e : launch_join(kind, type, out_type, p, stream);
 }
 
