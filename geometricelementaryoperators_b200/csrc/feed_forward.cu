@@ -94,9 +94,15 @@ struct Space {
     }
 };
 
-// Few rows are the weights' way through memory: one warp a column (feed_forward_plain.cu).
+// Few rows are the weights' way through memory: columns of the result by warps
+// (feed_forward_plain.cu). Of 16-bit types the tensor cores' tiles take over early
+// (4096 x 12288 bfloat16: 2 rows 70 us either way, 4 rows 95 and 70), later where the
+// weights are small (1024 x 2048: 4 rows 14 us, 5 rows in tiles 22) or would have to be
+// copied first.
 bool few_rows(const geo_b200_feed_forward_config_t &c) {
-    return c.rows <= (size_t)(type_bytes(c.type) == 2 ? kFewRows / 2 : kFewRows);
+    if (type_bytes(c.type) != 2) return c.rows <= (size_t)kFewRows;
+    const bool copied = c.gate_weight_stride % 8 != 0 || c.up_weight_stride % 8 != 0 || c.down_weight_stride % 8 != 0;
+    return c.rows <= 2 || (c.rows <= 4 && (copied || c.cols * c.hidden <= (size_t)1 << 22));
 }
 
 // The arrays of a call that TMA would read, by rows of `stride` values; those off 16

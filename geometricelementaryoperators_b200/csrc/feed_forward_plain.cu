@@ -203,64 +203,83 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Produ
 
 // A token or a few: every weight is read once and that is all the time it takes. A
 // column of the result (kGated: of gate and up) is `split` warps' work, each along its
-// part of K, vectors of 16 bytes side by side; the rows of x come from L1. `split`
-// grows until there are warps enough to keep HBM busy.
+// part of K, vectors of 16 bytes side by side; a lane asks for kBatch of them at a time
+// before it multiplies any, and L1 is left to the rows of x. `split` grows until there
+// are warps enough to keep HBM busy. kDown's weights are asked for before the kernel
+// that makes its rows has ended.
 constexpr int kFewThreads = 256, kFewWarps = kFewThreads / 32;
+
+template <typename T, int V>
+__device__ __forceinline__ Vec<T, V> load_once(const T *p) {
+    Vec<T, V> r;
+    if constexpr (Vec<T, V>::kBytes == 16)
+        asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(r.w[0]), "=r"(r.w[1]), "=r"(r.w[2]), "=r"(r.w[3])
+                     : "l"(p));
+    else
+        r = load<T, V>(p);
+    return r;
+}
 
 template <typename T, int KIND, int ROWS, bool ALIGNED>
 __global__ void __launch_bounds__(kFewThreads) few_kernel(const __grid_constant__ Product p, int split) {
     using W = Wide<T>;
-    constexpr int kOperands = KIND == kGated ? 2 : 1, V = ALIGNED ? 16 / (int)sizeof(T) : 1;
-    __shared__ W parts[kFewWarps][kOperands * ROWS];
+    // Several rows: as many columns a warp as make four streams of weights, which share what is read of the rows.
+    constexpr int kOperands = KIND == kGated ? 2 : 1, kColumns = ROWS == 1 ? 1 : 4 / kOperands;
+    constexpr int kStreams = kOperands * kColumns, V = ALIGNED ? 16 / (int)sizeof(T) : 1, kBatch = 8 / kStreams;
+    __shared__ W parts[kFewWarps][kStreams * ROWS];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int part = warp % split, columns = kFewWarps / split;
-    const int col = (int)blockIdx.x * columns + warp / split;
-    after_previous();
-    let_next_start();
-    W sum[kOperands][ROWS];
+    const int part = warp % split, columns = kFewWarps / split * kColumns;  // of the block
+    const int col = (int)blockIdx.x * columns + warp / split * kColumns;
+    W sum[kStreams][ROWS];
 #pragma unroll
-    for (int o = 0; o < kOperands; ++o)
+    for (int o = 0; o < kStreams; ++o)
 #pragma unroll
         for (int r = 0; r < ROWS; ++r) sum[o][r] = W(0);
-    if (col < p.n) {
-        const T *x = (const T *)p.a[0].p, *w[kOperands];
+    const T *x = (const T *)p.a[0].p, *w[kStreams];
 #pragma unroll
-        for (int o = 0; o < kOperands; ++o) w[o] = (const T *)p.b[o].p + (size_t)col * p.b[o].stride;
-        const int step = 32 * V * split;
-#pragma unroll 4
-        for (int k = (part * 32 + lane) * V; k < p.k; k += step) {
-            if constexpr (ALIGNED) {
-                Vec<T, V> piece[kOperands];
+    for (int o = 0; o < kStreams; ++o) {
+        const int c = col + o / kOperands;
+        w[o] = (const T *)p.b[o % kOperands].p + (size_t)(c < p.n ? c : 0) * p.b[o % kOperands].stride;
+    }
+    const int step = 32 * V * split, first = (part * 32 + lane) * V, last = col < p.n ? p.k : 0;
+    Vec<T, V> piece[kBatch][kStreams];
+    auto ask = [&](int k) {
 #pragma unroll
-                for (int o = 0; o < kOperands; ++o) piece[o] = load<T, V>(w[o] + k);
+        for (int i = 0; i < kBatch; ++i)
 #pragma unroll
-                for (int r = 0; r < ROWS; ++r) {
-                    if (r >= p.m) break;
-                    const Vec<T, V> xs = load<T, V>(x + (size_t)r * p.a[0].stride + k);
+            for (int o = 0; o < kStreams; ++o)
+                piece[i][o] = k + i * step < last ? load_once<T, V>(w[o] + k + i * step) : Vec<T, V>::zero();
+    };
+    if (KIND == kGated) after_previous();
+    ask(first);
+    if (KIND == kDown) after_previous();
+    let_next_start();
+    for (int k = first; k < last; k += kBatch * step) {
 #pragma unroll
-                    for (int o = 0; o < kOperands; ++o) {
+        for (int i = 0; i < kBatch; ++i) {
+            if (k + i * step >= last) break;
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r) {
+                if (r >= p.m) break;
+                const Vec<T, V> xs = load<T, V>(x + (size_t)r * p.a[0].stride + k + i * step);
+#pragma unroll
+                for (int o = 0; o < kStreams; ++o) {
+                    if constexpr (V == 1) {
+                        sum[o][r] += xs.one() * piece[i][o].one();
+                    } else {
                         Pair<W> two = both(W(0));
 #pragma unroll
-                        for (int q = 0; q < V / 2; ++q) two = fma(xs.pair(q), piece[o].pair(q), two);
+                        for (int q = 0; q < V / 2; ++q) two = fma(xs.pair(q), piece[i][o].pair(q), two);
                         sum[o][r] += two.x + two.y;
                     }
                 }
-            } else {
-                W v[kOperands];
-#pragma unroll
-                for (int o = 0; o < kOperands; ++o) v[o] = widen(w[o][k]);
-#pragma unroll
-                for (int r = 0; r < ROWS; ++r) {
-                    if (r >= p.m) break;
-                    const W xs = widen(x[(size_t)r * p.a[0].stride + k]);
-#pragma unroll
-                    for (int o = 0; o < kOperands; ++o) sum[o][r] += xs * v[o];
-                }
             }
         }
+        if (k + kBatch * step < last) ask(k + kBatch * step);
     }
 #pragma unroll
-    for (int o = 0; o < kOperands; ++o)
+    for (int o = 0; o < kStreams; ++o)
 #pragma unroll
         for (int r = 0; r < ROWS; ++r) {
             W v = sum[o][r];
@@ -275,19 +294,10 @@ __global__ void __launch_bounds__(kFewThreads) few_kernel(const __grid_constant_
 #pragma unroll
     for (int o = 0; o < kOperands; ++o) {
         total[o] = W(0);
-        for (int s = 0; s < split; ++s) total[o] += parts[c * split + s][o * ROWS + row];
+        for (int s = 0; s < split; ++s)
+            total[o] += parts[c / kColumns * split + s][(c % kColumns * kOperands + o) * ROWS + row];
     }
-    const size_t at = (size_t)blockIdx.x * columns + c;
-    auto put = [&](const OutMatrix &out, W v) {
-        if (out.p != nullptr) ((T *)out.p)[(size_t)row * out.stride + at] = narrow<T>(v);
-    };
-    if constexpr (KIND == kGated) {
-        put(p.out[0], total[0]);
-        put(p.out[1], total[kOperands - 1]);
-        put(p.out[2], activation<sizeof(T) == 2>(p.activation, total[0], (W *)nullptr) * total[kOperands - 1]);
-    } else {
-        put(p.out[0], total[0]);
-    }
+    finish<T, T, KIND>(p, 0, row, (size_t)blockIdx.x * columns + c, total[0], total[kOperands - 1]);
 }
 
 template <typename T, int KIND, int ROWS>
@@ -298,10 +308,11 @@ cudaError_t launch_rows(const Product &p, cudaStream_t stream) {
     };
     look(p.a[0], p.m);
     for (int o = 0; o < (KIND == kGated ? 2 : 1); ++o) look(p.b[o], p.n);
+    constexpr int kColumns = ROWS == 1 ? 1 : (KIND == kGated ? 2 : 4);
     int split = 1;
     const long long wanted = (long long)geo::device_sm_count() * 32;  // warps
-    while (split < kFewWarps && (long long)p.n * split < wanted && p.k > split * 512) split *= 2;
-    const int columns = kFewWarps / split;
+    while (split < kFewWarps && (long long)p.n * split < wanted * kColumns && p.k > split * 512) split *= 2;
+    const int columns = kFewWarps / split * kColumns;
     const unsigned grid = (unsigned)((p.n + columns - 1) / columns);
     return aligned ? launch_after(few_kernel<T, KIND, ROWS, true>, grid, kFewThreads, 0, 1, stream, p, split)
                    : launch_after(few_kernel<T, KIND, ROWS, false>, grid, kFewThreads, 0, 1, stream, p, split);

@@ -35,9 +35,9 @@ struct Entry {
     uint32_t first;  // piece
     uint32_t type;
 };
-// Entries of one launch. Few are the usual case of a small model, whose calls are
-// short: parameters take their time to arrive.
-constexpr int kSmall = 62, kLarge = 1000;
+// Entries of one launch, the fewest that hold the list: parameters take their time to
+// be handed over (1 microsecond for each 10 KB of them), which short calls notice.
+constexpr int kSmall = 62, kMiddle = 250, kLarge = 1000;
 template <int CAPACITY>
 struct Table {
     int count;
@@ -237,7 +237,7 @@ struct Part {
 // False when a type, a count or the whole is out of range.
 bool parts_of(const geo_b200_gradient_t *g, size_t count, std::vector<Part> &parts) {
     if (g == nullptr || count == 0 || count > GEO_B200_GRADIENT_MAX_TENSORS) return false;
-    const size_t each = count <= (size_t)kSmall ? kSmall : kLarge;
+    const size_t each = count <= (size_t)kLarge ? count : kLarge;
     for (size_t first = 0; first < count; first += each) {
         Part p = {first, first + each < count ? first + each : count, 0};
         size_t pieces = 0;
@@ -297,28 +297,36 @@ private:
     int next_ = 0;
 };
 
-// What is written overlaps nothing else of the call.
+// What is written overlaps nothing else of the call. Lists mostly lie in order, those
+// read and those written each.
 bool apart(const geo_b200_gradient_t *g, size_t count) {
     struct Range {
         uintptr_t first, last;
-        bool written;
     };
-    std::vector<Range> ranges;
+    auto before = [](const Range &a, const Range &b) { return a.first < b.first; };
+    std::vector<Range> read, written;
+    read.reserve(count);
+    written.reserve(count);
     for (size_t i = 0; i < count; ++i) {
         if (g[i].count == 0) continue;
         const size_t bytes = g[i].count * type_bytes(g[i].type);
         const uintptr_t in = (uintptr_t)g[i].gradient, out = (uintptr_t)g[i].clipped;
-        ranges.push_back({in, in + bytes, out == in});
-        if (out != 0 && out != in) ranges.push_back({out, out + bytes, true});
+        if (out != 0) written.push_back({out, out + bytes});
+        if (out != in) read.push_back({in, in + bytes});
     }
-    std::sort(ranges.begin(), ranges.end(), [](const Range &a, const Range &b) { return a.first < b.first; });
-    uintptr_t written = 0, any = 0;  // ends of what starts before
-    for (const Range &r : ranges) {
-        if (r.first < written || (r.written && r.first < any)) return false;
-        any = std::max(any, r.last);
-        if (r.written) written = std::max(written, r.last);
+    for (std::vector<Range> *ranges : {&read, &written})
+        if (!std::is_sorted(ranges->begin(), ranges->end(), before)) std::sort(ranges->begin(), ranges->end(), before);
+    uintptr_t read_end = 0, written_end = 0;  // of what starts before
+    auto r = read.begin();
+    for (const Range &w : written) {
+        for (; r != read.end() && r->first < w.first; ++r) {
+            if (r->first < written_end) return false;
+            read_end = std::max(read_end, r->last);
+        }
+        if (w.first < written_end || w.first < read_end) return false;
+        written_end = std::max(written_end, w.last);
     }
-    return true;
+    return r == read.end() || r->first >= written_end;
 }
 
 template <int CAPACITY>
@@ -405,11 +413,13 @@ extern "C" geo_b200_status_t geo_b200_gradient_clip(const geo_b200_gradient_t *g
     if (!apart(gradients, count) ||
         !arrays_usable({{device_norm, 8}, {device_scale, 8}, {device_workspace, 16}}))
         return GEO_B200_INVALID_ARGUMENT;
-    const cudaError_t e =
-        count <= (size_t)kSmall
-            ? launch<kSmall>(gradients, parts, max_norm, device_norm, device_scale, device_workspace, writes, stream)
-            : launch<kLarge>(gradients, parts, max_norm, device_norm, device_scale, device_workspace, writes, stream);
-    return status_of(e);
+    auto run = [&](auto capacity) {
+        return status_of(launch<decltype(capacity)::value>(gradients, parts, max_norm, device_norm, device_scale,
+                                                           device_workspace, writes, stream));
+    };
+    if (count <= (size_t)kSmall) return run(std::integral_constant<int, kSmall>{});
+    if (count <= (size_t)kMiddle) return run(std::integral_constant<int, kMiddle>{});
+    return run(std::integral_constant<int, kLarge>{});
 } catch (...) {
     return GEO_B200_RUNTIME_FAILURE;
 }

@@ -85,10 +85,11 @@ __global__ void __launch_bounds__(TEAM == kWarp ? kWarpBlock : kTeamThreads, TEA
                 if constexpr (MODE == kGatedNorm) {
                     ring.get(raw, u, 2, (const T *)a.gate + r * a.gate_stride);
 #pragma unroll
-                    for (int q = 0; q < Q; ++q) {
-                        const Pair<W> g = pair_at(raw, q);
-                        v[u][q] = v[u][q] * Pair<W>{gate_value<sizeof(T) == 2>(a.gate_kind, g.x, (W *)nullptr),
-                                                    gate_value<sizeof(T) == 2>(a.gate_kind, g.y, (W *)nullptr)};
+                    for (int i = 0; i < K; ++i) {
+                        Pair<W> f[V / 2], none[V / 2];
+                        gate_values<sizeof(T) == 2, false>(a.gate_kind, raw[i], f, none);
+#pragma unroll
+                        for (int q = 0; q < V / 2; ++q) v[u][i * V / 2 + q] = v[u][i * V / 2 + q] * f[q];
                     }
                 }
                 ring.get(raw, u, 1, (const T *)a.residual + r * a.residual_stride);

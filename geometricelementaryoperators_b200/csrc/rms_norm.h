@@ -54,6 +54,29 @@ __device__ __forceinline__ W gate_value(int kind, W g, W *slope) {
     return tanh(g);
 }
 
+// The gate's values, and where asked for their slopes, of a vector; the kind is looked
+// at once for all of them, whose functions are then worked out side by side (the
+// VJP of 16384 x 4096 bfloat16, sigmoid: 236 us with a look at each value).
+template <bool FAST, bool SLOPES, typename T, int V>
+__device__ __forceinline__ void gate_values(int kind, const Vec<T, V> &gate, Pair<Wide<T>> (&f)[V / 2],
+                                            Pair<Wide<T>> (&slope)[V / 2]) {
+    using W = Wide<T>;
+    auto all = [&](auto k) {
+#pragma unroll
+        for (int q = 0; q < V / 2; ++q) {
+            const Pair<W> g = gate.pair(q);
+            f[q].x = gate_value<FAST>(decltype(k)::value, g.x, SLOPES ? &slope[q].x : (W *)nullptr);
+            f[q].y = gate_value<FAST>(decltype(k)::value, g.y, SLOPES ? &slope[q].y : (W *)nullptr);
+        }
+    };
+    if (kind == GEO_B200_GATE_SIGMOID)
+        all(std::integral_constant<int, GEO_B200_GATE_SIGMOID>{});
+    else if (kind == GEO_B200_GATE_TANH)
+        all(std::integral_constant<int, GEO_B200_GATE_TANH>{});
+    else
+        all(std::integral_constant<int, GEO_B200_GATE_LINEAR>{});
+}
+
 // What the warps of a team sum up together: N values a warp (1, 2 or 4), from every
 // lane of it; the sums, the same on every thread. False: a wait gave up, sums are NaN.
 template <int N, int TEAM, int V, int K, typename W>

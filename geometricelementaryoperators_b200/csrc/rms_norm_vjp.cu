@@ -31,9 +31,15 @@ __device__ __forceinline__ void cut(Vec<T, V> &v, int i, const Place<TEAM, V, K>
     }
 }
 
+// Blocks a multiprocessor holds: 512 threads of up to 128 registers. A block norm's
+// passes within a warp, whose columns' places vary, want 170 of them.
+constexpr int resident_blocks(int mode, int team) {
+    return team == kWarp ? (mode == kRms ? 4 : 3) : 2;
+}
+
 // The arrays in the ring: x, y_bar, then (block norm) z, the gate, z_bar, as far as they are there.
 template <typename T, int MODE, int TEAM, bool SHIFT, bool FULL>
-__global__ void __launch_bounds__(TEAM == kWarp ? kWarpBlock : kTeamThreads, TEAM == kWarp ? 4 : 2)
+__global__ void __launch_bounds__(TEAM == kWarp ? kWarpBlock : kTeamThreads, resident_blocks(MODE, TEAM))
     rms_vjp_kernel(const RmsBackwardArgs a, int lanes, bool float_parameters, int stages, Wide<T> *partial, bool alone) {
     using W = Wide<T>;
     constexpr int V = 16 / (int)sizeof(T), K = values_per_thread(sizeof(T)) / V, Q = K * V / 2;
@@ -120,16 +126,14 @@ __global__ void __launch_bounds__(TEAM == kWarp ? kWarpBlock : kTeamThreads, TEA
                 Vec<T, V> gate = Vec<T, V>::zero(), dz = Vec<T, V>::zero();
                 if constexpr (kGates) gate = vector(i, 0, 3, a.gate, a.gate_stride);
                 if (has_dz) dz = vector(i, 0, kDz, a.dz, a.dz_stride);
+                Pair<W> act[V / 2], none[V / 2];
+                if constexpr (kGates) gate_values<kFast, false>(a.gate_kind, gate, act, none);
 #pragma unroll
                 for (int q = 0; q < V / 2; ++q) {
                     const int n = i * V / 2 + q;
                     const Pair<W> zh = z.pair(q) * both(rstd[0]), d = dy.pair(q), g = d * w[n];
                     Pair<W> f = x.pair(q) * both(x_rstd) * (post[n] * both(beta));
-                    if constexpr (kGates) {
-                        const Pair<W> k = gate.pair(q);
-                        f = f * Pair<W>{gate_value<kFast>(a.gate_kind, k.x, (W *)nullptr),
-                                        gate_value<kFast>(a.gate_kind, k.y, (W *)nullptr)};
-                    }
+                    if constexpr (kGates) f = f * act[q];
                     s1 = fma(g, zh, s1);
                     s2 = fma(f, fma(g, both(rstd[0]), dz.pair(q)), s2);
                     s3 = fma(f, zh, s3);
@@ -181,6 +185,8 @@ __global__ void __launch_bounds__(TEAM == kWarp ? kWarpBlock : kTeamThreads, TEA
                 Vec<T, V> gate = Vec<T, V>::zero(), dzs = Vec<T, V>::zero(), dresidual, dx, dgate;
                 if constexpr (kGates) gate = vector(i, 0, 3, a.gate, a.gate_stride);
                 if (has_dz) dzs = vector(i, 0, kDz, a.dz, a.dz_stride);
+                Pair<W> act[V / 2], slope[V / 2];
+                if constexpr (kGates) gate_values<kFast, true>(a.gate_kind, gate, act, slope);
 #pragma unroll
                 for (int q = 0; q < V / 2; ++q) {
                     const int n = i * V / 2 + q;
@@ -190,12 +196,8 @@ __global__ void __launch_bounds__(TEAM == kWarp ? kWarpBlock : kTeamThreads, TEA
                     Pair<W> dn = dz * both(beta);
                     dresidual.set(q, dz * both(alpha));
                     if constexpr (kGates) {
-                        const Pair<W> k = gate.pair(q);
-                        Pair<W> slope;
-                        const Pair<W> f = {gate_value<kFast>(a.gate_kind, k.x, &slope.x),
-                                           gate_value<kFast>(a.gate_kind, k.y, &slope.y)};
-                        dgate.set(q, dn * (xh * post[n]) * slope);
-                        dn = dn * f;
+                        dgate.set(q, dn * (xh * post[n]) * slope[q]);
+                        dn = dn * act[q];
                     }
                     dpost[n] = fma(dn, xh, dpost[n]);
                     dx.set(q, fma(xh, both(-c2), dn * post[n]) * both(x_rstd));
@@ -353,7 +355,8 @@ int at_once_of(NormMode mode, size_t bytes, const Shape &s) {
 }
 size_t team_grid(NormMode mode, const Shape &s, size_t bytes, size_t rows) {
     const size_t each = s.teams() * at_once_of(mode, bytes, s), wanted = (rows + each - 1) / each;
-    const size_t most = (size_t)geo::device_sm_count() * (512 / s.threads()) / s.blocks;
+    const int resident = s.team() == kWarp ? resident_blocks(mode, kWarp) : 512 / s.threads();
+    const size_t most = (size_t)geo::device_sm_count() * resident / s.blocks;
     return wanted < most ? wanted : most;
 }
 
