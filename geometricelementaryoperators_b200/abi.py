@@ -360,6 +360,8 @@ SIGNATURES: dict[str, tuple] = {
     "geo_b200_feed_forward_vjp_workspace": (_SZ, [ctypes.POINTER(FeedForwardConfig)]),
     "geo_b200_feed_forward": (_I, [ctypes.POINTER(FeedForwardConfig), *[_P] * 8, _SZ, _P]),
     "geo_b200_feed_forward_vjp": (_I, [ctypes.POINTER(FeedForwardConfig), *[_P] * 12, _SZ, _P]),
+    "geo_b200_feed_forward_wait_selftest": (
+        _I, [ctypes.POINTER(FeedForwardConfig), *[_P] * 8, _SZ, ctypes.c_uint32, ctypes.c_uint32, _P]),
     "geo_b200_gradient_clip_workspace": (_SZ, [ctypes.POINTER(Gradient), _SZ]),
     "geo_b200_gradient_clip": (_I, [ctypes.POINTER(Gradient), _SZ, _D, _P, _P, _P, _SZ, _P]),
 }

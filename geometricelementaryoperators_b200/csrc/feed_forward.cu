@@ -69,7 +69,7 @@ size_t partial_bytes(const geo_b200_feed_forward_config_t &c, std::initializer_l
 
 // Launches a product by the kernels that take it; `rest`: room for parts of its sums.
 cudaError_t launch_product(const geo_b200_feed_forward_config_t &c, bool tensor, ProductKind kind, Product &p, void *rest,
-                           cudaStream_t stream) {
+                           cudaStream_t stream, PipelineStarve starve = {UINT32_MAX, kPipelinePolls}) {
     p.partial = rest;
     if (type_bytes(c.type) != 2) {
         p.splits = cut_wide(kind, c.type, p.m, p.n, p.k).splits;
@@ -77,7 +77,7 @@ cudaError_t launch_product(const geo_b200_feed_forward_config_t &c, bool tensor,
     }
     if (tensor) {
         p.splits = cut_tensor(kind, kind == kWeights && c.gradient_type != c.type, p.m, p.n, p.k).splits;
-        return launch_product_tensor(kind, c.type, c.gradient_type, p, {UINT32_MAX, kPipelinePolls}, stream);
+        return launch_product_tensor(kind, c.type, c.gradient_type, p, starve, stream);
     }
     p.splits = cut_plain(kind, p.m, p.n, p.k).splits;
     return launch_product_plain(kind, c.type, c.gradient_type, p, stream);
@@ -179,12 +179,13 @@ extern "C" size_t geo_b200_feed_forward_vjp_workspace(const geo_b200_feed_forwar
     return space.used;
 }
 
-extern "C" geo_b200_status_t geo_b200_feed_forward(const geo_b200_feed_forward_config_t *config, const void *device_x,
-                                                   const void *device_gate_weight, const void *device_up_weight,
-                                                   const void *device_down_weight, void *device_gate, void *device_up,
-                                                   void *device_y, void *device_workspace, size_t workspace_bytes,
-                                                   cudaStream_t stream) {
-    geo::NvtxRange range("geo_b200.feed_forward");
+namespace {
+
+// `starve`: null, or for the self-test of the tensor-core kernels' waits, which are then the only ones taken.
+geo_b200_status_t forward(const geo_b200_feed_forward_config_t *config, const void *device_x,
+                          const void *device_gate_weight, const void *device_up_weight, const void *device_down_weight,
+                          void *device_gate, void *device_up, void *device_y, void *device_workspace,
+                          size_t workspace_bytes, const PipelineStarve *starve, cudaStream_t stream) {
     geo_b200_feed_forward_config_t c;
     if (!resolve(config, false, &c) || device_x == nullptr || device_gate_weight == nullptr ||
         device_up_weight == nullptr || device_down_weight == nullptr || device_y == nullptr ||
@@ -224,11 +225,39 @@ extern "C" geo_b200_status_t geo_b200_feed_forward(const geo_b200_feed_forward_c
     down.b[0] = wd.m;
     down.out[0] = {device_y, c.y_stride};
     void *const rest = space.take(0, 0, 1);
+    if (starve != nullptr) {
+        if (!tensor) return GEO_B200_INVALID_ARGUMENT;
+        const cudaError_t e = launch_product(c, tensor, kGated, gated, rest, stream, *starve);
+        return status_of(e != cudaSuccess ? e : launch_product(c, tensor, kDown, down, rest, stream));
+    }
     auto launch = [&](ProductKind kind, Product &p) {
         return few ? launch_product_few(kind, c.type, p, stream) : launch_product(c, tensor, kind, p, rest, stream);
     };
     const cudaError_t e = launch(kGated, gated);
     return status_of(e != cudaSuccess ? e : launch(kDown, down));
+}
+
+}  // namespace
+
+extern "C" geo_b200_status_t geo_b200_feed_forward(const geo_b200_feed_forward_config_t *config, const void *device_x,
+                                                   const void *device_gate_weight, const void *device_up_weight,
+                                                   const void *device_down_weight, void *device_gate, void *device_up,
+                                                   void *device_y, void *device_workspace, size_t workspace_bytes,
+                                                   cudaStream_t stream) {
+    geo::NvtxRange range("geo_b200.feed_forward");
+    return forward(config, device_x, device_gate_weight, device_up_weight, device_down_weight, device_gate, device_up,
+                   device_y, device_workspace, workspace_bytes, nullptr, stream);
+}
+
+extern "C" geo_b200_status_t geo_b200_feed_forward_wait_selftest(
+    const geo_b200_feed_forward_config_t *config, const void *device_x, const void *device_gate_weight,
+    const void *device_up_weight, const void *device_down_weight, void *device_gate, void *device_up, void *device_y,
+    void *device_workspace, size_t workspace_bytes, uint32_t block, uint32_t wait_limit, cudaStream_t stream) {
+    geo::NvtxRange range("geo_b200.feed_forward_wait_selftest");
+    if (wait_limit == 0 || wait_limit > kPipelinePolls) return GEO_B200_INVALID_ARGUMENT;
+    const PipelineStarve starve = {block, wait_limit};
+    return forward(config, device_x, device_gate_weight, device_up_weight, device_down_weight, device_gate, device_up,
+                   device_y, device_workspace, workspace_bytes, &starve, stream);
 }
 
 extern "C" geo_b200_status_t geo_b200_feed_forward_vjp(

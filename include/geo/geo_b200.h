@@ -698,6 +698,21 @@ geo_b200_status_t geo_b200_feed_forward_vjp(const geo_b200_feed_forward_config_t
                                             void *device_up_weight_cotangent, void *device_down_weight_cotangent,
                                             void *device_workspace, size_t workspace_bytes, cudaStream_t stream);
 
+/* The 16-bit types' products (more rows than a few) run through rings of shared memory
+ * that asynchronous copies fill. Every wait for a copy or a product gives up after a
+ * fixed number of polls (seconds, where a stage takes microseconds; it cannot happen
+ * unless a copy failed). A block whose wait gave up copies no more, waits for its copies
+ * in flight, and writes NaN for what it has not finished; the call ends and the context
+ * stays usable.
+ * Self-test of that path, for calls that those kernels take: the forward, in which every
+ * block (pair of blocks) stops copying before its block number `block` of 64 of K, all of
+ * its tiles counted one after another, of gate's and up's products; waits give up after
+ * wait_limit polls, 1 .. 2^20. */
+geo_b200_status_t geo_b200_feed_forward_wait_selftest(
+    const geo_b200_feed_forward_config_t *config, const void *device_x, const void *device_gate_weight,
+    const void *device_up_weight, const void *device_down_weight, void *device_gate, void *device_up, void *device_y,
+    void *device_workspace, size_t workspace_bytes, uint32_t block, uint32_t wait_limit, cudaStream_t stream);
+
 /* ---- 6. gradients of a training step ------------------------------------ */
 
 /* Norm over all gradients of a model, and clipping before the update:

@@ -302,3 +302,31 @@ def test_refusals_with_usable_arrays():
     host.copy_(c.x)
     assert call(x=host) == 0
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("rows,block", [(40, 0), (40, 2), (300, 0), (700, 3)])
+def test_waits_give_up(rows, block):
+    """Copies that stop (single blocks, parts of K, pairs of blocks): the call ends, what they were for is NaN, and the
+    next call is right."""
+    import torch
+
+    p, L = ff.pointer, abi.lib()
+    c = Case("bf16", rows, 640, 520)
+    a, u, y, _ = c.forward()
+    args = (ref(c.config), p(c.x), p(c.wg), p(c.wu), p(c.wd))
+    (ga, _), (gu, _), (gy, _) = (c.blank(rows, n, 0) for n in (520, 520, 640))
+    stream = torch.cuda.current_stream().cuda_stream
+    for limit in (1 << 8, 1 << 12):
+        assert L.geo_b200_feed_forward_wait_selftest(*args, p(ga), p(gu), p(gy), p(c.space), c.space.numel(), block,
+                                                     limit, stream) == 0
+        torch.cuda.synchronize()
+        assert ga.isnan().all() and gu.isnan().all() and gy.isnan().all()
+    for bad in (0, (1 << 20) + 1):
+        assert L.geo_b200_feed_forward_wait_selftest(*args, p(ga), p(gu), p(gy), p(c.space), c.space.numel(), 0, bad,
+                                                     stream) == 1
+    again = c.forward()
+    assert all(torch.equal(v, w) for v, w in zip(again[:3], (a, u, y)))
+    # A call that other kernels take has no such waits.
+    few = Case("bf16", 1, 640, 520)
+    assert L.geo_b200_feed_forward_wait_selftest(ref(few.config), p(few.x), p(few.wg), p(few.wu), p(few.wd), None, None,
+                                                 p(gy), p(few.space), few.space.numel(), 0, 16, stream) == 1
