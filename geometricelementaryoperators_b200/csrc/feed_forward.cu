@@ -114,12 +114,18 @@ struct Operand {
 size_t packed_bytes(const Operand &o) {
     return off16(o.m.stride) ? (o.rows * round8(o.cols) * 2 + kAlign - 1) / kAlign * kAlign : 0;
 }
-cudaError_t pack(Operand &o, Space &space, cudaStream_t stream) {
-    if (!off16(o.m.stride)) return cudaSuccess;
-    void *to = space.take(o.rows, round8(o.cols), 2);
-    const cudaError_t e = launch_pack_rows(o.m, o.rows, o.cols, to, round8(o.cols), stream);
-    o.m = {to, round8(o.cols)};
-    return e;
+cudaError_t pack(std::initializer_list<Operand *> operands, Space &space, cudaStream_t stream) {
+    Pack list = {};
+    size_t end = 0;
+    for (Operand *o : operands) {
+        if (o->m.p == nullptr || !off16(o->m.stride)) continue;
+        const size_t stride = round8(o->cols);
+        void *to = space.take(o->rows, stride, 2);
+        end += o->rows * (stride / 8);
+        list.arrays[list.count++] = {o->m, o->rows, (int)o->cols, to, stride, end};
+        o->m = {to, stride};
+    }
+    return launch_pack(list, stream);
 }
 // Whether the tensor-core kernels take these arrays, once those off 16 bytes by their stride are copied.
 bool tensor_call(const geo_b200_feed_forward_config_t &c, std::initializer_list<const Operand *> arrays) {
@@ -205,11 +211,10 @@ geo_b200_status_t forward(const geo_b200_feed_forward_config_t *config, const vo
             wu = {{device_up_weight, c.up_weight_stride}, c.hidden, c.cols},
             wd = {{device_down_weight, c.down_weight_stride}, c.cols, c.hidden};
     const bool few = few_rows(c), tensor = !few && tensor_call(c, {&x, &wg, &wu, &wd});
-    if (tensor)
-        for (Operand *o : {&x, &wg, &wu, &wd}) {
-            const cudaError_t e = pack(*o, space, stream);
-            if (e != cudaSuccess) return status_of(e);
-        }
+    if (tensor) {
+        const cudaError_t e = pack({&x, &wg, &wu, &wd}, space, stream);
+        if (e != cudaSuccess) return status_of(e);
+    }
     Product gated = {};
     gated.m = (int)c.rows, gated.n = (int)c.hidden, gated.k = (int)c.cols, gated.problems = 1;
     gated.activation = (int)c.activation;
@@ -298,11 +303,10 @@ extern "C" geo_b200_status_t geo_b200_feed_forward_vjp(
             wd = {{device_down_weight, c.down_weight_stride}, c.cols, c.hidden},
             dy = {{device_y_cotangent, c.y_cotangent_stride}, c.rows, c.cols};
     const bool tensor = tensor_call(c, {&x, &wg, &wu, &wd, &dy});
-    if (tensor)
-        for (Operand *o : {&x, &wg, &wu, &wd, &dy}) {
-            const cudaError_t e = o->m.p == nullptr ? cudaSuccess : pack(*o, space, stream);
-            if (e != cudaSuccess) return status_of(e);
-        }
+    if (tensor) {
+        const cudaError_t e = pack({&x, &wg, &wu, &wd, &dy}, space, stream);
+        if (e != cudaSuccess) return status_of(e);
+    }
     void *const rest = space.take(0, 0, 1);
     auto launch = [&](ProductKind kind, Product &p) { return launch_product(c, tensor, kind, p, rest, stream); };
     Product hidden = {};

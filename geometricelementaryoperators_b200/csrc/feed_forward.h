@@ -78,9 +78,20 @@ cudaError_t launch_product_plain(ProductKind kind, uint32_t type, uint32_t out_t
 // kGated, kDown with at most kFewRows rows.
 constexpr int kFewRows = 8;
 cudaError_t launch_product_few(ProductKind kind, uint32_t type, const Product &p, cudaStream_t stream);
-// Copies rows x cols values of 16 bits to rows of `to_stride` (a multiple of 8), zeros behind each row's end.
-cudaError_t launch_pack_rows(const Matrix &from, size_t rows, size_t cols, void *to, size_t to_stride,
-                             cudaStream_t stream);
+// Copies arrays of 16-bit values to rows of `to_stride` (a multiple of 8), zeros behind each row's end.
+constexpr int kPackMost = 5;
+struct Pack {
+    int count;
+    struct Array {
+        Matrix from;
+        size_t rows;
+        int cols;
+        void *to;
+        size_t to_stride;
+        size_t end;  // of its pieces of 8 values, all arrays counted one after another
+    } arrays[kPackMost];
+};
+cudaError_t launch_pack(const Pack &pack, cudaStream_t stream);
 // Whether the tensor-core products can run at all (the driver's tensor map encoder).
 bool tensor_products_available();
 

@@ -328,21 +328,25 @@ cudaError_t launch_few(const Product &p, cudaStream_t stream) {
 
 // ---- rows that start on 16 bytes -----------------------------------------------------
 
-__global__ void __launch_bounds__(256) pack_kernel(Matrix from, size_t rows, int cols, void *to, size_t to_stride) {
-    const size_t pieces = to_stride / 8, n = rows * pieces;
+__global__ void __launch_bounds__(256) pack_kernel(const __grid_constant__ Pack pack) {
     after_previous();
     let_next_start();
+    const size_t n = pack.arrays[pack.count - 1].end;
     for (size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (size_t)gridDim.x * blockDim.x) {
-        const size_t row = i / pieces;
-        const int col = (int)(i - row * pieces) * 8;
-        const unsigned short *x = (const unsigned short *)from.p + row * from.stride + col;
+        int which = 0;
+        while (i >= pack.arrays[which].end) ++which;
+        const Pack::Array &a = pack.arrays[which];
+        const size_t piece = i - (which > 0 ? pack.arrays[which - 1].end : 0), pieces = a.to_stride / 8;
+        const size_t row = piece / pieces;
+        const int col = (int)(piece - row * pieces) * 8;
+        const unsigned short *x = (const unsigned short *)a.from.p + row * a.from.stride + col;
         uint32_t w[4];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-            const uint32_t low = col + 2 * q < cols ? x[2 * q] : 0, high = col + 2 * q + 1 < cols ? x[2 * q + 1] : 0;
+            const uint32_t low = col + 2 * q < a.cols ? x[2 * q] : 0, high = col + 2 * q + 1 < a.cols ? x[2 * q + 1] : 0;
             w[q] = low | high << 16;
         }
-        ((uint4 *)to)[i] = make_uint4(w[0], w[1], w[2], w[3]);
+        ((uint4 *)a.to)[piece] = make_uint4(w[0], w[1], w[2], w[3]);
     }
 }
 
@@ -405,11 +409,10 @@ cudaError_t launch_product_few(ProductKind kind, uint32_t type, const Product &p
     });
 }
 
-cudaError_t launch_pack_rows(const Matrix &from, size_t rows, size_t cols, void *to, size_t to_stride,
-                             cudaStream_t stream) {
-    const size_t n = rows * (to_stride / 8), blocks = (n + 255) / 256, most = (size_t)geo::device_sm_count() * 32;
-    return launch_after(pack_kernel, (unsigned)(blocks < most ? blocks : most), 256, 0, 1, stream, from, rows, (int)cols,
-                        to, to_stride);
+cudaError_t launch_pack(const Pack &pack, cudaStream_t stream) {
+    if (pack.count == 0) return cudaSuccess;
+    const size_t blocks = (pack.arrays[pack.count - 1].end + 255) / 256, most = (size_t)geo::device_sm_count() * 32;
+    return launch_after(pack_kernel, (unsigned)(blocks < most ? blocks : most), 256, 0, 1, stream, pack);
 }
 
 }  // namespace layers

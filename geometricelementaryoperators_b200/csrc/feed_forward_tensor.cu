@@ -767,7 +767,7 @@ Cut cut_tensor(ProductKind kind, bool twice, size_t m, size_t n, size_t k) {
             const double sums = (double)sums_of(kind, 3) * splits * m * n * 4;
             if (splits > 1 && (waves > 1 || sums > (64 << 20))) break;
             const double cost = waves * ((blocks + splits - 1) / splits * block + 800) + 4000 +
-                                (splits > 1 ? 5000 + sums / 2500 : 0);
+                                (splits > 1 ? 6500 + sums / 1800 : 0);
             if (least < 0 || cost < 0.98 * least) least = cost, best = {bn, pair, (int)splits};
         }
     };
