@@ -40,10 +40,13 @@ constexpr int kBM = 128, kBK = 64;
 // Warps that take the sums out. The VJP's first product reads two more arrays and
 // writes up to six; float32 results of two-term operands are summed up in registers.
 constexpr int epilogue_warps(int kind, bool twice) { return kind == kHidden || twice ? 8 : 4; }
-// Blocks of K that are summed in tensor memory in one go, where the result is float32:
-// the tensor cores cut where float32 arithmetic rounds, which takes 1.8e-5 off the
-// size of sums over 8192 rows. The parts are added up in registers, rounded to nearest.
-constexpr int kChunk = 16;
+// Blocks of K that are summed in tensor memory in one go, where the results are float32
+// or two-term: the tensor cores cut where float32 arithmetic rounds, which takes 2e-8 of
+// the size off with each 16 of K (1.8e-5 over 8192 rows). The parts are added up in
+// registers, rounded to nearest. (VJP of 8192 x 4096 x 12288 to float32 cotangents: 16
+// blocks 5.66 ms and 4.9e-6 off, 8 blocks 5.74 ms, 4 blocks 5.98 ms and 3.6e-6; what two
+// 16-bit terms leave off is 2.2e-6.)
+constexpr int kChunk = 8;
 constexpr uint32_t bytes_a(bool twice) { return (twice ? 2 : 1) * kBM * kBK * 2; }
 constexpr uint32_t bytes_b(int bn) { return (uint32_t)bn * kBK * 2; }
 constexpr uint32_t kRows = 32 * 80;  // a warp's 32 rows of 64 bytes; 16 more keep banks apart
@@ -181,6 +184,19 @@ __device__ __forceinline__ void take_columns(uint32_t address, float (&v)[32]) {
     for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
 
+// And back: 32 columns of this thread's row.
+__device__ __forceinline__ void leave_columns(uint32_t address, const float *v) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(address),
+        "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]), "f"(v[8]), "f"(v[9]),
+        "f"(v[10]), "f"(v[11]), "f"(v[12]), "f"(v[13]), "f"(v[14]), "f"(v[15]), "f"(v[16]), "f"(v[17]), "f"(v[18]),
+        "f"(v[19]), "f"(v[20]), "f"(v[21]), "f"(v[22]), "f"(v[23]), "f"(v[24]), "f"(v[25]), "f"(v[26]), "f"(v[27]),
+        "f"(v[28]), "f"(v[29]), "f"(v[30]), "f"(v[31])
+        : "memory");
+}
+
 // Whether rows of this array can be read and written by 16 bytes.
 template <typename T>
 __device__ __forceinline__ bool by_16(const void *p, size_t stride) {
@@ -311,6 +327,7 @@ __global__ void __launch_bounds__(64 + 32 * epilogue_warps(KIND, TWICE), 1)
                    PipelineStarve starve) {
     constexpr bool kAMn = KIND == kWeights, kBMn = KIND == kHidden || KIND == kInput || KIND == kWeights;
     constexpr int kWarps = epilogue_warps(KIND, TWICE);
+    constexpr bool kInParts = TWICE || (KIND == kHidden && std::is_same_v<O, float>);  // of kChunk blocks
     constexpr int kStages = stages_of(KIND, BN, TWICE, PAIR), kColumns = KIND == kGated ? BN / 2 : BN;  // of the result, a tile
     constexpr uint32_t kBytesA = bytes_a(TWICE), kStageBytes = stage_bytes(BN, TWICE, PAIR), kSumColumns = 2 * BN < 32 ? 32 : 2 * BN;
     extern __shared__ unsigned char memory[];
@@ -425,7 +442,7 @@ __global__ void __launch_bounds__(64 + 32 * epilogue_warps(KIND, TWICE), 1)
             const int last = last_of(t);
             for (int i = first_of(t); i < last && good; ++round) {
                 const uint32_t to = round & 1, use = round >> 1;
-                const int first = i, end = TWICE && last - i > kChunk ? i + kChunk : last;
+                const int first = i, end = kInParts && last - i > kChunk ? i + kChunk : last;
                 good = barrier_wait(taken + 8 * to, (use & 1) ^ 1, starve.polls, &gave_up);
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 for (; i < end && good; ++i, ++step) {
@@ -513,12 +530,13 @@ __global__ void __launch_bounds__(64 + 32 * epilogue_warps(KIND, TWICE), 1)
                 }
                 put_columns<O>(mine, v, from, p.out[KIND == kWeights ? t.problem : 0], row0, col0, p.m, p.n);
             };
-            if constexpr (TWICE) {
-                float sum[kPart];
+            // The sums of all parts of K but the last to be released, in registers.
+            auto add_parts = [&](float (&sum)[kPart]) {
 #pragma unroll
                 for (int j = 0; j < kPart; ++j) sum[j] = 0.0f;
                 const int last = last_of(t);
                 for (int i = first_of(t); i < last; i += kChunk) {
+                    if (i > first_of(t)) release();
                     wait();
 #pragma unroll
                     for (int c = 0; c < kPart; c += 32) {
@@ -527,8 +545,12 @@ __global__ void __launch_bounds__(64 + 32 * epilogue_warps(KIND, TWICE), 1)
 #pragma unroll
                         for (int j = 0; j < 32; ++j) sum[c + j] += v[j];
                     }
-                    release();
                 }
+            };
+            if constexpr (TWICE) {
+                float sum[kPart];
+                add_parts(sum);
+                release();
                 if (row0 < p.m) {
 #pragma unroll
                     for (int c = 0; c < kPart; c += 32) {
@@ -549,7 +571,17 @@ __global__ void __launch_bounds__(64 + 32 * epilogue_warps(KIND, TWICE), 1)
                 };
                 if constexpr (KIND == kHidden)
                     if (p.splits == 1) fetch(begin);
-                wait();
+                if constexpr (kInParts) {
+                    float sum[kPart];
+                    add_parts(sum);
+                    if (good) {  // to where the last part was, for what follows
+#pragma unroll
+                        for (int c = 0; c < kPart; c += 32) leave_columns(at + begin + c, sum + c);
+                        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                    }
+                } else {
+                    wait();
+                }
                 if (row0 < p.m) {
 #pragma unroll 1
                     for (int c = begin; c < begin + kPart; c += 32) {
