@@ -204,20 +204,26 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Produ
 // A token or a few: every weight is read once and that is all the time it takes. A
 // column of the result (kGated: of gate and up) is `split` warps' work, each along its
 // part of K, vectors of 16 bytes side by side; a lane asks for kBatch of them at a time
-// before it multiplies any, and L1 is left to the rows of x. `split` grows until there
-// are warps enough to keep HBM busy. kDown's weights are asked for before the kernel
-// that makes its rows has ended.
+// before it multiplies any, past L1, which is left to the rows of x. `split` grows until
+// there are warps enough to keep HBM busy. kDown's weights are asked for before the
+// kernel that makes its rows has ended: whatever wrote them had ended before that one
+// read anything, and L1 is not asked.
 constexpr int kFewThreads = 256, kFewWarps = kFewThreads / 32;
 
 template <typename T, int V>
 __device__ __forceinline__ Vec<T, V> load_once(const T *p) {
     Vec<T, V> r;
-    if constexpr (Vec<T, V>::kBytes == 16)
-        asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-                     : "=r"(r.w[0]), "=r"(r.w[1]), "=r"(r.w[2]), "=r"(r.w[3])
-                     : "l"(p));
-    else
-        r = load<T, V>(p);
+    if constexpr (Vec<T, V>::kBytes == 16) {
+        const uint4 v = __ldcg(reinterpret_cast<const uint4 *>(p));
+        r.w[0] = v.x, r.w[1] = v.y, r.w[2] = v.z, r.w[3] = v.w;
+    } else if constexpr (Vec<T, V>::kBytes == 8) {
+        const uint2 v = __ldcg(reinterpret_cast<const uint2 *>(p));
+        r.w[0] = v.x, r.w[1] = v.y;
+    } else if constexpr (Vec<T, V>::kBytes == 4) {
+        r.w[0] = __ldcg(reinterpret_cast<const uint32_t *>(p));
+    } else {
+        r.w[0] = __ldcg(reinterpret_cast<const unsigned short *>(p));
+    }
     return r;
 }
 

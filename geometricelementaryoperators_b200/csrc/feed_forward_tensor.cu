@@ -43,14 +43,17 @@ constexpr int epilogue_warps(int kind, bool twice) { return kind == kHidden || t
 // Blocks of K that are summed in tensor memory in one go, where the results are float32
 // or two-term: the tensor cores cut where float32 arithmetic rounds, which takes 2e-8 of
 // the size off with each 16 of K (1.8e-5 over 8192 rows). The parts are added up in
-// registers, rounded to nearest. (VJP of 8192 x 4096 x 12288 to float32 cotangents: 16
-// blocks 5.66 ms and 4.9e-6 off, 8 blocks 5.74 ms, 4 blocks 5.98 ms and 3.6e-6; what two
-// 16-bit terms leave off is 2.2e-6.)
-constexpr int kChunk = 8;
+// registers, rounded to nearest. (VJP of 8192 x 4096 x 12288 to float32 cotangents, this
+// many blocks in the last product alone: 16 blocks 5.66 ms, 8 blocks 5.74, 4 blocks 5.98;
+// 16 in both products leave 3.7e-6 off, of which what two 16-bit terms lose is 2.2e-6.)
+constexpr int kChunk = 16;
 constexpr uint32_t bytes_a(bool twice) { return (twice ? 2 : 1) * kBM * kBK * 2; }
 constexpr uint32_t bytes_b(int bn) { return (uint32_t)bn * kBK * 2; }
-constexpr uint32_t kRows = 32 * 80;  // a warp's 32 rows of 64 bytes; 16 more keep banks apart
-constexpr uint32_t staging_of(int kind) { return kind == kHidden ? 3 * kRows : kRows; }  // of a warp
+// A warp's shared memory: 32 rows of 64 bytes, 16 more bytes a row to keep banks apart.
+// kHidden: two of those for what it reads, and two of 32 x 64 bytes (swizzled, so that a
+// copy of the whole can take them out) for what it writes.
+constexpr uint32_t kRows = 32 * 80, kBox = 32 * 64;
+constexpr uint32_t staging_of(int kind) { return kind == kHidden ? 2 * kBox + 2 * kRows : kRows; }
 constexpr uint32_t kSharedMost = 227 * 1024;
 // A block's part of a stage.
 constexpr uint32_t stage_bytes(int bn, bool twice, bool pair) { return bytes_a(twice) + bytes_b(bn) / (pair ? 2 : 1); }
@@ -69,6 +72,7 @@ __host__ __device__ constexpr int box_rows(int m) { return m < kBM ? (m + 7) / 8
 
 struct Maps {
     CUtensorMap a[3], b[3], low[3];
+    CUtensorMap out[6];  // kHidden: out[0], out_low[0], out[1], ...
 };
 
 __device__ __forceinline__ void barrier_init(uint32_t barrier, uint32_t count) {
@@ -236,6 +240,28 @@ __device__ __forceinline__ void put_words(unsigned char *staging, const uint32_t
                     ((const O *)(staging + r * kPitch))[lane % kWidth];
     }
     __syncwarp();
+}
+// Writes 32 columns of 16-bit values of this thread's row as a box of the array that
+// `map` describes (columns and rows from col0 and row0), which its ends clip: one copy
+// for the warp instead of the loads and stores of put_words. `box`: the next of the
+// warp's two boxes, which the copy before the last one has read.
+__device__ __forceinline__ void put_box(unsigned char *box, const uint32_t (&words)[16], const CUtensorMap *map, int row0,
+                                        int col0) {
+    const int lane = threadIdx.x & 31;
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < 4; ++j)  // 64-byte swizzle
+        *(uint4 *)(box + lane * 64 + (j ^ (lane >> 1 & 3)) * 16) =
+            make_uint4(words[4 * j], words[4 * j + 1], words[4 * j + 2], words[4 * j + 3]);
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncwarp();
+    if (lane == 0) {
+        asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(col0),
+                     "r"(row0), "r"(shared_address(box))
+                     : "memory");
+        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+    }
 }
 // Two neighbours as a word of 16-bit values.
 template <typename T>
@@ -565,8 +591,8 @@ __global__ void __launch_bounds__(64 + 32 * epilogue_warps(KIND, TWICE), 1)
             } else {
                 auto fetch = [&](int c) {
                     const int col0 = t.column * kColumns + c;
-                    fetch_columns<T>(mine + kRows, p.saved[0], row0, col0, p.m, p.n);
-                    fetch_columns<T>(mine + 2 * kRows, p.saved[1], row0, col0, p.m, p.n);
+                    fetch_columns<T>(mine + 2 * kBox, p.saved[0], row0, col0, p.m, p.n);
+                    fetch_columns<T>(mine + 2 * kBox + kRows, p.saved[1], row0, col0, p.m, p.n);
                     commit_async();
                 };
                 if constexpr (KIND == kHidden)
@@ -614,8 +640,8 @@ __global__ void __launch_bounds__(64 + 32 * epilogue_warps(KIND, TWICE), 1)
                             float g[32], u[32];
                             wait_async<0>();
                             __syncwarp();
-                            get_columns<T>(mine + kRows, g);
-                            get_columns<T>(mine + 2 * kRows, u);
+                            get_columns<T>(mine + 2 * kBox, g);
+                            get_columns<T>(mine + 2 * kBox + kRows, u);
                             __syncwarp();
                             if (c + 32 < begin + kPart) fetch(c + 32);  // on its way meanwhile
                             uint32_t words[3][kTerms][16];
@@ -639,14 +665,18 @@ __global__ void __launch_bounds__(64 + 32 * epilogue_warps(KIND, TWICE), 1)
                                     }
                                 }
                             });
+                            int box = 0;
 #pragma unroll
                             for (int n = 0; n < 3; ++n) {
                                 if (p.out[n].p != nullptr)
-                                    put_words<T>(mine, words[n][0], p.out[n], row0, col0, p.m, p.n);
+                                    put_box(mine + (box++ & 1) * kBox, words[n][0], &maps.out[2 * n], row0, col0);
                                 if constexpr (kTerms == 2)
                                     if (p.out_low[n].p != nullptr)
-                                        put_words<T>(mine, words[n][1], p.out_low[n], row0, col0, p.m, p.n);
+                                        put_box(mine + (box++ & 1) * kBox, words[n][1], &maps.out[2 * n + 1], row0, col0);
                             }
+                            // The boxes in turn from chunk to chunk: an odd one out waits for both.
+                            if (box & 1)
+                                if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
                         } else {
                             put(v, 0, col0);
                         }
@@ -656,6 +686,8 @@ __global__ void __launch_bounds__(64 + 32 * epilogue_warps(KIND, TWICE), 1)
             }
         }
     }
+    if constexpr (KIND == kHidden)
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     __syncwarp();
     everyone();
     if (warp == 1) {
@@ -682,15 +714,15 @@ PFN_cuTensorMapEncodeTiled_v12000 map_encoder() {
     return fn;
 }
 
-// [rows][cols] in boxes of box_rows rows by 64 values (128 bytes, swizzled); zeros outside.
-bool encode(CUtensorMap *map, bool bfloat, const Matrix &x, int rows, int cols, int box_rows) {
+// [rows][cols] in boxes of box_rows rows by 64 values (128 bytes, swizzled), or 32; zeros outside.
+bool encode(CUtensorMap *map, bool bfloat, const Matrix &x, int rows, int cols, int box_rows, int box_cols = 64) {
     const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
     const cuuint64_t strides[1] = {(cuuint64_t)x.stride * 2};
-    const cuuint32_t box[2] = {64, (cuuint32_t)box_rows};
+    const cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows};
     const cuuint32_t each[2] = {1, 1};
     return map_encoder()(map, bfloat ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
                          const_cast<void *>(x.p), dims, strides, box, each, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         box_cols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
@@ -712,6 +744,13 @@ cudaError_t launch_tiles(const Product &p, PipelineStarve starve, cudaStream_t s
     for (int i = 0; i < pairs_b; ++i)
         good = good && (kBMn ? encode(&maps.b[i], kBfloat, p.b[i], p.k, p.n, kBK)
                              : encode(&maps.b[i], kBfloat, p.b[i], p.n, p.k, KIND == kGated || PAIR ? BN / 2 : BN));
+    if constexpr (KIND == kHidden)
+        for (int i = 0; i < 3; ++i) {
+            if (p.out[i].p != nullptr)
+                good = good && encode(&maps.out[2 * i], kBfloat, {p.out[i].p, p.out[i].stride}, p.m, p.n, 32, 32);
+            if (p.out_low[i].p != nullptr)
+                good = good && encode(&maps.out[2 * i + 1], kBfloat, {p.out_low[i].p, p.out_low[i].stride}, p.m, p.n, 32, 32);
+        }
     if (!good) return cudaErrorInvalidValue;
     constexpr int kRowsAtOnce = PAIR ? 2 * kBM : kBM;
     const int down = (p.m + kRowsAtOnce - 1) / kRowsAtOnce, across = (p.n + kColumns - 1) / kColumns;

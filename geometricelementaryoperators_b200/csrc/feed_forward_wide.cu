@@ -1,8 +1,9 @@
 // feed_forward_wide.cu -- the feed-forward block's products of float32 and float64
 // (geo/geo_b200.h section 5).
 //
-// C = A B over tiles of 128 rows by 64 (float64) or 128 (float32) columns, 256 threads a
-// tile, 16 of K at a time through a ring of three or four stages that asynchronous
+// C = A B over tiles of 128 rows (32 where there are no more than 64, whose time is the
+// weights' and what is multiplied for nothing) by 64 (float64) or 128 (float32) columns,
+// 256 threads a tile, 16 of K at a time through a ring of three or four stages that asynchronous
 // copies fill (16 bytes each, 8 or 4 where rows are off 16 bytes; zeros past the ends).
 // Multiply-adds bound both types. What they need from shared memory comes next, so each
 // type's tiles are read in the way that takes the fewest bytes a multiply-add:
@@ -20,7 +21,8 @@ namespace layers {
 
 namespace {
 
-constexpr int kThreads = 256, kBM = 128, kBK = 16;
+constexpr int kThreads = 256, kBK = 16;
+constexpr int tile_rows(size_t m) { return m <= 64 ? 32 : 128; }
 template <typename T>
 constexpr int kBN = sizeof(T) == 8 ? 64 : 128;
 template <typename T>
@@ -30,8 +32,12 @@ constexpr int pitch_mn(int rows) { return rows + 4; }  // of a row along M or N
 constexpr int held(int rows) {             // values of an operand's part of a stage, either way
     return rows * kPitchK > kBK * pitch_mn(rows) ? rows * kPitchK : kBK * pitch_mn(rows);
 }
-template <typename T>
-constexpr size_t kShared = (size_t)kStages<T> * (held(kBM) + held(kBN<T>)) * sizeof(T);
+// The ring, or the tile of sums that is left there at the end.
+template <typename T, int BM>
+constexpr size_t kShared =
+    ((size_t)kStages<T> * (held(BM) + held(kBN<T>)) > (size_t)BM * (kBN<T> + 1)
+         ? (size_t)kStages<T> * (held(BM) + held(kBN<T>))
+         : (size_t)BM * (kBN<T> + 1)) * sizeof(T);
 
 // BYTES at most, `valid` of them (zeros else).
 template <int BYTES>
@@ -49,8 +55,10 @@ template <typename T, int ROWS, bool K_MAJOR, int BYTES, typename F>
 __device__ __forceinline__ void fetch(uint32_t to, int k0, int k, int rows, F &&row_of) {
     constexpr int V = BYTES / (int)sizeof(T), kPerLine = (K_MAJOR ? kBK : ROWS) / V, kPieces = ROWS * kBK / V;
 #pragma unroll
-    for (int e = 0; e < kPieces / kThreads; ++e) {
-        const int n = threadIdx.x + e * kThreads, line = n / kPerLine, at = n % kPerLine * V;
+    for (int e = 0; e < (kPieces + kThreads - 1) / kThreads; ++e) {
+        const int n = threadIdx.x + e * kThreads;
+        if (kPieces % kThreads != 0 && n >= kPieces) break;
+        const int line = n / kPerLine, at = n % kPerLine * V;
         const int tile_row = K_MAJOR ? line : at, kk = k0 + (K_MAJOR ? at : line);
         const Matrix *m;
         int row;
@@ -69,62 +77,68 @@ __device__ __forceinline__ void multiply(double (&c)[2], double a, double b) {
                  : "d"(a), "d"(b));
 }
 
-// The sums of one thread. add(): a stage's 16 of K. each(f): f(tile row, tile column, sum).
-template <typename T, bool A_K, bool B_K>
+// The sums of one thread, kCount of them, and where they stand in the tile. add(): a stage's 16 of K.
+template <typename T, int BM, bool A_K, bool B_K>
 struct Sums;
 
-template <bool A_K, bool B_K>
-struct Sums<double, A_K, B_K> {
-    double c[4][4][2];
-    int lane, row, col;  // of the warp's 32 x 32
+// A warp holds 32 rows by 32 columns (8 where the tile has 32 rows).
+template <int BM, bool A_K, bool B_K>
+struct Sums<double, BM, A_K, B_K> {
+    static constexpr int kJ = BM == 128 ? 4 : 1, kCount = 4 * kJ * 2;
+    static constexpr int kTurn = 8;  // kGated: eight columns of gate, eight of up in turn
+    double c[4][kJ][2];
+    int lane, row, col;
     __device__ __forceinline__ Sums() : lane(threadIdx.x & 31) {
         const int warp = threadIdx.x >> 5;
-        row = warp % 4 * 32;
-        col = warp / 4 * 32;
+        row = warp % (BM / 32) * 32;
+        col = warp / (BM / 32) * kJ * 8;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) c[i][j][0] = c[i][j][1] = 0.0;
+            for (int j = 0; j < kJ; ++j) c[i][j][0] = c[i][j][1] = 0.0;
     }
     __device__ __forceinline__ void add(const double *a, const double *b) {
 #pragma unroll
         for (int k = 0; k < kBK; k += 4) {
-            double fa[4], fb[4];
+            double fa[4], fb[kJ];
             const int kk = k + lane % 4;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int m = row + i * 8 + lane / 4, n = col + i * 8 + lane / 4;
-                fa[i] = a[A_K ? m * kPitchK + kk : kk * pitch_mn(kBM) + m];
-                fb[i] = b[B_K ? n * kPitchK + kk : kk * pitch_mn(kBN<double>) + n];
+                const int m = row + i * 8 + lane / 4;
+                fa[i] = a[A_K ? m * kPitchK + kk : kk * pitch_mn(BM) + m];
+            }
+#pragma unroll
+            for (int j = 0; j < kJ; ++j) {
+                const int n = col + j * 8 + lane / 4;
+                fb[j] = b[B_K ? n * kPitchK + kk : kk * pitch_mn(kBN<double>) + n];
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) multiply(c[i][j], fa[i], fb[j]);
+                for (int j = 0; j < kJ; ++j) multiply(c[i][j], fa[i], fb[j]);
         }
     }
-    // Sums 0 ... kCount - 1 of the thread: where they stand, and their values.
-    static constexpr int kCount = 32;
-    __device__ __forceinline__ int row_at(int n) const { return row + n / 8 * 8 + lane / 4; }
-    __device__ __forceinline__ int column_at(int n) const { return col + n % 8 / 2 * 8 + lane % 4 * 2 + n % 2; }
-    __device__ __forceinline__ double at(int n) const { return c[n / 8][n % 8 / 2][n % 2]; }
-    // kGated: eight columns of gate, eight of up in turn.
-    static constexpr int kTurn = 8;
+    __device__ __forceinline__ int row_at(int n) const { return row + n / (2 * kJ) * 8 + lane / 4; }
+    __device__ __forceinline__ int column_at(int n) const { return col + n % (2 * kJ) / 2 * 8 + lane % 4 * 2 + n % 2; }
+    __device__ __forceinline__ double at(int n) const { return c[n / (2 * kJ)][n % (2 * kJ) / 2][n % 2]; }
 };
 
-template <bool A_K, bool B_K>
-struct Sums<float, A_K, B_K> {
+// A thread holds 8 x 8 (4 x 4 where the tile has 32 rows), in groups of four either way.
+template <int BM, bool A_K, bool B_K>
+struct Sums<float, BM, A_K, B_K> {
     static constexpr bool kAlongK = A_K && B_K;
-    Pair<float> c[8][kAlongK ? 8 : 4];
+    static constexpr int kI = BM == 128 ? 8 : 4, kJ = kI, kCount = kI * kJ;
+    static constexpr int kTurn = 64;  // kGated: 64 columns of gate, then 64 of up
+    Pair<float> c[kI][kAlongK ? kJ : kJ / 2];
     int lane, row, col;
     __device__ __forceinline__ Sums() : lane(threadIdx.x & 31) {
         const int warp = threadIdx.x >> 5;
-        row = warp % 2 * 64;
-        col = warp / 2 * 16;
+        row = BM == 128 ? warp % 2 * 64 : 0;
+        col = BM == 128 ? warp / 2 * 16 : warp * 16;
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
+        for (int i = 0; i < kI; ++i)
 #pragma unroll
-            for (int j = 0; j < (kAlongK ? 8 : 4); ++j) c[i][j] = both(0.0f);
+            for (int j = 0; j < (kAlongK ? kJ : kJ / 2); ++j) c[i][j] = both(0.0f);
     }
     __device__ __forceinline__ int row_of(int i) const {
         return row + i / 4 * 32 + (A_K ? i % 4 * 8 + lane / 4 : lane / 4 * 4 + i % 4);
@@ -135,57 +149,56 @@ struct Sums<float, A_K, B_K> {
     __device__ __forceinline__ void add(const float *a, const float *b) {
 #pragma unroll
         for (int k = 0; k < kBK; k += 4) {
-            Vec<float, 4> fa[8];  // A_K: four of K of each row; else four rows of each k, twice
+            Vec<float, 4> fa[kI];  // A_K: four of K of each row; else four rows (and four more) of each of four k
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
+            for (int i = 0; i < kI; ++i)
                 fa[i] = A_K ? load<float, 4>(a + row_of(i) * kPitchK + k)
-                            : load<float, 4>(a + (k + i / 2) * pitch_mn(kBM) + row_of(i % 2 * 4));
+                            : load<float, 4>(a + (k + i / (kI / 4)) * pitch_mn(BM) + row_of(i % (kI / 4) * 4));
             if constexpr (kAlongK) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
+                for (int j = 0; j < kJ; ++j) {
                     const Vec<float, 4> fb = load<float, 4>(b + col_of(j) * kPitchK + k);
 #pragma unroll
                     for (int q = 0; q < 2; ++q)
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) c[i][j] = fma(fa[i].pair(q), fb.pair(q), c[i][j]);
+                        for (int i = 0; i < kI; ++i) c[i][j] = fma(fa[i].pair(q), fb.pair(q), c[i][j]);
                 }
             } else {
                 static_assert(!B_K, "columns lie side by side");
 #pragma unroll
                 for (int kk = 0; kk < 4; ++kk) {
-                    Vec<float, 4> fb[2];
+                    Vec<float, 4> fb[kJ / 4];
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) fb[h] = load<float, 4>(b + (k + kk) * pitch_mn(kBN<float>) + col_of(4 * h));
+                    for (int h = 0; h < kJ / 4; ++h)
+                        fb[h] = load<float, 4>(b + (k + kk) * pitch_mn(kBN<float>) + col_of(4 * h));
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const Pair<float> two = A_K ? fa[i].pair(kk / 2) : fa[kk * 2 + i / 4].pair(i % 4 / 2);
+                    for (int i = 0; i < kI; ++i) {
+                        const Pair<float> two = A_K ? fa[i].pair(kk / 2) : fa[kk * (kI / 4) + i / 4].pair(i % 4 / 2);
                         const float v = (A_K ? kk : i) % 2 ? two.y : two.x;
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) c[i][j] = fma(both(v), fb[j / 2].pair(j % 2), c[i][j]);
+                        for (int j = 0; j < kJ / 2; ++j) c[i][j] = fma(both(v), fb[j / 2].pair(j % 2), c[i][j]);
                     }
                 }
             }
         }
     }
-    static constexpr int kCount = 64;
-    __device__ __forceinline__ int row_at(int n) const { return row_of(n / 8); }
-    __device__ __forceinline__ int column_at(int n) const { return col_of(n % 8); }
+    __device__ __forceinline__ int row_at(int n) const { return row_of(n / kJ); }
+    __device__ __forceinline__ int column_at(int n) const { return col_of(n % kJ); }
     __device__ __forceinline__ float at(int n) const {
         if constexpr (kAlongK)
-            return c[n / 8][n % 8].x + c[n / 8][n % 8].y;
+            return c[n / kJ][n % kJ].x + c[n / kJ][n % kJ].y;
         else
-            return n % 2 ? c[n / 8][n % 8 / 2].y : c[n / 8][n % 8 / 2].x;
+            return n % 2 ? c[n / kJ][n % kJ / 2].y : c[n / kJ][n % kJ / 2].x;
     }
-    static constexpr int kTurn = 64;
 };
 
 // Up to 128 registers a thread in float64, so that two blocks share a multiprocessor.
-template <typename T, int KIND, int BYTES>
+template <typename T, int KIND, int BYTES, int kBM>
 __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 2 : 1)
     wide_kernel(const __grid_constant__ Product p, int down, int across, int tiles) {
     constexpr bool kAK = KIND != kWeights, kBK_ = KIND == kGated || KIND == kDown;
     constexpr int BN = kBN<T>, kColumns = KIND == kGated ? BN / 2 : BN;
-    using S = Sums<T, kAK, kBK_>;
+    using S = Sums<T, kBM, kAK, kBK_>;
     extern __shared__ __align__(16) unsigned char memory[];
     T *const stages = (T *)memory;
     constexpr int kStage = held(kBM) + held(BN);
@@ -235,7 +248,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 2 : 1)
         // thread's sums (float64's functions are long: the VJP's first product of 16384 x 64
         // through 256 hidden values, GELU, 192 us so).
         constexpr int kPitch = BN + 1;
-        static_assert((size_t)kBM * kPitch * sizeof(T) <= kShared<T>, "the tile fits the ring");
+        static_assert((size_t)kBM * kPitch * sizeof(T) <= kShared<T, kBM>, "the tile fits the ring");
         wait_async<0>();
         __syncthreads();
 #pragma unroll
@@ -262,17 +275,17 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 8 ? 2 : 1)
     }
 }
 
-template <typename T, int KIND, int BYTES>
-cudaError_t launch_bytes(const Product &p, cudaStream_t stream) {
+template <typename T, int KIND, int BYTES, int kBM>
+cudaError_t launch_tiles(const Product &p, cudaStream_t stream) {
     constexpr int kColumns = KIND == kGated ? kBN<T> / 2 : kBN<T>;
     const int down = (p.m + kBM - 1) / kBM, across = (p.n + kColumns - 1) / kColumns;
     const long long tiles = (long long)down * across * p.problems * p.splits;
     if (tiles > INT32_MAX) return cudaErrorInvalidValue;
-    const auto kernel = wide_kernel<T, KIND, BYTES>;
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kShared<T>);
+    const auto kernel = wide_kernel<T, KIND, BYTES, kBM>;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kShared<T, kBM>);
     if (e != cudaSuccess) return e;
     const long long most = (long long)geo::device_sm_count() * (sizeof(T) == 8 ? 2 : 1);
-    return launch_after(kernel, (unsigned)(tiles < most ? tiles : most), kThreads, kShared<T>, 1, stream, p, down, across,
+    return launch_after(kernel, (unsigned)(tiles < most ? tiles : most), kThreads, kShared<T, kBM>, 1, stream, p, down, across,
                         (int)tiles);
 }
 
@@ -285,7 +298,12 @@ cudaError_t launch_kind(const Product &p, cudaStream_t stream) {
     };
     for (int i = 0; i < (KIND == kInput ? 2 : p.problems); ++i) look(p.a[i]);
     for (int i = 0; i < (KIND == kInput || KIND == kGated ? 2 : p.problems); ++i) look(p.b[i]);
-    return whole ? launch_bytes<T, KIND, 16>(p, stream) : launch_bytes<T, KIND, (int)sizeof(T)>(p, stream);
+    auto launch = [&](auto bytes) {
+        constexpr int kBytes = decltype(bytes)::value;
+        return tile_rows(p.m) == 32 ? launch_tiles<T, KIND, kBytes, 32>(p, stream)
+                                    : launch_tiles<T, KIND, kBytes, 128>(p, stream);
+    };
+    return whole ? launch(std::integral_constant<int, 16>{}) : launch(std::integral_constant<int, (int)sizeof(T)>{});
 }
 
 template <typename T>
@@ -308,7 +326,7 @@ cudaError_t launch_type(ProductKind kind, const Product &p, cudaStream_t stream)
 Cut cut_wide(ProductKind kind, uint32_t type, size_t m, size_t n, size_t k) {
     const bool f64 = type == GEO_B200_F64;
     const size_t wide = (f64 ? kBN<double> : kBN<float>) / (kind == kGated ? 2 : 1);
-    const size_t tiles = (kind == kWeights ? 3 : 1) * ((m + kBM - 1) / kBM) * ((n + wide - 1) / wide);
+    const size_t tiles = (kind == kWeights ? 3 : 1) * ((m + tile_rows(m) - 1) / tile_rows(m)) * ((n + wide - 1) / wide);
     const size_t wanted = (size_t)geo::device_sm_count() * (f64 ? 2 : 1) / tiles, most = k * (kind == kInput ? 2 : 1) / 128;
     const size_t splits = wanted < most ? wanted : most;
     return {(int)wide, false, splits < 1 ? 1 : (splits < 64 ? (int)splits : 64)};

@@ -6,8 +6,8 @@
 // byte of gradients, less what the second pass still finds in L2: it goes backwards.
 // A gradient is cut into pieces of 16 KB, whatever its type; the list travels in the
 // kernel's parameters (nothing to copy or keep, graphs capture it), a block finds a
-// piece's gradient by bisection. Squares and their sums are float64, in which no
-// smaller type's value overflows or vanishes. Each block leaves one partial sum; the
+// piece's gradient by bisection. Sums are float64, in which no smaller type's square
+// overflows or vanishes. Each block leaves one partial sum; the
 // second pass's blocks add them up in the same order each.
 #include <cuda.h>
 #include <cudaTypedefs.h>
@@ -45,15 +45,26 @@ struct Table {
     Entry entries[CAPACITY];
 };
 
-// Squares of V adjacent values: exact but for the sums' own roundings (a float32's square has 48 bits).
+// The square of a value, to be summed in float64: exact for the 16-bit types, rounded to
+// its own type otherwise, but exact for a float32 value whose square leaves float32's
+// range.
+template <typename T>
+__device__ __forceinline__ double square(Wide<T> v) {
+    if constexpr (std::is_same_v<T, float>) {
+        const float s = __fmul_rn(v, v);
+        return s > 0x1p-100f && s < 0x1p126f ? (double)s : (double)v * (double)v;
+    } else {
+        return (double)v * (double)v;
+    }
+}
 template <typename T, int V>
 __device__ __forceinline__ double squares(const Vec<T, V> &v) {
     double even = 0, odd = 0;
 #pragma unroll
     for (int q = 0; q < V / 2; ++q) {
-        const double a = v.pair(q).x, b = v.pair(q).y;
-        even = ::fma(a, a, even);
-        odd = ::fma(b, b, odd);
+        const Pair<Wide<T>> p = v.pair(q);
+        even += square<T>(p.x);
+        odd += square<T>(p.y);
     }
     return even + odd;
 }
@@ -81,8 +92,7 @@ __device__ double piece_squares(const Entry &e, uint32_t piece) {
         for (int i = 0; i < kEach; ++i) sum += squares<T, V>(v[i]);
     } else {
         for (size_t i = first + threadIdx.x; i < last; i += kThreads) {
-            const double v = (double)widen(g[i]);
-            sum = ::fma(v, v, sum);
+            sum += square<T>(widen(g[i]));
         }
     }
     return sum;

@@ -22,8 +22,12 @@
  *  4. Sparse fixed-multivector operators over a batch (reference
  *     src/operator_kernel.c:191-334, geo_operator_apply_*_f64 and VJPs).
  *  5. Layer operators over rows of coefficients (no counterpart in the
- *     reference): layer norm, dropout, the two fused with a residual, and
- *     rotary positions, each with its VJP; float64, float32, bfloat16, float16.
+ *     reference): layer norm, dropout, the two fused with a residual, rotary
+ *     positions, RMS norm, the norms before and after a block with its gate and
+ *     residual, and a gated feed-forward block, each with its VJP; float64,
+ *     float32, bfloat16, float16.
+ *  6. The norm over all gradients of a model, and clipping (no counterpart in
+ *     the reference).
  *
  * All device-pointer calls are asynchronous on the given stream; host-pointer
  * calls are synchronous. Arrays are sample-major [batch][2^n].
@@ -718,8 +722,9 @@ geo_b200_status_t geo_b200_feed_forward_wait_selftest(
 /* Norm over all gradients of a model, and clipping before the update:
  *   norm = sqrt(sum of squares of every value of every gradient),
  *   scale = min(1, max_norm / norm)  (1 for a norm of 0),  clipped = scale gradient,
- * each value rounded once to its type. Squares are summed in float64, in a fixed order:
- * the same call gives the same bits. A norm that is infinite or NaN (a gradient is) makes
+ * each value rounded once to its type. Squares (of float32 values rounded to float32
+ * where they are in its range) are summed in float64, in a fixed order: the same call
+ * gives the same bits. A norm that is infinite or NaN (a gradient is) makes
  * scale NaN; the clipped values are then scale times gradient, NaN as well: the
  * update must not be made. Asynchronous and allocating nothing as section 5. */
 typedef struct {
