@@ -98,9 +98,10 @@ struct Space {
 // (feed_forward_plain.cu). Of 16-bit types the tensor cores' tiles take over early
 // (4096 x 12288 bfloat16: 2 rows 70 us either way, 4 rows 95 and 70), later where the
 // weights are small (1024 x 2048: 4 rows 14 us, 5 rows in tiles 22) or would have to be
-// copied first.
+// copied first; of float64 before 8 rows (2048 x 4096: 107 us, 9 rows in tiles 99), of
+// float32 beyond (56 and 88 us).
 bool few_rows(const geo_b200_feed_forward_config_t &c) {
-    if (type_bytes(c.type) != 2) return c.rows <= (size_t)kFewRows;
+    if (type_bytes(c.type) != 2) return c.rows <= (size_t)(c.type == GEO_B200_F64 ? kFewRows / 2 : kFewRows);
     const bool copied = c.gate_weight_stride % 8 != 0 || c.up_weight_stride % 8 != 0 || c.down_weight_stride % 8 != 0;
     return c.rows <= 2 || (c.rows <= 4 && (copied || c.cols * c.hidden <= (size_t)1 << 22));
 }

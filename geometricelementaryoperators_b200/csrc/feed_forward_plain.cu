@@ -161,19 +161,25 @@ cudaError_t launch_tile(const Product &p, cudaStream_t stream) {
 
 // ---- parts of K -----------------------------------------------------------------------
 
-// Adds the parts of K up, in order, four columns a thread, and does with the sums what
-// the kernel that made them does where K is whole.
-template <typename T, typename O, int KIND>
+// Adds the parts of K up, four columns a thread, and does with the sums what the kernel
+// that made them does where K is whole. LANES: that many threads share the parts of a
+// place, each every so many in order, and add theirs up as a tree (three results of 256 x
+// 64 float64 in 49 parts: 28 us by one thread each).
+template <typename T, typename O, int KIND, int LANES>
 __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Product p) {
     using W = Wide<T>;
-    constexpr int kSums = KIND == kGated ? 2 : 1, V = 16 / (int)sizeof(W);
+    constexpr int kSums = KIND == kGated ? 2 : 1, V = 16 / (int)sizeof(W), kPlaces = 256 / LANES;
     after_previous();
     let_next_start();
     const size_t stride = partial_stride(p.n), groups = stride / 4, each = (size_t)p.m * groups;
-    const size_t part = (size_t)p.m * stride;
-    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < each * p.problems; i += (size_t)gridDim.x * 256) {
-        const int problem = (int)(i / each);
-        const size_t row = (i - problem * each) / groups, col = (i - problem * each) % groups * 4;
+    const size_t part = (size_t)p.m * stride, all = each * p.problems;
+    // The threads of a place are neighbours in a warp; all of them go through the same rounds.
+    const int lane = threadIdx.x % LANES;
+    for (size_t first = (size_t)blockIdx.x * kPlaces; first < all; first += (size_t)gridDim.x * kPlaces) {
+        const size_t i = first + threadIdx.x / LANES;
+        const bool live = i < all;
+        const int problem = live ? (int)(i / each) : 0;
+        const size_t place = live ? i - problem * each : 0, row = place / groups, col = place % groups * 4;
         W sum[kSums][4];
 #pragma unroll
         for (int z = 0; z < kSums; ++z) {
@@ -181,18 +187,22 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Produ
 #pragma unroll
             for (int j = 0; j < 4; ++j) sum[z][j] = W(0);
 #pragma unroll 4
-            for (int s = 0; s < p.splits; ++s, from += part)
+            for (int s = lane; s < p.splits; s += LANES)
 #pragma unroll
                 for (int v = 0; v < 4 / V; ++v) {
-                    const Vec<W, V> piece = load<W, V>(from + v * V);
+                    const Vec<W, V> piece = load<W, V>(from + s * part + v * V);
 #pragma unroll
                     for (int q = 0; q < V / 2; ++q) {
                         sum[z][v * V + 2 * q] += piece.pair(q).x;
                         sum[z][v * V + 2 * q + 1] += piece.pair(q).y;
                     }
                 }
+#pragma unroll
+            for (int o = LANES / 2; o > 0; o /= 2)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) sum[z][j] += __shfl_xor_sync(0xffffffffu, sum[z][j], o);
         }
-        const int held = (size_t)p.n - col < 4 ? (int)((size_t)p.n - col) : 4;
+        const int held = !live || lane != 0 ? 0 : ((size_t)p.n - col < 4 ? (int)((size_t)p.n - col) : 4);
 #pragma unroll
         for (int j = 0; j < 4; ++j)
             if (j < held) finish<T, O, KIND>(p, problem, row, col + j, sum[0][j], sum[kSums - 1][j]);
@@ -203,19 +213,28 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Produ
 
 // A token or a few: every weight is read once and that is all the time it takes. A
 // column of the result (kGated: of gate and up) is `split` warps' work, each along its
-// part of K, vectors of 16 bytes side by side; a lane asks for kBatch of them at a time
-// before it multiplies any, past L1, which is left to the rows of x. `split` grows until
+// part of K, vectors of 16 bytes side by side; a lane has kBatch of them on their way,
+// past L1, which is left to the rows of x. `split` grows until
 // there are warps enough to keep HBM busy. kDown's weights are asked for before the
 // kernel that makes its rows has ended: whatever wrote them had ended before that one
 // read anything, and L1 is not asked.
 constexpr int kFewThreads = 256, kFewWarps = kFewThreads / 32;
 
-template <typename T, int V>
+// Volatile: all of a batch before anything waits for one. EARLY: before the kernel before
+// this one has ended; L1, which might hold what was there before, is passed by. (Later
+// loads only do not stay in it: .cg for all of them takes 64 us for one token of 4096 x
+// 12288 bfloat16, 58 so.)
+template <bool EARLY, typename T, int V>
 __device__ __forceinline__ Vec<T, V> load_once(const T *p) {
     Vec<T, V> r;
-    if constexpr (Vec<T, V>::kBytes == 16) {
-        const uint4 v = __ldcg(reinterpret_cast<const uint4 *>(p));
-        r.w[0] = v.x, r.w[1] = v.y, r.w[2] = v.z, r.w[3] = v.w;
+    if constexpr (Vec<T, V>::kBytes == 16 && EARLY) {
+        asm volatile("ld.global.cg.v4.u32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(r.w[0]), "=r"(r.w[1]), "=r"(r.w[2]), "=r"(r.w[3])
+                     : "l"(p));
+    } else if constexpr (Vec<T, V>::kBytes == 16) {
+        asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(r.w[0]), "=r"(r.w[1]), "=r"(r.w[2]), "=r"(r.w[3])
+                     : "l"(p));
     } else if constexpr (Vec<T, V>::kBytes == 8) {
         const uint2 v = __ldcg(reinterpret_cast<const uint2 *>(p));
         r.w[0] = v.x, r.w[1] = v.y;
@@ -233,6 +252,9 @@ __global__ void __launch_bounds__(kFewThreads) few_kernel(const __grid_constant_
     // Several rows: as many columns a warp as make four streams of weights, which share what is read of the rows.
     constexpr int kOperands = KIND == kGated ? 2 : 1, kColumns = ROWS == 1 ? 1 : 4 / kOperands;
     constexpr int kStreams = kOperands * kColumns, V = ALIGNED ? 16 / (int)sizeof(T) : 1, kBatch = 8 / kStreams;
+    // Up to two rows: the next vector as soon as one is used; more: a batch at a time (4096 x 12288 bfloat16, 2 rows 69
+    // and 79 us; 2048 x 4096 float64, 4 rows 72 and 66).
+    constexpr bool kRoll = ROWS <= 2;
     __shared__ W parts[kFewWarps][kStreams * ROWS];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int part = warp % split, columns = kFewWarps / split * kColumns;  // of the block
@@ -250,15 +272,14 @@ __global__ void __launch_bounds__(kFewThreads) few_kernel(const __grid_constant_
     }
     const int step = 32 * V * split, first = (part * 32 + lane) * V, last = col < p.n ? p.k : 0;
     Vec<T, V> piece[kBatch][kStreams];
-    auto ask = [&](int k) {
+    auto ask = [&](auto early, int i, int k) {
 #pragma unroll
-        for (int i = 0; i < kBatch; ++i)
-#pragma unroll
-            for (int o = 0; o < kStreams; ++o)
-                piece[i][o] = k + i * step < last ? load_once<T, V>(w[o] + k + i * step) : Vec<T, V>::zero();
+        for (int o = 0; o < kStreams; ++o)
+            piece[i][o] = k < last ? load_once<decltype(early)::value, T, V>(w[o] + k) : Vec<T, V>::zero();
     };
     if (KIND == kGated) after_previous();
-    ask(first);
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) ask(std::bool_constant<KIND == kDown>{}, i, first + i * step);
     if (KIND == kDown) after_previous();
     let_next_start();
     for (int k = first; k < last; k += kBatch * step) {
@@ -281,8 +302,13 @@ __global__ void __launch_bounds__(kFewThreads) few_kernel(const __grid_constant_
                     }
                 }
             }
+            if constexpr (kRoll) ask(std::false_type{}, i, k + (i + kBatch) * step);
         }
-        if (k + kBatch * step < last) ask(k + kBatch * step);
+        if constexpr (!kRoll)
+            if (k + kBatch * step < last) {
+#pragma unroll
+                for (int i = 0; i < kBatch; ++i) ask(std::false_type{}, i, k + (i + kBatch) * step);
+            }
     }
 #pragma unroll
     for (int o = 0; o < kStreams; ++o)
@@ -370,9 +396,13 @@ Cut cut_plain(ProductKind kind, size_t m, size_t n, size_t k) {
 
 template <typename T, typename O, int KIND>
 cudaError_t launch_join_kind(const Product &p, cudaStream_t stream) {
-    const size_t n = (size_t)p.m * (partial_stride(p.n) / 4) * p.problems, blocks = (n + 255) / 256;
-    const size_t most = (size_t)geo::device_sm_count() * 8;
-    return launch_after(join_kernel<T, O, KIND>, (unsigned)(blocks < most ? blocks : most), 256, 0, 1, stream, p);
+    const size_t n = (size_t)p.m * (partial_stride(p.n) / 4) * p.problems, most = (size_t)geo::device_sm_count() * 8;
+    // Threads that share a place where there are parts for them and threads to spare.
+    const bool share = p.splits >= 16 && n * 8 <= most * 256;
+    const size_t blocks = (n * (share ? 8 : 1) + 255) / 256;
+    const unsigned grid = (unsigned)(blocks < most ? blocks : most);
+    return share ? launch_after(join_kernel<T, O, KIND, 8>, grid, 256, 0, 1, stream, p)
+                 : launch_after(join_kernel<T, O, KIND, 1>, grid, 256, 0, 1, stream, p);
 }
 cudaError_t launch_join(ProductKind kind, uint32_t type, uint32_t out_type, const Product &p, cudaStream_t stream) {
     return by_type(type, [&](auto t) -> cudaError_t {
