@@ -143,13 +143,14 @@ __device__ __forceinline__ W activation(int kind, W a, W *slope) {
             return a * below;
         }
         default: {
+            if (slope == nullptr) {
+                const W alone = logistic<FAST>(a);
+                return kind == GEO_B200_ACTIVATION_SIGMOID ? alone : a * alone;
+            }
             W s, rest;
             logistic<FAST>(a, s, rest);
-            if (kind == GEO_B200_ACTIVATION_SIGMOID) {
-                if (slope != nullptr) *slope = s * rest;
-                return s;
-            }
-            if (slope != nullptr) *slope = s * (W(1) + a * rest);
+            *slope = kind == GEO_B200_ACTIVATION_SIGMOID ? s * rest : s * (W(1) + a * rest);
+            if (kind == GEO_B200_ACTIVATION_SIGMOID) return s;
             return a * s;
         }
     }

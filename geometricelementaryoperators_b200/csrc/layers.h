@@ -197,6 +197,14 @@ __device__ __forceinline__ void logistic(W a, W &s, W &rest) {
     s = a < W(0) ? e * d : d;
     rest = a < W(0) ? d : e * d;
 }
+// s alone: 0 where e^-a leaves the type's range (FAST: below -87).
+template <bool FAST, typename W>
+__device__ __forceinline__ W logistic(W a) {
+    if constexpr (FAST && sizeof(W) == 4)
+        return __fdividef(1.0f, 1.0f + __expf(-a));
+    else
+        return W(1) / (W(1) + exp(-a));
+}
 #endif
 
 inline size_t type_bytes(uint32_t type) {

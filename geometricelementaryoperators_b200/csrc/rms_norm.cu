@@ -44,7 +44,11 @@ __global__ void __launch_bounds__(TEAM == kWarp ? kWarpBlock : kTeamThreads, TEA
     const W over = W(1) / (W)a.cols, alpha = (W)a.residual_scale, beta = (W)a.block_scale;
     Pair<W> w[Q], post[MODE >= kBlockNorm ? Q : 1];
     load_parameters<T, V, K, SHIFT>(a.weight, float_parameters, at, a.cols, W(1), w);
-    if constexpr (MODE >= kBlockNorm) load_parameters<T, V, K, SHIFT>(a.post, float_parameters, at, a.cols, W(1), post);
+    if constexpr (MODE >= kBlockNorm) {
+        load_parameters<T, V, K, SHIFT>(a.post, float_parameters, at, a.cols, W(1), post);
+#pragma unroll
+        for (int q = 0; q < Q; ++q) post[q] = post[q] * both(beta);
+    }
     open_exchange(sums);
 
     uint32_t round = 0;
@@ -83,7 +87,7 @@ __global__ void __launch_bounds__(TEAM == kWarp ? kWarpBlock : kTeamThreads, TEA
                 if (live && at.lane == 0 && a.x_rstd != nullptr) ((W *)a.x_rstd)[row] = rstd[u];
                 Vec<T, V> raw[K];
 #pragma unroll
-                for (int q = 0; q < Q; ++q) v[u][q] = v[u][q] * both(rstd[u]) * (post[q] * both(beta));
+                for (int q = 0; q < Q; ++q) v[u][q] = v[u][q] * both(rstd[u]) * post[q];
                 if constexpr (MODE == kGatedNorm) {
                     ring.get(raw, u, 2, (const T *)a.gate + r * a.gate_stride);
 #pragma unroll

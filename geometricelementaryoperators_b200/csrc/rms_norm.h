@@ -43,8 +43,9 @@ __device__ __forceinline__ W gate_value(int kind, W g, W *slope) {
     }
     W s, rest;
     if (kind == GEO_B200_GATE_SIGMOID) {
+        if (slope == nullptr) return logistic<FAST>(g);
         logistic<FAST>(g, s, rest);
-        if (slope != nullptr) *slope = s * rest;
+        *slope = s * rest;
         return s;
     }
     if (slope != nullptr) {  // 1 - tanh^2 = 4 s (1 - s) at twice the argument, which does not cancel

@@ -69,7 +69,11 @@ __global__ void __launch_bounds__(TEAM == kWarp ? kWarpBlock : kTeamThreads, res
     const W over = W(1) / (W)a.cols, alpha = (W)a.residual_scale, beta = (W)a.block_scale;
     Pair<W> w[Q], dw[Q], post[kBlocks ? Q : 1], dpost[Q];
     load_parameters<T, V, K, SHIFT>(a.weight, float_parameters, at, a.cols, W(1), w);
-    if constexpr (kBlocks) load_parameters<T, V, K, SHIFT>(a.post, float_parameters, at, a.cols, W(1), post);
+    if constexpr (kBlocks) {
+        load_parameters<T, V, K, SHIFT>(a.post, float_parameters, at, a.cols, W(1), post);
+#pragma unroll
+        for (int q = 0; q < Q; ++q) post[q] = post[q] * both(beta);  // wherever it stands below, block_scale does too
+    }
 #pragma unroll
     for (int q = 0; q < Q; ++q) dw[q] = dpost[q] = both(W(0));
 
@@ -135,7 +139,7 @@ __global__ void __launch_bounds__(TEAM == kWarp ? kWarpBlock : kTeamThreads, res
                 for (int q = 0; q < V / 2; ++q) {
                     const int n = i * V / 2 + q;
                     const Pair<W> zh = z.pair(q) * both(rstd[0]), d = dy.pair(q), g = d * w[n];
-                    Pair<W> f = x.pair(q) * both(x_rstd) * (post[n] * both(beta));
+                    Pair<W> f = x.pair(q) * both(x_rstd) * post[n];
                     if constexpr (kGates) f = f * act[q];
                     s1 = fma(g, zh, s1);
                     s2 = fma(f, fma(g, both(rstd[0]), dz.pair(q)), s2);
@@ -196,7 +200,7 @@ __global__ void __launch_bounds__(TEAM == kWarp ? kWarpBlock : kTeamThreads, res
                     const Pair<W> zh = z.pair(q) * both(rstd[0]);
                     const Pair<W> dz = fma(fma(zh, both(-c1), dy.pair(q) * w[n]), both(rstd[0]), dzs.pair(q));
                     const Pair<W> xh = x.pair(q) * both(x_rstd);
-                    Pair<W> dn = dz * both(beta);
+                    Pair<W> dn = dz;  // without block_scale
                     dresidual.set(q, dz * both(alpha));
                     if constexpr (kGates) {
                         dgate.set(q, dn * (xh * post[n]) * slope[q]);
@@ -222,6 +226,10 @@ __global__ void __launch_bounds__(TEAM == kWarp ? kWarpBlock : kTeamThreads, res
     wait_async<0>();
     close_exchange<TEAM>();
     if (partial == nullptr) return;
+    if constexpr (kBlocks) {
+#pragma unroll
+        for (int q = 0; q < Q; ++q) dpost[q] = dpost[q] * both(beta);
+    }
     if (!complete) {
 #pragma unroll
         for (int q = 0; q < Q; ++q) dw[q] = dpost[q] = both((W)NAN);

@@ -330,3 +330,38 @@ def test_waits_give_up(rows, block):
     few = Case("bf16", 1, 640, 520)
     assert L.geo_b200_feed_forward_wait_selftest(ref(few.config), p(few.x), p(few.wg), p(few.wu), p(few.wd), None, None,
                                                  p(gy), p(few.space), few.space.numel(), 0, 16, stream) == 1
+
+
+def test_host_threads():
+    """Calls of several host threads at once, each on a stream and with a workspace of its own, of sizes that take other
+    kernels and other amounts of shared memory."""
+    import threading
+
+    import torch
+
+    cases = [Case("bf16", 300, 200, 136), Case("bf16", 40, 640, 520, gradient="f32"), Case("f64", 70, 33, 65),
+             Case("f32", 200, 136, 264), Case("f16", 2, 1000, 333)]
+    want = []
+    for c in cases:
+        a, u, y, _ = c.forward()
+        want.append((a, u, y, c.vjp(a, u)[0]))
+    torch.cuda.synchronize()
+    failed = []
+
+    def work(c, w):
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            for _ in range(20):
+                a, u, y, _ = c.forward()
+                grads, _ = c.vjp(w[0], w[1])
+                s.synchronize()
+                same = [torch.equal(p, q) for p, q in zip((a, u, y, *grads), (*w[:3], *w[3]))]
+                if not all(same):
+                    failed.append((c.rows, same))
+
+    threads = [threading.Thread(target=work, args=p) for p in zip(cases, want)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
