@@ -25,7 +25,7 @@
 // up of the same hidden values are in one tile of sums; kInput adds both its products
 // into one tile, K running through the first pair of operands, then the second.
 // Measured: 8192 x 4096 x 12288 bfloat16, gate and up 1.17 ms (1.41 PFLOP/s), down 0.59,
-// the VJP to float32 cotangents 5.7 to 6.3 ms with 7.4 TFLOP, its last product with 96% of
+// the VJP to float32 cotangents 5.75 to 6.6 ms with 7.4 TFLOP, its last product with 96% of
 // the tensor cycles: the board's power bounds them (1.3 GHz). The VJP's first product
 // reads two arrays more and writes six: 1.1 ms where its multiplications take 0.6.
 #include <cooperative_groups.h>
@@ -49,7 +49,7 @@ constexpr int epilogue_warps(int kind, bool twice) { return kind == kHidden || t
 // the size off with each 16 of K (1.8e-5 over 8192 rows). The parts are added up in
 // registers, rounded to nearest. (VJP of 8192 x 4096 x 12288 to float32 cotangents, this
 // many blocks in the last product alone: 16 blocks 5.66 ms, 8 blocks 5.74, 4 blocks 5.98;
-// 16 in both products leave 3.7e-6 off, of which what two 16-bit terms lose is 2.2e-6.)
+// 16 in both products leave 4.1e-6 off, of which what two 16-bit terms lose is 2.2e-6.)
 constexpr int kChunk = 16;
 constexpr uint32_t bytes_a(bool twice) { return (twice ? 2 : 1) * kBM * kBK * 2; }
 constexpr uint32_t bytes_b(int bn) { return (uint32_t)bn * kBK * 2; }
