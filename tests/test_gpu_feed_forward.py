@@ -365,3 +365,27 @@ def test_host_threads():
     for t in threads:
         t.join()
     assert not failed
+
+
+@pytest.mark.parametrize("kind,size", [("bf16", (200000, 40, 24)), ("f16", (3, 131072, 16)), ("bf16", (40, 8, 131072)),
+                                       ("f32", (1, 16, 1048576)), ("f64", (130, 100000, 24)), ("f32", (200000, 40, 24))])
+def test_long_and_wide(kind, size):
+    c = Case(kind, *size, "silu", gradient="f32" if kind == "bf16" else None)
+    a, u, y, buffers = c.forward()
+    c.check_forward(a, u, y)
+    outs, more = c.vjp(a, u)
+    c.check_vjp(a, u, outs)
+    untouched(buffers + more)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+def test_float32_cotangents_over_many_rows(kind):
+    """Their 2-norm's error does not grow with the rows: two terms leave 2^-18 of an inner value (bfloat16; and float16's
+    least, 2^-25 of values of some 2^-5), each of the 64 instructions of 16 that sum h_bar's parts, and each of the 128
+    that sum a cotangent's, may cut one unit, 2^-23, off a sum's size. Random signs keep the sums of parts to that."""
+    c = Case(kind, 8192, 512, 256, gradient="f32")
+    a, u, _, _ = c.forward()
+    outs, _ = c.vjp(a, u)
+    want = ff.vjp(*c.wide(), a.double(), u.double(), c.dy.double(), "silu")
+    for got, w in zip(outs[1:], want[1:]):
+        assert (got.double() - w).norm() <= (2.0 ** -18 + 192 * 2.0 ** -23) * w.norm()
