@@ -304,17 +304,18 @@ def test_refusals_with_usable_arrays():
     torch.cuda.synchronize()
 
 
-@pytest.mark.parametrize("rows,block", [(40, 0), (40, 2), (300, 0), (700, 3)])
-def test_waits_give_up(rows, block):
-    """Copies that stop (single blocks, parts of K, pairs of blocks): the call ends, what they were for is NaN, and the
-    next call is right."""
+@pytest.mark.parametrize("rows,cols,hidden,block", [(40, 640, 520, 0), (40, 640, 520, 2), (300, 640, 520, 0),
+                                                    (700, 640, 520, 3), (5000, 256, 2048, 0), (5000, 256, 2048, 3)])
+def test_waits_give_up(rows, cols, hidden, block):
+    """Copies that stop (single blocks, parts of K, pairs of blocks), before any tile is whole: the call ends, what they
+    were for is NaN, and the next call is right."""
     import torch
 
     p, L = ff.pointer, abi.lib()
-    c = Case("bf16", rows, 640, 520)
+    c = Case("bf16", rows, cols, hidden)
     a, u, y, _ = c.forward()
     args = (ref(c.config), p(c.x), p(c.wg), p(c.wu), p(c.wd))
-    (ga, _), (gu, _), (gy, _) = (c.blank(rows, n, 0) for n in (520, 520, 640))
+    (ga, _), (gu, _), (gy, _) = (c.blank(rows, n, 0) for n in (hidden, hidden, cols))
     stream = torch.cuda.current_stream().cuda_stream
     for limit in (1 << 8, 1 << 12):
         assert L.geo_b200_feed_forward_wait_selftest(*args, p(ga), p(gu), p(gy), p(c.space), c.space.numel(), block,
@@ -327,7 +328,7 @@ def test_waits_give_up(rows, block):
     again = c.forward()
     assert all(torch.equal(v, w) for v, w in zip(again[:3], (a, u, y)))
     # A call that other kernels take has no such waits.
-    few = Case("bf16", 1, 640, 520)
+    few = Case("bf16", 1, cols, hidden)
     assert L.geo_b200_feed_forward_wait_selftest(ref(few.config), p(few.x), p(few.wg), p(few.wu), p(few.wd), None, None,
                                                  p(gy), p(few.space), few.space.numel(), 0, 16, stream) == 1
 
