@@ -85,14 +85,21 @@ __device__ __forceinline__ void barrier_init(uint32_t barrier, uint32_t count) {
 __device__ __forceinline__ void barrier_expect(uint32_t barrier, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(barrier), "r"(bytes) : "memory");
 }
+// Takes bytes that will not come off what the phase expects.
+__device__ __forceinline__ void barrier_excuse(uint32_t barrier, uint32_t bytes) {
+    asm volatile("mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(barrier), "r"(bytes) : "memory");
+}
 __device__ __forceinline__ void barrier_arrive(uint32_t barrier) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(barrier) : "memory");
 }
-// The same barrier of the pair's block `rank`.
-__device__ __forceinline__ uint32_t barrier_of(uint32_t barrier, uint32_t rank) {
+// The same place of the shared memory of the pair's block `rank`.
+__device__ __forceinline__ uint32_t place_of(uint32_t here, uint32_t rank) {
     uint32_t there;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(barrier), "r"(rank));
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(here), "r"(rank));
     return there;
+}
+__device__ __forceinline__ void store_cluster(uint32_t there, uint32_t v) {
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(there), "r"(v) : "memory");
 }
 __device__ __forceinline__ void barrier_arrive_cluster(uint32_t there) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(there) : "memory");
@@ -364,6 +371,8 @@ __global__ void __launch_bounds__(64 + 32 * epilogue_warps(KIND, TWICE), 1)
     __shared__ __align__(8) uint64_t barriers[2 * kStages + 5];
     __shared__ uint32_t sums_address;
     __shared__ volatile int gave_up;
+    __shared__ uint32_t issued[2];   // blocks of K whose copies this block and (PAIR) the other one started, by rank
+    __shared__ int other_gave_up;    // PAIR: a wait of the other block
     const uint32_t base = (shared_address(memory) + 1023) & ~1023u;
     unsigned char *staging = memory + (base - shared_address(memory)) + kStages * kStageBytes;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -373,7 +382,7 @@ __global__ void __launch_bounds__(64 + 32 * epilogue_warps(KIND, TWICE), 1)
     const uint32_t full = shared_address(barriers), empty = full + 8 * kStages, ready = empty + 8 * kStages,
                    taken = ready + 16, drained = taken + 16;
     if (threadIdx.x == 0) {
-        gave_up = 0;
+        gave_up = other_gave_up = 0;
         for (int s = 0; s < kStages; ++s) barrier_init(full + 8 * s, 1), barrier_init(empty + 8 * s, 1);
         for (int i = 0; i < 2; ++i) barrier_init(ready + 8 * i, 1), barrier_init(taken + 8 * i, (PAIR ? 2 : 1) * kWarps);
         barrier_init(drained, 1);
@@ -425,7 +434,7 @@ __global__ void __launch_bounds__(64 + 32 * epilogue_warps(KIND, TWICE), 1)
                     break;
                 }
                 const uint32_t to = base + s * kStageBytes;
-                const uint32_t barrier = PAIR ? barrier_of(full + 8 * s, 0) : full + 8 * s;
+                const uint32_t barrier = PAIR ? place_of(full + 8 * s, 0) : full + 8 * s;
                 if (rank == 0) barrier_expect(full + 8 * s, (PAIR ? 2 : 1) * (kStageBytes - skipped));
                 const int second = KIND == kInput && i >= blocks_k ? 1 : 0, k = (i - second * blocks_k) * kBK;
                 const int row0 = (PAIR ? t.row * 2 + rank : t.row) * kBM;
@@ -455,14 +464,8 @@ __global__ void __launch_bounds__(64 + 32 * epilogue_warps(KIND, TWICE), 1)
                 }
             }
         }
-        if (!good) {
-            // Copies in flight land before the block ends. A stage's last copies were of its last round begun. (A
-            // pair's land at the first block's barriers, and the other one leaves no sooner than the first.)
-            for (uint32_t n = step < (uint32_t)kStages ? step : kStages; n > 0 && rank == 0; --n) {
-                const uint32_t last = step - n;
-                barrier_wait(full + 8 * (last % kStages), (last / kStages) & 1, starve.polls, nullptr);
-            }
-        }
+        issued[rank] = step;
+        if constexpr (PAIR) store_cluster(place_of(shared_address(&issued[rank]), rank ^ 1), step);
     } else if (warp == 1 && lane == 0 && rank == 0) {
         constexpr uint32_t kInstruction = instruction<T>(kAMn, kBMn, PAIR ? 2 * kBM : kBM, BN);
         uint32_t step = 0, round = 0;  // round: of the two places for sums
@@ -501,7 +504,7 @@ __global__ void __launch_bounds__(64 + 32 * epilogue_warps(KIND, TWICE), 1)
         }
         // Matrix instructions in flight end before tensor memory is given back.
         commit_to<PAIR>(drained);
-        barrier_wait(drained, 0, starve.polls, nullptr);
+        barrier_wait(drained, 0, kPipelinePolls, nullptr);
     } else if (warp >= 2) {
         unsigned char *mine = staging + (warp - 2) * staging_of(KIND);
         const int quarter = warp & 3;  // the rows of tensor memory that this warp may read
@@ -523,9 +526,10 @@ __global__ void __launch_bounds__(64 + 32 * epilogue_warps(KIND, TWICE), 1)
             auto release = [&] {
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) {
+                // A warp that gave up no longer says that it has taken what others may still be reading.
+                if (lane == 0 && good) {
                     if constexpr (PAIR)
-                        barrier_arrive_cluster(barrier_of(taken + 8 * (round & 1), 0));
+                        barrier_arrive_cluster(place_of(taken + 8 * (round & 1), 0));
                     else
                         barrier_arrive(taken + 8 * (round & 1));
                 }
@@ -693,7 +697,29 @@ __global__ void __launch_bounds__(64 + 32 * epilogue_warps(KIND, TWICE), 1)
     if constexpr (KIND == kHidden)
         if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     __syncwarp();
+    if constexpr (PAIR) {
+        __syncthreads();
+        if (threadIdx.x == 0 && gave_up) store_cluster(place_of(shared_address(&other_gave_up), rank ^ 1), 1);
+    }
     everyone();
+    if (PAIR && rank == 1 && threadIdx.x == 0)  // the first block's commits have arrived here too
+        barrier_wait(drained, 0, kPipelinePolls, nullptr);
+    if (gave_up || other_gave_up) {
+        // Whichever wait it was: copies in flight land before a block ends. A stage's last copies were of the last round
+        // begun; a pair's land at the first block's barriers, where one block may have come further than the other.
+        if (threadIdx.x == 0 && rank == 0) {
+            const uint32_t own = issued[0], other = PAIR ? issued[1] : own, most = own > other ? own : other;
+            for (uint32_t n = most > (uint32_t)kStages ? most - kStages : 0; n < most; ++n) {
+                const uint32_t barrier = full + 8 * (n % kStages);
+                if (n >= own)
+                    barrier_expect(barrier, kStageBytes);  // the other block's alone
+                else if (n >= other)
+                    barrier_excuse(barrier, kStageBytes);  // the other block's never began
+                barrier_wait(barrier, (n / kStages) & 1, kPipelinePolls, nullptr);
+            }
+        }
+        if constexpr (PAIR) cooperative_groups::this_cluster().sync();
+    }
     if (warp == 1) {
         if constexpr (PAIR)
             asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(sums), "r"(kSumColumns) : "memory");
