@@ -10,7 +10,8 @@
 // thousands of them in float32, so their roundings average out against the result's
 // own. A float32 result has no rounding to hide them (2.3e-3 of its size off, where its
 // sums are 2e-6): on their way to one, what was lost is kept as a second array of the
-// type and multiplied as well.
+// type and multiplied as well. float16's inner values of the VJP are multiplied by powers
+// of two while they are there (feed_forward_scale.cu).
 #include "feed_forward.h"
 
 #include <algorithm>
@@ -173,6 +174,7 @@ extern "C" size_t geo_b200_feed_forward_vjp_workspace(const geo_b200_feed_forwar
     Space space = {nullptr};
     const size_t b = type_bytes(c.type);
     for (int i = 0; i < (c.gradient_type != c.type ? 6 : 3); ++i) space.take(c.rows, round8(c.hidden), b);
+    if (c.type == GEO_B200_F16) space.take(1 + kScaleBlocks, 1, sizeof(float4));
     if (b == 2)
         for (const Operand &o : {Operand{{nullptr, c.x_stride}, c.rows, c.cols},
                                  Operand{{nullptr, c.y_cotangent_stride}, c.rows, c.cols},
@@ -299,6 +301,7 @@ extern "C" geo_b200_status_t geo_b200_feed_forward_vjp(
     for (void *&p : inside) p = space.take(c.rows, hidden_stride, b);
     if (c.gradient_type != c.type)
         for (void *&p : low) p = space.take(c.rows, hidden_stride, b);
+    float *const scale = c.type == GEO_B200_F16 ? (float *)space.take(1 + kScaleBlocks, 1, sizeof(float4)) : nullptr;
     Operand x = {{device_x, c.x_stride}, c.rows, c.cols}, wg = {{device_gate_weight, c.gate_weight_stride}, c.hidden, c.cols},
             wu = {{device_up_weight, c.up_weight_stride}, c.hidden, c.cols},
             wd = {{device_down_weight, c.down_weight_stride}, c.cols, c.hidden},
@@ -309,6 +312,15 @@ extern "C" geo_b200_status_t geo_b200_feed_forward_vjp(
         if (e != cudaSuccess) return status_of(e);
     }
     void *const rest = space.take(0, 0, 1);
+    if (scale != nullptr) {
+        InnerScale s = {dy.m, wd.m, {device_gate, c.gate_stride}, {device_up, c.up_stride}, c.rows, c.cols, c.hidden,
+                        (int)c.activation, (float4 *)scale};
+        if (!inner) s.dy.p = s.wd.p = nullptr;
+        const cudaError_t e = launch_scale(s, stream);
+        if (e != cudaSuccess) return status_of(e);
+    }
+    // Of the cotangents of gate and up (0, 1) and of h (2).
+    auto times = [&](int i, bool inverse) { return scale == nullptr ? nullptr : scale + (i == 2 ? 2 : 0) + (inverse ? 1 : 0); };
     auto launch = [&](ProductKind kind, Product &p) { return launch_product(c, tensor, kind, p, rest, stream); };
     Product hidden = {};
     hidden.m = (int)c.rows, hidden.n = (int)c.hidden, hidden.k = (int)c.cols, hidden.problems = 1;
@@ -320,6 +332,7 @@ extern "C" geo_b200_status_t geo_b200_feed_forward_vjp(
     for (int i = 0; i < 3; ++i) {
         const bool wanted = i == 2 ? device_down_weight_cotangent != nullptr : inner;
         if (wanted) hidden.out[i] = {inside[i], hidden_stride};
+        hidden.times[i] = times(i, false);
         if (wanted && (i == 2 || weights)) hidden.out_low[i] = {low[i], hidden_stride};
     }
     cudaError_t e = launch(kHidden, hidden);
@@ -330,6 +343,7 @@ extern "C" geo_b200_status_t geo_b200_feed_forward_vjp(
         input.b[0] = wg.m;
         input.b[1] = wu.m;
         input.out[0] = {device_x_cotangent, c.x_cotangent_stride};
+        input.times[0] = times(0, true);
         e = launch(kInput, input);
     }
     Product w = {};
@@ -343,6 +357,7 @@ extern "C" geo_b200_status_t geo_b200_feed_forward_vjp(
             w.low[w.problems] = {low[i], hidden_stride};
             w.b[w.problems] = i == 2 ? dy.m : x.m;
             w.transposed[w.problems] = i == 2;
+            w.times[w.problems] = times(i, true);
             w.out[w.problems++] = outs[i];
         }
     if (e == cudaSuccess && w.problems > 0) e = launch(kWeights, w);

@@ -39,6 +39,7 @@ struct Product {
     OutMatrix out[3];  // kGated: gate, up (may be null), h; kHidden: cotangents of gate and up, h; kWeights: [M][N], or
     bool transposed[3];     // ... [N][M]
     OutMatrix out_low[3];  // kHidden: what those lost to rounding, or null
+    const float *times[3]; // float16's VJP: device memory of what out[i] is multiplied by, a power of two; or null
     void *partial;     // splits > 1: [sum][split][M][partial_stride(N)] of the arithmetic type
 };
 __host__ __device__ inline size_t partial_stride(size_t n) { return (n + 3) / 4 * 4; }
@@ -92,6 +93,16 @@ struct Pack {
     } arrays[kPackMost];
 };
 cudaError_t launch_pack(const Pack &pack, cudaStream_t stream);
+// float16's VJP: found[0] = the power of two for the cotangents of gate and up, its
+// inverse, that for h, its inverse; behind it room for kScaleBlocks more.
+constexpr int kScaleBlocks = 1024;
+struct InnerScale {
+    Matrix dy, wd, gate, up;  // dy, wd: null where only h is wanted
+    size_t rows, cols, hidden;
+    int activation;
+    float4 *found;
+};
+cudaError_t launch_scale(const InnerScale &scale, cudaStream_t stream);
 // Whether the tensor-core products can run at all (the driver's tensor map encoder).
 bool tensor_products_available();
 
@@ -120,7 +131,8 @@ cudaError_t launch_after(void (*kernel)(P...), unsigned grid, unsigned threads, 
 }
 
 // What v loses to its rounding to T, itself to be rounded to T: together they hold
-// twice T's digits. (What T has no finite value for loses an infinity or NaN.)
+// twice T's digits as far as T's range goes (float16's inner values are brought into it
+// first, feed_forward_scale.cu). (What T has no finite value for loses an infinity or NaN.)
 template <typename T>
 __device__ __forceinline__ float lost_to(float v) {
     return v - widen(narrow<T>(v));
@@ -168,6 +180,15 @@ __device__ __forceinline__ void by_activation(int kind, F &&f) {
     }
 }
 
+// What result n is multiplied by.
+template <typename T>
+__device__ __forceinline__ Wide<T> times_of(const Product &p, int n) {
+    if constexpr (std::is_same_v<T, __half>)
+        return p.times[n] != nullptr ? *p.times[n] : 1.0f;
+    else
+        return Wide<T>(1);
+}
+
 // What is done with the sums of one place of a product's result: gate and up (kGated), or one.
 template <typename T, typename O, int KIND>
 __device__ __forceinline__ void finish(const Product &p, int problem, size_t row, size_t col, Wide<T> v, Wide<T> other) {
@@ -176,6 +197,7 @@ __device__ __forceinline__ void finish(const Product &p, int problem, size_t row
     auto put = [&](const OutMatrix &out, W x) {
         if (out.p != nullptr) ((T *)out.p)[row * out.stride + col] = narrow<T>(x);
     };
+    auto scaled = [&](int n, W x) { return x * times_of<T>(p, n); };
     if constexpr (KIND == kGated) {
         put(p.out[0], v);
         put(p.out[1], other);
@@ -186,6 +208,7 @@ __device__ __forceinline__ void finish(const Product &p, int problem, size_t row
         W slope;
         const W f = activation<kFast>(p.activation, g, &slope);
         auto put_two = [&](int n, W x) {
+            x = scaled(n, x);
             put(p.out[n], x);
             if constexpr (sizeof(T) == 2) put(p.out_low[n], lost_to<T>(x));
         };
@@ -194,9 +217,10 @@ __device__ __forceinline__ void finish(const Product &p, int problem, size_t row
         put_two(2, f * u);
     } else if constexpr (KIND == kWeights) {
         const OutMatrix &out = p.out[problem];
-        ((O *)out.p)[p.transposed[problem] ? col * out.stride + row : row * out.stride + col] = narrow<O>((Wide<O>)v);
+        ((O *)out.p)[p.transposed[problem] ? col * out.stride + row : row * out.stride + col] =
+            narrow<O>((Wide<O>)scaled(problem, v));
     } else {
-        put(p.out[0], v);
+        put(p.out[0], scaled(0, v));
     }
 }
 #endif

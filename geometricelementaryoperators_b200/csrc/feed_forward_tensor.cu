@@ -549,6 +549,19 @@ __global__ void __launch_bounds__(64 + 32 * epilogue_warps(KIND, TWICE), 1)
                 const size_t stride = partial_stride(p.n), part = (size_t)which * p.splits + t.split;
                 put_columns<float>(mine, v, from, {(float *)p.partial + part * p.m * stride, stride}, row0, col0, p.m, p.n);
             };
+            // float16's VJP: the powers of two of this tile's results.
+            constexpr bool kTimes = std::is_same_v<T, __half> && (KIND == kHidden || KIND == kInput || KIND == kWeights);
+            float times[3] = {1.0f, 1.0f, 1.0f};
+            if constexpr (kTimes) {
+#pragma unroll
+                for (int n = 0; n < (KIND == kHidden ? 3 : 1); ++n) times[n] = times_of<T>(p, KIND == kWeights ? t.problem : n);
+            }
+            auto scale = [&](auto &v) {
+                if constexpr (kTimes && KIND != kHidden) {
+#pragma unroll
+                    for (float &x : v) x *= times[0];
+                }
+            };
             // 32 columns of a result of kWeights, kDown, kInput.
             auto put = [&](const auto &v, int from, int col0) {
                 if constexpr (KIND == kWeights) {
@@ -585,6 +598,7 @@ __global__ void __launch_bounds__(64 + 32 * epilogue_warps(KIND, TWICE), 1)
                 float sum[kPart];
                 add_parts(sum);
                 release();
+                if (p.splits == 1) scale(sum);
                 if (row0 < p.m) {
 #pragma unroll
                     for (int c = 0; c < kPart; c += 32) {
@@ -660,7 +674,11 @@ __global__ void __launch_bounds__(64 + 32 * epilogue_warps(KIND, TWICE), 1)
                                     f.x = activation<true>(decltype(kind)::value, g[2 * q], &slope.x);
                                     f.y = activation<true>(decltype(kind)::value, g[2 * q + 1], &slope.y);
                                     const Pair<float> hb = {v[2 * q], v[2 * q + 1]}, up2 = {u[2 * q], u[2 * q + 1]};
-                                    const Pair<float> results[3] = {hb * up2 * slope, hb * f, f * up2};
+                                    Pair<float> results[3] = {hb * up2 * slope, hb * f, f * up2};
+                                    if constexpr (kTimes) {
+#pragma unroll
+                                        for (int n = 0; n < 3; ++n) results[n] = results[n] * both(times[n]);
+                                    }
 #pragma unroll
                                     for (int n = 0; n < 3; ++n) {
                                         words[n][0][q] = word_of<T>(results[n].x, results[n].y);
@@ -686,6 +704,7 @@ __global__ void __launch_bounds__(64 + 32 * epilogue_warps(KIND, TWICE), 1)
                             if (box & 1)
                                 if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
                         } else {
+                            scale(v);
                             put(v, 0, col0);
                         }
                     }

@@ -651,7 +651,10 @@ geo_b200_status_t geo_b200_block_norm_vjp(
  * multiplied exactly and summed in float32; h, and the VJP's cotangents of gate and
  * up, are rounded to `type` on their way to the next product, but to the sum of two
  * values of it on their way to float32 cotangents of weights, which costs that product
- * twice. An infinity may come out as NaN. */
+ * twice. float16's VJP multiplies them by powers of two meanwhile, chosen from its
+ * arrays' largest values, so that those of small cotangents keep their digits and none
+ * overflows; its forward does not: h beyond 65504 is infinite, and below 2^-14 has
+ * float16's steps of 2^-24. An infinity may come out as NaN. */
 typedef enum {
     GEO_B200_ACTIVATION_SILU = 1,
     GEO_B200_ACTIVATION_GELU = 2,

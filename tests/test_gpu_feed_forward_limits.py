@@ -1,4 +1,5 @@
-"""Gated feed-forward block (geo/geo_b200.h section 5) at its limits on the GPU: waits that give up anywhere."""
+"""Gated feed-forward block (geo/geo_b200.h section 5) at its limits on the GPU: waits that give up anywhere, float16
+values at both ends of its range."""
 from __future__ import annotations
 
 import ctypes
@@ -34,3 +35,62 @@ def test_any_wait_gives_up(rows, cols, hidden):
             for got, w in zip((a, u, y), want):
                 assert ((got == w) | got.isnan()).all()
     assert all(torch.equal(v, w) for v, w in zip(c.forward()[:3], want))
+
+
+def off(got, want):
+    """2-norm of the difference and of what it is of."""
+    return float((got.double() - want).norm()), float(want.norm())
+
+
+@pytest.mark.parametrize("size", [(3, 256, 136), (300, 520, 1032), (4000, 256, 136)])
+@pytest.mark.parametrize("before", [0, 1])  # on the tensor cores, and value by value
+@pytest.mark.parametrize("gradient", ["f32", "f16"])
+@pytest.mark.parametrize("scale", [1e-2, 1e-4, 1e-6])
+def test_small_float16_cotangents(gradient, scale, before, size):
+    """y_bar as small as a mean over many values makes it. Inner values are multiplied into float16's range, so that
+    they are one rounding off, 2^-11, or two terms' 2^-22 on their way to a float32 cotangent of weights; up to 64
+    instructions of 16 cut a unit, 2^-23, of a part of h_bar's and a cotangent's sums each, float32's functions leave
+    2^-20, and a float16 result has its own rounding, 2^-11 of it or 2^-25."""
+    c = Case("f16", *size, "silu", gradient=None if gradient == "f16" else gradient, before=before)
+    a, u, _, _ = c.forward()
+    c.dy.mul_(scale)
+    outs, _ = c.vjp(a, u)
+    want = ff.vjp(*c.wide(), a.double(), u.double(), c.dy.double(), "silu")
+    sums = 128 * 2.0 ** -23 + 2.0 ** -20
+    for n, (got, w) in enumerate(zip(outs, want)):
+        difference, of = off(got, w)
+        if n == 0 or gradient == "f16":
+            assert difference <= (2 * 2.0 ** -11 + sums) * of + 2.0 ** -25 * w.numel() ** 0.5, n
+        else:
+            assert difference <= (2.0 ** -22 + sums) * of, n
+
+
+@pytest.mark.parametrize("before", [0, 1])
+def test_float16_cotangents_with_infinite_rows(before):
+    """A row whose cotangent is not finite leaves the other rows' x_bar as exact as it is without it."""
+    c = Case("f16", 300, 256, 136, before=before)
+    a, u, _, _ = c.forward()
+    c.dy.mul_(1e-6)
+    want = ff.vjp(*c.wide(), a.double(), u.double(), c.dy.double(), "silu")[0]
+    c.dy[7, 5], c.dy[80, 0] = float("inf"), float("nan")
+    got = c.vjp(a, u)[0][0]
+    good = [r for r in range(300) if r not in (7, 80)]
+    assert (~got[[7, 80]].isfinite()).any(dim=1).all()
+    difference, of = off(got[good], want[good])
+    assert difference <= (2 * 2.0 ** -11 + 2.0 ** -16) * of + 2.0 ** -25 * want.numel() ** 0.5
+
+
+@pytest.mark.parametrize("gradient", ["f32", "f16"])
+@pytest.mark.parametrize("before", [0, 1])
+def test_float16_h_beyond_its_range(gradient, before):
+    """act(gate) up of up to 250000 in the VJP: down_weight's cotangent is finite and right."""
+    import torch
+
+    c = Case("f16", 200, 64, 72, gradient=None if gradient == "f16" else gradient, before=before)
+    a, u = (torch.rand(200, 72, device="cuda").mul(250).add(250).half() for _ in range(2))
+    c.dy.mul_(2.0 ** -14)
+    got = c.vjp(a, u)[0]
+    want = ff.vjp(*c.wide(), a.double(), u.double(), c.dy.double(), "silu")
+    for n, (g, w) in enumerate(zip(got, want)):
+        difference, of = off(g, w)
+        assert difference <= (2 * 2.0 ** -11 + 2.0 ** -16) * of + 2.0 ** -25 * w.numel() ** 0.5, n
