@@ -59,7 +59,7 @@ size_t partial_bytes(const geo_b200_feed_forward_config_t &c, std::initializer_l
     for (const Extent &x : products) {
         if (type_bytes(c.type) == 2) {
             const bool twice = x.kind == kWeights && c.gradient_type != c.type;
-            most = std::max(most, partial_values(x.kind, cut_tensor(x.kind, twice, x.m, x.n, x.k).splits, x.m, x.n));
+            most = std::max(most, partial_values(x.kind, cut_tensor(x.kind, c.type, twice, x.m, x.n, x.k).splits, x.m, x.n));
             most = std::max(most, partial_values(x.kind, cut_plain(x.kind, x.m, x.n, x.k).splits, x.m, x.n));
         } else {
             most = std::max(most, partial_values(x.kind, cut_wide(x.kind, c.type, x.m, x.n, x.k).splits, x.m, x.n));
@@ -77,7 +77,7 @@ cudaError_t launch_product(const geo_b200_feed_forward_config_t &c, bool tensor,
         return launch_product_wide(kind, c.type, p, stream);
     }
     if (tensor) {
-        p.splits = cut_tensor(kind, kind == kWeights && c.gradient_type != c.type, p.m, p.n, p.k).splits;
+        p.splits = cut_tensor(kind, c.type, kind == kWeights && c.gradient_type != c.type, p.m, p.n, p.k).splits;
         return launch_product_tensor(kind, c.type, c.gradient_type, p, starve, stream);
     }
     p.splits = cut_plain(kind, p.m, p.n, p.k).splits;

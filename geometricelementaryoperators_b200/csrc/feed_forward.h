@@ -53,7 +53,7 @@ struct Cut {
     bool pair;    // two blocks a tile
     int splits;
 };
-Cut cut_tensor(ProductKind kind, bool twice, size_t m, size_t n, size_t k);
+Cut cut_tensor(ProductKind kind, uint32_t type, bool twice, size_t m, size_t n, size_t k);
 Cut cut_wide(ProductKind kind, uint32_t type, size_t m, size_t n, size_t k);
 Cut cut_plain(ProductKind kind, size_t m, size_t n, size_t k);
 // Values of `partial`.

@@ -46,11 +46,17 @@ constexpr int kBM = 128, kBK = 64;
 constexpr int epilogue_warps(int kind, bool twice) { return kind == kHidden || twice ? 8 : 4; }
 // Blocks of K that are summed in tensor memory in one go, where the results are float32
 // or two-term: the tensor cores cut where float32 arithmetic rounds, which takes 2e-8 of
-// the size off with each 16 of K (1.8e-5 over 8192 rows). The parts are added up in
+// the size off with each 16 of K (1.8e-5 over 8192 rows; five times that where all
+// products have one sign). The parts are added up in
 // registers, rounded to nearest. (VJP of 8192 x 4096 x 12288 to float32 cotangents, this
 // many blocks in the last product alone: 16 blocks 5.66 ms, 8 blocks 5.74, 4 blocks 5.98;
 // 16 in both products leave 4.1e-6 off, of which what two 16-bit terms lose is 2.2e-6.)
 constexpr int kChunk = 16;
+// Blocks of K that are summed up in tensor memory in one go at most, by more parts of K
+// where there are more: sums of like signs lose 1.0e-7 with each 16 of K (of random signs
+// less), so that these leave 1.0e-4 (float16) and 2.1e-4, a fifth and a nineteenth of the
+// result's own rounding. 65536 of K in one go left 4.2e-4.
+constexpr int longest(uint32_t type) { return type == GEO_B200_F16 ? 256 : 512; }
 constexpr uint32_t bytes_a(bool twice) { return (twice ? 2 : 1) * kBM * kBK * 2; }
 constexpr uint32_t bytes_b(int bn) { return (uint32_t)bn * kBK * 2; }
 // A warp's shared memory: 32 rows of 64 bytes, 16 more bytes a row to keep banks apart.
@@ -843,7 +849,7 @@ template <typename T>
 cudaError_t launch_type(ProductKind kind, uint32_t type, uint32_t out_type, const Product &p, PipelineStarve starve,
                         cudaStream_t stream) {
     const bool to_float = out_type == GEO_B200_F32;
-    const Cut cut = cut_tensor(kind, kind == kWeights && to_float, p.m, p.n, p.k);
+    const Cut cut = cut_tensor(kind, type, kind == kWeights && to_float, p.m, p.n, p.k);
     cudaError_t e;
     switch (kind) {
         case kGated: e = launch_kind<T, T, false, kGated>(cut, p, starve, stream); break;
@@ -870,11 +876,12 @@ bool tensor_products_available() { return map_encoder() != nullptr; }
 // each row of 128 bytes: 600 cycles measured for 128 + 32 rows, 700 for 128 + 128, 670
 // for a pair's 128 + 128), whichever is more; parts of K cost the way of their sums
 // through L2 and one more launch.
-Cut cut_tensor(ProductKind kind, bool twice, size_t m, size_t n, size_t k) {
+Cut cut_tensor(ProductKind kind, uint32_t type, bool twice, size_t m, size_t n, size_t k) {
     const long long sms = geo::device_sm_count(), problems = kind == kWeights ? 3 : 1;
     const long long blocks = (long long)((k + kBK - 1) / kBK) * (kind == kInput ? 2 : 1);
     const long long rows_a = kind == kWeights ? kBM : box_rows((int)(m < (size_t)kBM ? m : kBM));
-    Cut best = {256, false, 1};
+    const long long fewest = twice ? 1 : (blocks + longest(type) - 1) / longest(type);  // twice: summed up in registers
+    Cut best = {256, false, (int)fewest};
     double least = -1;
     auto look = [&](int bn, bool pair) {
         const long long columns = kind == kGated ? bn / 2 : bn, high = pair ? 2 * kBM : kBM;
@@ -882,10 +889,10 @@ Cut cut_tensor(ProductKind kind, bool twice, size_t m, size_t n, size_t k) {
         const long long teams = pair ? sms / 2 : sms, terms = twice ? 2 : 1;
         const double copies = 2.1 * (terms * rows_a + (pair ? bn / 2 : bn)) + 150, products = 2.0 * bn * terms;
         const double block = copies > products ? copies : products;
-        for (long long splits = 1; splits <= 16 && splits * 4 <= (blocks > 4 ? blocks : 4); ++splits) {
+        for (long long splits = fewest; splits == fewest || (splits <= 16 && splits * 4 <= blocks); ++splits) {
             const long long waves = (tiles * splits + teams - 1) / teams;
             const double sums = (double)sums_of(kind, 3) * splits * m * n * 4;
-            if (splits > 1 && (waves > 1 || sums > (64 << 20))) break;
+            if (splits > fewest && (waves > 1 || sums > (64 << 20))) break;
             const double cost = waves * ((blocks + splits - 1) / splits * block + 800) + 4000 +
                                 (splits > 1 ? 6500 + sums / 1800 : 0);
             if (least < 0 || cost < 0.98 * least) least = cost, best = {bn, pair, (int)splits};

@@ -1,5 +1,5 @@
 """Gated feed-forward block (geo/geo_b200.h section 5) at its limits on the GPU: waits that give up anywhere, float16
-values at both ends of its range."""
+values at both ends of its range, sums of very many values of like signs."""
 from __future__ import annotations
 
 import ctypes
@@ -94,3 +94,30 @@ def test_float16_h_beyond_its_range(gradient, before):
     for n, (g, w) in enumerate(zip(got, want)):
         difference, of = off(g, w)
         assert difference <= (2 * 2.0 ** -11 + 2.0 ** -16) * of + 2.0 ** -25 * w.numel() ** 0.5, n
+
+
+@pytest.mark.parametrize("rows,cols,hidden", [(40, 1 << 20, 16), (40, 16, 1 << 20), (1 << 22, 16, 24)])
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+def test_long_sums_of_like_signs(kind, rows, cols, hidden):
+    """Positive values alone, the worst for sums that are cut where others are rounded: what the cuts of one product
+    take off is to stay below a quarter of a step of the type's own rounding, and below 2^-12. Two such products follow
+    one another, or three in the VJP, and 16-bit values between them and at the end add a rounding each."""
+    import torch
+
+    c = Case(kind, rows, cols, hidden, "relu")
+    for v, size in ((c.x, 1.0), (c.wg, 4.0 / cols), (c.wu, 4.0 / cols), (c.wd, 4.0 / hidden), (c.dy, 16.0 / rows)):
+        v.copy_(torch.rand(v.shape, device="cuda").add(1.0).mul(size))
+    t = torch.finfo(c.dtype).eps / 2
+    cut = min(t / 2, 2.0 ** -12)
+    a, u, y, _ = c.forward()
+    want = ff.forward(*c.wide(), "relu")
+    for n, (got, w) in enumerate(zip((a, u, y), want)):
+        far = ((got.double() - w) / w).abs().max()
+        assert far <= (3 * cut + 2 * t if n == 2 else cut + t) * 1.01, n
+    outs, _ = c.vjp(a, u)
+    want = ff.vjp(*c.wide(), a.double(), u.double(), c.dy.double(), "relu")
+    for n, (got, w) in enumerate(zip(outs, want)):
+        over = w > 1.1 * torch.finfo(c.dtype).max  # float16's weights' cotangents where cols are many
+        assert got[over].isinf().all(), n
+        far = ((got.double() - w) / w)[~over].abs()
+        assert (far <= ((2 * cut if n < 3 else cut) + 2 * t) * 1.01).all(), n
