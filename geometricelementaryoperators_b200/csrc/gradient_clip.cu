@@ -48,26 +48,15 @@ struct Table {
     Entry entries[CAPACITY];
 };
 
-// The square of a value, to be summed in float64: exact for the 16-bit types, rounded to
-// its own type otherwise, but exact for a float32 value whose square leaves float32's
-// range.
-template <typename T>
-__device__ __forceinline__ double square(Wide<T> v) {
-    if constexpr (std::is_same_v<T, float>) {
-        const float s = __fmul_rn(v, v);
-        return s > 0x1p-100f && s < 0x1p126f ? (double)s : (double)v * (double)v;
-    } else {
-        return (double)v * (double)v;
-    }
-}
+// Squares of V adjacent values: exact but for the sums' own roundings (a float32's square has 48 bits).
 template <typename T, int V>
 __device__ __forceinline__ double squares(const Vec<T, V> &v) {
     double even = 0, odd = 0;
 #pragma unroll
     for (int q = 0; q < V / 2; ++q) {
-        const Pair<Wide<T>> p = v.pair(q);
-        even += square<T>(p.x);
-        odd += square<T>(p.y);
+        const double a = v.pair(q).x, b = v.pair(q).y;
+        even = ::fma(a, a, even);
+        odd = ::fma(b, b, odd);
     }
     return even + odd;
 }
@@ -95,7 +84,8 @@ __device__ double piece_squares(const Entry &e, uint32_t piece) {
         for (int i = 0; i < kEach; ++i) sum += squares<T, V>(v[i]);
     } else {
         for (size_t i = first + threadIdx.x; i < last; i += kThreads) {
-            sum += square<T>(widen(g[i]));
+            const double v = (double)widen(g[i]);
+            sum = ::fma(v, v, sum);
         }
     }
     return sum;

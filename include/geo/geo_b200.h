@@ -725,9 +725,8 @@ geo_b200_status_t geo_b200_feed_forward_wait_selftest(
 /* Norm over all gradients of a model, and clipping before the update:
  *   norm = sqrt(sum of squares of every value of every gradient),
  *   scale = min(1, max_norm / norm)  (1 for a norm of 0),  clipped = scale gradient,
- * each value rounded once to its type. Squares (of float32 values rounded to float32
- * where they are in its range) are summed in float64, in a fixed order: the same call
- * gives the same bits. A norm that is infinite or NaN (a gradient is) makes
+ * each value rounded once to its type. Squares are summed in float64, in a fixed order:
+ * the same call gives the same bits. A norm that is infinite or NaN (a gradient is) makes
  * scale NaN; the clipped values are then scale times gradient, NaN as well: the
  * update must not be made. Asynchronous and allocating nothing as section 5. */
 typedef struct {
