@@ -726,9 +726,11 @@ geo_b200_status_t geo_b200_feed_forward_wait_selftest(
  *   norm = sqrt(sum of squares of every value of every gradient),
  *   scale = min(1, max_norm / norm)  (1 for a norm of 0),  clipped = scale gradient,
  * each value rounded once to its type. Squares are summed in float64, in a fixed order:
- * the same call gives the same bits. A norm that is infinite or NaN (a gradient is) makes
- * scale NaN; the clipped values are then scale times gradient, NaN as well: the
- * update must not be made. Asynchronous and allocating nothing as section 5. */
+ * the same call gives the same bits. No square leaves its range: only a norm that does
+ * is infinite. A norm that is infinite or NaN (a gradient is, or their norm is beyond
+ * float64's range) makes scale NaN; the clipped values are then scale times gradient,
+ * NaN as well: the update must not be made. Asynchronous and allocating nothing as
+ * section 5. */
 typedef struct {
     uint32_t type;              /* geo_b200_type_t */
     uint32_t reserved;          /* 0 */

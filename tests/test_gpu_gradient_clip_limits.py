@@ -17,3 +17,38 @@ def test_squares_are_exact(kind, sizes):
     g = [made(i, torch_type(kind), n) for i, n in enumerate(sizes)]
     want = norm_of(g)
     assert abs(clip(g, 1.0, None)[0] - want) <= CLOSE * want
+
+
+@pytest.mark.parametrize("outs", ["apart", "in place", None])
+@pytest.mark.parametrize("sizes,others", [
+    ((1e160,), ()), ((1e-170,), ()), ((1e300, 1e-300), ()), ((1e160, 1.0), ("f32", "bf16")), ((1e-170, 1e-150), ()),
+    ((2.0 ** 480, 2.0 ** 482), ()), ((2.0 ** -480, 2.0 ** -482), ()), ((1e-200, 1e-30), ("f16",)), ((5e-324,), ()),
+    ((2.0 ** -600,), ("f32",)), ((0.0, 1e-180, 0.0), ())])
+def test_float64_beyond_its_squares(sizes, others, outs):
+    """Float64 gradients whose squares leave float64's range, in whole pieces and in parts of some, alone and among
+    others: the norm and the clipped values as for any."""
+    import torch
+
+    g = [made(i, torch.float64, 5000 + i).mul_(v) for i, v in enumerate(sizes)]
+    g += [made(9 + i, torch_type(k), 300) for i, k in enumerate(others)]
+    before = [v.clone() for v in g]
+    back = 2.0 ** float(torch.stack([v.double().abs().max() for v in g]).max().log2().floor().clamp(min=-1000.0))
+    want = norm_of([v.double() / back for v in g]) * back
+    # A value as small as float64's least has no digits, and its quotient by 2^-1000 none of its own.
+    norm, scale, clipped = clip(g, float(want) / 4, outs)
+    assert want > 0 and abs(norm - want) <= CLOSE * want + 5e-324
+    assert abs(scale - 0.25) <= 0.25 * (2 * CLOSE + (0.1 if want < 1e-310 else 0.0))
+    for b, o in zip(before, clipped):
+        if o is not None and b.dtype == torch.float64:
+            assert torch.equal(o, b * scale)
+
+
+def test_a_norm_beyond_float64():
+    """Finite gradients whose norm is not: infinite, and scale NaN."""
+    import torch
+
+    g = [torch.full((100,), 1e308, device="cuda", dtype=torch.float64)]
+    norm, scale, clipped = clip(g, 1.0)
+    assert norm.isinf() and scale.isnan() and clipped[0].isnan().all()
+    g[0][3] = float("nan")
+    assert clip(g, 1.0)[0].isnan()
