@@ -131,6 +131,12 @@ __device__ void piece_clip(const Entry &e, uint32_t piece, double scale) {
     piece_range<T>(e, piece, first, last);
     const T *g = (const T *)e.gradient;
     T *out = (T *)e.clipped;
+    if (scale < 0x1p-126 && sizeof(W) == 4) {
+        // In float32 a scale as small has lost digits, or all of them; the product need not be small.
+        for (size_t i = first + threadIdx.x; i < last; i += kThreads)
+            out[i] = narrow<T>((W)((double)widen(g[i]) * scale));
+        return;
+    }
     const W by = (W)scale;
     if (((uintptr_t)g | (uintptr_t)out) % 16 == 0 && last - first == kPieceBytes / sizeof(T)) {
         Vec<T, V> v[kEach];

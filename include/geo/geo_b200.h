@@ -725,7 +725,8 @@ geo_b200_status_t geo_b200_feed_forward_wait_selftest(
 /* Norm over all gradients of a model, and clipping before the update:
  *   norm = sqrt(sum of squares of every value of every gradient),
  *   scale = min(1, max_norm / norm)  (1 for a norm of 0),  clipped = scale gradient,
- * each value rounded once to its type. Squares are summed in float64, in a fixed order:
+ * in float64 for float64, else in float32 (with scale rounded to it; in float64 where
+ * scale is below float32's normal range), rounded to the type. Squares are summed in float64, in a fixed order:
  * the same call gives the same bits. No square leaves its range: only a norm that does
  * is infinite. A norm that is infinite or NaN (a gradient is, or their norm is beyond
  * float64's range) makes scale NaN; the clipped values are then scale times gradient,

@@ -52,3 +52,22 @@ def test_a_norm_beyond_float64():
     assert norm.isinf() and scale.isnan() and clipped[0].isnan().all()
     g[0][3] = float("nan")
     assert clip(g, 1.0)[0].isnan()
+
+
+@pytest.mark.parametrize("outs", ["apart", "in place"])
+@pytest.mark.parametrize("most", [1e-7, 1e-12, 1e-18])
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_scales_below_float32(kind, most, outs):
+    """Gradients of some 1e30 clipped to a small norm: scale has no digits, or is 0, in float32, and the clipped values
+    are ordinary ones. The product is rounded to float32 and to the type."""
+    import torch
+
+    g = [made(1, torch_type(kind), 10007).mul_(1e30), made(2, torch_type(kind), 3).mul_(1e30)]
+    before = [v.clone() for v in g]
+    norm, scale, clipped = clip(g, most, outs)
+    assert 0 < scale < 2.0 ** -126
+    for b, o in zip(before, clipped):
+        want = b.double() * scale
+        t = torch.finfo(o.dtype).eps / 2 + 2.0 ** -24
+        assert ((o.double() - want).abs() <= t * want.abs() + torch.finfo(torch.float32).smallest_normal * t).all()
+    assert abs(norm_of(clipped) - most) <= most * (2.0 ** -7 if kind == "bf16" else 2.0 ** -22)
