@@ -1,5 +1,5 @@
 """Gated feed-forward block (geo/geo_b200.h section 5) at its limits on the GPU: waits that give up anywhere, float16
-values at both ends of its range, sums of very many values of like signs."""
+values at both ends of its range, sums of very many values."""
 from __future__ import annotations
 
 import ctypes
@@ -121,3 +121,41 @@ def test_long_sums_of_like_signs(kind, rows, cols, hidden):
         assert got[over].isinf().all(), n
         far = ((got.double() - w) / w)[~over].abs()
         assert (far <= ((2 * cut if n < 3 else cut) + 2 * t) * 1.01).all(), n
+
+
+@pytest.mark.parametrize("kind,size", [("bf16", (200000, 40, 24)), ("f16", (200000, 40, 24)), ("f16", (3, 131072, 16)),
+                                       ("bf16", (40, 8, 131072)), ("f32", (1, 16, 1 << 20)), ("f32", (200000, 40, 24)),
+                                       ("f64", (130, 100000, 24)), ("bf16", (2, 1 << 18, 40)), ("f32", (70, 200000, 24))])
+@pytest.mark.parametrize("gradient", ["f32", None])
+def test_long_sums_as_a_whole(kind, gradient, size):
+    """2-norms, which sums that leave anything out do not meet: a 64th of K is an eighth of a sum of random signs. 16-bit
+    results are two roundings off, twice half a step, the sums' own errors far below; float32 ones sqrt(K) u of rounding
+    (2^-14 at 2^20) or two 16-bit terms' 2^-18 and cut parts of 64 instructions, 2^-16: 2^-12 is above all of them and
+    their functions; float64 ones sqrt(K) 2^-53."""
+    import torch
+
+    if kind == "f64" and gradient:
+        pytest.skip("no such pair of types")
+    c = Case(kind, *size, "silu", gradient=gradient)
+    limit = {torch.float64: 2.0 ** -40, torch.float32: 2.0 ** -12, torch.float16: 2.0 ** -10, torch.bfloat16: 2.0 ** -7}
+    a, u, y, _ = c.forward()
+    want = ff.forward(*c.wide(), "silu")
+    for n, (got, w) in enumerate(zip((a, u, y), want)):
+        difference, of = off(got, w)
+        assert difference <= limit[got.dtype] * of, n
+    outs, _ = c.vjp(a, u)
+    args = (a.double(), u.double(), c.dy.double(), "silu")
+    want = ff.vjp(*c.wide(), *args)
+    for n, (got, w) in enumerate(zip(outs, want)):
+        difference, of = off(got, w)
+        assert difference <= limit[got.dtype] * of, n
+    # The check sees what a part of the rows leaves out of the weights' cotangents, or of hidden values out of x_bar.
+    rows, hidden = size[0] - (size[0] + 63) // 64, size[2] - (size[2] + 63) // 64
+    x, wg, wu, wd = c.wide()
+    fewer = ff.vjp(x[:rows], wg, wu, wd, *[v[:rows] for v in args[:3]], "silu")
+    for n in (1, 2, 3):
+        difference, of = off(outs[n], fewer[n])
+        assert difference > 4 * limit[outs[n].dtype] * of, n
+    narrow = ff.vjp(x, wg[:hidden], wu[:hidden], wd[:, :hidden], args[0][:, :hidden], args[1][:, :hidden], *args[2:])
+    difference, of = off(outs[0], narrow[0])
+    assert difference > 4 * limit[outs[0].dtype] * of
