@@ -356,6 +356,8 @@ SIGNATURES: dict[str, tuple] = {
     "geo_b200_block_norm": (_I, [ctypes.POINTER(BlockNormConfig), *[_P] * 10]),
     "geo_b200_block_norm_vjp_workspace": (_SZ, [ctypes.POINTER(BlockNormConfig)]),
     "geo_b200_block_norm_vjp": (_I, [ctypes.POINTER(BlockNormConfig), *[_P] * 15, _SZ, _P]),
+    "geo_b200_block_norm_wait_selftest": (
+        _I, [ctypes.POINTER(BlockNormConfig), *[_P] * 10, _SZ, ctypes.c_uint32, ctypes.c_uint32, _P]),
     "geo_b200_feed_forward_workspace": (_SZ, [ctypes.POINTER(FeedForwardConfig)]),
     "geo_b200_feed_forward_vjp_workspace": (_SZ, [ctypes.POINTER(FeedForwardConfig)]),
     "geo_b200_feed_forward": (_I, [ctypes.POINTER(FeedForwardConfig), *[_P] * 8, _SZ, _P]),

@@ -23,7 +23,7 @@ namespace layers {
 
 namespace {
 
-template <typename T, int MODE, int TEAM, bool SHIFT, bool FULL>
+template <typename T, int MODE, int TEAM, bool SHIFT, bool FULL, bool STARVE = false>
 __global__ void __launch_bounds__(TEAM == kWarp ? kWarpBlock : kTeamThreads, TEAM == kWarp ? 4 : 2)
     rms_kernel(const RmsForwardArgs a, int lanes, bool float_parameters, int stages) {
     using W = Wide<T>;
@@ -75,7 +75,11 @@ __global__ void __launch_bounds__(TEAM == kWarp ? kWarpBlock : kTeamThreads, TEA
             if constexpr (SHIFT) set_past(v[u], at, row < a.rows, a.cols, W(0));
             square(u);
         }
-        complete = team_sums<R>(sums, round++, at, part, complete);
+        auto join = [&] {
+            const bool silent = STARVE && round == a.starve.round && at.rank == at.ranks - 1;
+            complete = team_sums<R>(sums, round++, at, part, complete, STARVE ? a.starve.polls : kWaitPolls, silent);
+        };
+        join();
         W rstd[R];
 #pragma unroll
         for (int u = 0; u < R; ++u) rstd[u] = rsqrt(part[u] * over + (W)a.epsilon);
@@ -104,7 +108,7 @@ __global__ void __launch_bounds__(TEAM == kWarp ? kWarpBlock : kTeamThreads, TEA
                 if constexpr (SHIFT) set_past(v[u], at, row < a.rows, a.cols, W(0));
                 square(u);
             }
-            complete = team_sums<R>(sums, round++, at, part, complete);
+            join();
 #pragma unroll
             for (int u = 0; u < R; ++u) rstd[u] = rsqrt(part[u] * over + (W)a.epsilon);
         }
@@ -176,7 +180,7 @@ __global__ void __launch_bounds__(kThreads, 4) rms_any_kernel(const RmsForwardAr
     }
 }
 
-template <typename T, int MODE, int TEAM, bool SHIFT, bool FULL>
+template <typename T, int MODE, int TEAM, bool SHIFT, bool FULL, bool STARVE = false>
 cudaError_t launch_shape(const Shape &s, const RmsForwardArgs &a, bool float_parameters, cudaStream_t stream) {
     constexpr int at_once = rows_at_once(sizeof(T), SHIFT, TEAM);
     const size_t stage = (MODE + 1) * s.part(sizeof(T));
@@ -184,7 +188,7 @@ cudaError_t launch_shape(const Shape &s, const RmsForwardArgs &a, bool float_par
     const size_t each = s.teams() * at_once, wanted = (a.rows + each - 1) / each;
     const size_t most = (size_t)geo::device_sm_count() * (512 / s.threads()) / s.blocks;
     size_t grid = wanted < most ? wanted : most;
-    return launch_team(rms_kernel<T, MODE, TEAM, SHIFT, FULL>, s, grid, s.blocks, stages * stage, stream, a, s.lanes,
+    return launch_team(rms_kernel<T, MODE, TEAM, SHIFT, FULL, STARVE>, s, grid, s.blocks, stages * stage, stream, a, s.lanes,
                        float_parameters, stages);
 }
 
@@ -213,6 +217,10 @@ cudaError_t launch_rms(NormTypes n, NormMode mode, const RmsForwardArgs &a, cuda
             });
         });
     });
+}
+
+cudaError_t launch_rms_starved(const RmsForwardArgs &a, cudaStream_t stream) {
+    return launch_shape<float, kBlockNorm, kCluster, false, true, true>(shape_of(a.cols, 4, true), a, true, stream);
 }
 
 }  // namespace layers
@@ -452,4 +460,64 @@ extern "C" geo_b200_status_t geo_b200_block_norm_vjp(
     a.residual_scale = c.residual_scale;
     a.block_scale = c.block_scale;
     return status_of(launch_rms_vjp({c.type, c.parameter_type}, mode_of(c), a, device_workspace, stream));
+}
+
+extern "C" geo_b200_status_t geo_b200_block_norm_wait_selftest(
+    const geo_b200_block_norm_config_t *config, const void *device_x, const void *device_residual,
+    const void *device_y_cotangent, void *device_out, void *device_y, void *device_x_rstd, void *device_z_rstd,
+    void *device_post_weight_cotangent, void *device_pre_weight_cotangent, void *device_workspace,
+    size_t workspace_bytes, uint32_t round, uint32_t wait_limit, cudaStream_t stream) {
+    geo::NvtxRange range("geo_b200.block_norm_wait_selftest");
+    if (!config_valid(config) || config->type != GEO_B200_F32 || config->gate != GEO_B200_GATE_NONE || wait_limit == 0 ||
+        wait_limit > kWaitPolls || device_x == nullptr || device_residual == nullptr || device_out == nullptr ||
+        device_y == nullptr || device_x_rstd == nullptr || device_z_rstd == nullptr)
+        return GEO_B200_INVALID_ARGUMENT;
+    const geo_b200_block_norm_config_t &c = *config;
+    for (const size_t stride : {c.x_stride, c.residual_stride, c.z_stride, c.y_stride, c.y_cotangent_stride,
+                                c.residual_cotangent_stride, c.x_cotangent_stride})
+        if (stride != 0) return GEO_B200_INVALID_ARGUMENT;
+    const Shape s = shape_of(c.cols, 4, true);
+    if (s.team() != kCluster || s.lanes == 0 || !s.full ||
+        !arrays_usable({{device_x, 16}, {device_residual, 16}, {device_y_cotangent, 16}, {device_out, 16}, {device_y, 16},
+                        {device_x_rstd, 4}, {device_z_rstd, 4}, {device_post_weight_cotangent, 4},
+                        {device_pre_weight_cotangent, 4}}))
+        return GEO_B200_INVALID_ARGUMENT;
+    if (device_y_cotangent == nullptr) {
+        RmsForwardArgs a = {};
+        a.x = device_x;
+        a.residual = device_residual;
+        a.z = device_out;
+        a.y = device_y;
+        a.x_rstd = device_x_rstd;
+        a.rstd = device_z_rstd;
+        a.rows = c.rows;
+        a.x_stride = a.residual_stride = a.z_stride = a.y_stride = c.cols;
+        a.cols = (int)c.cols;
+        a.epsilon = c.epsilon;
+        a.residual_scale = c.residual_scale;
+        a.block_scale = c.block_scale;
+        a.starve = {round, wait_limit};
+        return status_of(launch_rms_starved(a, stream));
+    }
+    if (device_post_weight_cotangent == nullptr || device_pre_weight_cotangent == nullptr ||
+        !workspace_usable(rms_vjp_workspace({c.type, c.parameter_type}, kBlockNorm, c.rows, c.cols), device_workspace,
+                          workspace_bytes))
+        return GEO_B200_INVALID_ARGUMENT;
+    RmsBackwardArgs a = {};
+    a.x = device_x;
+    a.z = device_residual;
+    a.x_rstd = device_x_rstd;
+    a.rstd = device_z_rstd;
+    a.dy = device_y_cotangent;
+    a.dresidual = device_out;
+    a.dx = device_y;
+    a.dpost = device_post_weight_cotangent;
+    a.dweight = device_pre_weight_cotangent;
+    a.rows = c.rows;
+    a.x_stride = a.z_stride = a.dy_stride = a.dresidual_stride = a.dx_stride = c.cols;
+    a.cols = (int)c.cols;
+    a.residual_scale = c.residual_scale;
+    a.block_scale = c.block_scale;
+    a.starve = {round, wait_limit};
+    return status_of(launch_rms_vjp_starved(a, device_workspace, stream));
 }

@@ -18,6 +18,7 @@ struct RmsForwardArgs {
     size_t rows, x_stride, residual_stride, gate_stride, z_stride, y_stride;
     int cols, gate_kind;
     double epsilon, residual_scale, block_scale;
+    Starve starve;
 };
 
 struct RmsBackwardArgs {
@@ -26,10 +27,14 @@ struct RmsBackwardArgs {
     size_t rows, x_stride, z_stride, gate_stride, dy_stride, dz_stride, dresidual_stride, dx_stride, dgate_stride;
     int cols, gate_kind;
     double residual_scale, block_scale;
+    Starve starve;
 };
 
 cudaError_t launch_rms(NormTypes t, NormMode mode, const RmsForwardArgs &a, cudaStream_t stream);
 cudaError_t launch_rms_vjp(NormTypes t, NormMode mode, const RmsBackwardArgs &a, void *workspace, cudaStream_t stream);
+// Block norms without a gate of float32 rows that fill a cluster of blocks, with a.starve.
+cudaError_t launch_rms_starved(const RmsForwardArgs &a, cudaStream_t stream);
+cudaError_t launch_rms_vjp_starved(const RmsBackwardArgs &a, void *workspace, cudaStream_t stream);
 size_t rms_vjp_workspace(NormTypes t, NormMode mode, size_t rows, size_t cols);
 
 #ifdef __CUDACC__
@@ -82,7 +87,8 @@ __device__ __forceinline__ void gate_values(int kind, const Vec<T, V> &gate, Pai
 // lane of it; the sums, the same on every thread. False: a wait gave up, sums are NaN.
 template <int N, int TEAM, int V, int K, typename W>
 __device__ __forceinline__ bool team_sums(Exchange<W, N, TEAM> &sums, uint32_t round, const Place<TEAM, V, K> &at,
-                                          W (&part)[N], bool complete) {
+                                          W (&part)[N], bool complete, uint32_t polls = kWaitPolls,
+                                          bool silent = false) {
     if constexpr (TEAM == kWarp) {
 #pragma unroll
         for (int n = 0; n < N; ++n) part[n] = team_sum(part[n], at.threads);
@@ -92,7 +98,7 @@ __device__ __forceinline__ bool team_sums(Exchange<W, N, TEAM> &sums, uint32_t r
             mine = team_sum(part[0], 32);
         else
             mine = folded_sums(part);
-        complete = exchange(sums, round, at, mine, complete);
+        complete = exchange(sums, round, at, mine, complete, polls, silent);
         constexpr int kJoin = 32 / N;  // lanes that add one value up
         W total = 0;
 #pragma unroll

@@ -41,7 +41,7 @@ constexpr int resident_blocks(int mode, int team) {
 }
 
 // The arrays in the ring: x, y_bar, then (block norm) z, the gate, z_bar, as far as they are there.
-template <typename T, int MODE, int TEAM, bool SHIFT, bool FULL>
+template <typename T, int MODE, int TEAM, bool SHIFT, bool FULL, bool STARVE = false>
 __global__ void __launch_bounds__(TEAM == kWarp ? kWarpBlock : kTeamThreads, resident_blocks(MODE, TEAM))
     rms_vjp_kernel(const RmsBackwardArgs a, int lanes, bool float_parameters, int stages, Wide<T> *partial, bool alone) {
     using W = Wide<T>;
@@ -152,7 +152,8 @@ __global__ void __launch_bounds__(TEAM == kWarp ? kWarpBlock : kTeamThreads, res
             part[2] = s3.x + s3.y;
             part[3] = W(0);
         }
-        complete = team_sums<N>(sums, round, at, part, complete);
+        complete = team_sums<N>(sums, round, at, part, complete, STARVE ? a.starve.polls : kWaitPolls,
+                                STARVE && round == a.starve.round && at.rank == at.ranks - 1);
         if constexpr (!kBlocks) {
 #pragma unroll
             for (int u = 0; u < R; ++u) {
@@ -380,13 +381,13 @@ int stages_of(NormMode mode, int at_once, size_t stage, int threads) {
     return n > 4 ? 4 : (n > 1 ? n : 1);
 }
 
-template <typename T, int MODE, int TEAM, bool SHIFT, bool FULL>
+template <typename T, int MODE, int TEAM, bool SHIFT, bool FULL, bool STARVE = false>
 cudaError_t launch_shape(const Shape &s, const RmsBackwardArgs &a, bool float_parameters, Wide<T> *partial, bool alone,
                          size_t &blocks, cudaStream_t stream) {
     const int arrays = MODE == kRms ? 2 : 3 + (MODE == kGatedNorm) + (a.dz != nullptr);
     const size_t stage = arrays * s.part(sizeof(T));
     const int stages = stages_of((NormMode)MODE, at_once_of((NormMode)MODE, sizeof(T), s), stage, s.threads());
-    return launch_team(rms_vjp_kernel<T, MODE, TEAM, SHIFT, FULL>, s, blocks, alone ? blocks : s.blocks, stages * stage,
+    return launch_team(rms_vjp_kernel<T, MODE, TEAM, SHIFT, FULL, STARVE>, s, blocks, alone ? blocks : s.blocks, stages * stage,
                        stream, a, s.lanes, float_parameters, stages, partial, alone);
 }
 
@@ -454,6 +455,16 @@ cudaError_t launch_rms_vjp(NormTypes n, NormMode mode, const RmsBackwardArgs &a,
             return launch_join<W, P>(partial, blocks, a.cols, a.dweight, a.dpost, geo::device_sm_count(), stream);
         });
     });
+}
+
+cudaError_t launch_rms_vjp_starved(const RmsBackwardArgs &a, void *workspace, cudaStream_t stream) {
+    const Shape s = shape_of(a.cols, 4, true);
+    float *const partial = (float *)workspace;
+    size_t blocks = team_grid(kBlockNorm, s, 4, a.rows);
+    const cudaError_t e = launch_shape<float, kBlockNorm, kCluster, false, true, true>(s, a, true, partial, false, blocks,
+                                                                                      stream);
+    return e != cudaSuccess ? e : launch_join<float, float>(partial, blocks, a.cols, a.dweight, a.dpost,
+                                                             geo::device_sm_count(), stream);
 }
 
 }  // namespace layers

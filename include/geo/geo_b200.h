@@ -643,6 +643,21 @@ geo_b200_status_t geo_b200_block_norm_vjp(
     void *device_post_weight_cotangent, void *device_pre_weight_cotangent, void *device_workspace,
     size_t workspace_bytes, cudaStream_t stream);
 
+/* Long rows of these norms lie in clusters, as layer norm's do, and their waits give up
+ * in the same way: what is written from then on is NaN. Self-test of that path, float32
+ * without a gate and without weights, packed and 16-byte aligned rows that fill their
+ * cluster (as for layer norm's): the block norm of device_x and device_residual into
+ * device_out (z) and device_y (device_y_cotangent NULL, both rstd written), or its VJP
+ * (device_residual: z; device_out: residual_bar; device_y: x_bar; both rstd read). The
+ * forward sums up twice a row, first x, then z: in the round-th sum (VJP: row) that a
+ * cluster takes its last block sends nothing; waits give up after wait_limit polls, 1 ..
+ * 2^22. */
+geo_b200_status_t geo_b200_block_norm_wait_selftest(
+    const geo_b200_block_norm_config_t *config, const void *device_x, const void *device_residual,
+    const void *device_y_cotangent, void *device_out, void *device_y, void *device_x_rstd, void *device_z_rstd,
+    void *device_post_weight_cotangent, void *device_pre_weight_cotangent, void *device_workspace,
+    size_t workspace_bytes, uint32_t round, uint32_t wait_limit, cudaStream_t stream);
+
 /* Gated feed-forward block of rows of cols values through hidden values:
  *   gate = x gate_weight^T,  up = x up_weight^T,  h = act(gate) up,  y = h down_weight^T,
  * gate_weight and up_weight [hidden][cols], down_weight [cols][hidden].
