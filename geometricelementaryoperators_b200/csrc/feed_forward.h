@@ -1,7 +1,8 @@
 // feed_forward.h -- what the gated feed-forward block's entry points
 // (feed_forward.cu) and products (feed_forward_tensor.cu: 16-bit types on the tensor
 // cores; feed_forward_wide.cu: float32 and float64; feed_forward_plain.cu: few rows, and
-// 16-bit arrays that the tensor cores cannot be given) share.
+// 16-bit arrays that the tensor cores cannot be given; feed_forward_scale.cu: float16's
+// powers of two) share.
 #pragma once
 
 #include "layers.h"

@@ -12,8 +12,9 @@
 // digits then are all there (8192 rows, y_bar of 1e-5: weights' float32 cotangents 2.5e-6
 // off, 1.9e-3 without). Infinities and NaN are left out: they make what they enter so.
 // Two launches; HBM bounds the first, which reads y_bar, gate, up and down_weight once
-// more (VJP of 8192 x 4096 x 8192 within the boards' spread of bfloat16's, which has no
-// need of it; 300 x 1000 x 4000 86 and 73 us, 200000 x 40 x 24 248 and 236).
+// more: 150 MB in 34 us, 14 MB in 9 (what a VJP takes more than bfloat16's, which has no
+// need of it: 300 x 1000 x 4000 84 and 73 us, 200000 x 40 x 24 255 and 242, 8192 x 4096
+// x 8192 within the boards' spread of a tenth).
 #include "feed_forward.h"
 #include "geo_runtime.h"
 
@@ -59,51 +60,48 @@ __device__ __forceinline__ float look_at(const Scan &s, size_t piece) {
             sum = 0.0f;
         }
     };
-    auto vector = [&](const T *p, size_t at, size_t last) {
-        Vec<T, V> v = Vec<T, V>::zero();
-        if (s.aligned && at + V <= last)
-            v = load<T, V>(p + at);
-        else
-            for (size_t e = at; e < last && e < at + V; ++e) take(widen(p[e]));
-        return v;
-    };
     auto take_vector = [&](const Vec<T, V> &v) {
 #pragma unroll
         for (int q = 0; q < V / 2; ++q) take(v.pair(q).x), take(v.pair(q).y);
     };
+    const T *const base = (const T *)s.m.p;
     if (s.brief) {
-        // What `vector` takes by itself it takes before the row it is of ends: one row after the other.
         const size_t row = piece * teams * kAhead + team;
-        if (s.aligned && s.cols % V == 0) {
-            Vec<T, V> v[kAhead];
+        const int at = lane * V, held = (int)s.cols - at;  // values of the lane's vector, or more
+        Vec<T, V> v[kAhead];
 #pragma unroll
-            for (int i = 0; i < kAhead; ++i)
-                v[i] = vector((const T *)s.m.p + (row + i * teams) * s.m.stride, lane * V,
-                              row + i * teams < s.rows ? s.cols : 0);
+        for (int i = 0; i < kAhead; ++i) {
+            const bool live = row + i * teams < s.rows;
+            const T *p = base + (row + i * teams) * s.m.stride + at;
+            v[i] = Vec<T, V>::zero();
+            if (live && held >= V && s.aligned) {
+                v[i] = load<T, V>(p);
+            } else if (live) {
 #pragma unroll
-            for (int i = 0; i < kAhead; ++i) take_vector(v[i]), row_ends();
-        } else {
-#pragma unroll
-            for (int i = 0; i < kAhead; ++i) {
-                take_vector(vector((const T *)s.m.p + (row + i * teams) * s.m.stride, lane * V,
-                                   row + i * teams < s.rows ? s.cols : 0));
-                row_ends();
+                for (int q = 0; q < V / 2; ++q)
+                    v[i].set(q, {2 * q < held ? widen(p[2 * q]) : 0.0f, 2 * q + 1 < held ? widen(p[2 * q + 1]) : 0.0f});
             }
         }
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) take_vector(v[i]), row_ends();
         return most;
     }
     const size_t item = piece * teams + team, row = s.parts == 1 ? item : item / s.parts;
     const size_t first = (item - row * s.parts) * s.segment;
     const size_t last = row >= s.rows ? 0 : (first + s.segment < s.cols ? first + s.segment : s.cols);
-    const T *p = (const T *)s.m.p + row * s.m.stride;
+    const T *p = base + row * s.m.stride;
     if (s.aligned) {
-        for (size_t c = first + lane * V; c < last; c += (size_t)s.lanes * V * kAhead) {
+        const size_t gap = (size_t)s.lanes * V;
+        for (size_t c = first + lane * V; c < last; c += kAhead * gap) {
             Vec<T, V> v[kAhead];
 #pragma unroll
-            for (int i = 0; i < kAhead; ++i) v[i] = vector(p, c + (size_t)i * s.lanes * V, last);
+            for (int i = 0; i < kAhead; ++i)
+                v[i] = c + i * gap + V <= last ? load<T, V>(p + c + i * gap) : Vec<T, V>::zero();
 #pragma unroll
             for (int i = 0; i < kAhead; ++i) take_vector(v[i]);
         }
+        // What is less than a vector at the end.
+        for (size_t c = last / V * V + lane; c < last; c += s.lanes) take(widen(p[c]));
     } else {
         for (size_t c = first + lane; c < last; c += (size_t)s.lanes * 16) {
             T v[16];
@@ -118,18 +116,23 @@ __device__ __forceinline__ float look_at(const Scan &s, size_t piece) {
 }
 
 // The largest over the block's threads, on its first warp.
-__device__ __forceinline__ float largest_of_block(float v) {
-    __shared__ float found[32];
-    __syncthreads();
+__device__ __forceinline__ void largest_of_block(float (&v)[4]) {
+    __shared__ float found[32][4];
+    auto of_warp = [&] {
 #pragma unroll
-    for (int o = 16; o > 0; o /= 2) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-    if ((threadIdx.x & 31) == 0) found[threadIdx.x / 32] = v;
-    __syncthreads();
-    v = threadIdx.x < blockDim.x / 32 ? found[threadIdx.x] : 0.0f;
-    if (threadIdx.x < 32)
+        for (int o = 16; o > 0; o /= 2)
 #pragma unroll
-        for (int o = 16; o > 0; o /= 2) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-    return v;
+            for (int n = 0; n < 4; ++n) v[n] = fmaxf(v[n], __shfl_xor_sync(0xffffffffu, v[n], o));
+    };
+    of_warp();
+#pragma unroll
+    for (int n = 0; n < 4; ++n)
+        if ((threadIdx.x & 31) == 0) found[threadIdx.x / 32][n] = v[n];
+    __syncthreads();
+    if (threadIdx.x >= 32) return;
+#pragma unroll
+    for (int n = 0; n < 4; ++n) v[n] = threadIdx.x < blockDim.x / 32 ? found[threadIdx.x][n] : 0.0f;
+    of_warp();
 }
 
 __global__ void __launch_bounds__(kThreads) largest_kernel(const __grid_constant__ Scans scans) {
@@ -146,19 +149,20 @@ __global__ void __launch_bounds__(kThreads) largest_kernel(const __grid_constant
             begin = scans.of[i].pieces_end;
         }
     }
+    largest_of_block(most);
     // A row's sum is at most the largest part's times the parts.
-    const float dy = largest_of_block(most[0]) * (float)scans.of[0].parts, wd = largest_of_block(most[1]);
-    const float gate = largest_of_block(most[2]), up = largest_of_block(most[3]);
-    if (threadIdx.x == 0) scans.found[1 + blockIdx.x] = make_float4(dy, wd, gate, up);
+    if (threadIdx.x == 0)
+        scans.found[1 + blockIdx.x] = make_float4(most[0] * (float)scans.of[0].parts, most[1], most[2], most[3]);
 }
 
 __global__ void __launch_bounds__(kScaleBlocks) scale_kernel(float4 *found, int activation, int blocks) {
     after_previous();
     let_next_start();
     const float4 mine = (int)threadIdx.x < blocks ? found[1 + threadIdx.x] : make_float4(0, 0, 0, 0);
-    const float dy = largest_of_block(mine.x), wd = largest_of_block(mine.y), gate = largest_of_block(mine.z),
-                up = largest_of_block(mine.w);
+    float most[4] = {mine.x, mine.y, mine.z, mine.w};
+    largest_of_block(most);
     if (threadIdx.x != 0) return;
+    const float dy = most[0], wd = most[1], gate = most[2], up = most[3];
     // |act'| <= 1.2; |act(a)| <= |a| but for the sigmoid.
     const float act = activation == GEO_B200_ACTIVATION_SIGMOID ? 1.0f : gate;
     auto power = [](float bound) { return bound > 0.0f ? 14 - ilogbf(bound) : 0; };

@@ -1,12 +1,20 @@
 // feed_forward_tensor.cu -- the feed-forward block's products of 16-bit types on
 // the tensor cores (geo/geo_b200.h section 5).
 //
-// All products are C = A B over tiles of 128 rows by BN columns, K in steps of 64.
-// One block a multiprocessor, persistent over its tiles, six warps:
+// All products are C = A B in steps of 64 of K. Large ones (PAIR) go over tiles of 256
+// rows by 256 columns, on which two blocks on neighbouring multiprocessors work
+// (tcgen05 cta_group::2): each copies its own 128 rows of A and half of the columns of
+// B, and the first block's instructions multiply for both, 256 x 256 x 16 at a time. 32
+// KB copied a block of K, where single blocks copy 48: their way from L2 into shared
+// memory is what bounds those (the instructions of the VJP's products waited 28 to 59%
+// of their time for data). Up to 128 rows, and where pairs would leave multiprocessors
+// idle, single blocks take tiles of 128 rows by BN = 64, 128 or 256 columns.
+// One block a multiprocessor, persistent over its tiles, six warps or ten:
 //   warp 0   one thread copies tiles of A and B into a ring of stages (TMA,
-//            128-byte swizzle, completion on the stage's `full` mbarrier);
-//   warp 1   one thread issues the matrix instructions of a stage (tcgen05.mma,
-//            128 x BN x 16) and commits them to the stage's `empty` mbarrier, a
+//            128-byte swizzle, completion on the stage's `full` mbarrier; a pair's on
+//            the first block's);
+//   warp 1   one thread (a pair's first block's) issues the matrix instructions of a
+//            stage (tcgen05.mma) and commits them to the stage's `empty` mbarrier, a
 //            tile's last to `ready`; the float32 sums stand in tensor memory, two
 //            tiles of BN columns in turn;
 //   warps 2-5 (2-9 where there is more to do) take a finished tile out of tensor
@@ -16,11 +24,6 @@
 // Operands whose sum index is not the adjacent one (weights in the VJP, both sides
 // of the weights' cotangents) are copied as they lie, [64 of K][64 values] boxes,
 // and read by the matrix instruction as "MN-major": nothing is transposed.
-// PAIR: two blocks on neighbouring multiprocessors work on one tile of 256 rows
-// (tcgen05 cta_group::2). Each copies its own 128 rows of A and half of the columns of
-// B, and the first block's instructions multiply for both: 32 KB copied a block of K
-// instead of 48. What bounds a single block is the way from L2 into its shared memory:
-// the instructions of the VJP's products waited 28 to 59% of their time for data.
 // kGated puts BN / 2 rows of each weight side by side in one B tile, so that gate and
 // up of the same hidden values are in one tile of sums; kInput adds both its products
 // into one tile, K running through the first pair of operands, then the second.

@@ -579,7 +579,9 @@ geo_b200_status_t geo_b200_rotary_vjp(const geo_b200_rotary_plan_t *plan, const 
  * No mean is taken off: where the rotors of an algebra leave the sum of squares of a
  * multivector's coefficients alone (every Cl(n,0)) and the weight is the same for all
  * of them, this norm commutes with rotors. config as for layer norm, weight and rstd
- * likewise (either may be NULL). */
+ * likewise (either may be NULL). mean(x^2) and epsilon are float32, float64 for float64:
+ * a row whose squares' sum leaves that range above (values of some 1e18, 1e153) has
+ * rstd 0 and y 0. */
 geo_b200_status_t geo_b200_rms_norm(const geo_b200_layer_norm_config_t *config, const void *device_x,
                                     const void *device_weight, void *device_y, void *device_rstd,
                                     cudaStream_t stream);
