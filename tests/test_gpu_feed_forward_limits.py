@@ -80,6 +80,23 @@ def test_float16_cotangents_with_infinite_rows(before):
     assert difference <= (2 * 2.0 ** -11 + 2.0 ** -16) * of + 2.0 ** -25 * want.numel() ** 0.5
 
 
+@pytest.mark.parametrize("size", [(3, 256, 3000), (300, 256, 136), (300, 1000, 4001), (5000, 24, 40), (2000, 33, 200)])
+@pytest.mark.parametrize("before", [0, 1])
+def test_float16_rows_of_unlike_sizes(before, size):
+    """One row's cotangent and another's projections far above all others: the other rows' x_bar has its digits, as in
+    the test of small cotangents."""
+    import torch
+
+    c = Case("f16", *size, before=before)
+    a, u, _, _ = c.forward()
+    c.dy[0] *= 3000.0
+    u[1, ::7] *= 4000.0
+    want = ff.vjp(*c.wide(), a.double(), u.double(), c.dy.double(), "silu")[0]
+    got = c.vjp(a, u)[0][0]
+    difference, of = off(got[2:], want[2:])
+    assert difference <= (2 * 2.0 ** -11 + 2.0 ** -16) * of + 2.0 ** -25 * want.numel() ** 0.5
+
+
 @pytest.mark.parametrize("gradient", ["f32", "f16"])
 @pytest.mark.parametrize("before", [0, 1])
 def test_float16_h_beyond_its_range(gradient, before):
