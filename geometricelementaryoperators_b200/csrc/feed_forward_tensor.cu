@@ -397,6 +397,10 @@ __global__ void __launch_bounds__(64 + 32 * epilogue_warps(KIND, TWICE), 1)
         barrier_init(drained, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    // Tensor memory is taken and given back by both blocks of a pair together, instructions
+    // without a limit to their wait: the other block has to run when one asks, and may not
+    // leave before both are through.
+    if constexpr (PAIR) cooperative_groups::this_cluster().sync();
     if (warp == 1) {
         if constexpr (PAIR) {
             asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
@@ -746,14 +750,15 @@ __global__ void __launch_bounds__(64 + 32 * epilogue_warps(KIND, TWICE), 1)
                 barrier_wait(barrier, (n / kStages) & 1, kPipelinePolls, nullptr);
             }
         }
-        if constexpr (PAIR) cooperative_groups::this_cluster().sync();
     }
+    __syncwarp();
     if (warp == 1) {
         if constexpr (PAIR)
             asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(sums), "r"(kSumColumns) : "memory");
         else
             asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(sums), "r"(kSumColumns) : "memory");
     }
+    if constexpr (PAIR) cooperative_groups::this_cluster().sync();
 }
 
 // ---- launches --------------------------------------------------------------------

@@ -176,3 +176,28 @@ def test_long_sums_as_a_whole(kind, gradient, size):
     narrow = ff.vjp(x, wg[:hidden], wu[:hidden], wd[:, :hidden], args[0][:, :hidden], args[1][:, :hidden], *args[2:])
     difference, of = off(outs[0], narrow[0])
     assert difference > 4 * limit[outs[0].dtype] * of
+
+
+def test_many_calls_in_a_row():
+    """Calls whose kernels take pairs of blocks and single ones by turns, each starting up while the one before ends, all
+    of them with tensor memory: a thousand one after another give the bits of one alone."""
+    import torch
+
+    cases = [Case("f16", 5182, 1913, 69, "gelu"), Case("bf16", 300, 640, 520, gradient="f32"),
+             Case("bf16", 40, 640, 520), Case("f16", 700, 24, 1000, gradient="f32")]
+    want = []
+    for c in cases:
+        a, u, y, _ = c.forward()
+        want.append((a, u, y, *c.vjp(a, u)[0]))
+    torch.cuda.synchronize()
+    p, L, stream = ff.pointer, abi.lib(), torch.cuda.current_stream().cuda_stream
+    outs = [[torch.empty_like(v) for v in w] for w in want]
+    for n in range(250):
+        for c, o, w in zip(cases, outs, want):
+            args = (ref(c.config), p(c.x), p(c.wg), p(c.wu), p(c.wd))
+            assert L.geo_b200_feed_forward(*args, p(o[0]), p(o[1]), p(o[2]), p(c.space), c.space.numel(), stream) == 0
+            assert L.geo_b200_feed_forward_vjp(*args, p(w[0]), p(w[1]), p(c.dy), *[p(v) for v in o[3:]], p(c.vjp_space),
+                                               c.vjp_space.numel(), stream) == 0
+    torch.cuda.synchronize()
+    for o, w in zip(outs, want):
+        assert all(torch.equal(v, e) for v, e in zip(o, w))
