@@ -50,7 +50,8 @@ constexpr int epilogue_warps(int kind, bool twice) { return kind == kHidden || t
 // Blocks of K that are summed in tensor memory in one go, where the results are float32
 // or two-term: the tensor cores cut where float32 arithmetic rounds, which takes 2e-8 of
 // the size off with each 16 of K (1.8e-5 over 8192 rows; five times that where all
-// products have one sign). The parts are added up in
+// products have one sign; float16 values below 2^-14 count as such of 2^-14 there, so that
+// sums of those alone are cut at 2^-39 of the other operand's size). The parts are added up in
 // registers, rounded to nearest. (VJP of 8192 x 4096 x 12288 to float32 cotangents, this
 // many blocks in the last product alone: 16 blocks 5.66 ms, 8 blocks 5.74, 4 blocks 5.98;
 // 16 in both products leave 4.1e-6 off, of which what two 16-bit terms lose is 2.2e-6.)

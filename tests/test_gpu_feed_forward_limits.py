@@ -201,3 +201,20 @@ def test_many_calls_in_a_row():
     torch.cuda.synchronize()
     for o, w in zip(outs, want):
         assert all(torch.equal(v, e) for v, e in zip(o, w))
+
+
+@pytest.mark.parametrize("gradient", ["f32", "f16"])
+@pytest.mark.parametrize("rows,before", [(3, 0), (200, 0), (200, 1)])
+def test_some_float16_cotangents(rows, before, gradient):
+    """Each cotangent has the same bits alone as among all, whatever the powers of two are taken from."""
+    import torch
+
+    c = Case("f16", rows, 72, 136, gradient=None if gradient == "f16" else gradient, before=before)
+    a, u, _, _ = c.forward()
+    outs, _ = c.vjp(a, u)
+    c.check_vjp(a, u, outs)
+    for wanted in [(True, False, False, False), (False, True, False, False), (False, False, True, False),
+                   (False, False, False, True), (True, False, True, True)]:
+        again, _ = c.vjp(a, u, wanted=wanted)
+        for on, one, other in zip(wanted, again, outs):
+            assert torch.equal(one, other) if on else one.isnan().all()
