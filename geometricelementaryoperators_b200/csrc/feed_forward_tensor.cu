@@ -52,10 +52,13 @@ constexpr int epilogue_warps(int kind, bool twice) { return kind == kHidden || t
 // the size off with each 16 of K (1.8e-5 over 8192 rows; five times that where all
 // products have one sign; float16 values below 2^-14 count as such of 2^-14 there, so that
 // sums of those alone are cut at 2^-39 of the other operand's size). The parts are added up in
-// registers, rounded to nearest. (VJP of 8192 x 4096 x 12288 to float32 cotangents, this
-// many blocks in the last product alone: 16 blocks 5.66 ms, 8 blocks 5.74, 4 blocks 5.98;
-// 16 in both products leave 4.1e-6 off, of which what two 16-bit terms lose is 2.2e-6.)
-constexpr int kChunk = 16;
+// registers, rounded to nearest. VJP of 8192 x 4096 x 12288 to float32 cotangents, this
+// many blocks, a weight's cotangent's error and the time in calls one after another:
+//   bfloat16  16 blocks 4.1e-6, 6.08 ms; 8 blocks 3.0e-6, 6.1 to 6.3; 4 blocks 2.6e-6, 6.5
+//   float16   16 blocks 3.5e-6, 7.0 ms;  8 blocks 1.8e-6, 7.1;        4 blocks 1.0e-6, 7.1
+// What two terms of bfloat16 lose is 2.2e-6 of it, of float16 nothing: it takes shorter parts.
+template <typename T>
+constexpr int kChunk = std::is_same_v<T, __half> ? 4 : 8;
 // Blocks of K that are summed up in tensor memory in one go at most, by more parts of K
 // where there are more: sums of like signs lose 1.0e-7 with each 16 of K (of random signs
 // less), so that these leave 1.0e-4 (float16) and 2.1e-4, a fifth and a nineteenth of the
@@ -374,7 +377,7 @@ __global__ void __launch_bounds__(64 + 32 * epilogue_warps(KIND, TWICE), 1)
                    PipelineStarve starve) {
     constexpr bool kAMn = KIND == kWeights, kBMn = KIND == kHidden || KIND == kInput || KIND == kWeights;
     constexpr int kWarps = epilogue_warps(KIND, TWICE);
-    constexpr bool kInParts = TWICE || (KIND == kHidden && std::is_same_v<O, float>);  // of kChunk blocks
+    constexpr bool kInParts = TWICE || (KIND == kHidden && std::is_same_v<O, float>);  // of kChunk<T> blocks
     constexpr int kStages = stages_of(KIND, BN, TWICE, PAIR), kColumns = KIND == kGated ? BN / 2 : BN;  // of the result, a tile
     constexpr uint32_t kBytesA = bytes_a(TWICE), kStageBytes = stage_bytes(BN, TWICE, PAIR), kSumColumns = 2 * BN < 32 ? 32 : 2 * BN;
     extern __shared__ unsigned char memory[];
@@ -489,7 +492,7 @@ __global__ void __launch_bounds__(64 + 32 * epilogue_warps(KIND, TWICE), 1)
             const int last = last_of(t);
             for (int i = first_of(t); i < last && good; ++round) {
                 const uint32_t to = round & 1, use = round >> 1;
-                const int first = i, end = kInParts && last - i > kChunk ? i + kChunk : last;
+                const int first = i, end = kInParts && last - i > kChunk<T> ? i + kChunk<T> : last;
                 good = barrier_wait(taken + 8 * to, (use & 1) ^ 1, starve.polls, &gave_up);
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 for (; i < end && good; ++i, ++step) {
@@ -596,7 +599,7 @@ __global__ void __launch_bounds__(64 + 32 * epilogue_warps(KIND, TWICE), 1)
 #pragma unroll
                 for (int j = 0; j < kPart; ++j) sum[j] = 0.0f;
                 const int last = last_of(t);
-                for (int i = first_of(t); i < last; i += kChunk) {
+                for (int i = first_of(t); i < last; i += kChunk<T>) {
                     if (i > first_of(t)) release();
                     wait();
 #pragma unroll

@@ -218,3 +218,17 @@ def test_some_float16_cotangents(rows, before, gradient):
         again, _ = c.vjp(a, u, wanted=wanted)
         for on, one, other in zip(wanted, again, outs):
             assert torch.equal(one, other) if on else one.isnan().all()
+
+
+@pytest.mark.parametrize("kind,limit", [("bf16", 2.0 ** -18), ("f16", 2.0 ** -19)])
+def test_float32_cotangents_over_long_sums(kind, limit):
+    """2-norms over 4096 columns and 8192 rows. Two terms leave at most 2^-18 of an inner value, 2^-18 / sqrt(3) of many
+    (float16's: nothing that counts); the up to 32 instructions of a part of h_bar's and a cotangent's sums (float16: 16)
+    cut some 2e-8 each; functions and the parts' own roundings leave 2^-21: below 2^-18, and 2^-19."""
+    c = Case(kind, 8192, 4096, 256, gradient="f32")
+    a, u, _, _ = c.forward()
+    outs, _ = c.vjp(a, u)
+    want = ff.vjp(*c.wide(), a.double(), u.double(), c.dy.double(), "silu")
+    for n in (1, 2, 3):
+        difference, of = off(outs[n], want[n])
+        assert difference <= limit * of, n
